@@ -383,6 +383,138 @@ int tw_optimal_path_f64(const double* cost, int B, int K, int T, int U, int max_
                         int start_view, double* r_ws, int* back_ws, int* path, int* length,
                         void* stream);
 
+/* ---------------------------------------------------------------------
+ * Encoder operators (no counterpart in the reference): what a sequence
+ * encoder in front of an alignment loss computes, for float (f32),
+ * bfloat16 (bf16) and half (f16) elements; `void*` tensors hold elements of
+ * the entry's type.  Rows may be strided: strides are in elements, the last
+ * dimension is contiguous.  Outputs are dense.  Sums, statistics and states
+ * are float32; a result is rounded once, when it is stored.
+ * ------------------------------------------------------------------- */
+
+/* Layer norm of rows of D values: y = (x - mean) / sqrt(var + eps) * weight +
+ * bias.  weight, bias: [D] or NULL (1 and 0), of the element type, or float32
+ * when params_f32.  mean, rstd: [rows] outputs for the backward, or both NULL.
+ * Backward: dx [rows, D], dweight, dbias [D] in the parameters' type; any of
+ * the three may be NULL.  Sums over rows have a fixed order. */
+size_t tw_layer_norm_workspace_bytes(size_t rows, int D);
+int tw_layer_norm_forward_f32(const void* x, size_t x_stride, const void* weight,
+                              const void* bias, int params_f32, size_t rows, int D, double eps,
+                              void* y, float* mean, float* rstd, void* stream);
+int tw_layer_norm_backward_f32(const void* dy, size_t dy_stride, const void* x, size_t x_stride,
+                               const void* weight, int params_f32, const float* mean,
+                               const float* rstd, size_t rows, int D, void* dx, void* dweight,
+                               void* dbias, void* workspace, size_t ws_bytes, void* stream);
+int tw_layer_norm_forward_bf16(const void* x, size_t x_stride, const void* weight,
+                              const void* bias, int params_f32, size_t rows, int D, double eps,
+                              void* y, float* mean, float* rstd, void* stream);
+int tw_layer_norm_backward_bf16(const void* dy, size_t dy_stride, const void* x, size_t x_stride,
+                               const void* weight, int params_f32, const float* mean,
+                               const float* rstd, size_t rows, int D, void* dx, void* dweight,
+                               void* dbias, void* workspace, size_t ws_bytes, void* stream);
+int tw_layer_norm_forward_f16(const void* x, size_t x_stride, const void* weight,
+                              const void* bias, int params_f32, size_t rows, int D, double eps,
+                              void* y, float* mean, float* rstd, void* stream);
+int tw_layer_norm_backward_f16(const void* dy, size_t dy_stride, const void* x, size_t x_stride,
+                               const void* weight, int params_f32, const float* mean,
+                               const float* rstd, size_t rows, int D, void* dx, void* dweight,
+                               void* dbias, void* workspace, size_t ws_bytes, void* stream);
+
+/* Linear layer: z = x w^T + bias, y = act(z) + residual.  x [M, K], w [N, K],
+ * bias [N] or NULL, residual [M, N] or NULL, y [M, N].  act: 0 none, 1 relu,
+ * 2 gelu (with erf), 3 silu, 4 sigmoid.  z: [M, N] output for the backward, or
+ * NULL; it is not needed without an activation.
+ * Backward: dz = dy act'(z), dx = dz w [M, K], dw = dz^T x [N, K],
+ * dbias = sum of dz's rows [N]; any of the three may be NULL.
+ * workspace: tw_linear_workspace_bytes(..., backward = 0 or 1). */
+size_t tw_linear_workspace_bytes(int M, int N, int K, int dtype_bytes, int act, int backward);
+int tw_linear_forward_f32(const void* x, size_t ldx, const void* w, size_t ldw, const void* bias,
+                          const void* residual, size_t ldr, int M, int N, int K, int act, void* y,
+                          void* z, void* workspace, size_t ws_bytes, void* stream);
+int tw_linear_backward_f32(const void* dy, size_t lddy, const void* x, size_t ldx, const void* w,
+                           size_t ldw, const void* z, int M, int N, int K, int act, void* dx,
+                           void* dw, void* dbias, void* workspace, size_t ws_bytes, void* stream);
+int tw_linear_forward_bf16(const void* x, size_t ldx, const void* w, size_t ldw, const void* bias,
+                          const void* residual, size_t ldr, int M, int N, int K, int act, void* y,
+                          void* z, void* workspace, size_t ws_bytes, void* stream);
+int tw_linear_backward_bf16(const void* dy, size_t lddy, const void* x, size_t ldx, const void* w,
+                           size_t ldw, const void* z, int M, int N, int K, int act, void* dx,
+                           void* dw, void* dbias, void* workspace, size_t ws_bytes, void* stream);
+int tw_linear_forward_f16(const void* x, size_t ldx, const void* w, size_t ldw, const void* bias,
+                          const void* residual, size_t ldr, int M, int N, int K, int act, void* y,
+                          void* z, void* workspace, size_t ws_bytes, void* stream);
+int tw_linear_backward_f16(const void* dy, size_t lddy, const void* x, size_t ldx, const void* w,
+                           size_t ldw, const void* z, int M, int N, int K, int act, void* dx,
+                           void* dw, void* dbias, void* workspace, size_t ws_bytes, void* stream);
+
+/* Gated linear recurrence: f = sigmoid(gate), h_t = f_t h_{t-1} + (1 - f_t) x_t.
+ * x, gate [B, T, D] with batch and time strides; h0 [B, D] float32 or NULL
+ * (zeros); lengths [B] or NULL: from frame lengths[b] on a sequence keeps its
+ * state, its outputs and gradients are 0 and its inputs are not read.
+ * y [B, T, D], state [B, D] float32: the last state.  carry: states saved for
+ * the backward (tw_gated_scan_carry_bytes), or NULL.
+ * Backward for dL/dy and dL/dstate (NULL: none): dx, dgate [B, T, D], dh0
+ * [B, D] float32 or NULL.
+ * Step: one frame, x, gate, y [B, D]; state is updated in place. */
+size_t tw_gated_scan_carry_bytes(int B, int T, int D);
+int tw_gated_scan_forward_f32(const void* x, size_t x_batch, size_t x_time, const void* gate,
+                              size_t g_batch, size_t g_time, const float* h0,
+                              const int64_t* lengths, int B, int T, int D, void* y, float* state,
+                              void* carry, size_t carry_bytes, void* stream);
+int tw_gated_scan_backward_f32(const void* dy, size_t dy_batch, size_t dy_time,
+                               const float* dstate, const void* x, size_t x_batch, size_t x_time,
+                               const void* gate, size_t g_batch, size_t g_time,
+                               const int64_t* lengths, const void* carry, size_t carry_bytes,
+                               int B, int T, int D, void* dx, void* dgate, float* dh0,
+                               void* stream);
+int tw_gated_scan_step_f32(const void* x, size_t x_batch, const void* gate, size_t g_batch,
+                           float* state, int B, int D, void* y, void* stream);
+int tw_gated_scan_forward_bf16(const void* x, size_t x_batch, size_t x_time, const void* gate,
+                              size_t g_batch, size_t g_time, const float* h0,
+                              const int64_t* lengths, int B, int T, int D, void* y, float* state,
+                              void* carry, size_t carry_bytes, void* stream);
+int tw_gated_scan_backward_bf16(const void* dy, size_t dy_batch, size_t dy_time,
+                               const float* dstate, const void* x, size_t x_batch, size_t x_time,
+                               const void* gate, size_t g_batch, size_t g_time,
+                               const int64_t* lengths, const void* carry, size_t carry_bytes,
+                               int B, int T, int D, void* dx, void* dgate, float* dh0,
+                               void* stream);
+int tw_gated_scan_step_bf16(const void* x, size_t x_batch, const void* gate, size_t g_batch,
+                           float* state, int B, int D, void* y, void* stream);
+int tw_gated_scan_forward_f16(const void* x, size_t x_batch, size_t x_time, const void* gate,
+                              size_t g_batch, size_t g_time, const float* h0,
+                              const int64_t* lengths, int B, int T, int D, void* y, float* state,
+                              void* carry, size_t carry_bytes, void* stream);
+int tw_gated_scan_backward_f16(const void* dy, size_t dy_batch, size_t dy_time,
+                               const float* dstate, const void* x, size_t x_batch, size_t x_time,
+                               const void* gate, size_t g_batch, size_t g_time,
+                               const int64_t* lengths, const void* carry, size_t carry_bytes,
+                               int B, int T, int D, void* dx, void* dgate, float* dh0,
+                               void* stream);
+int tw_gated_scan_step_f16(const void* x, size_t x_batch, const void* gate, size_t g_batch,
+                           float* state, int B, int D, void* y, void* stream);
+
+/* One AdamW step of many tensors of one element type.  table: HOST memory,
+ * four uint64 per tensor: parameter pointer, gradient pointer, number of
+ * values, offset of its states in the flat state buffers (a multiple of 256).
+ * It is read during the call.  state_bits 32: exp_avg, exp_avg_sq are float32
+ * and the scales NULL.  state_bits 8: exp_avg and exp_avg_sq hold e4m3 codes
+ * of m and sqrt(v), the scales one float32 per 256 values.  step: device int
+ * [2], {steps done, 0}; incremented here.  lr_device: a device float used in
+ * place of lr, or NULL.  seed: of the 8-bit codes' stochastic rounding. */
+int tw_adamw_step_f32(const uint64_t* table, int count, int state_bits, void* exp_avg,
+                      float* exp_avg_scale, void* exp_avg_sq, float* exp_avg_sq_scale, int* step,
+                      double lr, const float* lr_device, double beta1, double beta2, double eps,
+                      double weight_decay, size_t seed, void* stream);
+int tw_adamw_step_bf16(const uint64_t* table, int count, int state_bits, void* exp_avg,
+                      float* exp_avg_scale, void* exp_avg_sq, float* exp_avg_sq_scale, int* step,
+                      double lr, const float* lr_device, double beta1, double beta2, double eps,
+                      double weight_decay, size_t seed, void* stream);
+int tw_adamw_step_f16(const uint64_t* table, int count, int state_bits, void* exp_avg,
+                      float* exp_avg_scale, void* exp_avg_sq, float* exp_avg_sq_scale, int* step,
+                      double lr, const float* lr_device, double beta1, double beta2, double eps,
+                      double weight_decay, size_t seed, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -93,7 +93,30 @@ SIGNATURES = {
     "tw_jeanie_fused_backward_f32": (_c_i, [_c_p] * 5 + [_c_i] * 10 + [_c_d, _c_p, _c_sz, _c_p,
                                                                    _c_p, _c_p, _c_p]),
     "tw_optimal_path_f64": (_c_i, [_c_p] + [_c_i] * 6 + [_c_p] * 5),
+    "tw_layer_norm_workspace_bytes": (_c_sz, [_c_sz, _c_i]),
+    "tw_linear_workspace_bytes": (_c_sz, [_c_i] * 6),
+    "tw_gated_scan_carry_bytes": (_c_sz, [_c_i] * 3),
 }
+
+# the encoder operators, one entry per element type
+for _t in ("f32", "bf16", "f16"):
+    SIGNATURES.update({
+        "tw_layer_norm_forward_" + _t: (_c_i, [_c_p, _c_sz, _c_p, _c_p, _c_i, _c_sz, _c_i, _c_d]
+                                        + [_c_p] * 4),
+        "tw_layer_norm_backward_" + _t: (_c_i, [_c_p, _c_sz, _c_p, _c_sz, _c_p, _c_i, _c_p, _c_p,
+                                                _c_sz, _c_i] + [_c_p] * 4 + [_c_sz, _c_p]),
+        "tw_linear_forward_" + _t: (_c_i, [_c_p, _c_sz, _c_p, _c_sz, _c_p, _c_p, _c_sz]
+                                    + [_c_i] * 4 + [_c_p] * 3 + [_c_sz, _c_p]),
+        "tw_linear_backward_" + _t: (_c_i, [_c_p, _c_sz] * 3 + [_c_p] + [_c_i] * 4 + [_c_p] * 4
+                                     + [_c_sz, _c_p]),
+        "tw_gated_scan_forward_" + _t: (_c_i, [_c_p, _c_sz, _c_sz] * 2 + [_c_p] * 2 + [_c_i] * 3
+                                        + [_c_p] * 3 + [_c_sz, _c_p]),
+        "tw_gated_scan_backward_" + _t: (_c_i, [_c_p, _c_sz, _c_sz, _c_p] + [_c_p, _c_sz, _c_sz] * 2
+                                         + [_c_p] * 2 + [_c_sz] + [_c_i] * 3 + [_c_p] * 4),
+        "tw_gated_scan_step_" + _t: (_c_i, [_c_p, _c_sz] * 2 + [_c_p] + [_c_i] * 2 + [_c_p] * 2),
+        "tw_adamw_step_" + _t: (_c_i, [_c_p, _c_i, _c_i] + [_c_p] * 5 + [_c_d, _c_p] + [_c_d] * 4
+                                + [_c_sz, _c_p]),
+    })
 
 _LIB = None
 
@@ -149,6 +172,32 @@ def require_cuda(*tensors):
             raise RuntimeError(
                 "torchwarp_b200 runs only on CUDA tensors (B200, sm_100a); got a tensor on {}. "
                 "There is no CPU fallback.".format(t.device))
+
+
+_SUFFIX16 = {torch.float32: "f32", torch.bfloat16: "bf16", torch.float16: "f16"}
+
+
+def entry(name, dtype):
+    """The C entry of an encoder operator for an element type."""
+    suffix = _SUFFIX16.get(dtype)
+    if suffix is None:
+        raise TypeError("the encoder operators take float32, bfloat16 or float16, got {}".format(
+            dtype))
+    return getattr(lib(), name + "_" + suffix)
+
+
+def launch(name, fn, device, *args):
+    """Calls ``fn(*args, stream)`` with `device` current and its current stream, and checks the
+    status.  Pointers are plain integers (``data_ptr()``): this is the path of calls whose time is
+    the host's."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = call(name, fn, *args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            status = call(name, fn, *args, torch.cuda.current_stream(index).cuda_stream)
+    if status != 0:
+        check(status, "tw_" + name)
 
 
 # ------------------------------------------------------------ launch timing

@@ -1,0 +1,256 @@
+// One AdamW step over many tensors in one launch, states in 32 or 8 bits.
+//
+//   m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2
+//   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// The states of all tensors lie in flat buffers, each tensor's on a boundary
+// of 256 values.  In 8 bits m and sqrt(v) are e4m3 codes with one float32
+// scale per 256 values (scale = largest magnitude / 448); sqrt(v), not v,
+// because its square then spans 2^36 within a block.  Codes are rounded
+// stochastically: a moving average moves by (1 - b2) of its distance a step,
+// far less than half an e4m3 spacing, so rounding to nearest would never
+// move it.  The random bits are a hash of the value's place, the step and
+// the seed, so a step is reproducible.  The weight's update uses m and v in
+// float32, before they are rounded.
+//
+// The step count lives on the device, so a step can be captured in a CUDA
+// graph: every block reads it, the last block to have read it stores the new
+// one.
+#include <cuda_fp8.h>
+
+#include "../../include/torchwarp_b200.h"
+#include "element.cuh"
+
+namespace tw {
+namespace {
+
+constexpr int AD_UNIT = 256;     // values per scale, and per warp and turn
+constexpr int AD_THREADS = 256;
+constexpr int AD_TENSORS = 480;  // per launch
+
+struct AdamEntry {
+  void* p;
+  const void* g;
+  unsigned long long n;       // values
+  unsigned long long offset;  // of its states, a multiple of AD_UNIT
+};
+struct AdamTable {
+  AdamEntry e[AD_TENSORS];
+  unsigned first[AD_TENSORS + 1];  // units before tensor i
+  int count;
+};
+struct AdamState {
+  float* m32;
+  float* v32;
+  uint8_t* m8;
+  float* ms;
+  uint8_t* r8;
+  float* rs;
+};
+struct AdamScalars {
+  double lr, b1, b2, eps, wd;
+  const float* lr_dev;
+  uint32_t seed;
+  int* step;  // [0] steps done, [1] blocks that have read it
+  int last;   // this launch ends the step
+};
+
+__device__ __forceinline__ uint32_t lowbias32(uint32_t h) {  // C. Wellons, hash prospector
+  h ^= h >> 16;
+  h *= 0x7FEB352Du;
+  h ^= h >> 15;
+  h *= 0x846CA68Bu;
+  return h ^ (h >> 16);
+}
+
+// The e4m3 code of y >= 0 (in units of the scale), rounded up when the
+// fraction of a spacing that is cut off plus u in [0, 1) reaches 1.
+__device__ __forceinline__ float round_e4m3(float y, float u) {
+  int e = (int)(__float_as_uint(y) >> 23) - 127;
+  e = e < -6 ? -6 : e;
+  const float ulp = __uint_as_float((unsigned)(e - 3 + 127) << 23);
+  const float inv = __uint_as_float((unsigned)(3 - e + 127) << 23);
+  return fminf(floorf(__fadd_rn(y * inv, u)) * ulp, 448.f);
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+__device__ __forceinline__ float decode(uint8_t c) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+}
+
+template <typename T, bool BITS8>
+__global__ void __launch_bounds__(AD_THREADS)
+    adamw_kernel(const __grid_constant__ AdamTable tab, AdamState s, AdamScalars a) {
+  __shared__ float sc[4];
+  __shared__ uint32_t skey;
+  if (threadIdx.x == 0) {
+    const int t = *(volatile int*)a.step + 1;
+    const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
+    sc[0] = (float)(1.0 - lr * a.wd);
+    sc[1] = (float)(lr / (1.0 - pow(a.b1, (double)t)));
+    sc[2] = (float)sqrt(1.0 - pow(a.b2, (double)t));
+    skey = a.seed * 0x9E3779B1u + (uint32_t)t * 0x85EBCA77u;
+    __threadfence();
+    if (a.last && atomicAdd(&a.step[1], 1) == (int)gridDim.x - 1) {
+      a.step[1] = 0;
+      a.step[0] = t;
+    }
+  }
+  __syncthreads();
+  const float keep = sc[0], alpha = sc[1], root2 = sc[2];
+  const float b1 = (float)a.b1, c1 = (float)(1.0 - a.b1), b2 = (float)a.b2,
+              c2 = (float)(1.0 - a.b2), eps = (float)a.eps;
+  const uint32_t key = skey;
+  const int lane = threadIdx.x & 31;
+  const unsigned units = tab.first[tab.count];
+  for (unsigned u = blockIdx.x * (AD_THREADS / 32) + (threadIdx.x >> 5); u < units;
+       u += gridDim.x * (AD_THREADS / 32)) {
+    int lo = 0, hi = tab.count - 1;  // the tensor of this unit
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (tab.first[mid] <= u) lo = mid; else hi = mid - 1;
+    }
+    const unsigned long long at = (unsigned long long)(u - tab.first[lo]) * AD_UNIT;
+    const unsigned long long so = tab.e[lo].offset + at;
+    const int n = (int)min((unsigned long long)AD_UNIT, tab.e[lo].n - at);
+    T* p = (T*)tab.e[lo].p + at;
+    const T* g = (const T*)tab.e[lo].g + at;
+    float m[8], r[8], mmax = 0.f, rmax = 0.f;
+    const float ms = BITS8 ? s.ms[so / AD_UNIT] : 0.f, rs = BITS8 ? s.rs[so / AD_UNIT] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = k * 32 + lane;
+      m[k] = r[k] = 0.f;
+      if (i < n) {
+        const float gv = to_f(g[i]);
+        float v;
+        if (BITS8) {
+          m[k] = decode(s.m8[so + i]) * ms;
+          v = decode(s.r8[so + i]) * rs;
+          v *= v;
+        } else {
+          m[k] = s.m32[so + i];
+          v = s.v32[so + i];
+        }
+        m[k] = fmaf(b1, m[k], c1 * gv);
+        v = fmaf(b2, v, c2 * (gv * gv));
+        r[k] = sqrtf(v);
+        const float pv = to_f(p[i]) * keep - alpha * (m[k] / (r[k] / root2 + eps));
+        p[i] = from_f<T>(pv);
+        if (!BITS8) {
+          s.m32[so + i] = m[k];
+          s.v32[so + i] = v;
+        }
+        mmax = fmaxf(mmax, fabsf(m[k]));
+        rmax = fmaxf(rmax, r[k]);
+      }
+    }
+    if (BITS8) {
+      const float nms = warp_max(mmax) / 448.f, nrs = warp_max(rmax) / 448.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = k * 32 + lane;
+        if (i < n) {
+          const uint32_t h = lowbias32((uint32_t)(so + i) ^ key);
+          const float ym = nms > 0.f ? fabsf(m[k]) / nms : fabsf(m[k]);
+          const float yr = nrs > 0.f ? r[k] / nrs : r[k];
+          const float qm = round_e4m3(ym, (float)(h & 0xFFFFu) * (1.f / 65536.f));
+          float qr = round_e4m3(yr, (float)(h >> 16) * (1.f / 65536.f));
+          // a second moment that is not zero stays above zero: it divides m
+          if (yr > 0.f) qr = fmaxf(qr, 0.001953125f);
+          s.m8[so + i] = __nv_cvt_float_to_fp8(copysignf(qm, m[k]), __NV_SATFINITE, __NV_E4M3);
+          s.r8[so + i] = __nv_cvt_float_to_fp8(qr, __NV_SATFINITE, __NV_E4M3);
+        }
+      }
+      if (lane == 0) {
+        s.ms[so / AD_UNIT] = nms;
+        s.rs[so / AD_UNIT] = nrs;
+      }
+    }
+  }
+}
+
+template <typename T>
+int step(const uint64_t* table, int count, int bits, void* m, float* ms, void* v, float* vs,
+         int* step_state, double lr, const float* lr_dev, double b1, double b2, double eps,
+         double wd, size_t seed, void* stream) {
+  set_error(kOk, "%s", "");
+  if (count < 0 || (bits != 8 && bits != 32))
+    return set_error(kInvalid, "tw_adamw_step: invalid count=%d or state_bits=%d (8 or 32)", count,
+                     bits);
+  if (!(b1 >= 0 && b1 < 1 && b2 >= 0 && b2 < 1 && eps >= 0))
+    return set_error(kInvalid, "tw_adamw_step: need 0 <= beta < 1 and eps >= 0");
+  if (!step_state || (count && (!table || !m || !v || (bits == 8 && (!ms || !vs)))))
+    return set_error(kInvalid, "tw_adamw_step: null pointer argument");
+  AdamState s = {};
+  if (bits == 32) {
+    s.m32 = (float*)m;
+    s.v32 = (float*)v;
+  } else {
+    s.m8 = (uint8_t*)m;
+    s.ms = ms;
+    s.r8 = (uint8_t*)v;
+    s.rs = vs;
+  }
+  AdamScalars a = {lr, b1, b2, eps, wd, lr_dev, (uint32_t)seed, step_state, 0};
+  int at = 0;
+  do {
+    AdamTable tab;
+    tab.count = 0;
+    unsigned long long units = 0;
+    tab.first[0] = 0;
+    for (; at < count && tab.count < AD_TENSORS; ++at) {
+      const uint64_t* e = table + 4 * (size_t)at;
+      if (e[2] == 0) continue;
+      if (!e[0] || !e[1] || e[3] % AD_UNIT)
+        return set_error(kInvalid, "tw_adamw_step: tensor %d has a null pointer or a state offset "
+                         "that is no multiple of %d", at, AD_UNIT);
+      const unsigned long long mine = (e[2] + AD_UNIT - 1) / AD_UNIT;
+      if (mine >= 0x7fffffffull)
+        return set_error(kUnsupported, "tw_adamw_step: tensor %d is too large", at);
+      if (units + mine >= 0x7fffffffull) break;
+      units += mine;
+      tab.e[tab.count] = {(void*)e[0], (const void*)e[1], e[2], e[3]};
+      tab.first[++tab.count] = (unsigned)units;
+    }
+    a.last = at >= count;
+    const unsigned long long blocks = (units + AD_THREADS / 32 - 1) / (AD_THREADS / 32);
+    const unsigned grid = (unsigned)(blocks < 1 ? 1 : blocks < 148 * 8 ? blocks : 148 * 8);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (bits == 8)
+      adamw_kernel<T, true><<<grid, AD_THREADS, 0, st>>>(tab, s, a);
+    else
+      adamw_kernel<T, false><<<grid, AD_THREADS, 0, st>>>(tab, s, a);
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess)
+      return set_error(kLaunch, "tw_adamw_step: %s", cudaGetErrorString(err));
+  } while (at < count);
+  return kOk;
+}
+
+}  // namespace
+}  // namespace tw
+
+extern "C" {
+
+#define TW_ADAMW(SUFFIX, T)                                                                       \
+  int tw_adamw_step_##SUFFIX(const uint64_t* table, int count, int state_bits, void* exp_avg,     \
+                             float* exp_avg_scale, void* exp_avg_sq, float* exp_avg_sq_scale,     \
+                             int* step, double lr, const float* lr_device, double beta1,          \
+                             double beta2, double eps, double weight_decay, size_t seed,          \
+                             void* stream) {                                                      \
+    return tw::step<T>(table, count, state_bits, exp_avg, exp_avg_scale, exp_avg_sq,              \
+                       exp_avg_sq_scale, step, lr, lr_device, beta1, beta2, eps, weight_decay,    \
+                       seed, stream);                                                             \
+  }
+
+TW_ADAMW(f32, float)
+TW_ADAMW(bf16, __nv_bfloat16)
+TW_ADAMW(f16, __half)
+
+}  // extern "C"

@@ -1,0 +1,73 @@
+// Element types of the encoder operators (layer norm, linear, gated scan,
+// AdamW): float, bfloat16 and half in memory, float in registers.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace tw {
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+
+// One rounding, to nearest even, when a result leaves the registers.
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <> __device__ __forceinline__ __half from_f<__half>(float v) {
+  return __float2half_rn(v);
+}
+
+// f = sigmoid(z) and 1 - f: the smaller of the two from exp(-|z|), which
+// neither overflows nor cancels, to a few ulp of itself; the larger is one
+// minus it, correctly rounded.
+__device__ __forceinline__ void sigmoid_pair(float z, float& f, float& omf) {
+  const float e = ex2(-1.4426950408889634f * fabsf(z));
+  const float lo = e * rcp(1.f + e), hi = 1.f - lo;
+  f = z >= 0.f ? hi : lo;
+  omf = z >= 0.f ? lo : hi;
+}
+
+// Activations of the linear operator (values of the `act` argument).
+enum Act : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3, kActSigmoid = 4 };
+
+// The roundings are explicit: a call that saves z gives the bits of one that
+// does not, whatever the compiler contracts around it.
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+  if (ACT == kActRelu) return z < 0.f ? 0.f : z;  // a NaN stays a NaN
+  if (ACT == kActGelu) {
+    const float h = mul_rn(0.5f, z);
+    return __fmaf_rn(h, erff(mul_rn(z, 0.70710678118654752f)), h);
+  }
+  if (ACT == kActSilu || ACT == kActSigmoid) {
+    float f, omf;
+    sigmoid_pair(z, f, omf);
+    return ACT == kActSilu ? mul_rn(z, f) : f;
+  }
+  return z;
+}
+
+// d act / dz at z.
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+  if (ACT == kActRelu) return z > 0.f ? 1.f : (z != z ? z : 0.f);
+  if (ACT == kActGelu) {
+    const float cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+    const float pdf = 0.39894228040143268f * ex2(-0.72134752044448170f * z * z);
+    return fmaf(z, pdf, cdf);
+  }
+  if (ACT == kActSilu || ACT == kActSigmoid) {
+    float f, omf;
+    sigmoid_pair(z, f, omf);
+    return ACT == kActSilu ? f * fmaf(z, omf, 1.f) : f * omf;
+  }
+  return 1.f;
+}
+
+}  // namespace tw

@@ -1,0 +1,162 @@
+"""AdamW over all parameters of a group in one launch, with 32-bit or 8-bit states."""
+
+from array import array
+
+import torch
+
+from .. import _native as nat
+
+_BLOCK = 256  # values that share a scale; every tensor's states start on such a boundary
+
+
+class _Bucket:
+    """The parameters of one group with one type on one device, and their flat states."""
+
+    def __init__(self, params, bits):
+        self.params = params
+        self.device, self.dtype = params[0].device, params[0].dtype
+        nat.require_cuda(params[0])
+        self.fn = nat.entry("tw_adamw_step", self.dtype)
+        self.offsets, at = [], 0
+        for p in params:
+            self.offsets.append(at)
+            at += -(-p.numel() // _BLOCK) * _BLOCK
+        dev = self.device
+        self.step = torch.zeros(2, dtype=torch.int32, device=dev)
+        if bits == 32:
+            self.state = {"exp_avg": torch.zeros(at, device=dev),
+                          "exp_avg_sq": torch.zeros(at, device=dev)}
+        else:
+            code = dict(dtype=torch.float8_e4m3fn, device=dev)
+            self.state = {"exp_avg": torch.zeros(at, **code),
+                          "exp_avg_scale": torch.zeros(at // _BLOCK, device=dev),
+                          "exp_avg_sqrt": torch.zeros(at, **code),
+                          "exp_avg_sqrt_scale": torch.zeros(at // _BLOCK, device=dev)}
+        self.bits = bits
+
+    def pointers(self):
+        s = self.state
+        if self.bits == 32:
+            return s["exp_avg"].data_ptr(), None, s["exp_avg_sq"].data_ptr(), None
+        return tuple(s[k].data_ptr() for k in ("exp_avg", "exp_avg_scale", "exp_avg_sqrt",
+                                               "exp_avg_sqrt_scale"))
+
+    def table(self):
+        """Four numbers a tensor for the native step; a tensor without a gradient is left out."""
+        rows, keep = [], []
+        for p, offset in zip(self.params, self.offsets):
+            g = p.grad
+            if g is None:
+                continue
+            if g.dtype != self.dtype or g.is_sparse:
+                raise TypeError("a gradient must be dense and of its parameter's type {}, got {}"
+                                .format(self.dtype, g.dtype))
+            if not p.is_contiguous():
+                raise ValueError("parameters must be contiguous")
+            if not g.is_contiguous():
+                g = g.contiguous()
+                keep.append(g)
+            rows += (p.data_ptr(), g.data_ptr(), p.numel(), offset)
+        return array("Q", rows), keep
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) in one kernel launch per group and type.
+
+    Args:
+        params: Parameters or groups of them: float32, bfloat16 or float16 CUDA tensors.
+        lr: Learning rate, a number or a one-element float32 CUDA tensor.  A step captured in a
+            CUDA graph reads the tensor at each replay; a number is captured as it is.
+        betas, eps, weight_decay: As in ``torch.optim.AdamW``.
+        state_bits: 32, or 8: the first moment and the root of the second as e4m3 codes with a
+            float32 scale per 256 values, rounded stochastically.
+        seed: Of that rounding; one seed gives one result.
+
+    The states of a group's parameters lie in flat buffers (``flat_state``).  The step count is
+    the group's and lives on the device; a parameter without a gradient is left out of a step.
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *,
+                 state_bits=32, seed=0):
+        if not isinstance(lr, torch.Tensor) and not lr >= 0:
+            raise ValueError("lr must be >= 0")
+        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+            raise ValueError("betas must be in [0, 1)")
+        if not eps >= 0:
+            raise ValueError("eps must be >= 0")
+        if not weight_decay >= 0:
+            raise ValueError("weight_decay must be >= 0")
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        self._bits, self._seed, self._buckets = state_bits, int(seed), {}
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def _group_buckets(self, index):
+        """Made at the first step, when the parameters are where they will stay."""
+        group = self.param_groups[index]["params"]
+        have = self._buckets.get(index)
+        if have is None or sum(len(b.params) for b in have) != len(group):
+            kinds = {}
+            for p in group:
+                kinds.setdefault((p.device, p.dtype), []).append(p)
+            have = self._buckets[index] = [_Bucket(ps, self._bits) for ps in kinds.values()]
+        return have
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for index, group in enumerate(self.param_groups):
+            lr = group["lr"]
+            for b in self._group_buckets(index):
+                table, keep = b.table()
+                lr_device = None
+                if isinstance(lr, torch.Tensor):
+                    if lr.device != b.device or lr.dtype != torch.float32 or lr.numel() != 1:
+                        raise ValueError("lr must be a number or one float32 value on {}".format(
+                            b.device))
+                    lr_device = lr.data_ptr()
+                m, ms, v, vs = b.pointers()
+                nat.launch("adamw_step", b.fn, b.device, table.buffer_info()[0], len(table) // 4,
+                           self._bits, m, ms, v, vs, b.step.data_ptr(),
+                           0.0 if lr_device else float(lr), lr_device, group["betas"][0],
+                           group["betas"][1], group["eps"], group["weight_decay"],
+                           self._seed & 0xFFFFFFFF)
+                # written through raw pointers: autograd has to see the change
+                torch.autograd.graph.increment_version([p for p in b.params if p.grad is not None])
+        return loss
+
+    def flat_state(self, index=0):
+        """The flat state buffers of bucket ``index`` (groups in order, a bucket for each type in
+        them): ``exp_avg`` and ``exp_avg_sq``, or in 8 bits ``exp_avg`` and ``exp_avg_sqrt`` with
+        their ``*_scale``.  Each tensor's states start on a multiple of 256 values, in the order
+        of the parameters."""
+        buckets = [b for i in range(len(self.param_groups)) for b in self._group_buckets(i)]
+        return dict(buckets[index].state)
+
+    def state_dict(self):
+        """Hyperparameters by group, and the flat states of every bucket."""
+        out = super().state_dict()
+        out["state_bits"] = self._bits
+        out["seed"] = self._seed
+        out["buckets"] = [{"step": b.step[:1].clone(), **b.state}
+                          for i in range(len(self.param_groups)) for b in self._group_buckets(i)]
+        return out
+
+    def load_state_dict(self, state_dict):
+        if state_dict.get("state_bits") != self._bits:
+            raise ValueError("the saved states have {} bits, this optimizer's {}".format(
+                state_dict.get("state_bits"), self._bits))
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        mine = [b for i in range(len(self.param_groups)) for b in self._group_buckets(i)]
+        saved = state_dict["buckets"]
+        if len(mine) != len(saved) or any(v.shape != s[k].shape for b, s in zip(mine, saved)
+                                          for k, v in b.state.items()):
+            raise ValueError("the saved states belong to other parameters")
+        self._seed = int(state_dict["seed"])
+        for b, s in zip(mine, saved):
+            b.step[:1].copy_(s["step"])
+            for k, v in b.state.items():
+                v.copy_(s[k])

@@ -3,6 +3,8 @@
     import torchwarp_b200.functional as TF
 """
 
+from .encoder.functional import (GatedScanOutput, gated_scan, gated_scan_step, layer_norm,
+                                 linear)
 from .jeanie.distances import euclidean_cost, rbf_cost, squared_euclidean_cost
 from .jeanie.functional import jeanie, jeanie_from_cost
 from .jeanie.fvm import fvm, fvm_from_cost
@@ -25,4 +27,9 @@ __all__ = [
     "euclidean_cost",
     "squared_euclidean_cost",
     "rbf_cost",
+    "layer_norm",
+    "linear",
+    "gated_scan",
+    "gated_scan_step",
+    "GatedScanOutput",
 ]
