@@ -426,8 +426,11 @@ int tw_layer_norm_backward_f16(const void* dy, size_t dy_stride, const void* x, 
  * NULL; it is not needed without an activation.
  * Backward: dz = dy act'(z), dx = dz w [M, K], dw = dz^T x [N, K],
  * dbias = sum of dz's rows [N]; any of the three may be NULL.
- * workspace: tw_linear_workspace_bytes(..., backward = 0 or 1). */
-size_t tw_linear_workspace_bytes(int M, int N, int K, int dtype_bytes, int act, int backward);
+ * workspace: 256-byte aligned, tw_linear_workspace_bytes(); unaligned: 0 when
+ * every row of x, w and dy starts on a 16-byte boundary wherever K (of x, w)
+ * or N (of dy) is a multiple of 8, else 1. */
+size_t tw_linear_workspace_bytes(int M, int N, int K, int dtype_bytes, int act, int backward,
+                                 int unaligned);
 int tw_linear_forward_f32(const void* x, size_t ldx, const void* w, size_t ldw, const void* bias,
                           const void* residual, size_t ldr, int M, int N, int K, int act, void* y,
                           void* z, void* workspace, size_t ws_bytes, void* stream);

@@ -94,7 +94,7 @@ SIGNATURES = {
                                                                    _c_p, _c_p, _c_p]),
     "tw_optimal_path_f64": (_c_i, [_c_p] + [_c_i] * 6 + [_c_p] * 5),
     "tw_layer_norm_workspace_bytes": (_c_sz, [_c_sz, _c_i]),
-    "tw_linear_workspace_bytes": (_c_sz, [_c_i] * 6),
+    "tw_linear_workspace_bytes": (_c_sz, [_c_i] * 7),
     "tw_gated_scan_carry_bytes": (_c_sz, [_c_i] * 3),
 }
 

@@ -14,6 +14,8 @@
 
 namespace tw {
 
+int linear_take_device_error();
+
 static thread_local char g_err[512] = "";
 
 int set_error(int code, const char* fmt, ...) {
@@ -218,7 +220,8 @@ int tw_device_error(void) {
   if (cudaDeviceSynchronize() != cudaSuccess) return set_error(kLaunch, "device synchronize failed");
   const int tc_err = tc_take_device_error();
   const int dp_err = dp_take_device_error();
-  return tc_err != 0 ? tc_err : dp_err;
+  const int lin_err = linear_take_device_error();
+  return tc_err != 0 ? tc_err : dp_err != 0 ? dp_err : lin_err;
 }
 
 size_t tw_sdtw_saved_bytes(int B, int N, int M, int dtype_bytes, int has_penalty) {

@@ -36,11 +36,30 @@ __device__ __forceinline__ void sigmoid_pair(float z, float& f, float& omf) {
 // Activations of the linear operator (values of the `act` argument).
 enum Act : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3, kActSigmoid = 4 };
 
+// FAST (results rounded to 16 bits): the normal distribution function
+// through Abramowitz & Stegun 7.1.26, erfc(x) = (a1 t + .. + a5 t^5) e^(-x^2)
+// with t = 1 / (1 + p x), |error| <= 1.5e-7: one exponential and one
+// reciprocal in place of erff's two polynomial branches.  e is e^(-z^2/2).
+__device__ __forceinline__ float normal_cdf_fast(float z, float& e) {
+  const float t = rcp(__fmaf_rn(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
+  e = ex2(mul_rn(mul_rn(-0.72134752044448170f, z), z));
+  float q = __fmaf_rn(1.061405429f, t, -1.453152027f);
+  q = __fmaf_rn(q, t, 1.421413741f);
+  q = __fmaf_rn(q, t, -0.284496736f);
+  q = __fmaf_rn(q, t, 0.254829592f);
+  q = mul_rn(mul_rn(mul_rn(q, t), 0.5f), e);
+  return z < 0.f ? q : add_rn(1.f, -q);
+}
+
 // The roundings are explicit: a call that saves z gives the bits of one that
 // does not, whatever the compiler contracts around it.
-template <int ACT>
+template <int ACT, bool FAST>
 __device__ __forceinline__ float act_value(float z) {
   if (ACT == kActRelu) return z < 0.f ? 0.f : z;  // a NaN stays a NaN
+  if (ACT == kActGelu && FAST) {
+    float e;
+    return mul_rn(z, normal_cdf_fast(z, e));
+  }
   if (ACT == kActGelu) {
     const float h = mul_rn(0.5f, z);
     return __fmaf_rn(h, erff(mul_rn(z, 0.70710678118654752f)), h);
@@ -54,13 +73,18 @@ __device__ __forceinline__ float act_value(float z) {
 }
 
 // d act / dz at z.
-template <int ACT>
+template <int ACT, bool FAST>
 __device__ __forceinline__ float act_slope(float z) {
   if (ACT == kActRelu) return z > 0.f ? 1.f : (z != z ? z : 0.f);
   if (ACT == kActGelu) {
-    const float cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-    const float pdf = 0.39894228040143268f * ex2(-0.72134752044448170f * z * z);
-    return fmaf(z, pdf, cdf);
+    float cdf, e;
+    if (FAST) {
+      cdf = normal_cdf_fast(z, e);
+    } else {
+      cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+      e = ex2(-0.72134752044448170f * z * z);
+    }
+    return fmaf(z, 0.39894228040143268f * e, cdf);
   }
   if (ACT == kActSilu || ACT == kActSigmoid) {
     float f, omf;

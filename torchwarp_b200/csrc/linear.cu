@@ -4,91 +4,315 @@
 //   z = x w^T + b, y = act(z) + residual
 //   dz = dy act'(z), dx = dz w, dw = dz^T x, db = sum_rows dz
 //
-// Products accumulate in float32; z is saved in the element type (only when
-// there is an activation), the activation itself is taken of the unrounded z.
+// Products run on the tensor cores (linear_gemm.cuh) and accumulate in
+// float32.  Up to SMALL_ROWS rows (single tokens) the forward reads the
+// weight once with plain loads instead.  z is saved in the element type and
+// only when there is an activation; the activation itself is taken of the
+// unrounded z.  dz is rounded to the element type once, as the operand of its
+// two products; db sums it before that rounding.
+//
+// An operand goes to the tensor cores as it lies in memory when TMA can read
+// it (16-byte aligned rows).  Otherwise, and for float32, which is taken as
+// three bfloat16 planes, a pass writes it to the workspace first.
 #include "../../include/torchwarp_b200.h"
 #include "element.cuh"
+#include "linear_gemm.h"
 
 namespace tw {
+
+// One CTA pair computes a 256 x 256 tile at the tensor cores' full rate; it
+// takes 48 such tiles (of the 74 pairs) to beat single CTAs with narrower
+// tiles, which spread a small product over more SMs.  Where even those leave
+// a third of the SMs idle, the contraction is split, down to 4 chunks (256
+// values) a part (2 chunks for float32, whose chunks take six products).
+GemmPlan gemm_plan(int M, int N, int K, int planes) {
+  const long long nK = (K + 63) / 64;
+  if (planes == 1) {
+    const long long pairs = (long long)((M + 255) / 256) * ((N + 255) / 256);
+    if (pairs >= 48) return {2, 256, 1};
+  }
+  const long long rows = (M + 127) / 128;
+  const int tn = N > 64 && rows * ((N + 127) / 128) >= 74 ? 128 : 64;
+  const long long tiles = rows * ((N + tn - 1) / tn);
+  long long splits = 1;
+  if (tiles < 100) {
+    splits = 148 / tiles;
+    const long long most = nK / (planes == 1 ? 4 : 2);
+    if (splits > most) splits = most;
+    if (splits < 1) splits = 1;
+  }
+  return {1, tn, (int)splits};
+}
+
 namespace {
 
-constexpr int LT = 64;   // tile of the output
-constexpr int LK = 16;   // depth of a step
-constexpr int L_THREADS = 256;
+constexpr int SMALL_ROWS = 8;
+constexpr int SMALL_COLS = 4;  // output columns of a warp
 
-// out[m, n] = epilogue(sum_k A(m, k) B(n, k)), A(m, k) = A[m * am + k * ak].
-template <typename T, int ACT>
-__global__ void __launch_bounds__(L_THREADS)
-    linear_kernel(const T* __restrict__ A, size_t am, size_t ak, const T* __restrict__ Bm,
-                  size_t bn, size_t bk, int M, int N, int K, const T* __restrict__ bias,
-                  const T* __restrict__ res, size_t ldr, T* __restrict__ out,
-                  T* __restrict__ z) {
-  __shared__ float sa[LK][LT + 1], sb[LK][LT + 1];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int tiles_n = (N + LT - 1) / LT;
-  const int m0 = (int)(blockIdx.x / tiles_n) * LT, n0 = (int)(blockIdx.x % tiles_n) * LT;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < K; k0 += LK) {
-    for (int i = threadIdx.x; i < LT * LK; i += L_THREADS) {
-      const int r = i / LK, k = i % LK;
-      const bool in = k0 + k < K;
-      sa[k][r] = in && m0 + r < M ? to_f(A[(size_t)(m0 + r) * am + (size_t)(k0 + k) * ak]) : 0.f;
-      sb[k][r] = in && n0 + r < N ? to_f(Bm[(size_t)(n0 + r) * bn + (size_t)(k0 + k) * bk]) : 0.f;
+// --------------------------------------------------------- few rows
+
+// 16 bytes of T as floats (VEC), or one value.
+template <typename T, bool VEC> struct Lanes {
+  static constexpr int N = VEC ? 16 / (int)sizeof(T) : 1;
+  static __device__ __forceinline__ void load(const T* p, float (&v)[N]) {
+    if (VEC) {
+      union { uint4 u; T t[16 / sizeof(T)]; } q;
+      q.u = __ldg(reinterpret_cast<const uint4*>(p));
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = to_f(q.t[i]);
+    } else {
+      v[0] = to_f(*p);
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < LK; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[i][j] = fmaf(sa[k][ty + 16 * i], sb[k][tx + 16 * j], acc[i][j]);
-    __syncthreads();
   }
+};
+
+// Sums C values over the warp so that lane l ends with value l / (32 / C):
+// each step sends the half of the values that the other lanes keep.
+template <int C>
+__device__ __forceinline__ float scatter_sum(float (&v)[C], int lane) {
+  int o = 16;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int n = C; n > 1; n /= 2, o /= 2) {
+    const bool up = lane & o;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m < M && n < N) {
-        const float zv = add_rn(acc[i][j], bias ? to_f(bias[n]) : 0.f);
-        if (z) z[(size_t)m * N + n] = from_f<T>(zv);
-        const float v = add_rn(act_value<ACT>(zv), res ? to_f(res[(size_t)m * ldr + n]) : 0.f);
-        out[(size_t)m * N + n] = from_f<T>(v);
+    for (int i = 0; i < n / 2; ++i) {
+      const float send = up ? v[i] : v[i + n / 2], keep = up ? v[i + n / 2] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+  float s = v[0];
+#pragma unroll
+  for (; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+template <bool FAST>
+__device__ __forceinline__ float activate1(float v, int act) {
+  switch (act) {
+    case kActRelu: return act_value<kActRelu, FAST>(v);
+    case kActGelu: return act_value<kActGelu, FAST>(v);
+    case kActSilu: return act_value<kActSilu, FAST>(v);
+    case kActSigmoid: return act_value<kActSigmoid, FAST>(v);
+    default: return v;
+  }
+}
+
+// M <= MT rows: a warp owns 4 output columns, its lanes the contraction.
+// Bound by the one read of the weight; x stays in the caches.
+template <typename T, int MT, bool VEC>
+__global__ void __launch_bounds__(128)
+    linear_small_kernel(const T* __restrict__ x, size_t ldx, const T* __restrict__ w, size_t ldw,
+                        int M, int N, int K, const T* __restrict__ bias,
+                        const T* __restrict__ res, size_t ldr, int act, T* __restrict__ y,
+                        T* __restrict__ z) {
+  constexpr int V = Lanes<T, VEC>::N;
+  const int lane = threadIdx.x & 31;
+  const int n0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * SMALL_COLS;
+  if (n0 >= N) return;
+  const T* wr[SMALL_COLS];
+  const T* xr[MT];
+#pragma unroll
+  for (int j = 0; j < SMALL_COLS; ++j) wr[j] = w + (size_t)min(n0 + j, N - 1) * ldw;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) xr[i] = x + (size_t)min(i, M - 1) * ldx;
+  float acc[MT * SMALL_COLS];
+#pragma unroll
+  for (int i = 0; i < MT * SMALL_COLS; ++i) acc[i] = 0.f;
+  const int whole = K / V * V;
+#pragma unroll 2
+  for (int k = lane * V; k < whole; k += 32 * V) {
+    float wv[SMALL_COLS][V];
+#pragma unroll
+    for (int j = 0; j < SMALL_COLS; ++j) Lanes<T, VEC>::load(wr[j] + k, wv[j]);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      float xv[V];
+      Lanes<T, VEC>::load(xr[i] + k, xv);
+#pragma unroll
+      for (int j = 0; j < SMALL_COLS; ++j)
+#pragma unroll
+        for (int q = 0; q < V; ++q)
+          acc[i * SMALL_COLS + j] = fmaf(xv[q], wv[j][q], acc[i * SMALL_COLS + j]);
+    }
+  }
+  if (whole + lane < K) {  // fewer than V values are left
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < SMALL_COLS; ++j)
+        acc[i * SMALL_COLS + j] = fmaf(to_f(xr[i][whole + lane]), to_f(wr[j][whole + lane]),
+                                       acc[i * SMALL_COLS + j]);
+  }
+  constexpr int C = MT * SMALL_COLS, REP = 32 / C;
+  float v = scatter_sum<C>(acc, lane);
+  const int id = lane / REP, m = id / SMALL_COLS, n = n0 + id % SMALL_COLS;
+  if (lane % REP || m >= M || n >= N) return;
+  v = add_rn(v, bias ? to_f(bias[n]) : 0.f);
+  if (z) z[(size_t)m * N + n] = from_f<T>(v);
+  v = activate1<sizeof(T) == 2>(v, act);
+  y[(size_t)m * N + n] = from_f<T>(add_rn(v, res ? to_f(res[(size_t)m * ldr + n]) : 0.f));
+}
+
+template <typename T>
+int launch_small(const T* x, size_t ldx, const T* w, size_t ldw, int M, int N, int K,
+                 const T* bias, const T* res, size_t ldr, int act, T* y, T* z, cudaStream_t st) {
+  const bool vec = (uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0 &&
+                   (M == 1 || ldx * sizeof(T) % 16 == 0) && (N == 1 || ldw * sizeof(T) % 16 == 0);
+  const unsigned grid = (unsigned)((N + 4 * SMALL_COLS - 1) / (4 * SMALL_COLS));
+#define TW_SMALL(MT)                                                                             \
+  (vec ? linear_small_kernel<T, MT, true><<<grid, 128, 0, st>>>(x, ldx, w, ldw, M, N, K, bias,   \
+                                                                res, ldr, act, y, z)             \
+       : linear_small_kernel<T, MT, false><<<grid, 128, 0, st>>>(x, ldx, w, ldw, M, N, K, bias,  \
+                                                                 res, ldr, act, y, z))
+  if (M == 1) TW_SMALL(1);
+  else if (M == 2) TW_SMALL(2);
+  else if (M <= 4) TW_SMALL(4);
+  else TW_SMALL(8);
+#undef TW_SMALL
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_error(kLaunch, "tw_linear_forward: %s", cudaGetErrorString(e));
+  return kOk;
+}
+
+// ------------------------------------------- operands for the tensor cores
+
+template <typename T> struct Packed {
+  using E = T;
+  static constexpr int PL = 1;
+};
+template <> struct Packed<float> {
+  using E = __nv_bfloat16;
+  static constexpr int PL = 3;
+};
+
+// x = p0 + p1 + p2 exactly (8 + 8 + 8 bits), each rounded to nearest.  An
+// infinity or NaN stays in p0.
+__device__ __forceinline__ void split3(float x, __nv_bfloat16& p0, __nv_bfloat16& p1,
+                                       __nv_bfloat16& p2) {
+  p0 = __float2bfloat16_rn(x);
+  float h = __bfloat162float(p0);
+  if (fabsf(h) == INFINITY && fabsf(x) < INFINITY) {  // rounded past the largest value
+    h = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+    p0 = __float2bfloat16_rn(h);
+  }
+  const float r = fabsf(x) < INFINITY ? x - h : 0.f;
+  p1 = __float2bfloat16_rn(r);
+  p2 = __float2bfloat16_rn(r - __bfloat162float(p1));
+}
+
+constexpr int PACK_ROWS = 8, PACK_COLS = 256;  // rows and columns of a block's step
+
+// src [R, C], or src * act'(z), as the tensor cores read it: rows of Cp
+// (a multiple of 8) values, in planes.  dst NULL: no copy; sums: column sums
+// over this block's `rb` rows, in float32 before rounding, or NULL.
+// Bound by HBM: each value is read once with 16-byte loads where the rows
+// are aligned and written once.
+template <typename T, int ACT>
+__global__ void __launch_bounds__(256)
+    linear_pack_kernel(const T* __restrict__ src, size_t ld, const T* __restrict__ z, int R, int C,
+                       int Cp, typename Packed<T>::E* __restrict__ dst, size_t plane, int rb,
+                       float* __restrict__ sums, int vec) {
+  constexpr int PL = Packed<T>::PL;
+  using E = typename Packed<T>::E;
+  __shared__ float red[PACK_ROWS][PACK_COLS + 8];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int c0 = blockIdx.x * PACK_COLS + tx * 8;
+  const int r1 = min(R, (int)(blockIdx.y + 1) * rb);
+  float s[8] = {};
+  if (c0 < Cp) {
+#pragma unroll 2
+    for (int r = blockIdx.y * rb + ty; r < r1; r += PACK_ROWS) {
+      const T* p = src + (size_t)r * ld + c0;
+      const T* zp = ACT == kActNone ? nullptr : z + (size_t)r * C + c0;
+      float v[8];
+      if (vec && c0 + 8 <= C) {
+        constexpr int PER = 16 / sizeof(T);
+        union { uint4 u[8 / PER]; T t[8]; } q, qz;
+#pragma unroll
+        for (int i = 0; i < 8 / PER; ++i) q.u[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        if (ACT != kActNone)
+#pragma unroll
+          for (int i = 0; i < 8 / PER; ++i)
+            qz.u[i] = __ldg(reinterpret_cast<const uint4*>(zp) + i);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          v[i] = to_f(q.t[i]);
+          if (ACT != kActNone) v[i] *= act_slope<ACT, sizeof(T) == 2>(to_f(qz.t[i]));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          v[i] = c0 + i < C ? to_f(p[i]) : 0.f;
+          if (ACT != kActNone && c0 + i < C)
+            v[i] *= act_slope<ACT, sizeof(T) == 2>(to_f(zp[i]));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += v[i];
+      if (dst) {
+        union { E t[8]; uint4 u; } q[PL];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (PL == 3) split3(v[i], q[0].t[i], q[1].t[i], q[2].t[i]);
+          else q[0].t[i] = from_f<E>(v[i]);
+        }
+#pragma unroll
+        for (int k = 0; k < PL; ++k)
+          *reinterpret_cast<uint4*>(dst + k * plane + (size_t)r * Cp + c0) = q[k].u;
       }
     }
-}
-
-template <typename T, int ACT>
-__global__ void __launch_bounds__(L_THREADS)
-    linear_dz_kernel(const T* __restrict__ dy, size_t ldy, const T* __restrict__ z, int M, int N,
-                     T* __restrict__ dz) {
-  const size_t n = (size_t)M * N;
-  for (size_t i = (size_t)blockIdx.x * L_THREADS + threadIdx.x; i < n;
-       i += (size_t)gridDim.x * L_THREADS) {
-    const size_t m = i / N, c = i - m * N;
-    const float s = ACT == kActNone ? 1.f : act_slope<ACT>(to_f(z[i]));
-    dz[i] = from_f<T>(to_f(dy[m * ldy + c]) * s);
   }
-}
-
-template <typename T, int ACT>
-__global__ void __launch_bounds__(L_THREADS)
-    linear_db_kernel(const T* __restrict__ dy, size_t ldy, const T* __restrict__ z, int M, int N,
-                     T* __restrict__ db) {
-  __shared__ float sh[8][33];
-  const int c = threadIdx.x & 31, g = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
-  float s = 0.f;
-  if (n < N)
-    for (int m = g; m < M; m += 8)
-      s += to_f(dy[(size_t)m * ldy + n]) *
-           (ACT == kActNone ? 1.f : act_slope<ACT>(to_f(z[(size_t)m * N + n])));
-  sh[g][c] = s;
+  if (!sums) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) red[ty][tx * 8 + i] = s[i];
   __syncthreads();
-  if (g == 0 && n < N) {
-    for (int i = 1; i < 8; ++i) s += sh[i][c];
-    db[n] = from_f<T>(s);
+  const int c = blockIdx.x * PACK_COLS + threadIdx.x;
+  if (c < C) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < PACK_ROWS; ++k) t += red[k][threadIdx.x];
+    sums[(size_t)blockIdx.y * C + c] = t;
   }
+}
+
+// db[c] = the blocks' column sums, in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    linear_db_kernel(const float* __restrict__ sums, int blocks, int C, T* __restrict__ db) {
+  __shared__ float red[8][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 32 + tx;
+  float s = 0.f;
+  if (c < C)
+    for (int b = ty; b < blocks; b += 8) s += sums[(size_t)b * C + c];
+  red[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && c < C) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += red[i][tx];
+    db[c] = from_f<T>(s);
+  }
+}
+
+size_t up8(size_t n) { return (n + 7) / 8 * 8; }
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Rows of a block of the pack kernel: 64, or more where that makes over 256
+// blocks along the rows (their sums are read back).
+int rows_per_block(int R) {
+  const int rb = (R + 255) / 256;
+  return (rb < 64 ? 64 : (rb + 7) / 8 * 8);
+}
+int row_blocks(int R) { return (R + rows_per_block(R) - 1) / rows_per_block(R); }
+
+template <typename T>
+bool tma_reads(const void* p, size_t ld, int rows, int cols) {
+  return sizeof(T) == 2 && (uintptr_t)p % 16 == 0 &&
+         (rows == 1 || (ld % 8 == 0 && ld >= (size_t)cols));
+}
+
+template <typename T>
+size_t packed_bytes(int R, int C) {
+  return up256((size_t)Packed<T>::PL * R * up8(C) * 2);
 }
 
 int launched(const char* who) {
@@ -98,12 +322,60 @@ int launched(const char* who) {
 }
 
 template <typename T, int ACT>
-int product(const T* A, size_t am, size_t ak, const T* B, size_t bn, size_t bk, int M, int N,
-            int K, const T* bias, const T* res, size_t ldr, T* out, T* z, cudaStream_t st) {
-  const unsigned grid = (unsigned)(((M + LT - 1) / LT) * (size_t)((N + LT - 1) / LT));
-  linear_kernel<T, ACT><<<grid, L_THREADS, 0, st>>>(A, am, ak, B, bn, bk, M, N, K, bias, res, ldr,
-                                                    out, z);
-  return launched("tw_linear");
+void pack(const T* src, size_t ld, const T* z, int R, int C, void* dst, float* sums,
+          cudaStream_t st) {
+  const int Cp = (int)up8(C);
+  const int vec = (uintptr_t)src % 16 == 0 && ld * sizeof(T) % 16 == 0 &&
+                  (ACT == kActNone || ((uintptr_t)z % 16 == 0 && C * sizeof(T) % 16 == 0));
+  const dim3 grid((Cp + PACK_COLS - 1) / PACK_COLS, row_blocks(R));
+  linear_pack_kernel<T, ACT><<<grid, 256, 0, st>>>(
+      src, ld, z, R, C, Cp, (typename Packed<T>::E*)dst, (size_t)R * Cp, rows_per_block(R), sums,
+      vec);
+}
+
+// src as an operand: as it lies, or packed into `ws` (taken when `packs`).
+template <typename T>
+GemmOperand operand(const T* src, size_t ld, int R, int C, bool k_major, bool packs, void* ws,
+                    cudaStream_t st) {
+  if (!packs)
+    return {src, R == 1 ? up8(C) : ld, 0, R, C, k_major};
+  pack<T, kActNone>(src, ld, nullptr, R, C, ws, nullptr, st);
+  return {ws, up8(C), (size_t)R * up8(C), R, C, k_major};
+}
+
+size_t partial_bytes(int M, int N, int K, int planes) {
+  const GemmPlan p = gemm_plan(M, N, K, planes);
+  return p.splits > 1 ? up256((size_t)p.splits * M * N * sizeof(float)) : 0;
+}
+
+// Workspace of a call, in this order.
+struct Layout {
+  size_t dz, x, w, sums, partial, total;
+};
+
+template <typename T>
+Layout layout(int M, int N, int K, int act, bool backward, bool pack_dy, bool pack_x, bool pack_w) {
+  constexpr int PL = Packed<T>::PL;
+  Layout l = {};
+  if (M <= 0 || (!backward && M <= SMALL_ROWS)) return l;
+  size_t at = 0;
+  l.dz = at;
+  if (backward && (act != kActNone || pack_dy)) at += packed_bytes<T>(M, N);
+  l.x = at;
+  if (pack_x) at += packed_bytes<T>(M, K);
+  l.w = at;
+  if (pack_w) at += packed_bytes<T>(N, K);
+  l.sums = at;
+  if (backward) at += up256((size_t)row_blocks(M) * N * sizeof(float));
+  l.partial = at;
+  if (backward) {
+    const size_t a = partial_bytes(M, K, N, PL), b = partial_bytes(N, K, M, PL);
+    at += a > b ? a : b;
+  } else {
+    at += partial_bytes(M, N, K, PL);
+  }
+  l.total = at;
+  return l;
 }
 
 int check(const char* who, int M, int N, int K, int act) {
@@ -112,91 +384,140 @@ int check(const char* who, int M, int N, int K, int act) {
                      N, K);
   if (act < kActNone || act > kActSigmoid)
     return set_error(kInvalid, "%s: unknown activation %d", who, act);
-  const size_t big = 0x7fffffff;
-  if ((size_t)((M + LT - 1) / LT) * ((N + LT - 1) / LT) > big ||
-      (size_t)((M + LT - 1) / LT) * ((K + LT - 1) / LT) > big ||
-      (size_t)((N + LT - 1) / LT) * ((K + LT - 1) / LT) > big)
-    return set_error(kUnsupported, "%s: too many tiles", who);
+  if (M > 0x7fffffff - 512 || N > 0x7fffffff - 512 || K > 0x7fffffff - 512)
+    return set_error(kUnsupported, "%s: a size is too large", who);
+  return kOk;
+}
+
+int check_ws(const char* who, size_t have, size_t need, const void* ws) {
+  if (have < need || (need && (!ws || (uintptr_t)ws % 256)))
+    return set_error(kWorkspace, "%s: workspace needs %zu bytes, 256-byte aligned", who, need);
   return kOk;
 }
 
 template <typename T>
-int fwd(const void* x, size_t ldx, const void* w, size_t ldw, const void* bias, const void* res,
-        size_t ldr, int M, int N, int K, int act, void* y, void* z, void* stream) {
+int fwd(const void* xv, size_t ldx, const void* wv, size_t ldw, const void* bias, const void* res,
+        size_t ldr, int M, int N, int K, int act, void* y, void* z, void* ws, size_t ws_bytes,
+        void* stream) {
   set_error(kOk, "%s", "");
   if (int e = check("tw_linear_forward", M, N, K, act)) return e;
   if (M == 0) return kOk;
-  if (!x || !w || !y) return set_error(kInvalid, "tw_linear_forward: null pointer argument");
+  if (!xv || !wv || !y) return set_error(kInvalid, "tw_linear_forward: null pointer argument");
   cudaStream_t st = (cudaStream_t)stream;
-#define TW_CASE(A)                                                                               \
-  case A:                                                                                        \
-    return product<T, A>((const T*)x, ldx, 1, (const T*)w, ldw, 1, M, N, K, (const T*)bias,      \
-                         (const T*)res, ldr, (T*)y, (T*)z, st)
-  switch (act) {
-    TW_CASE(kActNone);
-    TW_CASE(kActRelu);
-    TW_CASE(kActGelu);
-    TW_CASE(kActSilu);
-    default:
-      TW_CASE(kActSigmoid);
-  }
-#undef TW_CASE
-}
-
-template <typename T, int ACT>
-int bwd_act(const T* dy, size_t ldy, const T* x, size_t ldx, const T* w, size_t ldw, const T* z,
-            int M, int N, int K, T* dx, T* dw, T* db, T* dz, cudaStream_t st) {
-  if (db) linear_db_kernel<T, ACT><<<(N + 31) / 32, L_THREADS, 0, st>>>(dy, ldy, z, M, N, db);
-  size_t ldz = ldy;
-  if (ACT != kActNone && M) {
-    linear_dz_kernel<T, ACT><<<148 * 8, L_THREADS, 0, st>>>(dy, ldy, z, M, N, dz);
-    dy = dz;
-    ldz = N;
-  }
-  int e = launched("tw_linear_backward");
-  if (!e && dx && M)
-    e = product<T, kActNone>(dy, ldz, 1, w, 1, ldw, M, K, N, nullptr, nullptr, 0, dx, nullptr, st);
-  if (!e && dw)
-    e = product<T, kActNone>(dy, 1, ldz, x, 1, ldx, N, K, M, nullptr, nullptr, 0, dw, nullptr, st);
-  return e;
+  const T* x = (const T*)xv;
+  const T* w = (const T*)wv;
+  if (M <= SMALL_ROWS)
+    return launch_small<T>(x, ldx, w, ldw, M, N, K, (const T*)bias, (const T*)res, ldr, act,
+                           (T*)y, (T*)z, st);
+  const bool px = !tma_reads<T>(x, ldx, M, K), pw = !tma_reads<T>(w, ldw, N, K);
+  const Layout l = layout<T>(M, N, K, act, false, false, px, pw);
+  if (int e = check_ws("tw_linear_forward", ws_bytes, l.total, ws)) return e;
+  char* base = (char*)ws;
+  GemmProblem p = {};
+  p.a = operand<T>(x, ldx, M, K, true, px, base + l.x, st);
+  p.b = operand<T>(w, ldw, N, K, true, pw, base + l.w, st);
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.bias = bias;
+  p.residual = res;
+  p.ldr = ldr;
+  p.act = act;
+  p.out = y;
+  p.z = act == kActNone ? nullptr : z;
+  p.partial = (float*)(base + l.partial);
+  if (int e = launched("tw_linear_forward")) return e;
+  return gemm_run<T>(p, st);
 }
 
 template <typename T>
-int bwd(const void* dy, size_t ldy, const void* x, size_t ldx, const void* w, size_t ldw,
+void pack_dz(const T* dy, size_t ldy, const T* z, int M, int N, int act, void* dst, float* sums,
+             cudaStream_t st) {
+  switch (act) {
+    case kActRelu: pack<T, kActRelu>(dy, ldy, z, M, N, dst, sums, st); break;
+    case kActGelu: pack<T, kActGelu>(dy, ldy, z, M, N, dst, sums, st); break;
+    case kActSilu: pack<T, kActSilu>(dy, ldy, z, M, N, dst, sums, st); break;
+    case kActSigmoid: pack<T, kActSigmoid>(dy, ldy, z, M, N, dst, sums, st); break;
+    default: pack<T, kActNone>(dy, ldy, nullptr, M, N, dst, sums, st); break;
+  }
+}
+
+template <typename T>
+int bwd(const void* dyv, size_t ldy, const void* xv, size_t ldx, const void* wv, size_t ldw,
         const void* z, int M, int N, int K, int act, void* dx, void* dw, void* db, void* ws,
         size_t ws_bytes, void* stream) {
   set_error(kOk, "%s", "");
   if (int e = check("tw_linear_backward", M, N, K, act)) return e;
+  const T* dy = (const T*)dyv;
+  const T* x = (const T*)xv;
+  const T* w = (const T*)wv;
   if (M && (!dy || (dx && !w) || (dw && !x) || (act != kActNone && !z)))
     return set_error(kInvalid, "tw_linear_backward: null pointer argument");
-  const size_t need = tw_linear_workspace_bytes(M, N, K, (int)sizeof(T), act, 1);
-  if (ws_bytes < need || (need && !ws))
-    return set_error(kWorkspace, "tw_linear_backward: workspace needs %zu bytes", need);
   cudaStream_t st = (cudaStream_t)stream;
-#define TW_CASE(A)                                                                              \
-  case A:                                                                                       \
-    return bwd_act<T, A>((const T*)dy, ldy, (const T*)x, ldx, (const T*)w, ldw, (const T*)z, M, \
-                         N, K, (T*)dx, (T*)dw, (T*)db, (T*)ws, st)
-  switch (act) {
-    TW_CASE(kActNone);
-    TW_CASE(kActRelu);
-    TW_CASE(kActGelu);
-    TW_CASE(kActSilu);
-    default:
-      TW_CASE(kActSigmoid);
+  if (M == 0) {  // sums over no rows
+    if (dw) cudaMemsetAsync(dw, 0, (size_t)N * K * sizeof(T), st);
+    if (db) cudaMemsetAsync(db, 0, (size_t)N * sizeof(T), st);
+    return launched("tw_linear_backward");
   }
-#undef TW_CASE
+  const bool px = dw && !tma_reads<T>(x, ldx, M, K), pw = dx && !tma_reads<T>(w, ldw, N, K);
+  const bool pdy = !tma_reads<T>(dy, ldy, M, N);
+  const Layout l = layout<T>(M, N, K, act, true, pdy, px, pw);
+  if (int e = check_ws("tw_linear_backward", ws_bytes, l.total, ws)) return e;
+  char* base = (char*)ws;
+  const bool packs = (dx || dw) && (act != kActNone || pdy);
+  if (packs || db) {
+    float* sums = db ? (float*)(base + l.sums) : nullptr;
+    pack_dz<T>(dy, ldy, (const T*)z, M, N, act, packs ? base + l.dz : nullptr, sums, st);
+    if (db) linear_db_kernel<T><<<(N + 31) / 32, 256, 0, st>>>(sums, row_blocks(M), N, (T*)db);
+  }
+  GemmOperand dz = {dy, M == 1 ? up8(N) : ldy, 0, M, N, true};
+  if (packs) dz = {base + l.dz, up8(N), (size_t)M * up8(N), M, N, true};
+  GemmProblem p = {};
+  p.partial = (float*)(base + l.partial);
+  if (dx) {
+    p.a = dz;
+    p.b = operand<T>(w, ldw, N, K, false, pw, base + l.w, st);
+    p.M = M;
+    p.N = K;
+    p.K = N;
+    p.out = dx;
+    if (int e = launched("tw_linear_backward")) return e;
+    if (int e = gemm_run<T>(p, st)) return e;
+  }
+  if (dw) {
+    p.a = dz;
+    p.a.k_major = false;
+    p.b = operand<T>(x, ldx, M, K, false, px, base + l.x, st);
+    p.M = N;
+    p.N = K;
+    p.K = M;
+    p.out = dw;
+    if (int e = launched("tw_linear_backward")) return e;
+    if (int e = gemm_run<T>(p, st)) return e;
+  }
+  return launched("tw_linear_backward");
 }
 
 }  // namespace
+
+// Errors of the product's kernels, of all types.
+int linear_take_device_error() {
+  const int a = gemm_take_device_error<float>(), b = gemm_take_device_error<__nv_bfloat16>(),
+            c = gemm_take_device_error<__half>();
+  return a != 0 ? a : b != 0 ? b : c;
+}
+
 }  // namespace tw
 
 extern "C" {
 
-size_t tw_linear_workspace_bytes(int M, int N, int K, int dtype_bytes, int act, int backward) {
-  (void)K;
-  if (!backward || act == tw::kActNone || M <= 0) return 0;
-  return (size_t)M * N * dtype_bytes;
+size_t tw_linear_workspace_bytes(int M, int N, int K, int dtype_bytes, int act, int backward,
+                                 int unaligned) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const bool u = unaligned != 0;
+  if (dtype_bytes == 4) return tw::layout<float>(M, N, K, act, backward != 0, true, true, true).total;
+  return tw::layout<__nv_bfloat16>(M, N, K, act, backward != 0, u || N % 8, u || K % 8,
+                                   u || K % 8).total;
 }
 
 #define TW_LINEAR(SUFFIX, T)                                                                     \
@@ -204,9 +525,8 @@ size_t tw_linear_workspace_bytes(int M, int N, int K, int dtype_bytes, int act, 
                                  const void* bias, const void* residual, size_t ldr, int M,      \
                                  int N, int K, int act, void* y, void* z, void* workspace,       \
                                  size_t ws_bytes, void* stream) {                                \
-    (void)workspace;                                                                             \
-    (void)ws_bytes;                                                                              \
-    return tw::fwd<T>(x, ldx, w, ldw, bias, residual, ldr, M, N, K, act, y, z, stream);          \
+    return tw::fwd<T>(x, ldx, w, ldw, bias, residual, ldr, M, N, K, act, y, z, workspace,        \
+                      ws_bytes, stream);                                                         \
   }                                                                                              \
   int tw_linear_backward_##SUFFIX(const void* dy, size_t lddy, const void* x, size_t ldx,        \
                                   const void* w, size_t ldw, const void* z, int M, int N, int K, \

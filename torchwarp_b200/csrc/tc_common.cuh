@@ -298,6 +298,12 @@ __device__ __forceinline__ uint32_t sw128b32_elem(int r, int w) {
 int make_map_3d_f32(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t dim1,
                     uint64_t dim2, uint32_t box0, uint32_t box1, bool granule32 = false);
 
+// 3-D tensor map with the caller's type, byte strides (of dim1 and dim2), box
+// and swizzle; errors as above.
+int make_map_3d(CUtensorMap* map, CUtensorMapDataType type, const void* base,
+                const uint64_t (&dims)[3], const uint64_t (&strides)[2], const uint32_t (&box)[3],
+                CUtensorMapSwizzle swizzle);
+
 // Reads and clears the device error word set by a tensor-core kernel whose
 // bounded wait ran out (0 = none).
 int tc_take_device_error();

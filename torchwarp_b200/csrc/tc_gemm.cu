@@ -1412,8 +1412,9 @@ bool aligned16(const void* p) { return p == nullptr || ((uintptr_t)p & 15u) == 0
 
 // ------------------------------------------------------------------ host
 
-int make_map_3d_f32(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t dim1,
-                    uint64_t dim2, uint32_t box0, uint32_t box1, bool granule32) {
+int make_map_3d(CUtensorMap* map, CUtensorMapDataType type, const void* base,
+                const uint64_t (&dims)[3], const uint64_t (&strides)[2], const uint32_t (&box)[3],
+                CUtensorMapSwizzle swizzle) {
   using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -1429,18 +1430,25 @@ int make_map_3d_f32(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t 
       encode = reinterpret_cast<EncodeFn>(fn);
   });
   if (encode == nullptr) return set_error(kUnsupported, "cuTensorMapEncodeTiled unavailable");
-  const cuuint64_t dims[3] = {dim0, dim1, dim2};
-  const cuuint64_t strides[2] = {dim0 * 4, dim0 * dim1 * 4};
-  const cuuint32_t box[3] = {box0, box1, 1};
+  const cuuint64_t d[3] = {dims[0], dims[1], dims[2]};
+  const cuuint64_t st[2] = {strides[0], strides[1]};
+  const cuuint32_t bx[3] = {box[0], box[1], box[2]};
   const cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(base), dims,
-                            strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            granule32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B
-                                      : CU_TENSOR_MAP_SWIZZLE_128B,
+  const CUresult r = encode(map, type, 3, const_cast<void*>(base), d, st, bx, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(kUnsupported, "tensor map rejected (CUresult %d)", (int)r);
   return kOk;
+}
+
+int make_map_3d_f32(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t dim1,
+                    uint64_t dim2, uint32_t box0, uint32_t box1, bool granule32) {
+  const uint64_t dims[3] = {dim0, dim1, dim2};
+  const uint64_t strides[2] = {dim0 * 4, dim0 * dim1 * 4};
+  const uint32_t box[3] = {box0, box1, 1};
+  return make_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, dims, strides, box,
+                     granule32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 int tc_take_device_error() {

@@ -149,6 +149,12 @@ layer_norm_op.register_autograd(_layer_norm_bwd, setup_context=_layer_norm_setup
 
 # ------------------------------------------------------------------ linear
 
+def _unaligned(a, stride_a, b, stride_b):
+    """1 when a row of 16-bit elements may start off a 16-byte boundary."""
+    return int((a.data_ptr() | b.data_ptr()) & 15 != 0 or (stride_a | stride_b) & 7 != 0
+               or stride_a < a.shape[-1] or stride_b < b.shape[-1])
+
+
 def linear_forward(x, weight, bias, residual, act, save):
     n, k = weight.shape
     m = x.numel() // k
@@ -157,7 +163,10 @@ def linear_forward(x, weight, bias, residual, act, save):
     if m:
         (xr, xs), (wr, wst) = rows_of(x), rows_of(weight)
         rr, rs = (None, 0) if residual is None else rows_of(residual)
-        nbytes = nat.lib().tw_linear_workspace_bytes(m, n, k, x.element_size(), act, 0)
+        nbytes = 0
+        if m > 8:  # fewer rows take none
+            nbytes = nat.lib().tw_linear_workspace_bytes(m, n, k, x.element_size(), act, 0,
+                                                         _unaligned(xr, xs, wr, wst))
         ws = _workspace(nbytes, x.device)
         nat.launch("linear_forward", nat.entry("tw_linear_forward", x.dtype), x.device,
                    xr.data_ptr(), xs, wr.data_ptr(), wst,
@@ -178,7 +187,9 @@ def linear_backward(dy, x, weight, z, act, need):
         if dy.dtype != x.dtype:
             dy = dy.to(x.dtype)
         (gr, gs), (xr, xs), (wr, wst) = rows_of(dy), rows_of(x), rows_of(weight)
-        nbytes = nat.lib().tw_linear_workspace_bytes(m, n, k, x.element_size(), act, 1)
+        nbytes = nat.lib().tw_linear_workspace_bytes(
+            m, n, k, x.element_size(), act, 1,
+            _unaligned(xr, xs, wr, wst) or _unaligned(gr, gs, gr, gs))
         ws = _workspace(nbytes, dev)
         nat.launch("linear_backward", nat.entry("tw_linear_backward", x.dtype), dev,
                    gr.data_ptr(), gs, xr.data_ptr(), xs, wr.data_ptr(), wst, _p(z), m, n, k, act,
