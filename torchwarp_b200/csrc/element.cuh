@@ -23,6 +23,41 @@ template <> __device__ __forceinline__ __half from_f<__half>(float v) {
   return __float2half_rn(v);
 }
 
+// N consecutive elements as floats, and back; with VEC in pieces of 16 bytes
+// (the address is 16-byte aligned), else one by one.
+template <bool VEC, int N, typename T>
+__device__ __forceinline__ void load_n(const T* p, float* v) {
+  constexpr int PER = 16 / sizeof(T);
+  if constexpr (VEC && N % PER == 0) {
+#pragma unroll
+    for (int i = 0; i < N / PER; ++i) {
+      union { uint4 u; T t[PER]; } q;
+      q.u = __ldg(reinterpret_cast<const uint4*>(p) + i);
+#pragma unroll
+      for (int k = 0; k < PER; ++k) v[i * PER + k] = to_f(q.t[k]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = to_f(p[i]);
+  }
+}
+template <bool VEC, int N, typename T>
+__device__ __forceinline__ void store_n(T* p, const float* v) {
+  constexpr int PER = 16 / sizeof(T);
+  if constexpr (VEC && N % PER == 0) {
+#pragma unroll
+    for (int i = 0; i < N / PER; ++i) {
+      union { uint4 u; T t[PER]; } q;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) q.t[k] = from_f<T>(v[i * PER + k]);
+      reinterpret_cast<uint4*>(p)[i] = q.u;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = from_f<T>(v[i]);
+  }
+}
+
 // f = sigmoid(z) and 1 - f: the smaller of the two from exp(-|z|), which
 // neither overflows nor cancels, to a few ulp of itself; the larger is one
 // minus it, correctly rounded.

@@ -9,17 +9,29 @@
 // A sequence of length L < T keeps its state from frame L on: its outputs
 // there are 0, its gradients 0, and x and g are not read.
 //
-// The forward saves the state before every SCAN_CHUNK-th frame in float32;
-// the backward recomputes the states inside a chunk from it, so no rounded
-// output enters a gradient and the outputs are not read again.
+// One pass over the data.  The channels of all sequences, c = b D + d, are
+// numbered through; a block owns 32 (or 64 of 16 bits, as pairs) of them and
+// walks time in tiles of 8 warps x 16 frames.  A thread reads its 16 frames
+// into registers, composes them to (A, B) with h_out = A h_in + B, learns its
+// h_in from the warps before it, and runs its frames again from the registers
+// to write the outputs.  Few channels: up to 8 blocks of a cluster take
+// neighbouring tiles and compose their (A, B) through each other's shared
+// memory, so that a long sequence still fills the GPU.  Everything is summed
+// in a fixed order.
+//
+// The forward saves h before every 16th frame in float32 (0.25 bytes a value);
+// the backward recomputes the states of a thread's frames from it, so no
+// rounded output enters a gradient and the outputs are not read again.
 #include "../../include/torchwarp_b200.h"
 #include "element.cuh"
 
 namespace tw {
 namespace {
 
-constexpr int SCAN_CHUNK = 32;
-constexpr int SCAN_THREADS = 128;
+constexpr int SCAN_FRAMES = 16;  // of a thread
+constexpr int SCAN_WARPS = 8;
+constexpr int SCAN_TILE = SCAN_FRAMES * SCAN_WARPS;
+constexpr int SCAN_THREADS = 32 * SCAN_WARPS;
 
 __device__ __forceinline__ int live_len(const int64_t* lengths, int b, int T) {
   if (!lengths) return T;
@@ -27,77 +39,293 @@ __device__ __forceinline__ int live_len(const int64_t* lengths, int b, int T) {
   return n < 0 ? 0 : n > T ? T : (int)n;
 }
 
-// One frame: f h + (1 - f) x as a step from the nearer of the two, so that the
-// rounding of a gate near 1 does not decay a state that should last.
-__device__ __forceinline__ float advance(float f, float omf, float h, float x) {
-  return f >= 0.5f ? fmaf(omf, x - h, h) : fmaf(f, h - x, x);
+// A gate as one number: the smaller of 1 - f and f, which keeps its relative
+// precision, negative when it is f.  +0 keeps the state.
+__device__ __forceinline__ float gate_of(float z) {
+  const float e = ex2(-1.4426950408889634f * fabsf(z));
+  return copysignf(e * rcp(1.f + e), z);
 }
-// f l, likewise.
-__device__ __forceinline__ float decay(float f, float omf, float l) {
-  return f >= 0.5f ? fmaf(-omf, l, l) : f * l;
+__device__ __forceinline__ bool opens(float s) { return __float_as_int(s) < 0; }
+// f h + (1 - f) x as a step from the nearer of the two, so that the rounding
+// of a gate near 1 does not decay a state that should last.
+__device__ __forceinline__ float advance(float s, float h, float x) {
+  return fmaf(s, x - h, opens(s) ? x : h);
+}
+// f l and (1 - f) l, likewise.
+__device__ __forceinline__ float decay(float s, float l) {
+  return fmaf(-s, l, opens(s) ? 0.f : l);
+}
+__device__ __forceinline__ float passed(float s, float l) {
+  return fmaf(s, l, opens(s) ? l : 0.f);
+}
+// f (1 - f)
+__device__ __forceinline__ float slope_of(float s) {
+  const float a = fabsf(s);
+  return fmaf(-a, a, a);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(SCAN_THREADS)
+// VC neighbouring channels of a frame.
+template <typename T, int VC> struct Frame { T t[VC]; };
+template <> struct __align__(4) Frame<__nv_bfloat16, 2> { __nv_bfloat16 t[2]; };
+template <> struct __align__(4) Frame<__half, 2> { __half t[2]; };
+
+template <typename T, int VC>
+__device__ __forceinline__ Frame<T, VC> load_frame(const T* p, bool in) {
+  Frame<T, VC> f;
+  if (in) {
+    f = *reinterpret_cast<const Frame<T, VC>*>(p);
+  } else {
+#pragma unroll
+    for (int v = 0; v < VC; ++v) f.t[v] = from_f<T>(0.f);
+  }
+  return f;
+}
+template <typename T, int VC>
+__device__ __forceinline__ void store_frame(T* p, const float (&v)[VC]) {
+  Frame<T, VC> f;
+#pragma unroll
+  for (int i = 0; i < VC; ++i) f.t[i] = from_f<T>(v[i]);
+  *reinterpret_cast<Frame<T, VC>*>(p) = f;
+}
+
+__device__ __forceinline__ float peer_read(const float* p, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int VC> struct ScanShared {
+  float a[2][SCAN_WARPS][32 * VC], b[2][SCAN_WARPS][32 * VC];  // of the warps' frames
+  float tile_a[2][32 * VC], tile_b[2][32 * VC];                // of the block's tile
+  float start[2][32 * VC];                                     // before the tile
+};
+
+// Composes the warps' (A, B) of step `it` and returns what enters this
+// thread's frames; REV: time runs from the last warp and the last block of
+// the cluster.  `run` is what enters the cluster's tiles, kept by warp 0.
+// One block barrier a step when S is 1 (the buffers alternate), else one of
+// the cluster and one more of the block.
+template <int VC, bool REV>
+__device__ __forceinline__ void compose(ScanShared<VC>& sh, int it, int S, int rank, int warp,
+                                        int lane, const float (&A)[VC], const float (&B)[VC],
+                                        float (&run)[VC], float (&enter)[VC]) {
+  const int p = it & 1;
+#pragma unroll
+  for (int v = 0; v < VC; ++v) {
+    sh.a[p][warp][lane * VC + v] = A[v];
+    sh.b[p][warp][lane * VC + v] = B[v];
+  }
+  __syncthreads();
+  if (S > 1) {
+    if (warp == 0) {
+#pragma unroll
+      for (int v = 0; v < VC; ++v) {
+        float ta = 1.f, tb = 0.f;
+#pragma unroll
+        for (int i = 0; i < SCAN_WARPS; ++i) {
+          const int w = REV ? SCAN_WARPS - 1 - i : i;
+          const float wa = sh.a[p][w][lane * VC + v];
+          tb = fmaf(wa, tb, sh.b[p][w][lane * VC + v]);
+          ta *= wa;
+        }
+        sh.tile_a[p][lane * VC + v] = ta;
+        sh.tile_b[p][lane * VC + v] = tb;
+      }
+    }
+    cluster_sync_all();
+    if (warp == 0) {
+#pragma unroll
+      for (int v = 0; v < VC; ++v) {
+        float h = run[v];
+        for (int i = 0; i < S; ++i) {
+          const int r = REV ? S - 1 - i : i;
+          if (r == rank) sh.start[p][lane * VC + v] = h;
+          h = fmaf(peer_read(&sh.tile_a[p][lane * VC + v], r), h,
+                   peer_read(&sh.tile_b[p][lane * VC + v], r));
+        }
+        run[v] = h;
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int v = 0; v < VC; ++v) {
+    float h = sh.start[p][lane * VC + v];
+#pragma unroll
+    for (int i = 0; i < SCAN_WARPS; ++i) {
+      const int w = REV ? SCAN_WARPS - 1 - i : i;
+      if (REV ? w > warp : w < warp)
+        h = fmaf(sh.a[p][w][lane * VC + v], h, sh.b[p][w][lane * VC + v]);
+    }
+    enter[v] = h;
+  }
+}
+
+template <typename T, int VC>
+__global__ void __launch_bounds__(SCAN_THREADS, VC == 1 ? 3 : 2)
     scan_fwd_kernel(const T* __restrict__ x, size_t xb, size_t xt, const T* __restrict__ g,
                     size_t gb, size_t gt, const float* __restrict__ h0,
-                    const int64_t* __restrict__ lengths, int B, int TT, int D, T* __restrict__ y,
-                    float* __restrict__ state, float* __restrict__ carry) {
-  const size_t id = (size_t)blockIdx.x * SCAN_THREADS + threadIdx.x;
-  if (id >= (size_t)B * D) return;
-  const int b = (int)(id / D), d = (int)(id - (size_t)b * D);
-  const int L = live_len(lengths, b, TT), nC = (TT + SCAN_CHUNK - 1) / SCAN_CHUNK;
-  float h = h0 ? h0[id] : 0.f;
-  for (int t = 0; t < L; ++t) {
-    if (carry && t % SCAN_CHUNK == 0) carry[((size_t)b * nC + t / SCAN_CHUNK) * D + d] = h;
-    float f, omf;
-    sigmoid_pair(to_f(g[b * gb + t * gt + d]), f, omf);
-    h = advance(f, omf, h, to_f(x[b * xb + t * xt + d]));
-    y[((size_t)b * TT + t) * D + d] = from_f<T>(h);
+                    const int64_t* __restrict__ lengths, size_t BD, int TT, int D, int S,
+                    T* __restrict__ y, float* __restrict__ state, float* __restrict__ carry) {
+  __shared__ ScanShared<VC> sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % S;
+  const size_t c = (size_t)(blockIdx.x / S) * (32 * VC) + lane * VC;
+  const bool live = c < BD;
+  const size_t b = live ? c / D : 0, d = live ? c - b * D : 0;
+  const int L = live ? live_len(lengths, (int)b, TT) : 0;
+  const T* xp = x + b * xb + d;
+  const T* gp = g + b * gb + d;
+  T* yp = y + b * (size_t)TT * D + d;
+  float run[VC];
+#pragma unroll
+  for (int v = 0; v < VC; ++v) {
+    run[v] = live && h0 ? h0[c + v] : 0.f;
+    if (warp == 0) sh.start[0][lane * VC + v] = run[v];
   }
-  for (int t = L; t < TT; ++t) y[((size_t)b * TT + t) * D + d] = from_f<T>(0.f);
-  state[id] = h;
+  const int steps = (TT + SCAN_TILE * S - 1) / (SCAN_TILE * S);
+  for (int it = 0; it < steps; ++it) {
+    const int t0 = (it * S + rank) * SCAN_TILE + warp * SCAN_FRAMES;
+    Frame<T, VC> xr[SCAN_FRAMES], gr[SCAN_FRAMES];
+#pragma unroll
+    for (int k = 0; k < SCAN_FRAMES; ++k) {
+      gr[k] = load_frame<T, VC>(gp + (size_t)(t0 + k) * gt, t0 + k < L);
+      xr[k] = load_frame<T, VC>(xp + (size_t)(t0 + k) * xt, t0 + k < L);
+    }
+    float s[SCAN_FRAMES][VC], A[VC], B[VC], h[VC];
+#pragma unroll
+    for (int v = 0; v < VC; ++v) {
+      A[v] = 1.f;
+      B[v] = 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < SCAN_FRAMES; ++k)
+#pragma unroll
+      for (int v = 0; v < VC; ++v) {
+        s[k][v] = t0 + k < L ? gate_of(to_f(gr[k].t[v])) : 0.f;
+        B[v] = advance(s[k][v], B[v], to_f(xr[k].t[v]));
+        A[v] = decay(s[k][v], A[v]);
+      }
+    compose<VC, false>(sh, it, S, rank, warp, lane, A, B, run, h);
+    if (carry && live && t0 < TT)
+#pragma unroll
+      for (int v = 0; v < VC; ++v) carry[(size_t)(t0 / SCAN_FRAMES) * BD + c + v] = h[v];
+#pragma unroll
+    for (int k = 0; k < SCAN_FRAMES; ++k) {
+      float o[VC];
+#pragma unroll
+      for (int v = 0; v < VC; ++v) {
+        h[v] = advance(s[k][v], h[v], to_f(xr[k].t[v]));
+        o[v] = t0 + k < L ? h[v] : 0.f;
+      }
+      if (live && t0 + k < TT) store_frame<T, VC>(yp + (size_t)(t0 + k) * D, o);
+    }
+    if (S == 1 && warp == SCAN_WARPS - 1)
+#pragma unroll
+      for (int v = 0; v < VC; ++v) sh.start[(it + 1) & 1][lane * VC + v] = h[v];
+  }
+  __syncthreads();
+  if (live && warp == 0 && rank == 0)
+#pragma unroll
+    for (int v = 0; v < VC; ++v)
+      state[c + v] = S > 1 ? run[v] : sh.start[steps & 1][lane * VC + v];
+  if (S > 1) cluster_sync_all();  // the others may still read this block's tile
 }
 
-template <typename T>
-__global__ void __launch_bounds__(SCAN_THREADS)
+template <typename T, int VC>
+__global__ void __launch_bounds__(SCAN_THREADS, 2)
     scan_bwd_kernel(const T* __restrict__ dy, size_t yb, size_t yt,
                     const float* __restrict__ dstate, const T* __restrict__ x, size_t xb,
                     size_t xt, const T* __restrict__ g, size_t gb, size_t gt,
-                    const int64_t* __restrict__ lengths, const float* __restrict__ carry, int B,
-                    int TT, int D, T* __restrict__ dx, T* __restrict__ dg,
+                    const int64_t* __restrict__ lengths, const float* __restrict__ carry,
+                    size_t BD, int TT, int D, int S, T* __restrict__ dx, T* __restrict__ dg,
                     float* __restrict__ dh0) {
-  const size_t id = (size_t)blockIdx.x * SCAN_THREADS + threadIdx.x;
-  if (id >= (size_t)B * D) return;
-  const int b = (int)(id / D), d = (int)(id - (size_t)b * D);
-  const int L = live_len(lengths, b, TT), nC = (TT + SCAN_CHUNK - 1) / SCAN_CHUNK;
-  for (int t = L; t < TT; ++t) {
-    dx[((size_t)b * TT + t) * D + d] = from_f<T>(0.f);
-    dg[((size_t)b * TT + t) * D + d] = from_f<T>(0.f);
+  __shared__ ScanShared<VC> sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % S;
+  const size_t c = (size_t)(blockIdx.x / S) * (32 * VC) + lane * VC;
+  const bool live = c < BD;
+  const size_t b = live ? c / D : 0, d = live ? c - b * D : 0;
+  const int L = live ? live_len(lengths, (int)b, TT) : 0;
+  const T* xp = x + b * xb + d;
+  const T* gp = g + b * gb + d;
+  const T* yp = dy + b * yb + d;
+  const size_t at = b * (size_t)TT * D + d;
+  float run[VC];  // f_{t+1} lam_{t+1} beyond the frames done
+#pragma unroll
+  for (int v = 0; v < VC; ++v) {
+    run[v] = live && dstate ? dstate[c + v] : 0.f;
+    if (warp == 0) sh.start[0][lane * VC + v] = run[v];
   }
-  float lam = dstate ? dstate[id] : 0.f;  // f_{t+1} lam_{t+1}
-  for (int c = (L + SCAN_CHUNK - 1) / SCAN_CHUNK - 1; c >= 0; --c) {
-    const int t0 = c * SCAN_CHUNK, n = min(SCAN_CHUNK, L - t0);
-    float hp[SCAN_CHUNK];
-    float h = carry[((size_t)b * nC + c) * D + d];
-    for (int k = 0; k < n; ++k) {
-      hp[k] = h;
-      float f, omf;
-      sigmoid_pair(to_f(g[b * gb + (t0 + k) * gt + d]), f, omf);
-      h = advance(f, omf, h, to_f(x[b * xb + (t0 + k) * xt + d]));
+  const int steps = (TT + SCAN_TILE * S - 1) / (SCAN_TILE * S);
+  for (int it = 0; it < steps; ++it) {
+    const int t0 = ((steps - 1 - it) * S + rank) * SCAN_TILE + warp * SCAN_FRAMES;
+    Frame<T, VC> xr[SCAN_FRAMES], gr[SCAN_FRAMES], yr[SCAN_FRAMES];
+    float h[VC], lam[VC];
+#pragma unroll
+    for (int k = 0; k < SCAN_FRAMES; ++k) {
+      gr[k] = load_frame<T, VC>(gp + (size_t)(t0 + k) * gt, t0 + k < L);
+      yr[k] = load_frame<T, VC>(yp + (size_t)(t0 + k) * yt, t0 + k < L);
+      xr[k] = load_frame<T, VC>(xp + (size_t)(t0 + k) * xt, t0 + k < L);
     }
-    for (int k = n - 1; k >= 0; --k) {
-      const int t = t0 + k;
-      float f, omf;
-      sigmoid_pair(to_f(g[b * gb + t * gt + d]), f, omf);
-      const float l = to_f(dy[b * yb + t * yt + d]) + lam;
-      dx[((size_t)b * TT + t) * D + d] = from_f<T>(omf * l);
-      dg[((size_t)b * TT + t) * D + d] =
-          from_f<T>(l * (hp[k] - to_f(x[b * xb + t * xt + d])) * (f * omf));
-      lam = decay(f, omf, l);
+#pragma unroll
+    for (int v = 0; v < VC; ++v)
+      h[v] = live && t0 < TT ? carry[(size_t)(t0 / SCAN_FRAMES) * BD + c + v] : 0.f;
+    float s[SCAN_FRAMES][VC], A[VC], B[VC];
+#pragma unroll
+    for (int v = 0; v < VC; ++v) {
+      A[v] = 1.f;
+      B[v] = 0.f;
     }
+#pragma unroll
+    for (int k = SCAN_FRAMES - 1; k >= 0; --k)
+#pragma unroll
+      for (int v = 0; v < VC; ++v) {
+        s[k][v] = t0 + k < L ? gate_of(to_f(gr[k].t[v])) : 0.f;
+        B[v] = decay(s[k][v], to_f(yr[k].t[v]) + B[v]);
+        A[v] = decay(s[k][v], A[v]);
+      }
+    compose<VC, true>(sh, it, S, rank, warp, lane, A, B, run, lam);
+    float diff[SCAN_FRAMES][VC];  // h_{t-1} - x_t
+#pragma unroll
+    for (int k = 0; k < SCAN_FRAMES; ++k)
+#pragma unroll
+      for (int v = 0; v < VC; ++v) {
+        const float xv = to_f(xr[k].t[v]);
+        diff[k][v] = h[v] - xv;
+        h[v] = advance(s[k][v], h[v], xv);
+      }
+#pragma unroll
+    for (int k = SCAN_FRAMES - 1; k >= 0; --k) {
+      float ox[VC], og[VC];
+#pragma unroll
+      for (int v = 0; v < VC; ++v) {
+        const float l = to_f(yr[k].t[v]) + lam[v];
+        lam[v] = decay(s[k][v], l);
+        ox[v] = t0 + k < L ? passed(s[k][v], l) : 0.f;
+        og[v] = t0 + k < L ? l * diff[k][v] * slope_of(s[k][v]) : 0.f;
+      }
+      if (live && t0 + k < TT) {
+        store_frame<T, VC>(dx + at + (size_t)(t0 + k) * D, ox);
+        store_frame<T, VC>(dg + at + (size_t)(t0 + k) * D, og);
+      }
+    }
+    if (S == 1 && warp == 0)
+#pragma unroll
+      for (int v = 0; v < VC; ++v) sh.start[(it + 1) & 1][lane * VC + v] = lam[v];
   }
-  if (dh0) dh0[id] = lam;
+  __syncthreads();
+  if (live && dh0 && warp == 0 && rank == 0)
+#pragma unroll
+    for (int v = 0; v < VC; ++v)
+      dh0[c + v] = S > 1 ? run[v] : sh.start[steps & 1][lane * VC + v];
+  if (S > 1) cluster_sync_all();
 }
 
 template <typename T>
@@ -107,9 +335,7 @@ __global__ void __launch_bounds__(SCAN_THREADS)
   const size_t id = (size_t)blockIdx.x * SCAN_THREADS + threadIdx.x;
   if (id >= (size_t)B * D) return;
   const size_t b = id / D, d = id - b * D;
-  float f, omf;
-  sigmoid_pair(to_f(g[b * gs + d]), f, omf);
-  const float h = advance(f, omf, state[id], to_f(x[b * xs + d]));
+  const float h = advance(gate_of(to_f(g[b * gs + d])), state[id], to_f(x[b * xs + d]));
   state[id] = h;
   y[id] = from_f<T>(h);
 }
@@ -118,8 +344,8 @@ int check(const char* who, int B, int TT, int D) {
   if (B < 0 || TT < 0 || D <= 0)
     return set_error(kInvalid, "%s: invalid sizes B=%d T=%d D=%d (need B, T >= 0, D > 0)", who, B,
                      TT, D);
-  if ((size_t)B * D / SCAN_THREADS >= 0x7fffffffu)
-    return set_error(kUnsupported, "%s: B * D too large", who);
+  if ((size_t)B * D / 32 >= 0x7fffffffu / 8 || TT > 0x7fffffff - 8 * SCAN_TILE)
+    return set_error(kUnsupported, "%s: sizes too large", who);
   return kOk;
 }
 
@@ -131,6 +357,36 @@ int launched(const char* who) {
 
 unsigned grid_of(int B, int D) {
   return (unsigned)(((size_t)B * D + SCAN_THREADS - 1) / SCAN_THREADS);
+}
+
+// Blocks that share the time of their channels: as many as three blocks a SM
+// leave room for, and no more than there are tiles.
+int time_blocks(size_t groups, int TT) {
+  int S = 8;
+  while (S > 1 && (groups * S > 148 * 3 || (long long)(S / 2) * SCAN_TILE >= TT)) S /= 2;
+  return S;
+}
+
+template <typename... Params, typename... Args>
+int launch(const char* who, void (*kernel)(Params...), size_t groups, int S, void* stream,
+           Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(groups * S));
+  cfg.blockDim = dim3(SCAN_THREADS);
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = S;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = S > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return set_error(kLaunch, "%s: %s", who, cudaGetErrorString(e));
+  return kOk;
+}
+
+bool pairs_ok(const void* p, size_t s1, size_t s2) {
+  return (uintptr_t)p % 4 == 0 && s1 % 2 == 0 && s2 % 2 == 0;
 }
 
 template <typename T>
@@ -145,10 +401,19 @@ int fwd(const void* x, size_t xb, size_t xt, const void* g, size_t gb, size_t gt
   if (carry && carry_bytes < tw_gated_scan_carry_bytes(B, TT, D))
     return set_error(kWorkspace, "tw_gated_scan_forward: carry needs %zu bytes",
                      tw_gated_scan_carry_bytes(B, TT, D));
-  scan_fwd_kernel<T><<<grid_of(B, D), SCAN_THREADS, 0, (cudaStream_t)stream>>>(
-      (const T*)x, xb, xt, (const T*)g, gb, gt, h0, lengths, B, TT, D, (T*)y, state,
-      (float*)carry);
-  return launched("tw_gated_scan_forward");
+  const char* who = "tw_gated_scan_forward";
+  const size_t BD = (size_t)B * D;
+  if constexpr (sizeof(T) == 2) if (D % 2 == 0 && pairs_ok(x, xb, xt) && pairs_ok(g, gb, gt) &&
+                                    pairs_ok(y, 0, 0)) {
+    const size_t groups = (BD + 63) / 64;
+    const int S = time_blocks(groups, TT);
+    return launch(who, scan_fwd_kernel<T, 2>, groups, S, stream, (const T*)x, xb, xt, (const T*)g,
+                  gb, gt, h0, lengths, BD, TT, D, S, (T*)y, state, (float*)carry);
+  }
+  const size_t groups = (BD + 31) / 32;
+  const int S = time_blocks(groups, TT);
+  return launch(who, scan_fwd_kernel<T, 1>, groups, S, stream, (const T*)x, xb, xt, (const T*)g,
+                gb, gt, h0, lengths, BD, TT, D, S, (T*)y, state, (float*)carry);
 }
 
 template <typename T>
@@ -163,10 +428,22 @@ int bwd(const void* dy, size_t yb, size_t yt, const float* dstate, const void* x
   if (carry_bytes < tw_gated_scan_carry_bytes(B, TT, D))
     return set_error(kWorkspace, "tw_gated_scan_backward: carry needs %zu bytes",
                      tw_gated_scan_carry_bytes(B, TT, D));
-  scan_bwd_kernel<T><<<grid_of(B, D), SCAN_THREADS, 0, (cudaStream_t)stream>>>(
-      (const T*)dy, yb, yt, dstate, (const T*)x, xb, xt, (const T*)g, gb, gt, lengths,
-      (const float*)carry, B, TT, D, (T*)dx, (T*)dg, dh0);
-  return launched("tw_gated_scan_backward");
+  const char* who = "tw_gated_scan_backward";
+  const size_t BD = (size_t)B * D;
+  if constexpr (sizeof(T) == 2) if (D % 2 == 0 && pairs_ok(x, xb, xt) && pairs_ok(g, gb, gt) &&
+                                    pairs_ok(dy, yb, yt) && pairs_ok(dx, 0, 0) &&
+                                    pairs_ok(dg, 0, 0)) {
+    const size_t groups = (BD + 63) / 64;
+    const int S = time_blocks(groups, TT);
+    return launch(who, scan_bwd_kernel<T, 2>, groups, S, stream, (const T*)dy, yb, yt, dstate,
+                  (const T*)x, xb, xt, (const T*)g, gb, gt, lengths, (const float*)carry, BD, TT,
+                  D, S, (T*)dx, (T*)dg, dh0);
+  }
+  const size_t groups = (BD + 31) / 32;
+  const int S = time_blocks(groups, TT);
+  return launch(who, scan_bwd_kernel<T, 1>, groups, S, stream, (const T*)dy, yb, yt, dstate,
+                (const T*)x, xb, xt, (const T*)g, gb, gt, lengths, (const float*)carry, BD, TT, D,
+                S, (T*)dx, (T*)dg, dh0);
 }
 
 template <typename T>
@@ -189,7 +466,7 @@ extern "C" {
 
 size_t tw_gated_scan_carry_bytes(int B, int T, int D) {
   if (B <= 0 || T <= 0 || D <= 0) return 0;
-  return (size_t)B * ((T + tw::SCAN_CHUNK - 1) / tw::SCAN_CHUNK) * D * sizeof(float);
+  return (size_t)B * D * ((T + tw::SCAN_FRAMES - 1) / tw::SCAN_FRAMES) * sizeof(float);
 }
 
 #define TW_GATED_SCAN(SUFFIX, E)                                                                 \

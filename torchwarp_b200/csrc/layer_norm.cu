@@ -25,16 +25,229 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < LN_THREADS / 32; ++i) s += red[i];
+  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) s += red[i];
   return s;
 }
 
-template <typename T, typename P>
+// Sum over the threads of a row: `tpr` lanes of a warp, or the block.
+template <bool BLOCK>
+__device__ __forceinline__ float row_sum(float v, int tpr, float* red) {
+  if constexpr (BLOCK) {
+    return block_sum(v, red);
+  } else {
+    for (int o = tpr >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
+}
+
+// Rows that fit the registers of `tpr` threads, E values each (VEC: in
+// 16-byte pieces, so that a row is read with whole-sector loads; else value
+// by value, neighbours in neighbouring lanes).  BLOCK: one row a block, else
+// 32 / tpr rows a warp.  x is read once; the two passes of the statistics run
+// on registers.  Bound by HBM.
+template <typename T, typename P, bool VEC, int E, bool BLOCK>
 __global__ void __launch_bounds__(LN_THREADS)
     ln_fwd_kernel(const T* __restrict__ x, size_t xs, const P* __restrict__ w,
-                  const P* __restrict__ b, size_t rows, int D, float eps, T* __restrict__ y,
-                  float* __restrict__ mean, float* __restrict__ rstd) {
+                  const P* __restrict__ b, size_t rows, int D, int tpr, float eps,
+                  T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
+  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, NV = E / V;
+  __shared__ float red[LN_THREADS / 32];
+  const int t = BLOCK ? threadIdx.x : threadIdx.x & (tpr - 1);
+  const size_t r = BLOCK ? blockIdx.x
+                         : (size_t)blockIdx.x * (LN_THREADS / tpr) + threadIdx.x / tpr;
+  const bool in = r < rows;
+  const T* xr = x + (in ? r : rows - 1) * xs;
+  float v[E];
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int d = (j * tpr + t) * V;
+    if (d < D) {
+      load_n<VEC, V>(xr + d, v + j * V);
+    } else {
+#pragma unroll
+      for (int q = 0; q < V; ++q) v[j * V + q] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) s += v[i];
+  const float mu = row_sum<BLOCK>(s, tpr, red) / D;
+  s = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if ((j * tpr + t) * V < D)
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        v[j * V + q] -= mu;
+        s = fmaf(v[j * V + q], v[j * V + q], s);
+      }
+  const float rs = 1.f / sqrtf(row_sum<BLOCK>(s, tpr, red) / D + eps);
+  if (!in) return;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int d = (j * tpr + t) * V;
+    if (d < D) {
+      float wv[V], bv[V];
+      if (w) load_n<VEC, V>(w + d, wv);
+      if (b) load_n<VEC, V>(b + d, bv);
+#pragma unroll
+      for (int q = 0; q < V; ++q)
+        wv[q] = __fmaf_rn(mul_rn(v[j * V + q], rs), w ? wv[q] : 1.f, b ? bv[q] : 0.f);
+      store_n<VEC, V>(y + r * D + d, wv);
+    }
+  }
+  if (mean && t == 0) {
+    mean[r] = mu;
+    rstd[r] = rs;
+  }
+}
+
+// dx, and this block's sums for dw and db: a thread keeps the same columns
+// for all its rows, so both sums stay in registers until the block's last
+// row.  x and dy are read once.  part: [gridDim.x][2][D] (NULL: only dx).
+template <typename T, typename P, bool VEC, int E, bool BLOCK>
+__global__ void __launch_bounds__(LN_THREADS)
+    ln_bwd_kernel(const T* __restrict__ dy, size_t dys, const T* __restrict__ x, size_t xs,
+                  const P* __restrict__ w, const float* __restrict__ mean,
+                  const float* __restrict__ rstd, size_t rows, int D, int tpr,
+                  T* __restrict__ dx, float* __restrict__ part) {
+  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, NV = E / V;
+  extern __shared__ float acc_s[];  // [2][D] of the block's warps, one after the other
+  __shared__ float red[LN_THREADS / 32];
+  const int t = BLOCK ? threadIdx.x : threadIdx.x & (tpr - 1);
+  const int per = BLOCK ? 1 : LN_THREADS / tpr;  // rows of a block's step
+  const float inv_d = 1.f / D;
+  float aw[E], ab[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) aw[i] = ab[i] = 0.f;
+  for (size_t r0 = (size_t)blockIdx.x * per; r0 < rows; r0 += (size_t)gridDim.x * per) {
+    const size_t r = r0 + (BLOCK ? 0 : threadIdx.x / tpr);
+    const bool in = r < rows;
+    const size_t rc = in ? r : rows - 1;
+    const float mu = mean[rc], rs = rstd[rc];
+    float g[E], h[E];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int d = (j * tpr + t) * V;
+      if (in && d < D) {
+        load_n<VEC, V>(dy + rc * dys + d, g + j * V);
+        load_n<VEC, V>(x + rc * xs + d, h + j * V);
+      } else {
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+          g[j * V + q] = 0.f;
+          h[j * V + q] = mu;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int d = (j * tpr + t) * V;
+      float wv[V];
+      if (w && d < D) load_n<VEC, V>(w + d, wv);
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        const int i = j * V + q;
+        h[i] = (h[i] - mu) * rs;
+        ab[i] += g[i];
+        aw[i] = fmaf(g[i], h[i], aw[i]);
+        if (w && d < D) g[i] *= wv[q];
+        s1 += g[i];
+        s2 = fmaf(g[i], h[i], s2);
+      }
+    }
+    if (dx) {
+      const float c1 = row_sum<BLOCK>(s1, tpr, red) * inv_d;
+      const float c2 = row_sum<BLOCK>(s2, tpr, red) * inv_d;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int d = (j * tpr + t) * V;
+        if (in && d < D) {
+#pragma unroll
+          for (int q = 0; q < V; ++q) {
+            const int i = j * V + q;
+            g[i] = rs * (g[i] - c1 - h[i] * c2);
+          }
+          store_n<VEC, V>(dx + r * D + d, g + j * V);
+        }
+      }
+    }
+  }
+  if (!part) return;
+  if (!BLOCK) {  // the rows of a warp's other lanes, then the warps in their order
+    for (int o = tpr; o < 32; o <<= 1)
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        aw[i] += __shfl_xor_sync(0xffffffffu, aw[i], o);
+        ab[i] += __shfl_xor_sync(0xffffffffu, ab[i], o);
+      }
+    const int warp = threadIdx.x >> 5;
+    for (int k = 0; k < LN_THREADS / 32; ++k) {
+      __syncthreads();
+      if (warp == k && (threadIdx.x & 31) < tpr) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int d = (j * tpr + t) * V;
+          if (d < D)
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+              const int i = j * V + q;
+              if (k == 0) {
+                acc_s[d + q] = aw[i];
+                acc_s[D + d + q] = ab[i];
+              } else {
+                acc_s[d + q] += aw[i];
+                acc_s[D + d + q] += ab[i];
+              }
+            }
+        }
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * D; i += LN_THREADS)
+      part[(size_t)blockIdx.x * 2 * D + i] = acc_s[i];
+  } else {
+    float* o = part + (size_t)blockIdx.x * 2 * D;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int d = (j * tpr + t) * V;
+      if (d < D) {
+        store_n<false, V>(o + d, aw + j * V);
+        store_n<false, V>(o + D + d, ab + j * V);
+      }
+    }
+  }
+}
+
+// dw and db from the blocks' sums, in a fixed order: 32 columns a block.
+template <typename P>
+__global__ void __launch_bounds__(LN_THREADS)
+    ln_join_kernel(const float* __restrict__ part, int blocks, int D, P* __restrict__ dw,
+                   P* __restrict__ db) {
+  __shared__ float red[LN_THREADS / 32][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 32 + tx;
+  float s = 0.f;
+  if (c < 2 * D)
+#pragma unroll 8
+    for (int k = ty; k < blocks; k += LN_THREADS / 32) s += part[(size_t)k * 2 * D + c];
+  red[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && c < 2 * D) {
+#pragma unroll
+    for (int i = 1; i < LN_THREADS / 32; ++i) s += red[i][tx];
+    if (c < D && dw) dw[c] = from_f<P>(s);
+    if (c >= D && db) db[c - D] = from_f<P>(s);
+  }
+}
+
+// ---- rows longer than a block's registers: read again from the caches
+
+template <typename T, typename P>
+__global__ void __launch_bounds__(LN_THREADS)
+    ln_fwd_long_kernel(const T* __restrict__ x, size_t xs, const P* __restrict__ w,
+                       const P* __restrict__ b, size_t rows, int D, float eps, T* __restrict__ y,
+                       float* __restrict__ mean, float* __restrict__ rstd) {
   __shared__ float red[LN_THREADS / 32];
   for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* xr = x + r * xs;
@@ -48,8 +261,8 @@ __global__ void __launch_bounds__(LN_THREADS)
     }
     const float rs = 1.f / sqrtf(block_sum(s, red) / D + eps);
     for (int d = threadIdx.x; d < D; d += LN_THREADS) {
-      const float xh = (to_f(xr[d]) - mu) * rs;
-      y[r * D + d] = from_f<T>(fmaf(xh, w ? to_f(w[d]) : 1.f, b ? to_f(b[d]) : 0.f));
+      const float xh = mul_rn(to_f(xr[d]) - mu, rs);
+      y[r * D + d] = from_f<T>(__fmaf_rn(xh, w ? to_f(w[d]) : 1.f, b ? to_f(b[d]) : 0.f));
     }
     if (mean && threadIdx.x == 0) {
       mean[r] = mu;
@@ -60,9 +273,9 @@ __global__ void __launch_bounds__(LN_THREADS)
 
 template <typename T, typename P>
 __global__ void __launch_bounds__(LN_THREADS)
-    ln_dx_kernel(const T* __restrict__ dy, size_t dys, const T* __restrict__ x, size_t xs,
-                 const P* __restrict__ w, const float* __restrict__ mean,
-                 const float* __restrict__ rstd, size_t rows, int D, T* __restrict__ dx) {
+    ln_dx_long_kernel(const T* __restrict__ dy, size_t dys, const T* __restrict__ x, size_t xs,
+                      const P* __restrict__ w, const float* __restrict__ mean,
+                      const float* __restrict__ rstd, size_t rows, int D, T* __restrict__ dx) {
   __shared__ float red[LN_THREADS / 32];
   for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const float mu = mean[r], rs = rstd[r];
@@ -84,9 +297,9 @@ __global__ void __launch_bounds__(LN_THREADS)
 // One block: 32 columns, all rows, in a fixed order.
 template <typename T, typename P>
 __global__ void __launch_bounds__(LN_THREADS)
-    ln_dw_kernel(const T* __restrict__ dy, size_t dys, const T* __restrict__ x, size_t xs,
-                 const float* __restrict__ mean, const float* __restrict__ rstd, size_t rows,
-                 int D, P* __restrict__ dw, P* __restrict__ db) {
+    ln_dw_long_kernel(const T* __restrict__ dy, size_t dys, const T* __restrict__ x, size_t xs,
+                      const float* __restrict__ mean, const float* __restrict__ rstd, size_t rows,
+                      int D, P* __restrict__ dw, P* __restrict__ db) {
   __shared__ float sw[8][33], sb[8][33];
   const int c = threadIdx.x & 31, g = threadIdx.x >> 5, d = blockIdx.x * 32 + c;
   float aw = 0.f, ab = 0.f;
@@ -109,6 +322,35 @@ __global__ void __launch_bounds__(LN_THREADS)
   }
 }
 
+// How a row of D values is spread: E values a thread (the fewest of 8, 16, 32
+// that let a warp hold the row), `tpr` threads; a longer row over a block.
+// Read value by value (not vec) a thread takes at most 16, as its bounds
+// checks are one a value and 32 of them spill.  tpr 0: too long for a block.
+struct RowPlan {
+  int e, tpr, per;  // per: rows of a block
+};
+
+RowPlan row_plan(int D, bool vec) {
+  const int most = vec ? 32 : 16;
+  RowPlan p = {most, 0, 1};
+  if (D > most * LN_THREADS) return p;
+  if (D <= 32 * most) {
+    p.e = D <= 256 ? 8 : D <= 512 ? 16 : 32;
+    p.tpr = 1;
+    while (p.tpr * p.e < D) p.tpr *= 2;
+    p.per = LN_THREADS / p.tpr;
+  } else {
+    p.tpr = (D + 32 * most - 1) / (32 * most) * 32;
+  }
+  return p;
+}
+
+// Blocks of the backward: two a SM, fewer when there are fewer rows.
+int bwd_blocks(size_t rows, const RowPlan& p) {
+  const size_t steps = (rows + p.per - 1) / p.per, most = 148 * 2 * (p.tpr > 32 ? 2 : 1);
+  return (int)(steps < most ? steps : most);
+}
+
 int check(const char* who, size_t rows, int D, size_t xs) {
   if (D <= 0) return set_error(kInvalid, "%s: invalid D=%d (need D > 0)", who, D);
   if (rows > (size_t)1 << 40) return set_error(kInvalid, "%s: too many rows", who);
@@ -125,11 +367,34 @@ int launched(const char* who) {
 
 int grid_of(size_t rows) { return (int)(rows < 148 * 8 ? rows : 148 * 8); }
 
+bool aligned16(const void* p, size_t stride_bytes) {
+  return (uintptr_t)p % 16 == 0 && stride_bytes % 16 == 0;
+}
+
+// The instance of a row kernel for a plan.
+#define TW_ROW_KERNEL(KERNEL)                                                          \
+  (!vec ? (plan.tpr > 32 ? KERNEL<T, P, false, 16, true>                               \
+           : plan.e == 8 ? KERNEL<T, P, false, 8, false> : KERNEL<T, P, false, 16, false>) \
+   : plan.tpr > 32 ? KERNEL<T, P, true, 32, true>                                      \
+   : plan.e == 8 ? KERNEL<T, P, true, 8, false>                                        \
+   : plan.e == 16 ? KERNEL<T, P, true, 16, false> : KERNEL<T, P, true, 32, false>)
+
 template <typename T, typename P>
 int fwd_p(const void* x, size_t xs, const void* w, const void* b, size_t rows, int D, float eps,
           void* y, float* mean, float* rstd, cudaStream_t st) {
-  ln_fwd_kernel<T, P><<<grid_of(rows), LN_THREADS, 0, st>>>(
-      (const T*)x, xs, (const P*)w, (const P*)b, rows, D, eps, (T*)y, mean, rstd);
+  const bool vec = D * sizeof(T) % 16 == 0 && aligned16(x, xs * sizeof(T)) && aligned16(y, 0) &&
+                   aligned16(w, 0) && aligned16(b, 0);
+  const RowPlan plan = row_plan(D, vec);
+  if (plan.tpr == 0) {
+    ln_fwd_long_kernel<T, P><<<grid_of(rows), LN_THREADS, 0, st>>>(
+        (const T*)x, xs, (const P*)w, (const P*)b, rows, D, eps, (T*)y, mean, rstd);
+    return launched("tw_layer_norm_forward");
+  }
+  const size_t blocks = (rows + plan.per - 1) / plan.per;
+  if (blocks > 0x7fffffff) return set_error(kUnsupported, "tw_layer_norm_forward: too many rows");
+  auto kernel = TW_ROW_KERNEL(ln_fwd_kernel);
+  kernel<<<(unsigned)blocks, plan.tpr > 32 ? plan.tpr : LN_THREADS, 0, st>>>(
+      (const T*)x, xs, (const P*)w, (const P*)b, rows, D, plan.tpr, eps, (T*)y, mean, rstd);
   return launched("tw_layer_norm_forward");
 }
 
@@ -149,14 +414,31 @@ int fwd(const void* x, size_t xs, const void* w, const void* b, int pf32, size_t
 
 template <typename T, typename P>
 int bwd_p(const void* dy, size_t dys, const void* x, size_t xs, const void* w, const float* mean,
-          const float* rstd, size_t rows, int D, void* dx, void* dw, void* db, cudaStream_t st) {
-  if (dx && rows)
-    ln_dx_kernel<T, P><<<grid_of(rows), LN_THREADS, 0, st>>>((const T*)dy, dys, (const T*)x, xs,
-                                                             (const P*)w, mean, rstd, rows, D,
-                                                             (T*)dx);
+          const float* rstd, size_t rows, int D, void* dx, void* dw, void* db, void* ws,
+          cudaStream_t st) {
+  const bool vec = D * sizeof(T) % 16 == 0 && aligned16(x, xs * sizeof(T)) &&
+                   aligned16(dy, dys * sizeof(T)) && aligned16(w, 0) && aligned16(dx, 0);
+  const RowPlan plan = row_plan(D, vec);
+  if (plan.tpr == 0) {
+    if (dx && rows)
+      ln_dx_long_kernel<T, P><<<grid_of(rows), LN_THREADS, 0, st>>>(
+          (const T*)dy, dys, (const T*)x, xs, (const P*)w, mean, rstd, rows, D, (T*)dx);
+    if (dw || db)
+      ln_dw_long_kernel<T, P><<<(D + 31) / 32, LN_THREADS, 0, st>>>(
+          (const T*)dy, dys, (const T*)x, xs, mean, rstd, rows, D, (P*)dw, (P*)db);
+    return launched("tw_layer_norm_backward");
+  }
+  const int blocks = bwd_blocks(rows, plan);
+  float* part = dw || db ? (float*)ws : nullptr;
+  if (blocks) {
+    auto kernel = TW_ROW_KERNEL(ln_bwd_kernel);
+    const size_t smem = part && plan.tpr <= 32 ? 2 * (size_t)D * sizeof(float) : 0;
+    kernel<<<blocks, plan.tpr > 32 ? plan.tpr : LN_THREADS, smem, st>>>(
+        (const T*)dy, dys, (const T*)x, xs, (const P*)w, mean, rstd, rows, D, plan.tpr, (T*)dx,
+        part);
+  }
   if (dw || db)
-    ln_dw_kernel<T, P><<<(D + 31) / 32, LN_THREADS, 0, st>>>(
-        (const T*)dy, dys, (const T*)x, xs, mean, rstd, rows, D, (P*)dw, (P*)db);
+    ln_join_kernel<P><<<(2 * D + 31) / 32, LN_THREADS, 0, st>>>(part, blocks, D, (P*)dw, (P*)db);
   return launched("tw_layer_norm_backward");
 }
 
@@ -173,8 +455,8 @@ int bwd(const void* dy, size_t dys, const void* x, size_t xs, const void* w, int
     return set_error(kWorkspace, "tw_layer_norm_backward: workspace needs %zu bytes",
                      tw_layer_norm_workspace_bytes(rows, D));
   cudaStream_t st = (cudaStream_t)stream;
-  return pf32 ? bwd_p<T, float>(dy, dys, x, xs, w, mean, rstd, rows, D, dx, dw, db, st)
-              : bwd_p<T, T>(dy, dys, x, xs, w, mean, rstd, rows, D, dx, dw, db, st);
+  return pf32 ? bwd_p<T, float>(dy, dys, x, xs, w, mean, rstd, rows, D, dx, dw, db, ws, st)
+              : bwd_p<T, T>(dy, dys, x, xs, w, mean, rstd, rows, D, dx, dw, db, ws, st);
 }
 
 }  // namespace
@@ -183,9 +465,14 @@ int bwd(const void* dy, size_t dys, const void* x, size_t xs, const void* w, int
 extern "C" {
 
 size_t tw_layer_norm_workspace_bytes(size_t rows, int D) {
-  (void)rows;
-  (void)D;
-  return 0;
+  if (D <= 0) return 0;
+  int blocks = 0;  // of either way to read a row
+  for (int vec = 0; vec < 2; ++vec) {
+    const tw::RowPlan p = tw::row_plan(D, vec != 0);
+    const int b = p.tpr ? tw::bwd_blocks(rows, p) : 0;
+    if (b > blocks) blocks = b;
+  }
+  return (size_t)blocks * 2 * D * sizeof(float);
 }
 
 #define TW_LAYER_NORM(SUFFIX, T)                                                                \
