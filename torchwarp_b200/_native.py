@@ -175,15 +175,19 @@ def require_cuda(*tensors):
 
 
 _SUFFIX16 = {torch.float32: "f32", torch.bfloat16: "bf16", torch.float16: "f16"}
+_ENTRIES = {}
 
 
 def entry(name, dtype):
     """The C entry of an encoder operator for an element type."""
-    suffix = _SUFFIX16.get(dtype)
-    if suffix is None:
-        raise TypeError("the encoder operators take float32, bfloat16 or float16, got {}".format(
-            dtype))
-    return getattr(lib(), name + "_" + suffix)
+    fn = _ENTRIES.get((name, dtype))
+    if fn is None:
+        suffix = _SUFFIX16.get(dtype)
+        if suffix is None:
+            raise TypeError("the encoder operators take float32, bfloat16 or float16, got "
+                            "{}".format(dtype))
+        fn = _ENTRIES[name, dtype] = getattr(lib(), name + "_" + suffix)
+    return fn
 
 
 def launch(name, fn, device, *args):
@@ -191,11 +195,11 @@ def launch(name, fn, device, *args):
     status.  Pointers are plain integers (``data_ptr()``): this is the path of calls whose time is
     the host's."""
     index = device.index
-    if index == torch.cuda.current_device():
-        status = call(name, fn, *args, torch.cuda.current_stream(index).cuda_stream)
-    else:
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
-            status = call(name, fn, *args, torch.cuda.current_stream(index).cuda_stream)
+            return launch(name, fn, device, *args)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    status = fn(*args, stream) if _RECORDER is None else call(name, fn, *args, stream)
     if status != 0:
         check(status, "tw_" + name)
 

@@ -79,10 +79,42 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-__device__ __forceinline__ float decode(uint8_t c) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+// Eight neighbours.  Plain loads: the kernel writes these arrays too.
+template <typename T>
+__device__ __forceinline__ void read8(const T* p, float* v) {
+  constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+  for (int i = 0; i < 8 / PER; ++i)
+    unpack16<T>(reinterpret_cast<const uint4*>(p)[i], v + i * PER);
 }
 
+// Eight neighbouring e4m3 codes as floats, and back.
+__device__ __forceinline__ void decode8(uint2 c, float scale, float* v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_fp8x2_storage_t two = (__nv_fp8x2_storage_t)((i < 2 ? c.x : c.y) >> (16 * (i & 1)));
+    const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+    v[2 * i] = f.x * scale;
+    v[2 * i + 1] = f.y * scale;
+  }
+}
+__device__ __forceinline__ uint2 encode8(const float* v) {
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * i], v[4 * i + 1]), __NV_SATFINITE,
+                                              __NV_E4M3) |
+           (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2], v[4 * i + 3]),
+                                              __NV_SATFINITE, __NV_E4M3)
+               << 16;
+  return make_uint2(w[0], w[1]);
+}
+
+// A warp takes a unit of 256 values a turn, 8 neighbours a lane.  Bound by HBM
+// (28 bytes a float32 weight with 32-bit states, 16 with 8-bit ones): every
+// array is read with 16-byte loads, all issued before the first is used.  A
+// unit whose parameter or gradient is not 16-byte aligned, and a tensor's
+// last, partial unit, go value by value.
 template <typename T, bool BITS8>
 __global__ void __launch_bounds__(AD_THREADS)
     adamw_kernel(const __grid_constant__ AdamTable tab, AdamState s, AdamScalars a) {
@@ -93,7 +125,7 @@ __global__ void __launch_bounds__(AD_THREADS)
     const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
     sc[0] = (float)(1.0 - lr * a.wd);
     sc[1] = (float)(lr / (1.0 - pow(a.b1, (double)t)));
-    sc[2] = (float)sqrt(1.0 - pow(a.b2, (double)t));
+    sc[2] = (float)(1.0 / sqrt(1.0 - pow(a.b2, (double)t)));
     skey = a.seed * 0x9E3779B1u + (uint32_t)t * 0x85EBCA77u;
     __threadfence();
     if (a.last && atomicAdd(&a.step[1], 1) == (int)gridDim.x - 1) {
@@ -108,65 +140,82 @@ __global__ void __launch_bounds__(AD_THREADS)
   const uint32_t key = skey;
   const int lane = threadIdx.x & 31;
   const unsigned units = tab.first[tab.count];
+  int lo = 0;
   for (unsigned u = blockIdx.x * (AD_THREADS / 32) + (threadIdx.x >> 5); u < units;
        u += gridDim.x * (AD_THREADS / 32)) {
-    int lo = 0, hi = tab.count - 1;  // the tensor of this unit
+    int hi = tab.count - 1;  // the tensor of this unit: not before the last one's
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (tab.first[mid] <= u) lo = mid; else hi = mid - 1;
     }
     const unsigned long long at = (unsigned long long)(u - tab.first[lo]) * AD_UNIT;
     const unsigned long long so = tab.e[lo].offset + at;
-    const int n = (int)min((unsigned long long)AD_UNIT, tab.e[lo].n - at);
-    T* p = (T*)tab.e[lo].p + at;
-    const T* g = (const T*)tab.e[lo].g + at;
-    float m[8], r[8], mmax = 0.f, rmax = 0.f;
-    const float ms = BITS8 ? s.ms[so / AD_UNIT] : 0.f, rs = BITS8 ? s.rs[so / AD_UNIT] : 0.f;
+    const int n = (int)min((unsigned long long)AD_UNIT, tab.e[lo].n - at) - 8 * lane;  // lane's
+    T* p = (T*)tab.e[lo].p + at + 8 * lane;
+    const T* g = (const T*)tab.e[lo].g + at + 8 * lane;
+    const unsigned long long sl = so + 8 * lane;
+    const bool vec = n >= 8 && (((uintptr_t)p | (uintptr_t)g) & 15) == 0;
+    float m[8], r[8], pv[8], gv[8];
+    // the states' buffers are padded to whole units
+    if (BITS8) {
+      const uint2 mc = *reinterpret_cast<const uint2*>(s.m8 + sl);
+      const uint2 rc = *reinterpret_cast<const uint2*>(s.r8 + sl);
+      const float ms = s.ms[so / AD_UNIT], rs = s.rs[so / AD_UNIT];
+      decode8(mc, ms, m);
+      decode8(rc, rs, r);
+    } else {
+      read8(s.m32 + sl, m);
+      read8(s.v32 + sl, r);
+    }
+    if (vec) {
+      load_n<true, 8>(g, gv);
+      read8(p, pv);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int i = k * 32 + lane;
-      m[k] = r[k] = 0.f;
-      if (i < n) {
-        const float gv = to_f(g[i]);
-        float v;
-        if (BITS8) {
-          m[k] = decode(s.m8[so + i]) * ms;
-          v = decode(s.r8[so + i]) * rs;
-          v *= v;
-        } else {
-          m[k] = s.m32[so + i];
-          v = s.v32[so + i];
-        }
-        m[k] = fmaf(b1, m[k], c1 * gv);
-        v = fmaf(b2, v, c2 * (gv * gv));
-        r[k] = sqrtf(v);
-        const float pv = to_f(p[i]) * keep - alpha * (m[k] / (r[k] / root2 + eps));
-        p[i] = from_f<T>(pv);
-        if (!BITS8) {
-          s.m32[so + i] = m[k];
-          s.v32[so + i] = v;
-        }
-        mmax = fmaxf(mmax, fabsf(m[k]));
-        rmax = fmaxf(rmax, r[k]);
+      for (int i = 0; i < 8; ++i) {
+        gv[i] = i < n ? to_f(g[i]) : 0.f;
+        pv[i] = i < n ? to_f(p[i]) : 0.f;
       }
     }
-    if (BITS8) {
-      const float nms = warp_max(mmax) / 448.f, nrs = warp_max(rmax) / 448.f;
+    float mmax = 0.f, rmax = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int i = k * 32 + lane;
-        if (i < n) {
-          const uint32_t h = lowbias32((uint32_t)(so + i) ^ key);
-          const float ym = nms > 0.f ? fabsf(m[k]) / nms : fabsf(m[k]);
-          const float yr = nrs > 0.f ? r[k] / nrs : r[k];
-          const float qm = round_e4m3(ym, (float)(h & 0xFFFFu) * (1.f / 65536.f));
-          float qr = round_e4m3(yr, (float)(h >> 16) * (1.f / 65536.f));
-          // a second moment that is not zero stays above zero: it divides m
-          if (yr > 0.f) qr = fmaxf(qr, 0.001953125f);
-          s.m8[so + i] = __nv_cvt_float_to_fp8(copysignf(qm, m[k]), __NV_SATFINITE, __NV_E4M3);
-          s.r8[so + i] = __nv_cvt_float_to_fp8(qr, __NV_SATFINITE, __NV_E4M3);
-        }
+    for (int i = 0; i < 8; ++i) {
+      const float v = fmaf(b2, BITS8 ? r[i] * r[i] : r[i], c2 * (gv[i] * gv[i]));
+      m[i] = fmaf(b1, m[i], c1 * gv[i]);
+      r[i] = sqrtf(v);
+      pv[i] = pv[i] * keep - alpha * __fdividef(m[i], fmaf(r[i], root2, eps));
+      if (!BITS8) r[i] = v;
+      mmax = fmaxf(mmax, fabsf(m[i]));
+      rmax = fmaxf(rmax, r[i]);
+    }
+    if (vec) {
+      store_n<true, 8>(p, pv);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) p[i] = from_f<T>(pv[i]);
+    }
+    if (!BITS8) {
+      store_n<true, 8>(s.m32 + sl, m);
+      store_n<true, 8>(s.v32 + sl, r);
+    } else {
+      // a block below 1e-37, whose scale has no reciprocal, is zero
+      float nms = warp_max(mmax) / 448.f, nrs = warp_max(rmax) / 448.f;
+      if (nms < 1e-37f) nms = 0.f;
+      if (nrs < 1e-37f) nrs = 0.f;
+      const float ims = nms > 0.f ? 1.f / nms : 0.f, irs = nrs > 0.f ? 1.f / nrs : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t h = lowbias32((uint32_t)(sl + i) ^ key);
+        const float yr = r[i] * irs;
+        m[i] = copysignf(round_e4m3(fabsf(m[i]) * ims, (float)(h & 0xFFFFu) * (1.f / 65536.f)),
+                         m[i]);
+        r[i] = round_e4m3(yr, (float)(h >> 16) * (1.f / 65536.f));
+        // a second moment that is not zero stays above zero: it divides m
+        if (yr > 0.f) r[i] = fmaxf(r[i], 0.001953125f);
       }
+      *reinterpret_cast<uint2*>(s.m8 + sl) = encode8(m);
+      *reinterpret_cast<uint2*>(s.r8 + sl) = encode8(r);
       if (lane == 0) {
         s.ms[so / AD_UNIT] = nms;
         s.rs[so / AD_UNIT] = nrs;

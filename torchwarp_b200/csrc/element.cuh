@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace tw {
@@ -23,6 +25,55 @@ template <> __device__ __forceinline__ __half from_f<__half>(float v) {
   return __float2half_rn(v);
 }
 
+// Two 16-bit elements of a word as floats, and back: one conversion a pair.
+template <typename T> struct Pair;
+template <> struct Pair<__nv_bfloat16> {
+  static __device__ __forceinline__ void unpack(uint32_t u, float& a, float& b) {
+    a = __uint_as_float(u << 16);
+    b = __uint_as_float(u & 0xFFFF0000u);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+};
+template <> struct Pair<__half> {
+  static __device__ __forceinline__ void unpack(uint32_t u, float& a, float& b) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+    a = f.x;
+    b = f.y;
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+};
+
+// The 16 / sizeof(T) elements of 16 bytes as floats, and back.
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4& u, float* v) {
+  if constexpr (sizeof(T) == 4) {
+    v[0] = __uint_as_float(u.x);
+    v[1] = __uint_as_float(u.y);
+    v[2] = __uint_as_float(u.z);
+    v[3] = __uint_as_float(u.w);
+  } else {
+    Pair<T>::unpack(u.x, v[0], v[1]);
+    Pair<T>::unpack(u.y, v[2], v[3]);
+    Pair<T>::unpack(u.z, v[4], v[5]);
+    Pair<T>::unpack(u.w, v[6], v[7]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float* v) {
+  if constexpr (sizeof(T) == 4)
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                      __float_as_uint(v[3]));
+  else
+    return make_uint4(Pair<T>::pack(v[0], v[1]), Pair<T>::pack(v[2], v[3]),
+                      Pair<T>::pack(v[4], v[5]), Pair<T>::pack(v[6], v[7]));
+}
+
 // N consecutive elements as floats, and back; with VEC in pieces of 16 bytes
 // (the address is 16-byte aligned), else one by one.
 template <bool VEC, int N, typename T>
@@ -30,12 +81,8 @@ __device__ __forceinline__ void load_n(const T* p, float* v) {
   constexpr int PER = 16 / sizeof(T);
   if constexpr (VEC && N % PER == 0) {
 #pragma unroll
-    for (int i = 0; i < N / PER; ++i) {
-      union { uint4 u; T t[PER]; } q;
-      q.u = __ldg(reinterpret_cast<const uint4*>(p) + i);
-#pragma unroll
-      for (int k = 0; k < PER; ++k) v[i * PER + k] = to_f(q.t[k]);
-    }
+    for (int i = 0; i < N / PER; ++i)
+      unpack16<T>(__ldg(reinterpret_cast<const uint4*>(p) + i), v + i * PER);
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = to_f(p[i]);
@@ -46,17 +93,48 @@ __device__ __forceinline__ void store_n(T* p, const float* v) {
   constexpr int PER = 16 / sizeof(T);
   if constexpr (VEC && N % PER == 0) {
 #pragma unroll
-    for (int i = 0; i < N / PER; ++i) {
-      union { uint4 u; T t[PER]; } q;
-#pragma unroll
-      for (int k = 0; k < PER; ++k) q.t[k] = from_f<T>(v[i * PER + k]);
-      reinterpret_cast<uint4*>(p)[i] = q.u;
-    }
+    for (int i = 0; i < N / PER; ++i)
+      reinterpret_cast<uint4*>(p)[i] = pack16<T>(v + i * PER);
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) p[i] = from_f<T>(v[i]);
   }
 }
+
+// What load_n reads, kept as it is until it is used: half the registers of
+// 16-bit elements as floats.
+template <bool VEC, int N, typename T> struct Raw {
+  static constexpr int PER = 16 / sizeof(T);
+  static constexpr int WORDS = VEC ? N / PER : N;
+  typename std::conditional<VEC, uint4, T>::type w[WORDS];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) w[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void zero() {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) w[i] = make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) w[i] = from_f<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ void get(float* v) const {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) unpack16<T>(w[i], v + i * PER);
+    } else {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) v[i] = to_f(w[i]);
+    }
+  }
+};
 
 // f = sigmoid(z) and 1 - f: the smaller of the two from exp(-|z|), which
 // neither overflows nor cancels, to a few ulp of itself; the larger is one

@@ -39,53 +39,138 @@ __device__ __forceinline__ int live_len(const int64_t* lengths, int b, int T) {
   return n < 0 ? 0 : n > T ? T : (int)n;
 }
 
+// V floats that go through the arithmetic together: pairs use the packed
+// instructions (two results each), which halve the issue slots of what a
+// frame costs beside its loads and two special functions.
+template <int V> struct Vec { float v[V]; };
+
+template <int V>
+__device__ __forceinline__ Vec<V> splat(float x) {
+  Vec<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = x;
+  return r;
+}
+__device__ __forceinline__ uint64_t two(const Vec<2>& a) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.v[0]), "f"(a.v[1]));
+  return r;
+}
+__device__ __forceinline__ Vec<2> of_two(uint64_t a) {
+  Vec<2> r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.v[0]), "=f"(r.v[1]) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ Vec<1> fma_v(Vec<1> a, Vec<1> b, Vec<1> c) {
+  return {{fmaf(a.v[0], b.v[0], c.v[0])}};
+}
+__device__ __forceinline__ Vec<2> fma_v(Vec<2> a, Vec<2> b, Vec<2> c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(two(a)), "l"(two(b)), "l"(two(c)));
+  return of_two(r);
+}
+__device__ __forceinline__ Vec<1> add_v(Vec<1> a, Vec<1> b) { return {{a.v[0] + b.v[0]}}; }
+__device__ __forceinline__ Vec<2> add_v(Vec<2> a, Vec<2> b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(two(a)), "l"(two(b)));
+  return of_two(r);
+}
+__device__ __forceinline__ Vec<1> mul_v(Vec<1> a, Vec<1> b) { return {{a.v[0] * b.v[0]}}; }
+__device__ __forceinline__ Vec<2> mul_v(Vec<2> a, Vec<2> b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(two(a)), "l"(two(b)));
+  return of_two(r);
+}
+template <int V>
+__device__ __forceinline__ Vec<V> sub_v(Vec<V> a, Vec<V> b) {  // a - b
+  return fma_v(b, splat<V>(-1.f), a);
+}
+
 // A gate as one number: the smaller of 1 - f and f, which keeps its relative
 // precision, negative when it is f.  +0 keeps the state.
-__device__ __forceinline__ float gate_of(float z) {
-  const float e = ex2(-1.4426950408889634f * fabsf(z));
-  return copysignf(e * rcp(1.f + e), z);
+template <int V>
+__device__ __forceinline__ Vec<V> gate_of(Vec<V> z) {
+  const Vec<V> t = mul_v(z, splat<V>(1.4426950408889634f));
+  Vec<V> e, r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) e.v[i] = ex2(-fabsf(t.v[i]));
+  r = add_v(e, splat<V>(1.f));
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = rcp(r.v[i]);
+  r = mul_v(e, r);
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = copysignf(r.v[i], z.v[i]);
+  return r;
 }
-__device__ __forceinline__ bool opens(float s) { return __float_as_int(s) < 0; }
+// b where the gate is f (opens), else a.
+template <int V>
+__device__ __forceinline__ Vec<V> pick(Vec<V> s, Vec<V> a, Vec<V> b) {
+  Vec<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = __float_as_int(s.v[i]) < 0 ? b.v[i] : a.v[i];
+  return r;
+}
 // f h + (1 - f) x as a step from the nearer of the two, so that the rounding
 // of a gate near 1 does not decay a state that should last.
-__device__ __forceinline__ float advance(float s, float h, float x) {
-  return fmaf(s, x - h, opens(s) ? x : h);
+template <int V>
+__device__ __forceinline__ Vec<V> advance(Vec<V> s, Vec<V> h, Vec<V> x) {
+  return fma_v(s, sub_v(x, h), pick(s, h, x));
 }
-// f l and (1 - f) l, likewise.
-__device__ __forceinline__ float decay(float s, float l) {
-  return fmaf(-s, l, opens(s) ? 0.f : l);
+// f l and (1 - f) l, likewise: together they are l.
+template <int V>
+__device__ __forceinline__ Vec<V> decay(Vec<V> ns, Vec<V> s, Vec<V> l) {
+  return fma_v(ns, l, pick(s, l, splat<V>(0.f)));
 }
-__device__ __forceinline__ float passed(float s, float l) {
-  return fmaf(s, l, opens(s) ? l : 0.f);
+template <int V>
+__device__ __forceinline__ Vec<V> passed(Vec<V> s, Vec<V> l) {
+  return fma_v(s, l, pick(s, splat<V>(0.f), l));
 }
-// f (1 - f)
-__device__ __forceinline__ float slope_of(float s) {
-  const float a = fabsf(s);
-  return fmaf(-a, a, a);
+template <int V>
+__device__ __forceinline__ Vec<V> negated(Vec<V> s) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) s.v[i] = -s.v[i];
+  return s;
+}
+// f (1 - f) = |s| (1 - |s|)
+template <int V>
+__device__ __forceinline__ Vec<V> slope_of(Vec<V> s) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) s.v[i] = fabsf(s.v[i]);
+  return fma_v(negated(s), s, s);
 }
 
-// VC neighbouring channels of a frame.
-template <typename T, int VC> struct Frame { T t[VC]; };
-template <> struct __align__(4) Frame<__nv_bfloat16, 2> { __nv_bfloat16 t[2]; };
-template <> struct __align__(4) Frame<__half, 2> { __half t[2]; };
+// VC neighbouring channels of a frame, as they lie in memory.
+template <typename T, int VC> struct Frame {
+  T t;
+  __device__ __forceinline__ Vec<1> get() const { return {{to_f(t)}}; }
+  static __device__ __forceinline__ Frame zero() { return {from_f<T>(0.f)}; }
+  static __device__ __forceinline__ Frame of(Vec<1> v) { return {from_f<T>(v.v[0])}; }
+};
+template <typename T> struct Frame<T, 2> {
+  uint32_t u;
+  __device__ __forceinline__ Vec<2> get() const {
+    Vec<2> r;
+    Pair<T>::unpack(u, r.v[0], r.v[1]);
+    return r;
+  }
+  static __device__ __forceinline__ Frame zero() { return {0u}; }
+  static __device__ __forceinline__ Frame of(Vec<2> v) { return {Pair<T>::pack(v.v[0], v.v[1])}; }
+};
 
+// A thread's frames t0.. of an array whose frames are `step` bytes apart;
+// frames from `n` on are zero and not read.
 template <typename T, int VC>
-__device__ __forceinline__ Frame<T, VC> load_frame(const T* p, bool in) {
-  Frame<T, VC> f;
-  if (in) {
-    f = *reinterpret_cast<const Frame<T, VC>*>(p);
+__device__ __forceinline__ void load_frames(Frame<T, VC> (&f)[SCAN_FRAMES], const char* p,
+                                            size_t step, int n) {
+  if (n >= SCAN_FRAMES) {
+#pragma unroll
+    for (int k = 0; k < SCAN_FRAMES; ++k, p += step)
+      f[k] = *reinterpret_cast<const Frame<T, VC>*>(p);
   } else {
 #pragma unroll
-    for (int v = 0; v < VC; ++v) f.t[v] = from_f<T>(0.f);
+    for (int k = 0; k < SCAN_FRAMES; ++k, p += step)
+      f[k] = k < n ? *reinterpret_cast<const Frame<T, VC>*>(p) : Frame<T, VC>::zero();
   }
-  return f;
-}
-template <typename T, int VC>
-__device__ __forceinline__ void store_frame(T* p, const float (&v)[VC]) {
-  Frame<T, VC> f;
-#pragma unroll
-  for (int i = 0; i < VC; ++i) f.t[i] = from_f<T>(v[i]);
-  *reinterpret_cast<Frame<T, VC>*>(p) = f;
 }
 
 __device__ __forceinline__ float peer_read(const float* p, uint32_t rank) {
@@ -113,13 +198,13 @@ template <int VC> struct ScanShared {
 // the cluster and one more of the block.
 template <int VC, bool REV>
 __device__ __forceinline__ void compose(ScanShared<VC>& sh, int it, int S, int rank, int warp,
-                                        int lane, const float (&A)[VC], const float (&B)[VC],
-                                        float (&run)[VC], float (&enter)[VC]) {
+                                        int lane, Vec<VC> A, Vec<VC> B, Vec<VC>& run,
+                                        Vec<VC>& enter) {
   const int p = it & 1;
 #pragma unroll
   for (int v = 0; v < VC; ++v) {
-    sh.a[p][warp][lane * VC + v] = A[v];
-    sh.b[p][warp][lane * VC + v] = B[v];
+    sh.a[p][warp][lane * VC + v] = A.v[v];
+    sh.b[p][warp][lane * VC + v] = B.v[v];
   }
   __syncthreads();
   if (S > 1) {
@@ -142,14 +227,14 @@ __device__ __forceinline__ void compose(ScanShared<VC>& sh, int it, int S, int r
     if (warp == 0) {
 #pragma unroll
       for (int v = 0; v < VC; ++v) {
-        float h = run[v];
+        float h = run.v[v];
         for (int i = 0; i < S; ++i) {
           const int r = REV ? S - 1 - i : i;
           if (r == rank) sh.start[p][lane * VC + v] = h;
           h = fmaf(peer_read(&sh.tile_a[p][lane * VC + v], r), h,
                    peer_read(&sh.tile_b[p][lane * VC + v], r));
         }
-        run[v] = h;
+        run.v[v] = h;
       }
     }
     __syncthreads();
@@ -163,12 +248,27 @@ __device__ __forceinline__ void compose(ScanShared<VC>& sh, int it, int S, int r
       if (REV ? w > warp : w < warp)
         h = fmaf(sh.a[p][w][lane * VC + v], h, sh.b[p][w][lane * VC + v]);
     }
-    enter[v] = h;
+    enter.v[v] = h;
   }
 }
 
+// What a block works on: its channels' sequence, feature and length.
+struct Channel {
+  size_t c, b, d;
+  bool live;
+  int L;
+  __device__ __forceinline__ Channel(size_t first, int lane, int vc, size_t BD, int D, int TT,
+                                     const int64_t* lengths) {
+    c = first + lane * vc;
+    live = c < BD;
+    b = live ? c / D : 0;
+    d = live ? c - b * D : 0;
+    L = live ? live_len(lengths, (int)b, TT) : 0;
+  }
+};
+
 template <typename T, int VC>
-__global__ void __launch_bounds__(SCAN_THREADS, VC == 1 ? 3 : 2)
+__global__ void __launch_bounds__(SCAN_THREADS, 2)
     scan_fwd_kernel(const T* __restrict__ x, size_t xb, size_t xt, const T* __restrict__ g,
                     size_t gb, size_t gt, const float* __restrict__ h0,
                     const int64_t* __restrict__ lengths, size_t BD, int TT, int D, int S,
@@ -176,68 +276,79 @@ __global__ void __launch_bounds__(SCAN_THREADS, VC == 1 ? 3 : 2)
   __shared__ ScanShared<VC> sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x % S;
-  const size_t c = (size_t)(blockIdx.x / S) * (32 * VC) + lane * VC;
-  const bool live = c < BD;
-  const size_t b = live ? c / D : 0, d = live ? c - b * D : 0;
-  const int L = live ? live_len(lengths, (int)b, TT) : 0;
-  const T* xp = x + b * xb + d;
-  const T* gp = g + b * gb + d;
-  T* yp = y + b * (size_t)TT * D + d;
-  float run[VC];
+  const Channel ch((size_t)(blockIdx.x / S) * (32 * VC), lane, VC, BD, D, TT, lengths);
+  const char* xp = reinterpret_cast<const char*>(x + ch.b * xb + ch.d);
+  const char* gp = reinterpret_cast<const char*>(g + ch.b * gb + ch.d);
+  char* yp = reinterpret_cast<char*>(y + ch.b * (size_t)TT * D + ch.d);
+  const size_t xs = xt * sizeof(T), gs = gt * sizeof(T), ys = D * sizeof(T);
+  Vec<VC> run;
 #pragma unroll
   for (int v = 0; v < VC; ++v) {
-    run[v] = live && h0 ? h0[c + v] : 0.f;
-    if (warp == 0) sh.start[0][lane * VC + v] = run[v];
+    run.v[v] = ch.live && h0 ? h0[ch.c + v] : 0.f;
+    if (warp == 0) sh.start[0][lane * VC + v] = run.v[v];
   }
   const int steps = (TT + SCAN_TILE * S - 1) / (SCAN_TILE * S);
-  for (int it = 0; it < steps; ++it) {
-    const int t0 = (it * S + rank) * SCAN_TILE + warp * SCAN_FRAMES;
-    Frame<T, VC> xr[SCAN_FRAMES], gr[SCAN_FRAMES];
+  int t0 = rank * SCAN_TILE + warp * SCAN_FRAMES;
+  Frame<T, VC> xr[SCAN_FRAMES], gr[SCAN_FRAMES];
+  load_frames<T, VC>(gr, gp + (size_t)t0 * gs, gs, ch.L - t0);
+  load_frames<T, VC>(xr, xp + (size_t)t0 * xs, xs, ch.L - t0);
+  for (int it = 0; it < steps; ++it, t0 += SCAN_TILE * S) {
+    const int n = ch.L - t0;
+    Vec<VC> s[SCAN_FRAMES], xv[SCAN_FRAMES];
 #pragma unroll
     for (int k = 0; k < SCAN_FRAMES; ++k) {
-      gr[k] = load_frame<T, VC>(gp + (size_t)(t0 + k) * gt, t0 + k < L);
-      xr[k] = load_frame<T, VC>(xp + (size_t)(t0 + k) * xt, t0 + k < L);
+      s[k] = gate_of(gr[k].get());
+      xv[k] = xr[k].get();
     }
-    float s[SCAN_FRAMES][VC], A[VC], B[VC], h[VC];
+    if (n < SCAN_FRAMES)
 #pragma unroll
-    for (int v = 0; v < VC; ++v) {
-      A[v] = 1.f;
-      B[v] = 0.f;
+      for (int k = 0; k < SCAN_FRAMES; ++k)
+        if (k >= n) s[k] = splat<VC>(0.f);
+    // the next tile's loads are under way while the blocks wait for each other
+    const int t1 = t0 + SCAN_TILE * S;
+    load_frames<T, VC>(gr, gp + (size_t)t1 * gs, gs, ch.L - t1);
+    load_frames<T, VC>(xr, xp + (size_t)t1 * xs, xs, ch.L - t1);
+    Vec<VC> A = splat<VC>(1.f), B = splat<VC>(0.f), h;
+#pragma unroll
+    for (int k = 0; k < SCAN_FRAMES; ++k) {
+      B = advance(s[k], B, xv[k]);
+      A = decay(negated(s[k]), s[k], A);
     }
-#pragma unroll
-    for (int k = 0; k < SCAN_FRAMES; ++k)
-#pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        s[k][v] = t0 + k < L ? gate_of(to_f(gr[k].t[v])) : 0.f;
-        B[v] = advance(s[k][v], B[v], to_f(xr[k].t[v]));
-        A[v] = decay(s[k][v], A[v]);
-      }
     compose<VC, false>(sh, it, S, rank, warp, lane, A, B, run, h);
-    if (carry && live && t0 < TT)
+    if (carry && ch.live && t0 < TT)
 #pragma unroll
-      for (int v = 0; v < VC; ++v) carry[(size_t)(t0 / SCAN_FRAMES) * BD + c + v] = h[v];
+      for (int v = 0; v < VC; ++v)
+        carry[(size_t)(t0 / SCAN_FRAMES) * BD + ch.c + v] = h.v[v];
+    char* o = yp + (size_t)t0 * ys;
+    if (n >= SCAN_FRAMES) {
 #pragma unroll
-    for (int k = 0; k < SCAN_FRAMES; ++k) {
-      float o[VC];
-#pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        h[v] = advance(s[k][v], h[v], to_f(xr[k].t[v]));
-        o[v] = t0 + k < L ? h[v] : 0.f;
+      for (int k = 0; k < SCAN_FRAMES; ++k, o += ys) {
+        h = advance(s[k], h, xv[k]);
+        *reinterpret_cast<Frame<T, VC>*>(o) = Frame<T, VC>::of(h);
       }
-      if (live && t0 + k < TT) store_frame<T, VC>(yp + (size_t)(t0 + k) * D, o);
+    } else {
+#pragma unroll
+      for (int k = 0; k < SCAN_FRAMES; ++k, o += ys) {
+        h = advance(s[k], h, xv[k]);
+        if (ch.live && t0 + k < TT)
+          *reinterpret_cast<Frame<T, VC>*>(o) = k < n ? Frame<T, VC>::of(h) : Frame<T, VC>::zero();
+      }
     }
     if (S == 1 && warp == SCAN_WARPS - 1)
 #pragma unroll
-      for (int v = 0; v < VC; ++v) sh.start[(it + 1) & 1][lane * VC + v] = h[v];
+      for (int v = 0; v < VC; ++v) sh.start[(it + 1) & 1][lane * VC + v] = h.v[v];
   }
   __syncthreads();
-  if (live && warp == 0 && rank == 0)
+  if (ch.live && warp == 0 && rank == 0)
 #pragma unroll
     for (int v = 0; v < VC; ++v)
-      state[c + v] = S > 1 ? run[v] : sh.start[steps & 1][lane * VC + v];
+      state[ch.c + v] = S > 1 ? run.v[v] : sh.start[steps & 1][lane * VC + v];
   if (S > 1) cluster_sync_all();  // the others may still read this block's tile
 }
 
+// The same walk from the end.  Pairs of 16 bits load a tile when its turn
+// comes (its registers leave no room for the next one's); single channels
+// load a tile ahead.
 template <typename T, int VC>
 __global__ void __launch_bounds__(SCAN_THREADS, 2)
     scan_bwd_kernel(const T* __restrict__ dy, size_t yb, size_t yt,
@@ -246,85 +357,92 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2)
                     const int64_t* __restrict__ lengths, const float* __restrict__ carry,
                     size_t BD, int TT, int D, int S, T* __restrict__ dx, T* __restrict__ dg,
                     float* __restrict__ dh0) {
+  constexpr bool AHEAD = VC == 1;
   __shared__ ScanShared<VC> sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x % S;
-  const size_t c = (size_t)(blockIdx.x / S) * (32 * VC) + lane * VC;
-  const bool live = c < BD;
-  const size_t b = live ? c / D : 0, d = live ? c - b * D : 0;
-  const int L = live ? live_len(lengths, (int)b, TT) : 0;
-  const T* xp = x + b * xb + d;
-  const T* gp = g + b * gb + d;
-  const T* yp = dy + b * yb + d;
-  const size_t at = b * (size_t)TT * D + d;
-  float run[VC];  // f_{t+1} lam_{t+1} beyond the frames done
+  const Channel ch((size_t)(blockIdx.x / S) * (32 * VC), lane, VC, BD, D, TT, lengths);
+  const char* xp = reinterpret_cast<const char*>(x + ch.b * xb + ch.d);
+  const char* gp = reinterpret_cast<const char*>(g + ch.b * gb + ch.d);
+  const char* yp = reinterpret_cast<const char*>(dy + ch.b * yb + ch.d);
+  const size_t at = ch.b * (size_t)TT * D + ch.d;
+  const size_t xs = xt * sizeof(T), gs = gt * sizeof(T), ys = yt * sizeof(T);
+  const ptrdiff_t os = (ptrdiff_t)(D * sizeof(T));
+  Vec<VC> run;  // f_{t+1} lam_{t+1} beyond the frames done
 #pragma unroll
   for (int v = 0; v < VC; ++v) {
-    run[v] = live && dstate ? dstate[c + v] : 0.f;
-    if (warp == 0) sh.start[0][lane * VC + v] = run[v];
+    run.v[v] = ch.live && dstate ? dstate[ch.c + v] : 0.f;
+    if (warp == 0) sh.start[0][lane * VC + v] = run.v[v];
   }
   const int steps = (TT + SCAN_TILE * S - 1) / (SCAN_TILE * S);
-  for (int it = 0; it < steps; ++it) {
-    const int t0 = ((steps - 1 - it) * S + rank) * SCAN_TILE + warp * SCAN_FRAMES;
-    Frame<T, VC> xr[SCAN_FRAMES], gr[SCAN_FRAMES], yr[SCAN_FRAMES];
-    float h[VC], lam[VC];
-#pragma unroll
-    for (int k = 0; k < SCAN_FRAMES; ++k) {
-      gr[k] = load_frame<T, VC>(gp + (size_t)(t0 + k) * gt, t0 + k < L);
-      yr[k] = load_frame<T, VC>(yp + (size_t)(t0 + k) * yt, t0 + k < L);
-      xr[k] = load_frame<T, VC>(xp + (size_t)(t0 + k) * xt, t0 + k < L);
-    }
+  int t0 = ((steps - 1) * S + rank) * SCAN_TILE + warp * SCAN_FRAMES;
+  Frame<T, VC> xr[SCAN_FRAMES], gr[SCAN_FRAMES], yr[SCAN_FRAMES];
+  Vec<VC> hr;
+  auto load = [&](int t) {
+    const int n = t >= 0 ? ch.L - t : 0;
+    const size_t tt = t >= 0 ? t : 0;
+    load_frames<T, VC>(gr, gp + tt * gs, gs, n);
+    load_frames<T, VC>(yr, yp + tt * ys, ys, n);
+    load_frames<T, VC>(xr, xp + tt * xs, xs, n);
 #pragma unroll
     for (int v = 0; v < VC; ++v)
-      h[v] = live && t0 < TT ? carry[(size_t)(t0 / SCAN_FRAMES) * BD + c + v] : 0.f;
-    float s[SCAN_FRAMES][VC], A[VC], B[VC];
+      hr.v[v] = n > 0 ? carry[(tt / SCAN_FRAMES) * BD + ch.c + v] : 0.f;
+  };
+  if (AHEAD) load(t0);
+  for (int it = 0; it < steps; ++it, t0 -= SCAN_TILE * S) {
+    const int n = ch.L - t0;
+    if (!AHEAD) load(t0);
+    Vec<VC> s[SCAN_FRAMES], diff[SCAN_FRAMES];  // the gates; h_{t-1} - x_t
+    Vec<VC> yv[AHEAD ? SCAN_FRAMES : 1], h = hr, lam;
 #pragma unroll
-    for (int v = 0; v < VC; ++v) {
-      A[v] = 1.f;
-      B[v] = 0.f;
+    for (int k = 0; k < SCAN_FRAMES; ++k) {
+      s[k] = gate_of(gr[k].get());
+      if (AHEAD) yv[k] = yr[k].get();
     }
+    if (n < SCAN_FRAMES)
 #pragma unroll
-    for (int k = SCAN_FRAMES - 1; k >= 0; --k)
+      for (int k = 0; k < SCAN_FRAMES; ++k)
+        if (k >= n) s[k] = splat<VC>(0.f);
 #pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        s[k][v] = t0 + k < L ? gate_of(to_f(gr[k].t[v])) : 0.f;
-        B[v] = decay(s[k][v], to_f(yr[k].t[v]) + B[v]);
-        A[v] = decay(s[k][v], A[v]);
-      }
-    compose<VC, true>(sh, it, S, rank, warp, lane, A, B, run, lam);
-    float diff[SCAN_FRAMES][VC];  // h_{t-1} - x_t
-#pragma unroll
-    for (int k = 0; k < SCAN_FRAMES; ++k)
-#pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        const float xv = to_f(xr[k].t[v]);
-        diff[k][v] = h[v] - xv;
-        h[v] = advance(s[k][v], h[v], xv);
-      }
+    for (int k = 0; k < SCAN_FRAMES; ++k) {
+      diff[k] = sub_v(h, xr[k].get());
+      h = fma_v(negated(s[k]), diff[k], pick(s[k], h, xr[k].get()));
+    }
+    if (AHEAD) load(t0 - SCAN_TILE * S);
+    Vec<VC> A = splat<VC>(1.f), B = splat<VC>(0.f);
 #pragma unroll
     for (int k = SCAN_FRAMES - 1; k >= 0; --k) {
-      float ox[VC], og[VC];
+      const Vec<VC> ns = negated(s[k]);
+      B = decay(ns, s[k], add_v(AHEAD ? yv[k] : yr[k].get(), B));
+      A = decay(ns, s[k], A);
+    }
+    compose<VC, true>(sh, it, S, rank, warp, lane, A, B, run, lam);
+    const size_t last = (at + (size_t)(t0 + SCAN_FRAMES - 1) * D) * sizeof(T);
+    char* ox = reinterpret_cast<char*>(dx) + last;
+    char* og = reinterpret_cast<char*>(dg) + last;
 #pragma unroll
-      for (int v = 0; v < VC; ++v) {
-        const float l = to_f(yr[k].t[v]) + lam[v];
-        lam[v] = decay(s[k][v], l);
-        ox[v] = t0 + k < L ? passed(s[k][v], l) : 0.f;
-        og[v] = t0 + k < L ? l * diff[k][v] * slope_of(s[k][v]) : 0.f;
-      }
-      if (live && t0 + k < TT) {
-        store_frame<T, VC>(dx + at + (size_t)(t0 + k) * D, ox);
-        store_frame<T, VC>(dg + at + (size_t)(t0 + k) * D, og);
+    for (int k = SCAN_FRAMES - 1; k >= 0; --k, ox -= os, og -= os) {
+      const Vec<VC> l = add_v(AHEAD ? yv[k] : yr[k].get(), lam);
+      lam = decay(negated(s[k]), s[k], l);
+      const Frame<T, VC> vx = Frame<T, VC>::of(passed(s[k], l));
+      const Frame<T, VC> vg = Frame<T, VC>::of(mul_v(mul_v(l, diff[k]), slope_of(s[k])));
+      if (n >= SCAN_FRAMES) {
+        *reinterpret_cast<Frame<T, VC>*>(ox) = vx;
+        *reinterpret_cast<Frame<T, VC>*>(og) = vg;
+      } else if (ch.live && t0 + k < TT) {
+        *reinterpret_cast<Frame<T, VC>*>(ox) = k < n ? vx : Frame<T, VC>::zero();
+        *reinterpret_cast<Frame<T, VC>*>(og) = k < n ? vg : Frame<T, VC>::zero();
       }
     }
     if (S == 1 && warp == 0)
 #pragma unroll
-      for (int v = 0; v < VC; ++v) sh.start[(it + 1) & 1][lane * VC + v] = lam[v];
+      for (int v = 0; v < VC; ++v) sh.start[(it + 1) & 1][lane * VC + v] = lam.v[v];
   }
   __syncthreads();
-  if (live && dh0 && warp == 0 && rank == 0)
+  if (ch.live && dh0 && warp == 0 && rank == 0)
 #pragma unroll
     for (int v = 0; v < VC; ++v)
-      dh0[c + v] = S > 1 ? run[v] : sh.start[steps & 1][lane * VC + v];
+      dh0[ch.c + v] = S > 1 ? run.v[v] : sh.start[steps & 1][lane * VC + v];
   if (S > 1) cluster_sync_all();
 }
 
@@ -335,7 +453,8 @@ __global__ void __launch_bounds__(SCAN_THREADS)
   const size_t id = (size_t)blockIdx.x * SCAN_THREADS + threadIdx.x;
   if (id >= (size_t)B * D) return;
   const size_t b = id / D, d = id - b * D;
-  const float h = advance(gate_of(to_f(g[b * gs + d])), state[id], to_f(x[b * xs + d]));
+  const Vec<1> s = gate_of(Vec<1>{{to_f(g[b * gs + d])}});
+  const float h = advance(s, Vec<1>{{state[id]}}, Vec<1>{{to_f(x[b * xs + d])}}).v[0];
   state[id] = h;
   y[id] = from_f<T>(h);
 }

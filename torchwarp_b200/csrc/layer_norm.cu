@@ -16,6 +16,7 @@ namespace tw {
 namespace {
 
 constexpr int LN_THREADS = 256;
+constexpr int BWD_THREADS = 128;  // of a backward block whose warps hold whole rows
 
 // Sum over the block; every thread gets it.
 __device__ __forceinline__ float block_sum(float v, float* red) {
@@ -87,13 +88,20 @@ __global__ void __launch_bounds__(LN_THREADS)
   for (int j = 0; j < NV; ++j) {
     const int d = (j * tpr + t) * V;
     if (d < D) {
-      float wv[V], bv[V];
-      if (w) load_n<VEC, V>(w + d, wv);
-      if (b) load_n<VEC, V>(b + d, bv);
+      float o[V], p[V];
 #pragma unroll
-      for (int q = 0; q < V; ++q)
-        wv[q] = __fmaf_rn(mul_rn(v[j * V + q], rs), w ? wv[q] : 1.f, b ? bv[q] : 0.f);
-      store_n<VEC, V>(y + r * D + d, wv);
+      for (int q = 0; q < V; ++q) o[q] = mul_rn(v[j * V + q], rs);
+      if (w) {
+        load_n<VEC, V>(w + d, p);
+#pragma unroll
+        for (int q = 0; q < V; ++q) o[q] = mul_rn(o[q], p[q]);
+      }
+      if (b) {
+        load_n<VEC, V>(b + d, p);
+#pragma unroll
+        for (int q = 0; q < V; ++q) o[q] = add_rn(o[q], p[q]);
+      }
+      store_n<VEC, V>(y + r * D + d, o);
     }
   }
   if (mean && t == 0) {
@@ -104,9 +112,12 @@ __global__ void __launch_bounds__(LN_THREADS)
 
 // dx, and this block's sums for dw and db: a thread keeps the same columns
 // for all its rows, so both sums stay in registers until the block's last
-// row.  x and dy are read once.  part: [gridDim.x][2][D] (NULL: only dx).
+// row.  x and dy are read once and kept as they lie (half the registers).
+// With 32 values a thread that is about 150 registers: blocks of 4 warps, three
+// a SM, hold 12 warps where blocks of 8 held one of 178 registers each (146 us
+// for 32768 x 1024 bfloat16).  part: [gridDim.x][2][D] (NULL: only dx).
 template <typename T, typename P, bool VEC, int E, bool BLOCK>
-__global__ void __launch_bounds__(LN_THREADS)
+__global__ void __launch_bounds__(BLOCK ? LN_THREADS : BWD_THREADS, BLOCK ? 1 : 3)
     ln_bwd_kernel(const T* __restrict__ dy, size_t dys, const T* __restrict__ x, size_t xs,
                   const P* __restrict__ w, const float* __restrict__ mean,
                   const float* __restrict__ rstd, size_t rows, int D, int tpr,
@@ -115,7 +126,7 @@ __global__ void __launch_bounds__(LN_THREADS)
   extern __shared__ float acc_s[];  // [2][D] of the block's warps, one after the other
   __shared__ float red[LN_THREADS / 32];
   const int t = BLOCK ? threadIdx.x : threadIdx.x & (tpr - 1);
-  const int per = BLOCK ? 1 : LN_THREADS / tpr;  // rows of a block's step
+  const int per = BLOCK ? 1 : BWD_THREADS / tpr;  // rows of a block's step
   const float inv_d = 1.f / D;
   float aw[E], ab[E];
 #pragma unroll
@@ -125,36 +136,41 @@ __global__ void __launch_bounds__(LN_THREADS)
     const bool in = r < rows;
     const size_t rc = in ? r : rows - 1;
     const float mu = mean[rc], rs = rstd[rc];
-    float g[E], h[E];
+    Raw<VEC, V, T> gr[NV], hr[NV];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int d = (j * tpr + t) * V;
       if (in && d < D) {
-        load_n<VEC, V>(dy + rc * dys + d, g + j * V);
-        load_n<VEC, V>(x + rc * xs + d, h + j * V);
+        gr[j].load(dy + rc * dys + d);
+        hr[j].load(x + rc * xs + d);
       } else {
-#pragma unroll
-        for (int q = 0; q < V; ++q) {
-          g[j * V + q] = 0.f;
-          h[j * V + q] = mu;
-        }
+        gr[j].zero();
+        hr[j].zero();
       }
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int d = (j * tpr + t) * V;
-      float wv[V];
-      if (w && d < D) load_n<VEC, V>(w + d, wv);
+      float g[V], h[V];
+      gr[j].get(g);
+      hr[j].get(h);
 #pragma unroll
       for (int q = 0; q < V; ++q) {
-        const int i = j * V + q;
-        h[i] = (h[i] - mu) * rs;
-        ab[i] += g[i];
-        aw[i] = fmaf(g[i], h[i], aw[i]);
-        if (w && d < D) g[i] *= wv[q];
-        s1 += g[i];
-        s2 = fmaf(g[i], h[i], s2);
+        h[q] = (h[q] - mu) * rs;
+        ab[j * V + q] += g[q];
+        aw[j * V + q] = fmaf(g[q], h[q], aw[j * V + q]);
+      }
+      if (w && d < D) {
+        float wv[V];
+        load_n<VEC, V>(w + d, wv);
+#pragma unroll
+        for (int q = 0; q < V; ++q) g[q] *= wv[q];
+      }
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        s1 += g[q];
+        s2 = fmaf(g[q], h[q], s2);
       }
     }
     if (dx) {
@@ -164,12 +180,18 @@ __global__ void __launch_bounds__(LN_THREADS)
       for (int j = 0; j < NV; ++j) {
         const int d = (j * tpr + t) * V;
         if (in && d < D) {
+          float g[V], h[V];
+          gr[j].get(g);
+          hr[j].get(h);
+          if (w) {
+            float wv[V];
+            load_n<VEC, V>(w + d, wv);
 #pragma unroll
-          for (int q = 0; q < V; ++q) {
-            const int i = j * V + q;
-            g[i] = rs * (g[i] - c1 - h[i] * c2);
+            for (int q = 0; q < V; ++q) g[q] *= wv[q];
           }
-          store_n<VEC, V>(dx + r * D + d, g + j * V);
+#pragma unroll
+          for (int q = 0; q < V; ++q) g[q] = rs * (g[q] - c1 - (h[q] - mu) * rs * c2);
+          store_n<VEC, V>(dx + r * D + d, g);
         }
       }
     }
@@ -183,7 +205,7 @@ __global__ void __launch_bounds__(LN_THREADS)
         ab[i] += __shfl_xor_sync(0xffffffffu, ab[i], o);
       }
     const int warp = threadIdx.x >> 5;
-    for (int k = 0; k < LN_THREADS / 32; ++k) {
+    for (int k = 0; k < BWD_THREADS / 32; ++k) {
       __syncthreads();
       if (warp == k && (threadIdx.x & 31) < tpr) {
 #pragma unroll
@@ -205,7 +227,7 @@ __global__ void __launch_bounds__(LN_THREADS)
       }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * D; i += LN_THREADS)
+    for (int i = threadIdx.x; i < 2 * D; i += BWD_THREADS)
       part[(size_t)blockIdx.x * 2 * D + i] = acc_s[i];
   } else {
     float* o = part + (size_t)blockIdx.x * 2 * D;
@@ -262,7 +284,7 @@ __global__ void __launch_bounds__(LN_THREADS)
     const float rs = 1.f / sqrtf(block_sum(s, red) / D + eps);
     for (int d = threadIdx.x; d < D; d += LN_THREADS) {
       const float xh = mul_rn(to_f(xr[d]) - mu, rs);
-      y[r * D + d] = from_f<T>(__fmaf_rn(xh, w ? to_f(w[d]) : 1.f, b ? to_f(b[d]) : 0.f));
+      y[r * D + d] = from_f<T>(add_rn(mul_rn(xh, w ? to_f(w[d]) : 1.f), b ? to_f(b[d]) : 0.f));
     }
     if (mean && threadIdx.x == 0) {
       mean[r] = mu;
@@ -345,9 +367,11 @@ RowPlan row_plan(int D, bool vec) {
   return p;
 }
 
-// Blocks of the backward: two a SM, fewer when there are fewer rows.
+// Blocks of the backward: what a SM holds, fewer when there are fewer rows.
+int bwd_per(const RowPlan& p) { return p.tpr > 32 ? 1 : BWD_THREADS / p.tpr; }
 int bwd_blocks(size_t rows, const RowPlan& p) {
-  const size_t steps = (rows + p.per - 1) / p.per, most = 148 * 2 * (p.tpr > 32 ? 2 : 1);
+  const int per_sm = p.tpr > 32 ? 1024 / p.tpr / 2 : p.e == 8 ? 8 : p.e == 16 ? 5 : 3;
+  const size_t steps = (rows + bwd_per(p) - 1) / bwd_per(p), most = 148 * (per_sm < 1 ? 1 : per_sm);
   return (int)(steps < most ? steps : most);
 }
 
@@ -433,7 +457,7 @@ int bwd_p(const void* dy, size_t dys, const void* x, size_t xs, const void* w, c
   if (blocks) {
     auto kernel = TW_ROW_KERNEL(ln_bwd_kernel);
     const size_t smem = part && plan.tpr <= 32 ? 2 * (size_t)D * sizeof(float) : 0;
-    kernel<<<blocks, plan.tpr > 32 ? plan.tpr : LN_THREADS, smem, st>>>(
+    kernel<<<blocks, plan.tpr > 32 ? plan.tpr : BWD_THREADS, smem, st>>>(
         (const T*)dy, dys, (const T*)x, xs, (const P*)w, mean, rstd, rows, D, plan.tpr, (T*)dx,
         part);
   }

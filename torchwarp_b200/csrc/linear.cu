@@ -51,21 +51,6 @@ constexpr int SMALL_COLS = 4;  // output columns of a warp
 
 // --------------------------------------------------------- few rows
 
-// 16 bytes of T as floats (VEC), or one value.
-template <typename T, bool VEC> struct Lanes {
-  static constexpr int N = VEC ? 16 / (int)sizeof(T) : 1;
-  static __device__ __forceinline__ void load(const T* p, float (&v)[N]) {
-    if (VEC) {
-      union { uint4 u; T t[16 / sizeof(T)]; } q;
-      q.u = __ldg(reinterpret_cast<const uint4*>(p));
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = to_f(q.t[i]);
-    } else {
-      v[0] = to_f(*p);
-    }
-  }
-};
-
 // Sums C values over the warp so that lane l ends with value l / (32 / C):
 // each step sends the half of the values that the other lanes keep.
 template <int C>
@@ -105,7 +90,7 @@ __global__ void __launch_bounds__(128)
                         int M, int N, int K, const T* __restrict__ bias,
                         const T* __restrict__ res, size_t ldr, int act, T* __restrict__ y,
                         T* __restrict__ z) {
-  constexpr int V = Lanes<T, VEC>::N;
+  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
   const int lane = threadIdx.x & 31;
   const int n0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * SMALL_COLS;
   if (n0 >= N) return;
@@ -123,11 +108,11 @@ __global__ void __launch_bounds__(128)
   for (int k = lane * V; k < whole; k += 32 * V) {
     float wv[SMALL_COLS][V];
 #pragma unroll
-    for (int j = 0; j < SMALL_COLS; ++j) Lanes<T, VEC>::load(wr[j] + k, wv[j]);
+    for (int j = 0; j < SMALL_COLS; ++j) load_n<VEC, V>(wr[j] + k, wv[j]);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       float xv[V];
-      Lanes<T, VEC>::load(xr[i] + k, xv);
+      load_n<VEC, V>(xr[i] + k, xv);
 #pragma unroll
       for (int j = 0; j < SMALL_COLS; ++j)
 #pragma unroll
@@ -185,19 +170,16 @@ template <> struct Packed<float> {
   static constexpr int PL = 3;
 };
 
-// x = p0 + p1 + p2 exactly (8 + 8 + 8 bits), each rounded to nearest.  An
-// infinity or NaN stays in p0.
-__device__ __forceinline__ void split3(float x, __nv_bfloat16& p0, __nv_bfloat16& p1,
-                                       __nv_bfloat16& p2) {
-  p0 = __float2bfloat16_rn(x);
-  float h = __bfloat162float(p0);
-  if (fabsf(h) == INFINITY && fabsf(x) < INFINITY) {  // rounded past the largest value
+// x = p0 + p1 + p2 exactly (8 + 8 + 8 bits), each the bfloat16 nearest to what
+// is left: x becomes p0.  An infinity or NaN stays in p0.
+__device__ __forceinline__ void split3(float& x, float& p1, float& p2) {
+  float h = __bfloat162float(__float2bfloat16_rn(x));
+  if (fabsf(h) == INFINITY)  // x rounded past the largest value, or is infinite
     h = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
-    p0 = __float2bfloat16_rn(h);
-  }
   const float r = fabsf(x) < INFINITY ? x - h : 0.f;
-  p1 = __float2bfloat16_rn(r);
-  p2 = __float2bfloat16_rn(r - __bfloat162float(p1));
+  p1 = __bfloat162float(__float2bfloat16_rn(r));
+  p2 = r - p1;
+  x = h;
 }
 
 constexpr int PACK_ROWS = 8, PACK_COLS = 256;  // rows and columns of a block's step
@@ -226,18 +208,12 @@ __global__ void __launch_bounds__(256)
       const T* zp = ACT == kActNone ? nullptr : z + (size_t)r * C + c0;
       float v[8];
       if (vec && c0 + 8 <= C) {
-        constexpr int PER = 16 / sizeof(T);
-        union { uint4 u[8 / PER]; T t[8]; } q, qz;
+        load_n<true, 8>(p, v);
+        if (ACT != kActNone) {
+          float zv[8];
+          load_n<true, 8>(zp, zv);
 #pragma unroll
-        for (int i = 0; i < 8 / PER; ++i) q.u[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-        if (ACT != kActNone)
-#pragma unroll
-          for (int i = 0; i < 8 / PER; ++i)
-            qz.u[i] = __ldg(reinterpret_cast<const uint4*>(zp) + i);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          v[i] = to_f(q.t[i]);
-          if (ACT != kActNone) v[i] *= act_slope<ACT, sizeof(T) == 2>(to_f(qz.t[i]));
+          for (int i = 0; i < 8; ++i) v[i] *= act_slope<ACT, sizeof(T) == 2>(zv[i]);
         }
       } else {
 #pragma unroll
@@ -250,15 +226,17 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int i = 0; i < 8; ++i) s[i] += v[i];
       if (dst) {
-        union { E t[8]; uint4 u; } q[PL];
+        E* o = dst + (size_t)r * Cp + c0;
+        if constexpr (PL == 3) {
+          float p1[8], p2[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if constexpr (PL == 3) split3(v[i], q[0].t[i], q[1].t[i], q[2].t[i]);
-          else q[0].t[i] = from_f<E>(v[i]);
+          for (int i = 0; i < 8; ++i) split3(v[i], p1[i], p2[i]);
+          *reinterpret_cast<uint4*>(o) = pack16<E>(v);
+          *reinterpret_cast<uint4*>(o + plane) = pack16<E>(p1);
+          *reinterpret_cast<uint4*>(o + 2 * plane) = pack16<E>(p2);
+        } else {
+          *reinterpret_cast<uint4*>(o) = pack16<E>(v);
         }
-#pragma unroll
-        for (int k = 0; k < PL; ++k)
-          *reinterpret_cast<uint4*>(dst + k * plane + (size_t)r * Cp + c0) = q[k].u;
       }
     }
   }

@@ -246,10 +246,8 @@ template <typename T>
 __device__ __forceinline__ void stage_piece(uint8_t* box, const float (&v)[32], int lane) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    union { T t[8]; uint4 u; } q;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q.t[i] = from_f<T>(v[8 * c + i]);
-    *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = q.u;
+    *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+        pack16<T>(v + 8 * c);
   }
 }
 template <> __device__ __forceinline__ void stage_piece<float>(uint8_t*, const float (&)[32], int) {}
@@ -291,10 +289,10 @@ __device__ __forceinline__ void finish_piece(float (&v)[32], int m0, int n0, con
         constexpr int PER = 16 / sizeof(T);
 #pragma unroll
         for (int c = 0; c < 32 / PER; ++c) {
-          union { uint4 u; T t[PER]; } q;
-          q.u = __ldg(r + c);
+          float q[PER];
+          unpack16<T>(__ldg(r + c), q);
 #pragma unroll
-          for (int i = 0; i < PER; ++i) v[c * PER + i] = add_rn(v[c * PER + i], to_f(q.t[i]));
+          for (int i = 0; i < PER; ++i) v[c * PER + i] = add_rn(v[c * PER + i], q[i]);
         }
       }
     } else if (m0 + lane < g.M) {

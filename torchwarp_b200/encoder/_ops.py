@@ -18,6 +18,20 @@ from torch.autograd.function import once_differentiable
 
 from .. import _native as nat
 
+# [m, n] products of up to this many rows take no workspace (csrc/linear.cu)
+_SMALL_ROWS = 8
+
+
+def _first_order(fn):
+    """torch's ``once_differentiable``, at no cost to a backward that records no graph."""
+    guarded = once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else fn)(ctx, *grads)
+
+    return backward
+
+
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4}
 
 
@@ -35,6 +49,12 @@ def rows_of(x):
 def frames_of(x):
     """[B, T, D] with the last dimension contiguous."""
     return x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous()
+
+
+def _dense_like(x):
+    """An uninitialised contiguous tensor of x's shape and type."""
+    return torch.empty_like(x) if x.is_contiguous() else \
+        torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def _p(t):
@@ -58,7 +78,7 @@ def _mean_rstd(stats, rows):
 def layer_norm_forward(x, weight, bias, eps, save):
     d = x.shape[-1]
     rows = x.numel() // d
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _dense_like(x)
     stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if save else None
     if rows:
         xr, stride = rows_of(x)
@@ -75,7 +95,7 @@ def layer_norm_backward(dy, x, weight, bias_dtype, stats, need):
     d = x.shape[-1]
     rows = x.numel() // d
     ptype = weight.dtype if weight is not None else bias_dtype or x.dtype
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
+    dx = _dense_like(x) if need[0] else None
     dw = torch.empty(d, dtype=ptype, device=x.device) if need[1] else None
     db = torch.empty(d, dtype=ptype, device=x.device) if need[2] else None
     if any(need):
@@ -100,7 +120,7 @@ class LayerNormFunction(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         return (*layer_norm_backward(dy, x, weight, ctx.bias_dtype, stats,
@@ -164,7 +184,7 @@ def linear_forward(x, weight, bias, residual, act, save):
         (xr, xs), (wr, wst) = rows_of(x), rows_of(weight)
         rr, rs = (None, 0) if residual is None else rows_of(residual)
         nbytes = 0
-        if m > 8:  # fewer rows take none
+        if m > _SMALL_ROWS:
             nbytes = nat.lib().tw_linear_workspace_bytes(m, n, k, x.element_size(), act, 0,
                                                          _unaligned(xr, xs, wr, wst))
         ws = _workspace(nbytes, x.device)
@@ -180,8 +200,8 @@ def linear_backward(dy, x, weight, z, act, need):
     n, k = weight.shape
     m = x.numel() // k
     dev = x.device
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
-    dw = torch.empty((n, k), dtype=x.dtype, device=dev) if need[1] else None
+    dx = _dense_like(x) if need[0] else None
+    dw = _dense_like(weight) if need[1] else None
     db = torch.empty(n, dtype=x.dtype, device=dev) if need[2] else None
     if any(need):
         if dy.dtype != x.dtype:
@@ -206,7 +226,7 @@ class LinearFunction(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, weight, z = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -260,7 +280,7 @@ linear_op.register_autograd(_linear_bwd, setup_context=_linear_setup)
 
 def gated_scan_forward(x, gate, h0, lengths, save):
     b, t, d = x.shape
-    y = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
+    y = _dense_like(x)
     state = torch.empty((b, d), dtype=torch.float32, device=x.device)
     carry = None
     nbytes = 0
@@ -280,8 +300,7 @@ def gated_scan_forward(x, gate, h0, lengths, save):
 def gated_scan_backward(dy, dstate, x, gate, lengths, carry):
     """(dx, dgate, dh0) for dL/dy and dL/dstate (either may be None)."""
     b, t, d = x.shape
-    dx = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
-    dgate = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
+    dx, dgate = _dense_like(x), _dense_like(x)
     dh0 = torch.empty((b, d), dtype=torch.float32, device=x.device)
     if b:
         x, gate = frames_of(x), frames_of(gate)
@@ -304,7 +323,7 @@ class GatedScanFunction(torch.autograd.Function):
         return y, state
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy, dstate):
         if dy is None and dstate is None:
             return None, None, None, None
@@ -357,7 +376,7 @@ gated_scan_op.register_autograd(_gated_scan_bwd, setup_context=_gated_scan_setup
 
 def gated_scan_step(x, gate, state):
     b, d = x.shape
-    y = torch.empty((b, d), dtype=x.dtype, device=x.device)
+    y = _dense_like(x)
     if b:
         (xr, xs), (gr, gs) = rows_of(x), rows_of(gate)
         nat.launch("gated_scan_step", nat.entry("tw_gated_scan_step", x.dtype), x.device,

@@ -29,15 +29,31 @@ def _check_type(name, t):
 
 
 def _check_device(first, *rest):
-    nat.require_cuda(first, *rest)
+    device = first.device
+    if device.type != "cuda":
+        nat.require_cuda(first)
     for t in rest:
-        if t is not None and t.device != first.device:
+        if t is not None and t.device != device:
+            nat.require_cuda(t)
             raise ValueError("all tensors must be on one device, got {} and {}".format(
-                first.device, t.device))
+                device, t.device))
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _check_parameter(name, p, x):
+    if p.ndim != 1 or p.shape[0] != x.shape[-1]:
+        raise ValueError("{} must have shape [{}], got {}".format(name, x.shape[-1],
+                                                                  list(p.shape)))
+    if p.dtype != x.dtype and p.dtype != torch.float32:
+        raise TypeError("{} must be float32 or of x's type {}, got {}".format(name, x.dtype,
+                                                                              p.dtype))
 
 
 def layer_norm(x, weight=None, bias=None, *, eps=1e-5):
@@ -54,22 +70,19 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5):
     _check_type("x", x)
     if x.ndim < 1 or x.shape[-1] == 0:
         raise ValueError("x must have shape [..., D] with D > 0")
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        if p.shape != x.shape[-1:]:
-            raise ValueError("{} must have shape [{}], got {}".format(name, x.shape[-1],
-                                                                      list(p.shape)))
-        if p.dtype != x.dtype and p.dtype != torch.float32:
-            raise TypeError("{} must be float32 or of x's type {}, got {}".format(name, x.dtype,
-                                                                                  p.dtype))
+    if weight is not None:
+        _check_parameter("weight", weight, x)
+    if bias is not None:
+        _check_parameter("bias", bias, x)
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError("weight and bias must have one type")
     if not eps >= 0:
         raise ValueError("eps must be >= 0")
     _check_device(x, weight, bias)
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
     if torch.compiler.is_compiling():
         return _ops.layer_norm_op(x, weight, bias, float(eps))[0]
     if _wants_grad(x, weight, bias):

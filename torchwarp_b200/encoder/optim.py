@@ -21,6 +21,8 @@ class _Bucket:
         for p in params:
             self.offsets.append(at)
             at += -(-p.numel() // _BLOCK) * _BLOCK
+        self.rows = array("Q", [v for p, o in zip(params, self.offsets)
+                                for v in (0, 0, p.numel(), o)])
         dev = self.device
         self.step = torch.zeros(2, dtype=torch.int32, device=dev)
         if bits == 32:
@@ -42,22 +44,27 @@ class _Bucket:
                                                "exp_avg_sqrt_scale"))
 
     def table(self):
-        """Four numbers a tensor for the native step; a tensor without a gradient is left out."""
-        rows, keep = [], []
-        for p, offset in zip(self.params, self.offsets):
+        """Four numbers a tensor for the native step (a tensor without a gradient counts no
+        values), and the gradients that had to be copied."""
+        table, keep, at = array("Q", self.rows), [], 0
+        dtype = self.dtype
+        for p in self.params:
             g = p.grad
             if g is None:
-                continue
-            if g.dtype != self.dtype or g.is_sparse:
-                raise TypeError("a gradient must be dense and of its parameter's type {}, got {}"
-                                .format(self.dtype, g.dtype))
-            if not p.is_contiguous():
-                raise ValueError("parameters must be contiguous")
-            if not g.is_contiguous():
-                g = g.contiguous()
-                keep.append(g)
-            rows += (p.data_ptr(), g.data_ptr(), p.numel(), offset)
-        return array("Q", rows), keep
+                table[at + 2] = 0
+            else:
+                if g.dtype != dtype:
+                    raise TypeError("a gradient must be of its parameter's type {}, got {}".format(
+                        dtype, g.dtype))
+                if not p.is_contiguous():
+                    raise ValueError("parameters must be contiguous")
+                if not g.is_contiguous():
+                    g = g.contiguous()
+                    keep.append(g)
+                table[at] = p.data_ptr()
+                table[at + 1] = g.data_ptr()
+            at += 4
+        return table, keep
 
 
 class AdamW(torch.optim.Optimizer):
