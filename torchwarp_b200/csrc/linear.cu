@@ -184,101 +184,129 @@ __device__ __forceinline__ void split3(float& x, float& p1, float& p2) {
 
 constexpr int PACK_ROWS = 8, PACK_COLS = 256;  // rows and columns of a block's step
 
-// src [R, C], or src * act'(z), as the tensor cores read it: rows of Cp
-// (a multiple of 8) values, in planes.  dst NULL: no copy; sums: column sums
-// over this block's `rb` rows, in float32 before rounding, or NULL.
-// Bound by HBM: each value is read once with 16-byte loads where the rows
-// are aligned and written once.
+// One matrix to write as the tensor cores read it: src [R, C], or src *
+// act'(z), in rows of Cp (a multiple of 8) values, in planes.  dst NULL: no
+// copy; sums: column sums of each block's `rb` rows, in float32 before
+// rounding, or NULL.
+template <typename T> struct PackJob {
+  const T* src;
+  const T* z;
+  typename Packed<T>::E* dst;
+  float* sums;
+  size_t ld, plane;
+  int R, C, Cp, rb, vec, act, cols, first;  // blocks along the columns; number of the first block
+};
+// The matrices of a call go in one launch, side by side.
+constexpr int MOST_JOBS = 3;
+template <typename T> struct PackJobs {
+  PackJob<T> j[MOST_JOBS];
+  int count;
+};
+
+// Bound by HBM: each value is read once and written once, 8 neighbouring
+// columns a thread; with 16-byte loads where the rows are aligned (`vec`).
+// Single loads of neighbours still end in 16-byte stores: giving a thread
+// every 32nd column instead made the stores single too and took 44 in place of
+// 19 us for 7000 x 385 float32.
 template <typename T, int ACT>
-__global__ void __launch_bounds__(256)
-    linear_pack_kernel(const T* __restrict__ src, size_t ld, const T* __restrict__ z, int R, int C,
-                       int Cp, typename Packed<T>::E* __restrict__ dst, size_t plane, int rb,
-                       float* __restrict__ sums, int vec) {
+__device__ __forceinline__ void pack_block(const PackJob<T>& j, int bx, int by, float* s) {
   constexpr int PL = Packed<T>::PL;
   using E = typename Packed<T>::E;
-  __shared__ float red[PACK_ROWS][PACK_COLS + 8];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int c0 = blockIdx.x * PACK_COLS + tx * 8;
-  const int r1 = min(R, (int)(blockIdx.y + 1) * rb);
-  float s[8] = {};
-  if (c0 < Cp) {
+  const int c0 = bx * PACK_COLS + tx * 8, r1 = min(j.R, (by + 1) * j.rb), C = j.C;
+  if (c0 >= j.Cp) return;
 #pragma unroll 2
-    for (int r = blockIdx.y * rb + ty; r < r1; r += PACK_ROWS) {
-      const T* p = src + (size_t)r * ld + c0;
-      const T* zp = ACT == kActNone ? nullptr : z + (size_t)r * C + c0;
-      float v[8];
-      if (vec && c0 + 8 <= C) {
-        load_n<true, 8>(p, v);
-        if (ACT != kActNone) {
-          float zv[8];
-          load_n<true, 8>(zp, zv);
+  for (int r = by * j.rb + ty; r < r1; r += PACK_ROWS) {
+    const T* p = j.src + (size_t)r * j.ld + c0;
+    const T* zp = ACT == kActNone ? nullptr : j.z + (size_t)r * C + c0;
+    float v[8], zv[8];
+    if (j.vec) {  // then C is a multiple of 8
+      load_n<true, 8>(p, v);
+      if (ACT != kActNone) load_n<true, 8>(zp, zv);
+    } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] *= act_slope<ACT, sizeof(T) == 2>(zv[i]);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          v[i] = c0 + i < C ? to_f(p[i]) : 0.f;
-          if (ACT != kActNone && c0 + i < C)
-            v[i] *= act_slope<ACT, sizeof(T) == 2>(to_f(zp[i]));
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] += v[i];
-      if (dst) {
-        E* o = dst + (size_t)r * Cp + c0;
-        if constexpr (PL == 3) {
-          float p1[8], p2[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) split3(v[i], p1[i], p2[i]);
-          *reinterpret_cast<uint4*>(o) = pack16<E>(v);
-          *reinterpret_cast<uint4*>(o + plane) = pack16<E>(p1);
-          *reinterpret_cast<uint4*>(o + 2 * plane) = pack16<E>(p2);
-        } else {
-          *reinterpret_cast<uint4*>(o) = pack16<E>(v);
-        }
+      for (int i = 0; i < 8; ++i) {
+        v[i] = c0 + i < C ? to_f(p[i]) : 0.f;
+        if (ACT != kActNone) zv[i] = c0 + i < C ? to_f(zp[i]) : 0.f;
       }
     }
-  }
-  if (!sums) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) red[ty][tx * 8 + i] = s[i];
-  __syncthreads();
-  const int c = blockIdx.x * PACK_COLS + threadIdx.x;
-  if (c < C) {
-    float t = 0.f;
+    for (int i = 0; i < 8; ++i) {
+      if (ACT != kActNone) v[i] *= act_slope<ACT, sizeof(T) == 2>(zv[i]);
+      s[i] += v[i];
+    }
+    if (j.dst) {
+      E* o = j.dst + (size_t)r * j.Cp + c0;
+      if constexpr (PL == 3) {
+        float p1[8], p2[8];
 #pragma unroll
-    for (int k = 0; k < PACK_ROWS; ++k) t += red[k][threadIdx.x];
-    sums[(size_t)blockIdx.y * C + c] = t;
+        for (int i = 0; i < 8; ++i) split3(v[i], p1[i], p2[i]);
+        *reinterpret_cast<uint4*>(o + j.plane) = pack16<E>(p1);
+        *reinterpret_cast<uint4*>(o + 2 * j.plane) = pack16<E>(p2);
+      }
+      *reinterpret_cast<uint4*>(o) = pack16<E>(v);
+    }
   }
 }
 
-// db[c] = the blocks' column sums, in a fixed order.
 template <typename T>
 __global__ void __launch_bounds__(256)
+    linear_pack_kernel(const __grid_constant__ PackJobs<T> jobs) {
+  __shared__ float red[PACK_ROWS][PACK_COLS + 8];
+  int k = jobs.count - 1;
+  while (k > 0 && (int)blockIdx.x < jobs.j[k].first) --k;
+  const PackJob<T>& j = jobs.j[k];
+  const int block = blockIdx.x - j.first, by = block / j.cols, bx = block - by * j.cols;
+  float s[8] = {};
+  switch (j.act) {
+    case kActRelu: pack_block<T, kActRelu>(j, bx, by, s); break;
+    case kActGelu: pack_block<T, kActGelu>(j, bx, by, s); break;
+    case kActSilu: pack_block<T, kActSilu>(j, bx, by, s); break;
+    case kActSigmoid: pack_block<T, kActSigmoid>(j, bx, by, s); break;
+    default: pack_block<T, kActNone>(j, bx, by, s); break;
+  }
+  if (!j.sums) return;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) red[ty][tx * 8 + i] = s[i];
+  __syncthreads();
+  const int c = bx * PACK_COLS + threadIdx.x;
+  if (c < j.C) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < PACK_ROWS; ++i) t += red[i][threadIdx.x];
+    j.sums[(size_t)by * j.C + c] = t;
+  }
+}
+
+// db[c] = the blocks' column sums, in a fixed order: 32 columns a block, whose
+// 32 warps share the rows.
+template <typename T>
+__global__ void __launch_bounds__(1024)
     linear_db_kernel(const float* __restrict__ sums, int blocks, int C, T* __restrict__ db) {
-  __shared__ float red[8][33];
+  __shared__ float red[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 32 + tx;
   float s = 0.f;
   if (c < C)
-    for (int b = ty; b < blocks; b += 8) s += sums[(size_t)b * C + c];
+#pragma unroll 8
+    for (int b = ty; b < blocks; b += 32) s += sums[(size_t)b * C + c];
   red[ty][tx] = s;
   __syncthreads();
-  if (ty == 0 && c < C) {
+  s = red[tx][ty];  // warp ty sums column ty
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += red[i][tx];
-    db[c] = from_f<T>(s);
-  }
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int col = blockIdx.x * 32 + ty;
+  if (tx == 0 && col < C) db[col] = from_f<T>(s);
 }
 
 size_t up8(size_t n) { return (n + 7) / 8 * 8; }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Rows of a block of the pack kernel: 64, or more where that makes over 256
+// Rows of a block of the pack kernel: 16, or more where that makes over 256
 // blocks along the rows (their sums are read back).
 int rows_per_block(int R) {
   const int rb = (R + 255) / 256;
-  return (rb < 64 ? 64 : (rb + 7) / 8 * 8);
+  return rb < 16 ? 16 : (rb + 7) / 8 * 8;
 }
 int row_blocks(int R) { return (R + rows_per_block(R) - 1) / rows_per_block(R); }
 
@@ -299,27 +327,41 @@ int launched(const char* who) {
   return kOk;
 }
 
-template <typename T, int ACT>
-void pack(const T* src, size_t ld, const T* z, int R, int C, void* dst, float* sums,
-          cudaStream_t st) {
-  const int Cp = (int)up8(C);
-  const int vec = (uintptr_t)src % 16 == 0 && ld * sizeof(T) % 16 == 0 &&
-                  (ACT == kActNone || ((uintptr_t)z % 16 == 0 && C * sizeof(T) % 16 == 0));
-  const dim3 grid((Cp + PACK_COLS - 1) / PACK_COLS, row_blocks(R));
-  linear_pack_kernel<T, ACT><<<grid, 256, 0, st>>>(
-      src, ld, z, R, C, Cp, (typename Packed<T>::E*)dst, (size_t)R * Cp, rows_per_block(R), sums,
-      vec);
-}
+// The matrices of a call to be packed, and how many blocks they take.
+template <typename T> struct Packing {
+  PackJobs<T> jobs = {};
+  unsigned blocks = 0;
 
-// src as an operand: as it lies, or packed into `ws` (taken when `packs`).
-template <typename T>
-GemmOperand operand(const T* src, size_t ld, int R, int C, bool k_major, bool packs, void* ws,
-                    cudaStream_t st) {
-  if (!packs)
-    return {src, R == 1 ? up8(C) : ld, 0, R, C, k_major};
-  pack<T, kActNone>(src, ld, nullptr, R, C, ws, nullptr, st);
-  return {ws, up8(C), (size_t)R * up8(C), R, C, k_major};
-}
+  void add(const T* src, size_t ld, const T* z, int act, int R, int C, void* dst, float* sums) {
+    PackJob<T>& j = jobs.j[jobs.count++];
+    j.src = src;
+    j.z = z;
+    j.dst = (typename Packed<T>::E*)dst;
+    j.sums = sums;
+    j.ld = ld;
+    j.R = R;
+    j.C = C;
+    j.Cp = (int)up8(C);
+    j.plane = (size_t)R * j.Cp;
+    j.rb = rows_per_block(R);
+    j.act = act;
+    j.vec = C % 8 == 0 && (uintptr_t)src % 16 == 0 && ld * sizeof(T) % 16 == 0 &&
+            (act == kActNone || (uintptr_t)z % 16 == 0);
+    j.cols = (j.Cp + PACK_COLS - 1) / PACK_COLS;
+    j.first = (int)blocks;
+    blocks += (unsigned)(j.cols * row_blocks(R));
+  }
+  // src as an operand: as it lies, or packed into `ws` (taken when `packs`).
+  GemmOperand operand(const T* src, size_t ld, int R, int C, bool k_major, bool packs, void* ws) {
+    if (!packs) return {src, R == 1 ? up8(C) : ld, 0, R, C, k_major};
+    add(src, ld, nullptr, kActNone, R, C, ws, nullptr);
+    return {ws, up8(C), (size_t)R * up8(C), R, C, k_major};
+  }
+  int run(const char* who, cudaStream_t st) {
+    if (blocks) linear_pack_kernel<T><<<blocks, 256, 0, st>>>(jobs);
+    return launched(who);
+  }
+};
 
 size_t partial_bytes(int M, int N, int K, int planes) {
   const GemmPlan p = gemm_plan(M, N, K, planes);
@@ -392,8 +434,9 @@ int fwd(const void* xv, size_t ldx, const void* wv, size_t ldw, const void* bias
   if (int e = check_ws("tw_linear_forward", ws_bytes, l.total, ws)) return e;
   char* base = (char*)ws;
   GemmProblem p = {};
-  p.a = operand<T>(x, ldx, M, K, true, px, base + l.x, st);
-  p.b = operand<T>(w, ldw, N, K, true, pw, base + l.w, st);
+  Packing<T> packing;
+  p.a = packing.operand(x, ldx, M, K, true, px, base + l.x);
+  p.b = packing.operand(w, ldw, N, K, true, pw, base + l.w);
   p.M = M;
   p.N = N;
   p.K = K;
@@ -404,20 +447,8 @@ int fwd(const void* xv, size_t ldx, const void* wv, size_t ldw, const void* bias
   p.out = y;
   p.z = act == kActNone ? nullptr : z;
   p.partial = (float*)(base + l.partial);
-  if (int e = launched("tw_linear_forward")) return e;
+  if (int e = packing.run("tw_linear_forward", st)) return e;
   return gemm_run<T>(p, st);
-}
-
-template <typename T>
-void pack_dz(const T* dy, size_t ldy, const T* z, int M, int N, int act, void* dst, float* sums,
-             cudaStream_t st) {
-  switch (act) {
-    case kActRelu: pack<T, kActRelu>(dy, ldy, z, M, N, dst, sums, st); break;
-    case kActGelu: pack<T, kActGelu>(dy, ldy, z, M, N, dst, sums, st); break;
-    case kActSilu: pack<T, kActSilu>(dy, ldy, z, M, N, dst, sums, st); break;
-    case kActSigmoid: pack<T, kActSigmoid>(dy, ldy, z, M, N, dst, sums, st); break;
-    default: pack<T, kActNone>(dy, ldy, nullptr, M, N, dst, sums, st); break;
-  }
 }
 
 template <typename T>
@@ -443,34 +474,36 @@ int bwd(const void* dyv, size_t ldy, const void* xv, size_t ldx, const void* wv,
   if (int e = check_ws("tw_linear_backward", ws_bytes, l.total, ws)) return e;
   char* base = (char*)ws;
   const bool packs = (dx || dw) && (act != kActNone || pdy);
-  if (packs || db) {
-    float* sums = db ? (float*)(base + l.sums) : nullptr;
-    pack_dz<T>(dy, ldy, (const T*)z, M, N, act, packs ? base + l.dz : nullptr, sums, st);
-    if (db) linear_db_kernel<T><<<(N + 31) / 32, 256, 0, st>>>(sums, row_blocks(M), N, (T*)db);
-  }
+  float* sums = db ? (float*)(base + l.sums) : nullptr;
+  Packing<T> packing;
+  if (packs || db)
+    packing.add(dy, ldy, (const T*)z, act, M, N, packs ? base + l.dz : nullptr, sums);
   GemmOperand dz = {dy, M == 1 ? up8(N) : ldy, 0, M, N, true};
   if (packs) dz = {base + l.dz, up8(N), (size_t)M * up8(N), M, N, true};
+  GemmOperand bw = {}, bx = {};
+  if (dx) bw = packing.operand(w, ldw, N, K, false, pw, base + l.w);
+  if (dw) bx = packing.operand(x, ldx, M, K, false, px, base + l.x);
+  if (int e = packing.run("tw_linear_backward", st)) return e;
+  if (db) linear_db_kernel<T><<<(N + 31) / 32, 1024, 0, st>>>(sums, row_blocks(M), N, (T*)db);
   GemmProblem p = {};
   p.partial = (float*)(base + l.partial);
   if (dx) {
     p.a = dz;
-    p.b = operand<T>(w, ldw, N, K, false, pw, base + l.w, st);
+    p.b = bw;
     p.M = M;
     p.N = K;
     p.K = N;
     p.out = dx;
-    if (int e = launched("tw_linear_backward")) return e;
     if (int e = gemm_run<T>(p, st)) return e;
   }
   if (dw) {
     p.a = dz;
     p.a.k_major = false;
-    p.b = operand<T>(x, ldx, M, K, false, px, base + l.x, st);
+    p.b = bx;
     p.M = N;
     p.N = K;
     p.K = M;
     p.out = dw;
-    if (int e = launched("tw_linear_backward")) return e;
     if (int e = gemm_run<T>(p, st)) return e;
   }
   return launched("tw_linear_backward");

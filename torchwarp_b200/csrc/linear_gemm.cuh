@@ -16,9 +16,12 @@
 // its accumulator; every SEG_CHUNKS chunks the two are added to float32
 // registers, rounding to nearest, which keeps that bias to a few steps.
 //
-// Warps 0-7: epilogue (TMEM lane quadrant warp % 4, column half warp / 4);
-// warp 8: TMA; warp 9: TMEM allocation and MMA issue (of the pair's first
-// CTA).  Two accumulator sets let the epilogue of a tile overlap the next
+// Warps 0 .. EW - 1: epilogue (TMEM lane quadrant warp % 4, a share of the
+// columns each); then one warp for TMA and one for TMEM allocation and MMA
+// issue (of the pair's first CTA).  A warp's way through a piece is a chain of
+// latencies (TMEM, exponential and reciprocal, staging, fence), so wide tiles
+// take 16 of them: with 8 the gelu epilogue paced the 32768 x 1024 x 4096
+// product (262 us).  Two accumulator sets let the epilogue of a tile overlap the next
 // tile's products.  No atomics: results are reproducible.
 #pragma once
 
@@ -33,7 +36,6 @@ using namespace tc;
 
 __device__ int g_gemm_error;
 
-constexpr int GEMM_THREADS = 320;
 constexpr int BK = 64;                // contraction values per chunk: one 128-byte line
 constexpr int A_PLANE = 128 * BK * 2;
 constexpr int SMEM_MAX = 232448;
@@ -42,17 +44,17 @@ constexpr int SHARED_MAX = 2048;
 template <typename T> struct Elem {
   static constexpr int PL = 1;
   static constexpr uint32_t FMT = 1;  // bfloat16
-  static constexpr int STG = 8192;    // y and z, two buffers of 32 rows x 64 bytes each
+  static constexpr int STG = 4096;    // y and z: 32 rows x 64 bytes each, or 32 x 32 floats
 };
 template <> struct Elem<__half> {
   static constexpr int PL = 1;
   static constexpr uint32_t FMT = 0;
-  static constexpr int STG = 8192;
+  static constexpr int STG = 4096;
 };
 template <> struct Elem<float> {
   static constexpr int PL = 3;
   static constexpr uint32_t FMT = 1;
-  static constexpr int STG = 4224;    // 32 x 33 floats
+  static constexpr int STG = 4096;
 };
 
 template <typename T, int CG, int TN> struct Geom {
@@ -60,16 +62,20 @@ template <typename T, int CG, int TN> struct Geom {
   static constexpr int B_ROWS = TN / CG;
   static constexpr int B_PLANE = B_ROWS * BK * 2;
   static constexpr int STAGE = PL * (A_PLANE + B_PLANE);
-  static constexpr int FIT = (SMEM_MAX - SHARED_MAX - 8 * Elem<T>::STG) / STAGE;
+  // float32 keeps 8: its stages leave no room for more staging
+  static constexpr int EW = TN >= 128 && PL == 1 ? 16 : 8;  // epilogue warps
+  static constexpr int THREADS = 32 * (EW + 2);
+  static constexpr int FIT = (SMEM_MAX - SHARED_MAX - EW * Elem<T>::STG) / STAGE;
   static constexpr int STAGES = FIT < 8 ? FIT : 8;
   static constexpr int SEG_CHUNKS = 2;
   static constexpr int ACC = TN * (PL == 3 ? 2 : 1);  // TMEM columns of one accumulator set
-  static constexpr int SMEM = STAGES * STAGE + 8 * Elem<T>::STG + SHARED_MAX;
-  static constexpr int CHUNKS32 = TN / 64;            // 32-column pieces of a column half
+  static constexpr int SMEM = STAGES * STAGE + EW * Elem<T>::STG + SHARED_MAX;
+  static constexpr int COLS = TN / (EW / 4);          // of a warp
+  static constexpr int CHUNKS32 = COLS / 32;          // in pieces of 32
 };
 
 struct GemmShared {
-  float bias[8][32];
+  __align__(16) uint8_t bias[1024];  // of each epilogue warp: 32 elements
   uint64_t full[8], empty[8], accf[2], acce[2], mma_done;
   uint32_t tmem_base;
   int abort;
@@ -77,7 +83,7 @@ struct GemmShared {
 static_assert(sizeof(GemmShared) <= SHARED_MAX, "shared block");
 
 template <typename T> struct GemmArgs {
-  int M, N, nK, tiles_n, items, splits, per_split;
+  int M, N, K, nK, tiles_m, tiles_n, items, splits, per_split;
   const T* bias;
   const T* res;
   size_t ldr;
@@ -86,6 +92,21 @@ template <typename T> struct GemmArgs {
   float* partial;
   int act, res_vec, tma_store;
 };
+
+// The tile of an item: bands of TILE_BAND rows of tiles, down a band's columns,
+// so that the tiles in flight at once are near a square and share their A and
+// B panels in L2.
+constexpr int TILE_BAND = 8;
+struct TileAt {
+  int m, n, split;
+};
+template <typename T>
+__device__ __forceinline__ TileAt tile_at(int w, const GemmArgs<T>& g) {
+  const int tile = w / g.splits;
+  const int per_band = TILE_BAND * g.tiles_n, band = tile / per_band;
+  const int rows = min(TILE_BAND, g.tiles_m - band * TILE_BAND), r = tile - band * per_band;
+  return {band * TILE_BAND + r % rows, r / rows, w - tile * g.splits};
+}
 
 __device__ __forceinline__ uint32_t cta_rank() {
   uint32_t r;
@@ -129,6 +150,15 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, unsigned parity, volatil
     }
   }
   return true;
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
 }
 
 template <int CG>
@@ -231,13 +261,13 @@ __device__ __forceinline__ void store_piece(float* stg, const float (&v)[32], U*
                                             int n0, int M, int N, int lane) {
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 32; ++i) stg[lane * 33 + i] = v[i];
+  for (int i = 0; i < 32; ++i) stg[lane * 32 + (i ^ lane)] = v[i];
   __syncwarp();
   const int rows = min(32, M - m0);
   if (n0 + lane < N) {
     U* o = out + (size_t)m0 * N + n0 + lane;
 #pragma unroll 8
-    for (int r = 0; r < rows; ++r) o[(size_t)r * N] = from_f<U>(stg[r * 33 + lane]);
+    for (int r = 0; r < rows; ++r) o[(size_t)r * N] = from_f<U>(stg[r * 32 + (lane ^ r)]);
   }
 }
 
@@ -253,12 +283,12 @@ __device__ __forceinline__ void stage_piece(uint8_t* box, const float (&v)[32], 
 template <> __device__ __forceinline__ void stage_piece<float>(uint8_t*, const float (&)[32], int) {}
 
 // Bias, activation, residual and the stores of a warp's 32 x 32 piece at
-// (m0, n0); `use` counts the boxes this warp has stored.
+// (m0, n0); `bias` is that of column n0 + lane, bias_s the warp's room for 32.
 template <typename T>
 __device__ __forceinline__ void finish_piece(float (&v)[32], int m0, int n0, const GemmArgs<T>& g,
-                                             float* bias_s, uint8_t* stg, const CUtensorMap* mapY,
-                                             const CUtensorMap* mapZ, int lane, int& use,
-                                             int split) {
+                                             T bias, T* bias_s, uint8_t* stg,
+                                             const CUtensorMap* mapY, const CUtensorMap* mapZ,
+                                             int lane, int split) {
   if (m0 >= g.M || n0 >= g.N) return;
   if (g.partial) {
     store_piece<float>(reinterpret_cast<float*>(stg), v, g.partial + (size_t)split * g.M * g.N, m0,
@@ -267,17 +297,22 @@ __device__ __forceinline__ void finish_piece(float (&v)[32], int m0, int n0, con
   }
   constexpr bool FAST = sizeof(T) == 2;
   if (g.bias) {
+    constexpr int PER = 16 / sizeof(T);
     __syncwarp();
-    bias_s[lane] = n0 + lane < g.N ? to_f(g.bias[n0 + lane]) : 0.f;
+    bias_s[lane] = bias;
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = add_rn(v[i], bias_s[i]);
+    for (int c = 0; c < 32 / PER; ++c) {
+      float q[PER];
+      unpack16<T>(reinterpret_cast<const uint4*>(bias_s)[c], q);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[c * PER + i] = add_rn(v[c * PER + i], q[i]);
+    }
   }
-  uint8_t* box = stg + (use & 1) * 2048;
   if (g.tma_store) {
-    if (lane == 0) bulk_wait_read<1>();  // the boxes used two pieces ago are free
+    if (lane == 0) bulk_wait_read<0>();  // the boxes of the last piece are free
     __syncwarp();
-    if (g.z) stage_piece<T>(box + 4096, v, lane);
+    if (g.z) stage_piece<T>(stg + 2048, v, lane);
   } else if (g.z) {
     store_piece<T>(reinterpret_cast<float*>(stg), v, g.z, m0, n0, g.M, g.N, lane);
   }
@@ -303,32 +338,33 @@ __device__ __forceinline__ void finish_piece(float (&v)[32], int m0, int n0, con
     }
   }
   if (g.tma_store) {
-    stage_piece<T>(box, v, lane);
+    stage_piece<T>(stg, v, lane);
     fence_async_smem();
     __syncwarp();
     if (lane == 0) {
-      tma_store_3d(mapY, box, n0, m0, 0);
-      if (g.z) tma_store_3d(mapZ, box + 4096, n0, m0, 0);
+      tma_store_3d(mapY, stg, n0, m0, 0);
+      if (g.z) tma_store_3d(mapZ, stg + 2048, n0, m0, 0);
       bulk_commit();
     }
-    ++use;
   } else {
     store_piece<T>(reinterpret_cast<float*>(stg), v, g.out, m0, n0, g.M, g.N, lane);
   }
 }
 
 template <typename T, int CG, int TN, bool A_MN, bool B_MN>
-__global__ void __launch_bounds__(GEMM_THREADS, 1)
+__global__ void __launch_bounds__(Geom<T, CG, TN>::THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
                 const __grid_constant__ CUtensorMap mapY, const __grid_constant__ CUtensorMap mapZ,
                 const GemmArgs<T> g) {
   using G = Geom<T, CG, TN>;
-  constexpr int PL = G::PL, STAGES = G::STAGES, NP = G::CHUNKS32;
+  constexpr int PL = G::PL, STAGES = G::STAGES, NP = G::CHUNKS32, EW = G::EW;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* stg_base = smem + STAGES * G::STAGE;
-  GemmShared& sh = *reinterpret_cast<GemmShared*>(stg_base + 8 * Elem<T>::STG);
+  GemmShared& sh = *reinterpret_cast<GemmShared*>(stg_base + EW * Elem<T>::STG);
   volatile int* abort = &sh.abort;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  // the same in all lanes, and known to be: a role's loop runs on uniform registers
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int rank = CG == 2 ? (int)cta_rank() : 0;
   const int unit = blockIdx.x / CG, units = gridDim.x / CG;
 
@@ -344,12 +380,12 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&sh.accf[a], 1);
-      mbar_init(&sh.acce[a], 8 * CG);
+      mbar_init(&sh.acce[a], EW * CG);
     }
     mbar_init(&sh.mma_done, 1);
     fence_barrier_init();
   }
-  if (warp == 9) alloc_tmem<CG>(&sh.tmem_base, 2 * G::ACC);
+  if (warp == EW + 1) alloc_tmem<CG>(&sh.tmem_base, 2 * G::ACC);
   tc_fence_before();
   __syncthreads();
   if (CG == 2) cluster_sync_all();
@@ -359,19 +395,19 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
   // leaves together
   const bool dead = *abort != 0;
 
-  if (!dead && warp == 8) {
+  if (!dead && warp == EW) {
     // ---------------------------------------------------- TMA producer
     if (lane == 0) {
-      int it = 0;
+      int it = 0, s = 0;
+      uint32_t ph = 1;
       bool ok = true;
       for (int w = unit; ok && w < g.items; w += units) {
-        const int tile = w / g.splits, split = w - tile * g.splits;
-        const int m0 = (tile / g.tiles_n) * 128 * CG + rank * 128;
-        const int n0 = (tile % g.tiles_n) * TN + rank * G::B_ROWS;
-        const int k1 = min(g.nK, (split + 1) * g.per_split);
-        for (int kc = split * g.per_split; kc < k1; ++kc, ++it) {
-          const int s = it % STAGES;
-          if (!wait_for(&sh.empty[s], ((unsigned)(it / STAGES) & 1u) ^ 1u, abort)) {
+        const TileAt t = tile_at(w, g);
+        const int m0 = t.m * 128 * CG + rank * 128;
+        const int n0 = t.n * TN + rank * G::B_ROWS;
+        const int k1 = min(g.nK, (t.split + 1) * g.per_split);
+        for (int kc = t.split * g.per_split; kc < k1; ++kc, ++it) {
+          if (!wait_for(&sh.empty[s], ph, abort)) {
             ok = false;
             break;
           }
@@ -398,6 +434,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
               for (int j = 0; j < G::B_ROWS / 64; ++j)
                 load_box<CG>(pb + p * G::B_PLANE + j * 8192, &mapB, bar, n0 + 64 * j, kc * BK, p);
           }
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1;
+          }
         }
       }
       if (*abort && rank == 0) {  // copies in flight land before shared memory is given up
@@ -406,18 +446,26 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
       }
     }
     __syncwarp();
-  } else if (!dead && warp == 9) {
+  } else if (!dead && warp == EW + 1) {
     // ------------------------------------------------------ MMA issuer
-    if (lane == 0 && rank == 0) {
+    // The whole warp walks the loop, so that descriptors stay in uniform
+    // registers, where tcgen05.mma takes them, and one lane issues: moving
+    // them there for every product from one lane's registers cost 10% of the
+    // rate (8192^3: 823 against 720 us).
+    if (rank == 0) {
       constexpr uint32_t IDESC = (1u << 4) | (Elem<T>::FMT << 7) | (Elem<T>::FMT << 10) |
                                  ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) |
                                  ((uint32_t)(TN >> 3) << 17) |
                                  ((uint32_t)((128 * CG) >> 4) << 24);
       // a step of 16 contraction values: 32 bytes along a K-major line, 16
       // lines of an MN-major box
-      constexpr uint32_t STEP_A = A_MN ? 2048 : 32, STEP_B = B_MN ? 2048 : 32;
+      constexpr uint32_t STEP_A = (A_MN ? 2048 : 32) >> 4, STEP_B = (B_MN ? 2048 : 32) >> 4;
       constexpr uint32_t LBO = 8192;  // between 64-wide boxes of an MN-major operand
-      int it = 0, si = 0;
+      const uint64_t a0 = smem_desc_sw128(smem_u32(smem), LBO, 1024);
+      const uint64_t b0 = smem_desc_sw128(smem_u32(smem) + PL * A_PLANE, LBO, 1024);
+      const bool leader = elect_one();
+      int s = 0, si = 0;
+      uint32_t ph = 0;
       bool ok = true;
       for (int w = unit; ok && w < g.items; w += units) {
         const int split = w % g.splits;
@@ -425,68 +473,84 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         for (int kc = k0; ok && kc < k1;) {
           const int seg_end = PL == 3 ? min(k1, kc + G::SEG_CHUNKS) : k1;
           const int a = si & 1;
-          if (!wait_for(&sh.acce[a], ((unsigned)(si >> 1) & 1u) ^ 1u, abort)) {
-            ok = false;
-            break;
-          }
+          ok = __all_sync(0xffffffffu,
+                          wait_for(&sh.acce[a], ((unsigned)(si >> 1) & 1u) ^ 1u, abort));
+          if (!ok) break;
           tc_fence_after();
           const uint32_t d = tmem + (uint32_t)(a * G::ACC);
           uint32_t more = 0;
-          for (; kc < seg_end; ++kc, ++it) {
-            const int s = it % STAGES;
-            if (!wait_for(&sh.full[s], (unsigned)(it / STAGES) & 1u, abort)) {
-              ok = false;
-              break;
-            }
+          for (; kc < seg_end; ++kc) {
+            ok = __all_sync(0xffffffffu, wait_for(&sh.full[s], ph, abort));
+            if (!ok) break;
             tc_fence_after();
-            const uint32_t pa = smem_u32(smem + s * G::STAGE), pb = pa + PL * A_PLANE;
+            const uint64_t da = a0 + (uint64_t)(s * (G::STAGE >> 4));
+            const uint64_t db = b0 + (uint64_t)(s * (G::STAGE >> 4));
+            if (leader) {
 #pragma unroll
-            for (int kk = 0; kk < BK / 16; ++kk) {
-              uint64_t da[PL], db[PL];
-#pragma unroll
-              for (int p = 0; p < PL; ++p) {
-                da[p] = smem_desc_sw128(pa + p * A_PLANE + kk * STEP_A, LBO, 1024);
-                db[p] = smem_desc_sw128(pb + p * G::B_PLANE + kk * STEP_B, LBO, 1024);
+              for (int kk = 0; kk < BK / 16; ++kk) {
+                const uint64_t ka = da + kk * STEP_A, kb = db + kk * STEP_B;
+                const uint32_t acc = kk > 0 ? 1u : more;
+                mma_f16<CG>(d, ka, kb, IDESC, acc);
+                if (PL == 3) {
+                  constexpr uint32_t PA = A_PLANE >> 4, PB = G::B_PLANE >> 4;
+                  mma_f16<CG>(d + TN, ka, kb + 2 * PB, IDESC, acc);
+                  mma_f16<CG>(d + TN, ka + 2 * PA, kb, IDESC, 1);
+                  mma_f16<CG>(d + TN, ka + PA, kb + PB, IDESC, 1);
+                  mma_f16<CG>(d + TN, ka, kb + PB, IDESC, 1);
+                  mma_f16<CG>(d + TN, ka + PA, kb, IDESC, 1);
+                }
               }
-              mma_f16<CG>(d, da[0], db[0], IDESC, more);
-              if (PL == 3) {
-                mma_f16<CG>(d + TN, da[0], db[PL - 1], IDESC, more);
-                mma_f16<CG>(d + TN, da[PL - 1], db[0], IDESC, 1);
-                mma_f16<CG>(d + TN, da[PL / 2], db[PL / 2], IDESC, 1);
-                mma_f16<CG>(d + TN, da[0], db[PL / 2], IDESC, 1);
-                mma_f16<CG>(d + TN, da[PL / 2], db[0], IDESC, 1);
-              }
-              more = 1;
+              commit_to<CG>(&sh.empty[s]);
             }
-            commit_to<CG>(&sh.empty[s]);
+            __syncwarp();
+            more = 1;
+            if (++s == STAGES) {
+              s = 0;
+              ph ^= 1;
+            }
           }
           if (!ok) break;
-          commit_to<CG>(&sh.accf[a]);
+          if (leader) commit_to<CG>(&sh.accf[a]);
+          __syncwarp();
           ++si;
         }
       }
       // every MMA issued has finished before TMEM is released
-      if (CG == 2)
-        asm volatile(
-            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                smem_u32(&sh.mma_done))
-            : "memory");
-      else
-        mma_commit(&sh.mma_done);
+      if (leader) {
+        if (CG == 2)
+          asm volatile(
+              "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                  smem_u32(&sh.mma_done))
+              : "memory");
+        else
+          mma_commit(&sh.mma_done);
+      }
       wait_plain(&sh.mma_done, 0);
     }
     __syncwarp();
   } else if (!dead) {
     // -------------------------------------------------------- epilogue
-    const int quad = warp & 3, half = warp >> 2;
+    const int quad = warp & 3, share = warp >> 2;
     uint8_t* stg = stg_base + warp * Elem<T>::STG;
+    T* bias_s = reinterpret_cast<T*>(sh.bias) + 32 * warp;
     const uint32_t lanes = tmem + ((uint32_t)(32 * quad) << 16);
-    int si = 0, use = 0;
+    int si = 0;
     bool ok = true;
     for (int w = unit; ok && w < g.items; w += units) {
-      const int tile = w / g.splits, split = w - tile * g.splits;
-      const int m0 = (tile / g.tiles_n) * 128 * CG + rank * 128 + 32 * quad;
-      const int n0 = (tile % g.tiles_n) * TN + half * (TN / 2);
+      const TileAt t = tile_at(w, g);
+      const int split = t.split;
+      const int m0 = t.m * 128 * CG + rank * 128 + 32 * quad;
+      const int n0 = t.n * TN + share * G::COLS;
+      // what the epilogue adds is fetched while the products run
+      T bias[NP];
+#pragma unroll
+      for (int c = 0; c < NP; ++c) {
+        const int n = n0 + 32 * c + lane;
+        bias[c] = g.bias && n < g.N ? g.bias[n] : from_f<T>(0.f);
+        if (g.res && m0 + lane < g.M && n0 + 32 * c < g.N)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(g.res + (size_t)(m0 + lane) * g.ldr + n0 +
+                                                        32 * c));
+      }
       if (PL == 1) {
         const int a = si & 1;
         if (!wait_for(&sh.accf[a], (unsigned)(si >> 1) & 1u, abort)) {
@@ -494,10 +558,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         }
         ++si;
         tc_fence_after();
-#pragma unroll 1
+#pragma unroll
         for (int c = 0; c < NP; ++c) {
           float v[32];
-          tmem_ld32(lanes + (uint32_t)(a * G::ACC + half * (TN / 2) + 32 * c), v);
+          tmem_ld32(lanes + (uint32_t)(a * G::ACC + share * G::COLS + 32 * c), v);
           if (c == NP - 1) {
             tc_fence_before();
             __syncwarp();
@@ -506,7 +570,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
               else mbar_arrive(&sh.acce[a]);
             }
           }
-          finish_piece<T>(v, m0, n0 + 32 * c, g, sh.bias[warp], stg, &mapY, &mapZ, lane, use,
+          finish_piece<T>(v, m0, n0 + 32 * c, g, bias[c], bias_s, stg, &mapY, &mapZ, lane,
                           split);
         }
       } else {
@@ -526,7 +590,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
 #pragma unroll
           for (int c = 0; c < NP; ++c) {
             float big[32], small[32];
-            const uint32_t col = lanes + (uint32_t)(a * G::ACC + half * (TN / 2) + 32 * c);
+            const uint32_t col = lanes + (uint32_t)(a * G::ACC + share * G::COLS + 32 * c);
             tmem_ld32(col, big);
             tmem_ld32(col + TN, small);
 #pragma unroll
@@ -542,7 +606,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         if (!ok) break;
 #pragma unroll
         for (int c = 0; c < NP; ++c)
-          finish_piece<T>(acc[c], m0, n0 + 32 * c, g, sh.bias[warp], stg, &mapY, &mapZ, lane, use,
+          finish_piece<T>(acc[c], m0, n0 + 32 * c, g, bias[c], bias_s, stg, &mapY, &mapZ, lane,
                           split);
       }
     }
@@ -554,7 +618,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
   __syncthreads();
   if (CG == 2) cluster_sync_all();
   tc_fence_after();
-  if (warp == 9) free_tmem<CG>(tmem, 2 * G::ACC);
+  if (warp == EW + 1) free_tmem<CG>(tmem, 2 * G::ACC);
   if (CG == 2) cluster_sync_all();
 }
 
@@ -622,12 +686,13 @@ int gemm_launch(const GemmProblem& p, const GemmPlan& plan, cudaStream_t st) {
   GemmArgs<T> g;
   g.M = p.M;
   g.N = p.N;
+  g.K = p.K;
   g.nK = (p.K + BK - 1) / BK;
+  g.tiles_m = (p.M + 128 * CG - 1) / (128 * CG);
   g.tiles_n = (p.N + TN - 1) / TN;
   g.per_split = (g.nK + plan.splits - 1) / plan.splits;
   g.splits = (g.nK + g.per_split - 1) / g.per_split;
-  const long long items =
-      (long long)((p.M + 128 * CG - 1) / (128 * CG)) * g.tiles_n * g.splits;
+  const long long items = (long long)g.tiles_m * g.tiles_n * g.splits;
   if (items > 0x7fffffff / 2) return set_error(kUnsupported, "tw_linear: too many tiles");
   g.items = (int)items;
   g.bias = (const T*)p.bias;
@@ -651,7 +716,7 @@ int gemm_launch(const GemmProblem& p, const GemmPlan& plan, cudaStream_t st) {
   const int most = 148 / CG;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(CG * (g.items < most ? g.items : most)));
-  cfg.blockDim = dim3(GEMM_THREADS);
+  cfg.blockDim = dim3(G::THREADS);
   cfg.dynamicSmemBytes = G::SMEM;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
