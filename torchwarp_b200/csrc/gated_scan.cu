@@ -10,14 +10,14 @@
 // there are 0, its gradients 0, and x and g are not read.
 //
 // One pass over the data.  The channels of all sequences, c = b D + d, are
-// numbered through; a block owns 32 (or 64 of 16 bits, as pairs) of them and
-// walks time in tiles of 8 warps x 16 frames.  A thread reads its 16 frames
-// into registers, composes them to (A, B) with h_out = A h_in + B, learns its
-// h_in from the warps before it, and runs its frames again from the registers
-// to write the outputs.  Few channels: up to 8 blocks of a cluster take
-// neighbouring tiles and compose their (A, B) through each other's shared
-// memory, so that a long sequence still fills the GPU.  Everything is summed
-// in a fixed order.
+// numbered through; a block of 128 threads owns 32 (or 16) lanes of them,
+// pairs in 16 bits, and walks time in tiles of 4 (or 8) runs x 16 frames.  A
+// thread reads its 16 frames into registers, composes them to (A, B) with
+// h_out = A h_in + B, learns its h_in from the runs before it, and goes over
+// its frames again in registers to write the outputs.  Few channels: up to 8
+// blocks of a cluster take neighbouring tiles and compose their (A, B) through
+// each other's shared memory, so that a long sequence still fills the GPU.
+// Everything is summed in a fixed order.
 //
 // The forward saves h before every 16th frame in float32 (0.25 bytes a value);
 // the backward recomputes the states of a thread's frames from it, so no
@@ -29,9 +29,9 @@ namespace tw {
 namespace {
 
 constexpr int SCAN_FRAMES = 16;  // of a thread
-constexpr int SCAN_WARPS = 8;
-constexpr int SCAN_TILE = SCAN_FRAMES * SCAN_WARPS;
-constexpr int SCAN_THREADS = 32 * SCAN_WARPS;
+constexpr int SCAN_THREADS = 128;
+// LPR lanes a frame: 128 / LPR runs of 16 frames a tile.
+constexpr int tile_of(int lpr) { return SCAN_THREADS / lpr * SCAN_FRAMES; }
 
 __device__ __forceinline__ int live_len(const int64_t* lengths, int b, int T) {
   if (!lengths) return T;
@@ -185,36 +185,38 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <int VC> struct ScanShared {
-  float a[2][SCAN_WARPS][32 * VC], b[2][SCAN_WARPS][32 * VC];  // of the warps' frames
-  float tile_a[2][32 * VC], tile_b[2][32 * VC];                // of the block's tile
-  float start[2][32 * VC];                                     // before the tile
+template <int VC, int LPR> struct ScanShared {
+  static constexpr int RUNS = SCAN_THREADS / LPR, CH = LPR * VC;
+  float a[2][RUNS][CH], b[2][RUNS][CH];  // of the runs
+  float tile_a[2][CH], tile_b[2][CH];    // of the block's tile
+  float start[2][CH];                    // before the tile
 };
 
-// Composes the warps' (A, B) of step `it` and returns what enters this
-// thread's frames; REV: time runs from the last warp and the last block of
-// the cluster.  `run` is what enters the cluster's tiles, kept by warp 0.
+// Composes the runs' (A, B) of step `it` and returns what enters this
+// thread's frames; REV: time goes from the last run and the last block of the
+// cluster.  `run` is what enters the cluster's tiles, kept by run 0's threads.
 // One block barrier a step when S is 1 (the buffers alternate), else one of
 // the cluster and one more of the block.
-template <int VC, bool REV>
-__device__ __forceinline__ void compose(ScanShared<VC>& sh, int it, int S, int rank, int warp,
+template <int VC, int LPR, bool REV>
+__device__ __forceinline__ void compose(ScanShared<VC, LPR>& sh, int it, int S, int rank, int part,
                                         int lane, Vec<VC> A, Vec<VC> B, Vec<VC>& run,
                                         Vec<VC>& enter) {
+  constexpr int RUNS = ScanShared<VC, LPR>::RUNS;
   const int p = it & 1;
 #pragma unroll
   for (int v = 0; v < VC; ++v) {
-    sh.a[p][warp][lane * VC + v] = A.v[v];
-    sh.b[p][warp][lane * VC + v] = B.v[v];
+    sh.a[p][part][lane * VC + v] = A.v[v];
+    sh.b[p][part][lane * VC + v] = B.v[v];
   }
   __syncthreads();
   if (S > 1) {
-    if (warp == 0) {
+    if (part == 0) {
 #pragma unroll
       for (int v = 0; v < VC; ++v) {
         float ta = 1.f, tb = 0.f;
 #pragma unroll
-        for (int i = 0; i < SCAN_WARPS; ++i) {
-          const int w = REV ? SCAN_WARPS - 1 - i : i;
+        for (int i = 0; i < RUNS; ++i) {
+          const int w = REV ? RUNS - 1 - i : i;
           const float wa = sh.a[p][w][lane * VC + v];
           tb = fmaf(wa, tb, sh.b[p][w][lane * VC + v]);
           ta *= wa;
@@ -224,15 +226,24 @@ __device__ __forceinline__ void compose(ScanShared<VC>& sh, int it, int S, int r
       }
     }
     cluster_sync_all();
-    if (warp == 0) {
+    if (part == 0) {
 #pragma unroll
       for (int v = 0; v < VC; ++v) {
+        float ta[8], tb[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r < S) {
+            ta[r] = peer_read(&sh.tile_a[p][lane * VC + v], r);
+            tb[r] = peer_read(&sh.tile_b[p][lane * VC + v], r);
+          }
         float h = run.v[v];
-        for (int i = 0; i < S; ++i) {
-          const int r = REV ? S - 1 - i : i;
-          if (r == rank) sh.start[p][lane * VC + v] = h;
-          h = fmaf(peer_read(&sh.tile_a[p][lane * VC + v], r), h,
-                   peer_read(&sh.tile_b[p][lane * VC + v], r));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = REV ? 7 - i : i;
+          if (r < S) {
+            if (r == rank) sh.start[p][lane * VC + v] = h;
+            h = fmaf(ta[r], h, tb[r]);
+          }
         }
         run.v[v] = h;
       }
@@ -243,9 +254,9 @@ __device__ __forceinline__ void compose(ScanShared<VC>& sh, int it, int S, int r
   for (int v = 0; v < VC; ++v) {
     float h = sh.start[p][lane * VC + v];
 #pragma unroll
-    for (int i = 0; i < SCAN_WARPS; ++i) {
-      const int w = REV ? SCAN_WARPS - 1 - i : i;
-      if (REV ? w > warp : w < warp)
+    for (int i = 0; i < RUNS; ++i) {
+      const int w = REV ? RUNS - 1 - i : i;
+      if (REV ? w > part : w < part)
         h = fmaf(sh.a[p][w][lane * VC + v], h, sh.b[p][w][lane * VC + v]);
     }
     enter.v[v] = h;
@@ -267,16 +278,17 @@ struct Channel {
   }
 };
 
-template <typename T, int VC>
-__global__ void __launch_bounds__(SCAN_THREADS, 2)
+template <typename T, int VC, int LPR>
+__global__ void __launch_bounds__(SCAN_THREADS, 4)
     scan_fwd_kernel(const T* __restrict__ x, size_t xb, size_t xt, const T* __restrict__ g,
                     size_t gb, size_t gt, const float* __restrict__ h0,
                     const int64_t* __restrict__ lengths, size_t BD, int TT, int D, int S,
                     T* __restrict__ y, float* __restrict__ state, float* __restrict__ carry) {
-  __shared__ ScanShared<VC> sh;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int TILE = tile_of(LPR);
+  __shared__ ScanShared<VC, LPR> sh;
+  const int part = threadIdx.x / LPR, lane = threadIdx.x & (LPR - 1);
   const int rank = blockIdx.x % S;
-  const Channel ch((size_t)(blockIdx.x / S) * (32 * VC), lane, VC, BD, D, TT, lengths);
+  const Channel ch((size_t)(blockIdx.x / S) * (LPR * VC), lane, VC, BD, D, TT, lengths);
   const char* xp = reinterpret_cast<const char*>(x + ch.b * xb + ch.d);
   const char* gp = reinterpret_cast<const char*>(g + ch.b * gb + ch.d);
   char* yp = reinterpret_cast<char*>(y + ch.b * (size_t)TT * D + ch.d);
@@ -285,14 +297,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2)
 #pragma unroll
   for (int v = 0; v < VC; ++v) {
     run.v[v] = ch.live && h0 ? h0[ch.c + v] : 0.f;
-    if (warp == 0) sh.start[0][lane * VC + v] = run.v[v];
+    if (part == 0) sh.start[0][lane * VC + v] = run.v[v];
   }
-  const int steps = (TT + SCAN_TILE * S - 1) / (SCAN_TILE * S);
-  int t0 = rank * SCAN_TILE + warp * SCAN_FRAMES;
+  const int steps = (TT + TILE * S - 1) / (TILE * S);
+  int t0 = rank * TILE + part * SCAN_FRAMES;
   Frame<T, VC> xr[SCAN_FRAMES], gr[SCAN_FRAMES];
   load_frames<T, VC>(gr, gp + (size_t)t0 * gs, gs, ch.L - t0);
   load_frames<T, VC>(xr, xp + (size_t)t0 * xs, xs, ch.L - t0);
-  for (int it = 0; it < steps; ++it, t0 += SCAN_TILE * S) {
+  for (int it = 0; it < steps; ++it, t0 += TILE * S) {
     const int n = ch.L - t0;
     Vec<VC> s[SCAN_FRAMES], xv[SCAN_FRAMES];
 #pragma unroll
@@ -305,7 +317,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2)
       for (int k = 0; k < SCAN_FRAMES; ++k)
         if (k >= n) s[k] = splat<VC>(0.f);
     // the next tile's loads are under way while the blocks wait for each other
-    const int t1 = t0 + SCAN_TILE * S;
+    const int t1 = t0 + TILE * S;
     load_frames<T, VC>(gr, gp + (size_t)t1 * gs, gs, ch.L - t1);
     load_frames<T, VC>(xr, xp + (size_t)t1 * xs, xs, ch.L - t1);
     Vec<VC> A = splat<VC>(1.f), B = splat<VC>(0.f), h;
@@ -314,7 +326,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2)
       B = advance(s[k], B, xv[k]);
       A = decay(negated(s[k]), s[k], A);
     }
-    compose<VC, false>(sh, it, S, rank, warp, lane, A, B, run, h);
+    compose<VC, LPR, false>(sh, it, S, rank, part, lane, A, B, run, h);
     if (carry && ch.live && t0 < TT)
 #pragma unroll
       for (int v = 0; v < VC; ++v)
@@ -334,12 +346,12 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2)
           *reinterpret_cast<Frame<T, VC>*>(o) = k < n ? Frame<T, VC>::of(h) : Frame<T, VC>::zero();
       }
     }
-    if (S == 1 && warp == SCAN_WARPS - 1)
+    if (S == 1 && part == SCAN_THREADS / LPR - 1)
 #pragma unroll
       for (int v = 0; v < VC; ++v) sh.start[(it + 1) & 1][lane * VC + v] = h.v[v];
   }
   __syncthreads();
-  if (ch.live && warp == 0 && rank == 0)
+  if (ch.live && part == 0 && rank == 0)
 #pragma unroll
     for (int v = 0; v < VC; ++v)
       state[ch.c + v] = S > 1 ? run.v[v] : sh.start[steps & 1][lane * VC + v];
@@ -349,8 +361,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2)
 // The same walk from the end.  Pairs of 16 bits load a tile when its turn
 // comes (its registers leave no room for the next one's); single channels
 // load a tile ahead.
-template <typename T, int VC>
-__global__ void __launch_bounds__(SCAN_THREADS, 2)
+template <typename T, int VC, int LPR>
+__global__ void __launch_bounds__(SCAN_THREADS, 4)
     scan_bwd_kernel(const T* __restrict__ dy, size_t yb, size_t yt,
                     const float* __restrict__ dstate, const T* __restrict__ x, size_t xb,
                     size_t xt, const T* __restrict__ g, size_t gb, size_t gt,
@@ -358,10 +370,11 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2)
                     size_t BD, int TT, int D, int S, T* __restrict__ dx, T* __restrict__ dg,
                     float* __restrict__ dh0) {
   constexpr bool AHEAD = VC == 1;
-  __shared__ ScanShared<VC> sh;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int TILE = tile_of(LPR);
+  __shared__ ScanShared<VC, LPR> sh;
+  const int part = threadIdx.x / LPR, lane = threadIdx.x & (LPR - 1);
   const int rank = blockIdx.x % S;
-  const Channel ch((size_t)(blockIdx.x / S) * (32 * VC), lane, VC, BD, D, TT, lengths);
+  const Channel ch((size_t)(blockIdx.x / S) * (LPR * VC), lane, VC, BD, D, TT, lengths);
   const char* xp = reinterpret_cast<const char*>(x + ch.b * xb + ch.d);
   const char* gp = reinterpret_cast<const char*>(g + ch.b * gb + ch.d);
   const char* yp = reinterpret_cast<const char*>(dy + ch.b * yb + ch.d);
@@ -372,10 +385,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2)
 #pragma unroll
   for (int v = 0; v < VC; ++v) {
     run.v[v] = ch.live && dstate ? dstate[ch.c + v] : 0.f;
-    if (warp == 0) sh.start[0][lane * VC + v] = run.v[v];
+    if (part == 0) sh.start[0][lane * VC + v] = run.v[v];
   }
-  const int steps = (TT + SCAN_TILE * S - 1) / (SCAN_TILE * S);
-  int t0 = ((steps - 1) * S + rank) * SCAN_TILE + warp * SCAN_FRAMES;
+  const int steps = (TT + TILE * S - 1) / (TILE * S);
+  int t0 = ((steps - 1) * S + rank) * TILE + part * SCAN_FRAMES;
   Frame<T, VC> xr[SCAN_FRAMES], gr[SCAN_FRAMES], yr[SCAN_FRAMES];
   Vec<VC> hr;
   auto load = [&](int t) {
@@ -389,7 +402,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2)
       hr.v[v] = n > 0 ? carry[(tt / SCAN_FRAMES) * BD + ch.c + v] : 0.f;
   };
   if (AHEAD) load(t0);
-  for (int it = 0; it < steps; ++it, t0 -= SCAN_TILE * S) {
+  for (int it = 0; it < steps; ++it, t0 -= TILE * S) {
     const int n = ch.L - t0;
     if (!AHEAD) load(t0);
     Vec<VC> s[SCAN_FRAMES], diff[SCAN_FRAMES];  // the gates; h_{t-1} - x_t
@@ -408,7 +421,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2)
       diff[k] = sub_v(h, xr[k].get());
       h = fma_v(negated(s[k]), diff[k], pick(s[k], h, xr[k].get()));
     }
-    if (AHEAD) load(t0 - SCAN_TILE * S);
+    if (AHEAD) load(t0 - TILE * S);
     Vec<VC> A = splat<VC>(1.f), B = splat<VC>(0.f);
 #pragma unroll
     for (int k = SCAN_FRAMES - 1; k >= 0; --k) {
@@ -416,7 +429,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2)
       B = decay(ns, s[k], add_v(AHEAD ? yv[k] : yr[k].get(), B));
       A = decay(ns, s[k], A);
     }
-    compose<VC, true>(sh, it, S, rank, warp, lane, A, B, run, lam);
+    compose<VC, LPR, true>(sh, it, S, rank, part, lane, A, B, run, lam);
     const size_t last = (at + (size_t)(t0 + SCAN_FRAMES - 1) * D) * sizeof(T);
     char* ox = reinterpret_cast<char*>(dx) + last;
     char* og = reinterpret_cast<char*>(dg) + last;
@@ -434,12 +447,12 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2)
         *reinterpret_cast<Frame<T, VC>*>(og) = k < n ? vg : Frame<T, VC>::zero();
       }
     }
-    if (S == 1 && warp == 0)
+    if (S == 1 && part == 0)
 #pragma unroll
       for (int v = 0; v < VC; ++v) sh.start[(it + 1) & 1][lane * VC + v] = lam.v[v];
   }
   __syncthreads();
-  if (ch.live && dh0 && warp == 0 && rank == 0)
+  if (ch.live && dh0 && part == 0 && rank == 0)
 #pragma unroll
     for (int v = 0; v < VC; ++v)
       dh0[ch.c + v] = S > 1 ? run.v[v] : sh.start[steps & 1][lane * VC + v];
@@ -463,7 +476,7 @@ int check(const char* who, int B, int TT, int D) {
   if (B < 0 || TT < 0 || D <= 0)
     return set_error(kInvalid, "%s: invalid sizes B=%d T=%d D=%d (need B, T >= 0, D > 0)", who, B,
                      TT, D);
-  if ((size_t)B * D / 32 >= 0x7fffffffu / 8 || TT > 0x7fffffff - 8 * SCAN_TILE)
+  if ((size_t)B * D / 16 >= 0x7fffffffu / 8 || TT > 0x7fffffff - 8 * 256)
     return set_error(kUnsupported, "%s: sizes too large", who);
   return kOk;
 }
@@ -478,12 +491,23 @@ unsigned grid_of(int B, int D) {
   return (unsigned)(((size_t)B * D + SCAN_THREADS - 1) / SCAN_THREADS);
 }
 
-// Blocks that share the time of their channels: as many as three blocks a SM
-// leave room for, and no more than there are tiles.
-int time_blocks(size_t groups, int TT) {
-  int S = 8;
-  while (S > 1 && (groups * S > 148 * 3 || (long long)(S / 2) * SCAN_TILE >= TT)) S /= 2;
-  return S;
+// How the channels and the time of a call are spread over blocks.  Whole
+// 128-byte (pairs, float) or 64-byte lines a frame while that gives the SMs
+// three blocks each; else more blocks take part of the time, as many as there
+// are tiles; else half lines.
+struct ScanPlan {
+  int lpr, S;
+  size_t groups;
+};
+ScanPlan scan_plan(size_t BD, int vc, int TT) {
+  ScanPlan p = {32, 1, 0};
+  for (;;) {
+    p.groups = (BD + p.lpr * vc - 1) / (p.lpr * vc);
+    p.S = 1;
+    while (p.S < 8 && p.groups * p.S < 148 * 3 && (long long)p.S * tile_of(p.lpr) < TT) p.S *= 2;
+    if (p.lpr == 16 || p.groups * p.S >= 148 * 3) return p;
+    p.lpr = 16;
+  }
 }
 
 template <typename... Params, typename... Args>
@@ -524,15 +548,15 @@ int fwd(const void* x, size_t xb, size_t xt, const void* g, size_t gb, size_t gt
   const size_t BD = (size_t)B * D;
   if constexpr (sizeof(T) == 2) if (D % 2 == 0 && pairs_ok(x, xb, xt) && pairs_ok(g, gb, gt) &&
                                     pairs_ok(y, 0, 0)) {
-    const size_t groups = (BD + 63) / 64;
-    const int S = time_blocks(groups, TT);
-    return launch(who, scan_fwd_kernel<T, 2>, groups, S, stream, (const T*)x, xb, xt, (const T*)g,
-                  gb, gt, h0, lengths, BD, TT, D, S, (T*)y, state, (float*)carry);
+    const ScanPlan p = scan_plan(BD, 2, TT);
+    return launch(who, p.lpr == 32 ? scan_fwd_kernel<T, 2, 32> : scan_fwd_kernel<T, 2, 16>,
+                  p.groups, p.S, stream, (const T*)x, xb, xt, (const T*)g,
+                  gb, gt, h0, lengths, BD, TT, D, p.S, (T*)y, state, (float*)carry);
   }
-  const size_t groups = (BD + 31) / 32;
-  const int S = time_blocks(groups, TT);
-  return launch(who, scan_fwd_kernel<T, 1>, groups, S, stream, (const T*)x, xb, xt, (const T*)g,
-                gb, gt, h0, lengths, BD, TT, D, S, (T*)y, state, (float*)carry);
+  const ScanPlan p = scan_plan(BD, 1, TT);
+  return launch(who, p.lpr == 32 ? scan_fwd_kernel<T, 1, 32> : scan_fwd_kernel<T, 1, 16>, p.groups,
+                p.S, stream, (const T*)x, xb, xt, (const T*)g,
+                gb, gt, h0, lengths, BD, TT, D, p.S, (T*)y, state, (float*)carry);
 }
 
 template <typename T>
@@ -552,17 +576,17 @@ int bwd(const void* dy, size_t yb, size_t yt, const float* dstate, const void* x
   if constexpr (sizeof(T) == 2) if (D % 2 == 0 && pairs_ok(x, xb, xt) && pairs_ok(g, gb, gt) &&
                                     pairs_ok(dy, yb, yt) && pairs_ok(dx, 0, 0) &&
                                     pairs_ok(dg, 0, 0)) {
-    const size_t groups = (BD + 63) / 64;
-    const int S = time_blocks(groups, TT);
-    return launch(who, scan_bwd_kernel<T, 2>, groups, S, stream, (const T*)dy, yb, yt, dstate,
+    const ScanPlan p = scan_plan(BD, 2, TT);
+    return launch(who, p.lpr == 32 ? scan_bwd_kernel<T, 2, 32> : scan_bwd_kernel<T, 2, 16>,
+                  p.groups, p.S, stream, (const T*)dy, yb, yt, dstate,
                   (const T*)x, xb, xt, (const T*)g, gb, gt, lengths, (const float*)carry, BD, TT,
-                  D, S, (T*)dx, (T*)dg, dh0);
+                  D, p.S, (T*)dx, (T*)dg, dh0);
   }
-  const size_t groups = (BD + 31) / 32;
-  const int S = time_blocks(groups, TT);
-  return launch(who, scan_bwd_kernel<T, 1>, groups, S, stream, (const T*)dy, yb, yt, dstate,
+  const ScanPlan p = scan_plan(BD, 1, TT);
+  return launch(who, p.lpr == 32 ? scan_bwd_kernel<T, 1, 32> : scan_bwd_kernel<T, 1, 16>, p.groups,
+                p.S, stream, (const T*)dy, yb, yt, dstate,
                 (const T*)x, xb, xt, (const T*)g, gb, gt, lengths, (const float*)carry, BD, TT, D,
-                S, (T*)dx, (T*)dg, dh0);
+                p.S, (T*)dx, (T*)dg, dh0);
 }
 
 template <typename T>
