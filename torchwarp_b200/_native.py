@@ -7,6 +7,7 @@ CUDA stream into the ``void* stream`` argument.
 """
 
 import ctypes
+import importlib.util
 from pathlib import Path
 
 import torch
@@ -174,34 +175,24 @@ def require_cuda(*tensors):
                 "There is no CPU fallback.".format(t.device))
 
 
-_SUFFIX16 = {torch.float32: "f32", torch.bfloat16: "bf16", torch.float16: "f16"}
-_ENTRIES = {}
+_HOST = None
 
 
-def entry(name, dtype):
-    """The C entry of an encoder operator for an element type."""
-    fn = _ENTRIES.get((name, dtype))
-    if fn is None:
-        suffix = _SUFFIX16.get(dtype)
-        if suffix is None:
-            raise TypeError("the encoder operators take float32, bfloat16 or float16, got "
-                            "{}".format(dtype))
-        fn = _ENTRIES[name, dtype] = getattr(lib(), name + "_" + suffix)
-    return fn
-
-
-def launch(name, fn, device, *args):
-    """Calls ``fn(*args, stream)`` with `device` current and its current stream, and checks the
-    status.  Pointers are plain integers (``data_ptr()``): this is the path of calls whose time is
-    the host's."""
-    index = device.index
-    if index != torch._C._cuda_getDevice():
-        with torch.cuda.device(index):
-            return launch(name, fn, device, *args)
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    status = fn(*args, stream) if _RECORDER is None else call(name, fn, *args, stream)
-    if status != 0:
-        check(status, "tw_" + name)
+def host():
+    """The host extension of the encoder operators (loaded once; built with the library)."""
+    global _HOST
+    if _HOST is None:
+        path = LIB_PATH.with_name("_encoder_host.so")
+        if not path.exists():
+            raise RuntimeError(
+                "torchwarp_b200: host extension {} is missing; build it with "
+                "`python -m torchwarp_b200.build`".format(path))
+        lib()
+        spec = importlib.util.spec_from_file_location("_encoder_host", str(path))
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _HOST = module
+    return _HOST
 
 
 # ------------------------------------------------------------ launch timing

@@ -6,7 +6,10 @@
 Each ``csrc/*.cu`` is compiled to an object with
 ``nvcc -gencode arch=compute_100a,code=sm_100a -O3 -lineinfo`` and the
 objects are linked into ``torchwarp_b200/_lib/libtorchwarp_b200.so``.  The
-library depends only on the CUDA runtime.
+library depends only on the CUDA runtime.  ``csrc/host/encoder_host.cpp`` (eager
+calls of the encoder operators: checks, allocation, autograd) becomes the
+Python extension ``_lib/_encoder_host.so`` with g++; it needs torch's headers
+and calls the library through its C ABI.
 """
 
 import argparse
@@ -23,6 +26,8 @@ OUT_DIR = PKG / "_lib"
 LIB = OUT_DIR / "libtorchwarp_b200.so"
 OBJ_DIR = PKG.parent / "_build" / "obj"
 ROOT = PKG.parent
+HOST_SRC = CSRC / "host" / "encoder_host.cpp"
+HOST_LIB = OUT_DIR / "_encoder_host.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -52,6 +57,31 @@ def _compile(src, force):
     return obj, None
 
 
+def _build_host(force):
+    """The host extension; returns an error text or None."""
+    deps = [HOST_SRC, ROOT / "include" / "torchwarp_b200.h"]
+    if not force and HOST_LIB.exists() and \
+            HOST_LIB.stat().st_mtime >= max(d.stat().st_mtime for d in deps):
+        return None
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = Path(nvcc()).resolve().parents[1]
+    includes = [*cpp_extension.include_paths(), str(cuda / "include"),
+                sysconfig.get_paths()["include"]]
+    torch_lib = str(Path(torch.__file__).parent / "lib")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           "-DTORCH_EXTENSION_NAME=_encoder_host",
+           "-D_GLIBCXX_USE_CXX11_ABI={:d}".format(torch.compiled_with_cxx11_abi()),
+           *(a for i in includes for a in ("-isystem", i)), str(HOST_SRC), "-o", str(HOST_LIB),
+           "-L", str(OUT_DIR), "-l:" + LIB.name, "-L", torch_lib, "-lc10", "-lc10_cuda",
+           "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    return None if r.returncode == 0 else "{}\n{}{}".format(" ".join(cmd), r.stdout, r.stderr)
+
+
 def build(force=False, verbose=False):
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
     OUT_DIR.mkdir(parents=True, exist_ok=True)
@@ -70,6 +100,9 @@ def build(force=False, verbose=False):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("link failed:\n{}{}".format(r.stdout, r.stderr))
+    error = _build_host(force)
+    if error:
+        raise RuntimeError("host extension failed:\n" + error)
     if verbose:
         print("built", LIB)
     return LIB

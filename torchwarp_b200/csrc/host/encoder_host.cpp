@@ -1,0 +1,592 @@
+// Eager calls of the encoder operators: argument checks, allocation, autograd
+// and the calls of the C ABI in one C++ module.
+//
+// A call on a few rows takes less time on the GPU than its host side takes in
+// Python (layer norm of 4 rows: 2 us against 12; its training pass 107), so
+// the host side is C++: one conversion of the arguments, no interpreter in
+// the backward.  Backward passes are first order: their results carry a node
+// that raises when it is differentiated.
+#include <ATen/autocast_mode.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/extension.h>
+
+#include <optional>
+#include <string>
+#include <vector>
+
+#include "../../../include/torchwarp_b200.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<Tensor>;
+
+// A C ABI call's failure; Python sees torchwarp_b200._native.NativeError.
+struct NativeError : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+
+void check_status(int status, const char* what) {
+  if (status != TW_OK)
+    throw NativeError(std::string(what) + " failed (status " + std::to_string(status) +
+                      "): " + tw_last_error());
+}
+
+std::string shape_of(const Tensor& t) {
+  std::string s = "[";
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+  return s + "]";
+}
+
+std::string type_of(at::ScalarType t) {
+  std::string s = at::toString(t);
+  return t == at::kFloat ? "float32" : t == at::kBFloat16 ? "bfloat16" : t == at::kHalf ? "float16" : s;
+}
+
+[[noreturn]] void bad_value(const std::string& msg) { throw py::value_error(msg); }
+[[noreturn]] void bad_type(const std::string& msg) { throw py::type_error(msg); }
+
+bool supported(at::ScalarType t) {
+  return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf;
+}
+void check_type(const char* name, const Tensor& t) {
+  if (!supported(t.scalar_type()))
+    bad_type(std::string(name) + " must be float32, bfloat16 or float16, got " +
+             type_of(t.scalar_type()));
+}
+void check_same_type(const char* name, const Tensor& t, const Tensor& x) {
+  if (t.scalar_type() != x.scalar_type())
+    bad_type(std::string(name) + " must be of x's type " + type_of(x.scalar_type()) + ", got " +
+             type_of(t.scalar_type()));
+}
+void require_cuda(const Tensor& t) {
+  if (!t.is_cuda())
+    throw std::runtime_error("torchwarp_b200 runs only on CUDA tensors (B200, sm_100a); got a "
+                             "tensor on " + t.device().str() + ". There is no CPU fallback.");
+}
+void check_device(const Tensor& first, const Tensor& t) {
+  if (!t.defined()) return;
+  require_cuda(t);
+  if (t.device() != first.device())
+    bad_value("all tensors must be on one device, got " + first.device().str() + " and " +
+              t.device().str());
+}
+
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+Tensor dense_like(const Tensor& x) { return at::empty(x.sizes(), x.options()); }
+
+Tensor bytes(size_t n, const Tensor& like) {
+  return n ? at::empty({(int64_t)n}, like.options().dtype(at::kByte)) : Tensor();
+}
+
+// x with its last dimension contiguous and its leading ones collapsed to rows
+// `stride` elements apart: itself or a view where that is possible, else a
+// copy.
+struct Rows {
+  Tensor t;
+  int64_t stride;
+};
+Rows rows_of(const Tensor& x) {
+  if (x.is_contiguous()) return {x, x.size(-1)};
+  Tensor r = x.reshape({-1, x.size(-1)});
+  if (r.stride(1) != 1 && r.size(1) != 1) r = r.contiguous();
+  return {r, r.stride(0)};
+}
+Tensor frames_of(const Tensor& x) {
+  return x.stride(2) == 1 || x.size(2) == 1 ? x : x.contiguous();
+}
+
+// Optional arguments are undefined tensors here, but std::optional where
+// autograd sees them: an autograd Function counts only the tensors it is given.
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+Tensor def(const OptTensor& t) { return t.value_or(Tensor()); }
+
+// The entry of the element type.
+#define TW_PICK(NAME, TYPE)                                                        \
+  ((TYPE) == at::kFloat ? NAME##_f32 : (TYPE) == at::kBFloat16 ? NAME##_bf16 : NAME##_f16)
+
+void* stream_of(const Tensor& t) {
+  return (void*)c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
+}
+
+// Results of a first-order backward: under create_graph they stay tied to a
+// node that raises when a second derivative reaches it.
+variable_list first_order(variable_list out) {
+  if (!at::GradMode::is_enabled()) return out;
+  std::vector<size_t> at;
+  variable_list in;
+  for (size_t i = 0; i < out.size(); ++i)
+    if (out[i].defined()) {
+      at.push_back(i);
+      in.push_back(out[i].detach().requires_grad_(true));
+    }
+  auto node = std::make_shared<torch::autograd::DelayedError>(
+      "trying to differentiate twice a function that was marked once-differentiable "
+      "(a first-order native backward)", (int64_t)in.size());
+  variable_list tied = (*node)(std::move(in));
+  for (size_t i = 0; i < at.size(); ++i) out[at[i]] = tied[i];
+  return out;
+}
+
+// -------------------------------------------------------------- layer norm
+
+std::tuple<Tensor, Tensor> layer_norm_forward(const Tensor& x, const Tensor& w, const Tensor& b,
+                                              double eps, bool save) {
+  const int64_t d = x.size(-1), rows = x.numel() / d;
+  Tensor y = dense_like(x);
+  Tensor stats = save ? at::empty({2, rows}, x.options().dtype(at::kFloat)) : Tensor();
+  if (rows) {
+    c10::cuda::CUDAGuard guard(x.device());
+    const Rows r = rows_of(x);
+    const Tensor& param = w.defined() ? w : b;
+    float* mean = save ? stats.data_ptr<float>() : nullptr;
+    check_status(TW_PICK(tw_layer_norm_forward, x.scalar_type())(
+                     ptr(r.t), r.stride, ptr(w), ptr(b),
+                     param.defined() && param.scalar_type() != x.scalar_type(), rows, (int)d, eps,
+                     ptr(y), mean, save ? mean + rows : nullptr, stream_of(x)),
+                 "tw_layer_norm_forward");
+  }
+  return {y, stats};
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& dy_in, const Tensor& x,
+                                                       const Tensor& w, at::ScalarType ptype,
+                                                       const Tensor& stats, bool ndx, bool ndw,
+                                                       bool ndb) {
+  const int64_t d = x.size(-1), rows = x.numel() / d;
+  Tensor dx, dw, db;
+  if (ndx) dx = dense_like(x);
+  if (ndw) dw = at::empty({d}, x.options().dtype(ptype));
+  if (ndb) db = at::empty({d}, x.options().dtype(ptype));
+  if (ndx || ndw || ndb) {
+    c10::cuda::CUDAGuard guard(x.device());
+    const Rows r = rows_of(x), g = rows_of(dy_in.to(x.scalar_type()));
+    const size_t n = tw_layer_norm_workspace_bytes(rows, (int)d);
+    Tensor ws = bytes(n, x);
+    const float* mean = stats.data_ptr<float>();
+    check_status(TW_PICK(tw_layer_norm_backward, x.scalar_type())(
+                     ptr(g.t), g.stride, ptr(r.t), r.stride, ptr(w), ptype != x.scalar_type(),
+                     mean, mean + rows, rows, (int)d, ptr(dx), ptr(dw), ptr(db), ptr(ws), n,
+                     stream_of(x)),
+                 "tw_layer_norm_backward");
+  }
+  return {dx, dw, db};
+}
+
+struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight,
+                        const OptTensor& bias, double eps) {
+    const Tensor w = def(weight), b = def(bias);
+    auto [y, stats] = layer_norm_forward(x, w, b, eps, true);
+    ctx->save_for_backward({x, w, stats});
+    ctx->saved_data["ptype"] = (int64_t)(w.defined()   ? w.scalar_type()
+                                         : b.defined() ? b.scalar_type()
+                                                       : x.scalar_type());
+    ctx->saved_data["bias"] = b.defined();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const variable_list s = ctx->get_saved_variables();
+    const bool has_w = s[1].defined(), has_b = ctx->saved_data["bias"].toBool();
+    auto [dx, dw, db] = layer_norm_backward(
+        g[0], s[0], s[1], (at::ScalarType)ctx->saved_data["ptype"].toInt(), s[2],
+        ctx->needs_input_grad(0), has_w && ctx->needs_input_grad(1),
+        has_b && ctx->needs_input_grad(1 + has_w));
+    return first_order({dx, dw, db, Tensor()});
+  }
+};
+
+void check_parameter(const char* name, const Tensor& p, const Tensor& x) {
+  if (p.dim() != 1 || p.size(0) != x.size(-1))
+    bad_value(std::string(name) + " must have shape [" + std::to_string(x.size(-1)) + "], got " +
+              shape_of(p));
+  if (p.scalar_type() != x.scalar_type() && p.scalar_type() != at::kFloat)
+    bad_type(std::string(name) + " must be float32 or of x's type " + type_of(x.scalar_type()) +
+             ", got " + type_of(p.scalar_type()));
+}
+
+Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+  check_type("x", x);
+  if (x.dim() < 1 || x.size(-1) == 0) bad_value("x must have shape [..., D] with D > 0");
+  Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  if (w.defined()) check_parameter("weight", w, x);
+  if (b.defined()) check_parameter("bias", b, x);
+  if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type())
+    bad_type("weight and bias must have one type");
+  if (!(eps >= 0)) bad_value("eps must be >= 0");
+  require_cuda(x);
+  check_device(x, w);
+  check_device(x, b);
+  if (w.defined()) w = w.contiguous();
+  if (b.defined()) b = b.contiguous();
+  if (wants_grad({&x, &w, &b})) return LayerNormFn::apply(x, opt(w), opt(b), eps);
+  return std::get<0>(layer_norm_forward(x, w, b, eps, false));
+}
+
+// ------------------------------------------------------------------ linear
+
+// 1 when a row of 16-bit elements may start off a 16-byte boundary.
+int unaligned(const Rows& r) {
+  return ((uintptr_t)r.t.data_ptr() & 15) != 0 || (r.stride & 7) != 0 || r.stride < r.t.size(-1);
+}
+
+std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias,
+                                          const Tensor& res, int64_t act, bool save) {
+  const int64_t n = w.size(0), k = w.size(1), m = x.numel() / k;
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = n;
+  Tensor y = at::empty(shape, x.options());
+  Tensor z = save && act ? at::empty({m, n}, x.options()) : Tensor();
+  if (m) {
+    TORCH_CHECK(m <= INT_MAX && n <= INT_MAX && k <= INT_MAX, "linear: a size is too large");
+    c10::cuda::CUDAGuard guard(x.device());
+    const Rows xr = rows_of(x), wr = rows_of(w);
+    Rows rr{Tensor(), 0};
+    if (res.defined()) rr = rows_of(res);
+    const size_t bytes_needed = tw_linear_workspace_bytes(
+        (int)m, (int)n, (int)k, (int)x.element_size(), (int)act, 0, unaligned(xr) | unaligned(wr));
+    Tensor ws = bytes(bytes_needed, x);
+    check_status(TW_PICK(tw_linear_forward, x.scalar_type())(
+                     ptr(xr.t), xr.stride, ptr(wr.t), wr.stride, ptr(bias), ptr(rr.t), rr.stride,
+                     (int)m, (int)n, (int)k, (int)act, ptr(y), ptr(z), ptr(ws), bytes_needed,
+                     stream_of(x)),
+                 "tw_linear_forward");
+  }
+  return {y, z};
+}
+
+std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& dy_in, const Tensor& x,
+                                                   const Tensor& w, const Tensor& z, int64_t act,
+                                                   bool ndx, bool ndw, bool ndb) {
+  const int64_t n = w.size(0), k = w.size(1), m = x.numel() / k;
+  Tensor dx, dw, db;
+  if (ndx) dx = dense_like(x);
+  if (ndw) dw = dense_like(w);
+  if (ndb) db = at::empty({n}, x.options());
+  if (ndx || ndw || ndb) {
+    TORCH_CHECK(m <= INT_MAX, "linear: a size is too large");
+    c10::cuda::CUDAGuard guard(x.device());
+    const Rows g = rows_of(dy_in.to(x.scalar_type())), xr = rows_of(x), wr = rows_of(w);
+    const size_t bytes_needed = tw_linear_workspace_bytes(
+        (int)m, (int)n, (int)k, (int)x.element_size(), (int)act, 1,
+        unaligned(xr) | unaligned(wr) | unaligned(g));
+    Tensor ws = bytes(bytes_needed, x);
+    check_status(TW_PICK(tw_linear_backward, x.scalar_type())(
+                     ptr(g.t), g.stride, ptr(xr.t), xr.stride, ptr(wr.t), wr.stride, ptr(z), (int)m,
+                     (int)n, (int)k, (int)act, ptr(dx), ptr(dw), ptr(db), ptr(ws), bytes_needed,
+                     stream_of(x)),
+                 "tw_linear_backward");
+  }
+  return {dx, dw, db};
+}
+
+struct LinearFn : torch::autograd::Function<LinearFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w,
+                        const OptTensor& bias, const OptTensor& residual, int64_t act) {
+    auto [y, z] = linear_forward(x, w, def(bias), def(residual), act, true);
+    ctx->save_for_backward({x, w, z});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["residual"] = residual.has_value();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const variable_list s = ctx->get_saved_variables();
+    const bool has_b = ctx->saved_data["bias"].toBool();
+    const bool has_r = ctx->saved_data["residual"].toBool();
+    auto [dx, dw, db] = linear_backward(g[0], s[0], s[1], s[2], ctx->saved_data["act"].toInt(),
+                                        ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                                        has_b && ctx->needs_input_grad(2));
+    variable_list out = first_order({dx, dw, db});
+    out.push_back(has_r && ctx->needs_input_grad(2 + has_b) ? g[0] : Tensor());
+    out.push_back(Tensor());
+    return out;
+  }
+};
+
+Tensor linear(Tensor x, Tensor w, const OptTensor& bias, const OptTensor& residual, int64_t act) {
+  Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+  if (at::autocast::is_autocast_enabled(at::kCUDA)) {
+    const at::ScalarType t = at::autocast::get_autocast_dtype(at::kCUDA);
+    x = x.to(t);
+    w = w.to(t);
+    if (b.defined()) b = b.to(t);
+    if (r.defined()) r = r.to(t);
+  }
+  check_type("x", x);
+  if (w.dim() != 2 || w.size(0) == 0 || w.size(1) == 0)
+    bad_value("weight must have shape [N, K] with N, K > 0");
+  const int64_t n = w.size(0), k = w.size(1);
+  if (x.dim() < 1 || x.size(-1) != k)
+    bad_value("x must have shape [..., " + std::to_string(k) + "], got " + shape_of(x));
+  if (b.defined() && (b.dim() != 1 || b.size(0) != n))
+    bad_value("bias must have shape [" + std::to_string(n) + "], got " + shape_of(b));
+  if (r.defined()) {
+    bool same = r.dim() == x.dim() && r.size(-1) == n;
+    for (int64_t i = 0; same && i + 1 < x.dim(); ++i) same = r.size(i) == x.size(i);
+    if (!same)
+      bad_value("residual must have the result's shape [..., " + std::to_string(n) + "], got " +
+                shape_of(r));
+  }
+  check_same_type("weight", w, x);
+  if (b.defined()) check_same_type("bias", b, x);
+  if (r.defined()) check_same_type("residual", r, x);
+  require_cuda(x);
+  check_device(x, w);
+  check_device(x, b);
+  check_device(x, r);
+  if (b.defined()) b = b.contiguous();
+  if (wants_grad({&x, &w, &b, &r})) return LinearFn::apply(x, w, opt(b), opt(r), act);
+  return std::get<0>(linear_forward(x, w, b, r, act, false));
+}
+
+// -------------------------------------------------------------- gated scan
+
+int dim32(int64_t v) {
+  TORCH_CHECK(v <= INT_MAX, "gated_scan: a size is too large");
+  return (int)v;
+}
+
+std::tuple<Tensor, Tensor, Tensor> gated_scan_forward(const Tensor& x_in, const Tensor& gate_in,
+                                                      const Tensor& h0_in, const Tensor& lengths,
+                                                      bool save) {
+  const int64_t b = x_in.size(0), t = x_in.size(1), d = x_in.size(2);
+  Tensor y = dense_like(x_in);
+  Tensor state = at::empty({b, d}, x_in.options().dtype(at::kFloat));
+  Tensor carry;
+  size_t n = 0;
+  if (save) {
+    n = tw_gated_scan_carry_bytes(dim32(b), dim32(t), dim32(d));
+    carry = at::empty({(int64_t)n}, x_in.options().dtype(at::kByte));
+  }
+  if (b) {
+    c10::cuda::CUDAGuard guard(x_in.device());
+    const Tensor x = frames_of(x_in), gate = frames_of(gate_in);
+    const Tensor h0 = h0_in.defined() ? h0_in.contiguous() : h0_in;
+    check_status(TW_PICK(tw_gated_scan_forward, x.scalar_type())(
+                     ptr(x), x.stride(0), x.stride(1), ptr(gate), gate.stride(0), gate.stride(1),
+                     (const float*)ptr(h0), (const int64_t*)ptr(lengths), dim32(b), dim32(t),
+                     dim32(d), ptr(y), state.data_ptr<float>(), ptr(carry), n, stream_of(x)),
+                 "tw_gated_scan_forward");
+  }
+  return {y, state, carry};
+}
+
+// dL/dy or dL/dstate may be undefined: zero.
+std::tuple<Tensor, Tensor, Tensor> gated_scan_backward(const Tensor& dy_in, const Tensor& dstate_in,
+                                                       const Tensor& x_in, const Tensor& gate_in,
+                                                       const Tensor& lengths, const Tensor& carry) {
+  const int64_t b = x_in.size(0), t = x_in.size(1), d = x_in.size(2);
+  Tensor dx = dense_like(x_in), dgate = dense_like(x_in);
+  Tensor dh0 = at::empty({b, d}, x_in.options().dtype(at::kFloat));
+  if (b) {
+    c10::cuda::CUDAGuard guard(x_in.device());
+    const Tensor x = frames_of(x_in), gate = frames_of(gate_in);
+    const Tensor dy =
+        dy_in.defined() ? frames_of(dy_in.to(x.scalar_type())) : at::zeros_like(dx);
+    const Tensor ds =
+        dstate_in.defined() ? dstate_in.to(at::kFloat).contiguous() : dstate_in;
+    check_status(TW_PICK(tw_gated_scan_backward, x.scalar_type())(
+                     ptr(dy), dy.stride(0), dy.stride(1), (const float*)ptr(ds), ptr(x),
+                     x.stride(0), x.stride(1), ptr(gate), gate.stride(0), gate.stride(1),
+                     (const int64_t*)ptr(lengths), ptr(carry), (size_t)carry.numel(), dim32(b),
+                     dim32(t), dim32(d), ptr(dx), ptr(dgate), dh0.data_ptr<float>(), stream_of(x)),
+                 "tw_gated_scan_backward");
+  }
+  return {dx, dgate, dh0};
+}
+
+struct GatedScanFn : torch::autograd::Function<GatedScanFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate,
+                               const OptTensor& h0, const OptTensor& lengths) {
+    auto [y, state, carry] = gated_scan_forward(x, gate, def(h0), def(lengths), true);
+    ctx->save_for_backward({x, gate, def(lengths), carry});
+    ctx->saved_data["state"] = h0.has_value();
+    ctx->set_materialize_grads(false);
+    return {y, state};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    if (!g[0].defined() && !g[1].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const variable_list s = ctx->get_saved_variables();
+    auto [dx, dgate, dh0] = gated_scan_backward(g[0], g[1], s[0], s[1], s[2], s[3]);
+    return first_order({dx, dgate, ctx->saved_data["state"].toBool() ? dh0 : Tensor(), Tensor()});
+  }
+};
+
+void check_gate(const Tensor& gate, const Tensor& x) {
+  if (gate.sizes() != x.sizes())
+    bad_value("gate must have x's shape " + shape_of(x) + ", got " + shape_of(gate));
+  check_same_type("gate", gate, x);
+}
+void check_state(const Tensor& state, int64_t batch, int64_t dim) {
+  if (state.dim() != 2 || state.size(0) != batch || state.size(1) != dim)
+    bad_value("state must have shape [" + std::to_string(batch) + ", " + std::to_string(dim) +
+              "], got " + shape_of(state));
+  if (state.scalar_type() != at::kFloat)
+    bad_type("state must be float32, got " + type_of(state.scalar_type()));
+}
+
+std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gate, const OptTensor& state,
+                                      const OptTensor& lengths_in) {
+  check_type("x", x);
+  if (x.dim() != 3 || x.size(2) == 0)
+    bad_value("x must have shape [batch, time, feature] with features");
+  check_gate(gate, x);
+  Tensor h0 = state.value_or(Tensor()), lengths = lengths_in.value_or(Tensor());
+  if (h0.defined()) check_state(h0, x.size(0), x.size(2));
+  if (lengths.defined()) {
+    if (lengths.dim() != 1 || lengths.size(0) != x.size(0))
+      bad_value("lengths must have shape [" + std::to_string(x.size(0)) + "], got " +
+                shape_of(lengths));
+    if (lengths.scalar_type() != at::kLong && lengths.scalar_type() != at::kInt)
+      bad_type("lengths must be int64 or int32, got " + type_of(lengths.scalar_type()));
+  }
+  require_cuda(x);
+  check_device(x, gate);
+  check_device(x, h0);
+  check_device(x, lengths);
+  if (lengths.defined()) lengths = lengths.to(at::kLong).contiguous();
+  if (wants_grad({&x, &gate, &h0})) {
+    variable_list out = GatedScanFn::apply(x, gate, opt(h0), opt(lengths));
+    return {out[0], out[1]};
+  }
+  auto [y, last, carry] = gated_scan_forward(x, gate, h0, lengths, false);
+  return {y, last};
+}
+
+Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const OptTensor& state_in) {
+  check_type("x", x);
+  if (x.dim() != 2 || x.size(1) == 0)
+    bad_value("x must have shape [batch, feature] with features");
+  check_gate(gate, x);
+  if (!state_in.has_value()) bad_value("state must be a [B,D] tensor: it is updated in place");
+  const Tensor& state = *state_in;
+  const int64_t b = x.size(0), d = x.size(1);
+  check_state(state, b, d);
+  if (!state.is_contiguous()) bad_value("state must be contiguous: it is updated in place");
+  require_cuda(x);
+  check_device(x, gate);
+  check_device(x, state);
+  if (wants_grad({&x, &gate, &state}))
+    throw std::runtime_error("gated_scan_step is not differentiable; use gated_scan, or no_grad");
+  Tensor y = dense_like(x);
+  if (b) {
+    c10::cuda::CUDAGuard guard(x.device());
+    const Rows xr = rows_of(x), gr = rows_of(gate);
+    check_status(TW_PICK(tw_gated_scan_step, x.scalar_type())(
+                     ptr(xr.t), xr.stride, ptr(gr.t), gr.stride, state.data_ptr<float>(), dim32(b),
+                     dim32(d), ptr(y), stream_of(x)),
+                 "tw_gated_scan_step");
+  }
+  // written through a raw pointer: autograd has to see the change
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+  return y;
+}
+
+// ------------------------------------------------------------------ AdamW
+
+// One AdamW step over `params`, whose states start at `offsets` in the flat
+// buffers; a parameter without a gradient is left out.
+void adamw_step(const std::vector<Tensor>& params, const std::vector<int64_t>& offsets,
+                int64_t bits, const Tensor& m, const OptTensor& ms, const Tensor& v,
+                const OptTensor& vs, const Tensor& step, double lr, const OptTensor& lr_tensor,
+                double beta1, double beta2, double eps, double weight_decay, int64_t seed) {
+  TORCH_CHECK(params.size() == offsets.size(), "adamw_step: one offset a parameter");
+  std::vector<uint64_t> table;
+  std::vector<Tensor> keep;
+  table.reserve(4 * params.size());
+  const at::ScalarType type = params.empty() ? at::kFloat : params[0].scalar_type();
+  for (size_t i = 0; i < params.size(); ++i) {
+    const Tensor& p = params[i];
+    Tensor g = p.grad();
+    if (!g.defined()) continue;
+    if (p.scalar_type() != type || g.scalar_type() != type || g.layout() != at::kStrided)
+      bad_type("a gradient must be dense and of its parameter's type " + type_of(type) + ", got " +
+               type_of(g.scalar_type()));
+    if (!p.is_contiguous()) bad_value("parameters must be contiguous");
+    if (p.device() != m.device() || g.device() != m.device())
+      bad_value("parameters and gradients must stay on the device of their states, " +
+                m.device().str());
+    if (!g.is_contiguous()) {
+      g = g.contiguous();
+      keep.push_back(g);
+    }
+    table.insert(table.end(), {(uint64_t)p.data_ptr(), (uint64_t)g.data_ptr(), (uint64_t)p.numel(),
+                               (uint64_t)offsets[i]});
+  }
+  const float* lr_device = nullptr;
+  if (lr_tensor.has_value()) {
+    const Tensor& t = *lr_tensor;
+    if (t.device() != m.device() || t.scalar_type() != at::kFloat || t.numel() != 1)
+      bad_value("lr must be a number or one float32 value on " + m.device().str());
+    lr_device = t.data_ptr<float>();
+  }
+  c10::cuda::CUDAGuard guard(m.device());
+  check_status(TW_PICK(tw_adamw_step, type)(
+                   table.data(), (int)(table.size() / 4), (int)bits, ptr(m),
+                   (float*)ptr(ms.value_or(Tensor())), ptr(v), (float*)ptr(vs.value_or(Tensor())),
+                   step.data_ptr<int>(), lr, lr_device, beta1, beta2, eps, weight_decay,
+                   (size_t)(uint32_t)seed, stream_of(m)),
+               "tw_adamw_step");
+  for (const Tensor& p : params)
+    if (p.grad().defined() && !p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  static PyObject* native =
+      py::object(py::module_::import("torchwarp_b200._native").attr("NativeError")).release().ptr();
+  py::register_exception_translator([](std::exception_ptr p) {
+    try {
+      if (p) std::rethrow_exception(p);
+    } catch (const NativeError& e) {
+      PyErr_SetString(native, e.what());
+    }
+  });
+  m.def("layer_norm", &layer_norm);
+  m.def("linear", &linear);
+  m.def("gated_scan", &gated_scan);
+  m.def("gated_scan_step", &gated_scan_step);
+  m.def("adamw_step", &adamw_step);
+  // without autograd, for the custom ops of torch.compile
+  m.def("layer_norm_forward", [](const Tensor& x, const OptTensor& w, const OptTensor& b,
+                                 double eps) {
+    return layer_norm_forward(x, def(w), def(b), eps, true);
+  });
+  m.def("layer_norm_backward", [](const Tensor& dy, const Tensor& x, const OptTensor& w,
+                                  const OptTensor& param, const Tensor& stats) {
+    const Tensor p = w.has_value() ? *w : def(param);
+    return layer_norm_backward(dy, x, def(w), p.defined() ? p.scalar_type() : x.scalar_type(),
+                               stats, true, true, true);
+  });
+  m.def("linear_forward", [](const Tensor& x, const Tensor& w, const OptTensor& b,
+                             const OptTensor& r, int64_t act) {
+    auto [y, z] = linear_forward(x, w, def(b), def(r), act, true);
+    return std::make_tuple(y, opt(z));
+  });
+  m.def("linear_backward", [](const Tensor& dy, const Tensor& x, const Tensor& w,
+                              const OptTensor& z, int64_t act) {
+    return linear_backward(dy, x, w, def(z), act, true, true, true);
+  });
+  m.def("gated_scan_forward", [](const Tensor& x, const Tensor& g, const OptTensor& h0,
+                                 const OptTensor& n) {
+    return gated_scan_forward(x, g, def(h0), def(n), true);
+  });
+  m.def("gated_scan_backward", [](const OptTensor& dy, const OptTensor& ds, const Tensor& x,
+                                  const Tensor& g, const OptTensor& n, const Tensor& carry) {
+    return gated_scan_backward(def(dy), def(ds), x, g, def(n), carry);
+  });
+}

@@ -1,7 +1,5 @@
 """AdamW over all parameters of a group in one launch, with 32-bit or 8-bit states."""
 
-from array import array
-
 import torch
 
 from .. import _native as nat
@@ -16,13 +14,13 @@ class _Bucket:
         self.params = params
         self.device, self.dtype = params[0].device, params[0].dtype
         nat.require_cuda(params[0])
-        self.fn = nat.entry("tw_adamw_step", self.dtype)
+        if self.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise TypeError("parameters must be float32, bfloat16 or float16, got {}".format(
+                self.dtype))
         self.offsets, at = [], 0
         for p in params:
             self.offsets.append(at)
             at += -(-p.numel() // _BLOCK) * _BLOCK
-        self.rows = array("Q", [v for p, o in zip(params, self.offsets)
-                                for v in (0, 0, p.numel(), o)])
         dev = self.device
         self.step = torch.zeros(2, dtype=torch.int32, device=dev)
         if bits == 32:
@@ -36,35 +34,13 @@ class _Bucket:
                           "exp_avg_sqrt_scale": torch.zeros(at // _BLOCK, device=dev)}
         self.bits = bits
 
-    def pointers(self):
+    def buffers(self):
+        """First moments and their scales, second moments and theirs."""
         s = self.state
         if self.bits == 32:
-            return s["exp_avg"].data_ptr(), None, s["exp_avg_sq"].data_ptr(), None
-        return tuple(s[k].data_ptr() for k in ("exp_avg", "exp_avg_scale", "exp_avg_sqrt",
-                                               "exp_avg_sqrt_scale"))
-
-    def table(self):
-        """Four numbers a tensor for the native step (a tensor without a gradient counts no
-        values), and the gradients that had to be copied."""
-        table, keep, at = array("Q", self.rows), [], 0
-        dtype = self.dtype
-        for p in self.params:
-            g = p.grad
-            if g is None:
-                table[at + 2] = 0
-            else:
-                if g.dtype != dtype:
-                    raise TypeError("a gradient must be of its parameter's type {}, got {}".format(
-                        dtype, g.dtype))
-                if not p.is_contiguous():
-                    raise ValueError("parameters must be contiguous")
-                if not g.is_contiguous():
-                    g = g.contiguous()
-                    keep.append(g)
-                table[at] = p.data_ptr()
-                table[at + 1] = g.data_ptr()
-            at += 4
-        return table, keep
+            return s["exp_avg"], None, s["exp_avg_sq"], None
+        return tuple(s[k] for k in ("exp_avg", "exp_avg_scale", "exp_avg_sqrt",
+                                    "exp_avg_sqrt_scale"))
 
 
 class AdamW(torch.optim.Optimizer):
@@ -117,22 +93,13 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         for index, group in enumerate(self.param_groups):
             lr = group["lr"]
+            on_device = isinstance(lr, torch.Tensor)
             for b in self._group_buckets(index):
-                table, keep = b.table()
-                lr_device = None
-                if isinstance(lr, torch.Tensor):
-                    if lr.device != b.device or lr.dtype != torch.float32 or lr.numel() != 1:
-                        raise ValueError("lr must be a number or one float32 value on {}".format(
-                            b.device))
-                    lr_device = lr.data_ptr()
-                m, ms, v, vs = b.pointers()
-                nat.launch("adamw_step", b.fn, b.device, table.buffer_info()[0], len(table) // 4,
-                           self._bits, m, ms, v, vs, b.step.data_ptr(),
-                           0.0 if lr_device else float(lr), lr_device, group["betas"][0],
-                           group["betas"][1], group["eps"], group["weight_decay"],
-                           self._seed & 0xFFFFFFFF)
-                # written through raw pointers: autograd has to see the change
-                torch.autograd.graph.increment_version([p for p in b.params if p.grad is not None])
+                m, ms, v, vs = b.buffers()
+                nat.host().adamw_step(b.params, b.offsets, self._bits, m, ms, v, vs, b.step,
+                                      0.0 if on_device else lr, lr if on_device else None,
+                                      *group["betas"], group["eps"], group["weight_decay"],
+                                      self._seed & 0xFFFFFFFF)
         return loss
 
     def flat_state(self, index=0):
