@@ -136,6 +136,59 @@ template <bool VEC, int N, typename T> struct Raw {
   }
 };
 
+// V floats that go through the arithmetic together: pairs use the packed
+// instructions (two results each), which halve its issue slots.
+template <int V> struct Vec { float v[V]; };
+
+template <int V>
+__device__ __forceinline__ Vec<V> splat(float x) {
+  Vec<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = x;
+  return r;
+}
+__device__ __forceinline__ uint64_t two(const Vec<2>& a) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.v[0]), "f"(a.v[1]));
+  return r;
+}
+__device__ __forceinline__ Vec<2> of_two(uint64_t a) {
+  Vec<2> r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.v[0]), "=f"(r.v[1]) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ Vec<1> fma_v(Vec<1> a, Vec<1> b, Vec<1> c) {
+  return {{fmaf(a.v[0], b.v[0], c.v[0])}};
+}
+__device__ __forceinline__ Vec<2> fma_v(Vec<2> a, Vec<2> b, Vec<2> c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(two(a)), "l"(two(b)), "l"(two(c)));
+  return of_two(r);
+}
+__device__ __forceinline__ Vec<1> add_v(Vec<1> a, Vec<1> b) { return {{a.v[0] + b.v[0]}}; }
+__device__ __forceinline__ Vec<2> add_v(Vec<2> a, Vec<2> b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(two(a)), "l"(two(b)));
+  return of_two(r);
+}
+__device__ __forceinline__ Vec<1> mul_v(Vec<1> a, Vec<1> b) { return {{a.v[0] * b.v[0]}}; }
+__device__ __forceinline__ Vec<2> mul_v(Vec<2> a, Vec<2> b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(two(a)), "l"(two(b)));
+  return of_two(r);
+}
+template <int V>
+__device__ __forceinline__ Vec<V> sub_v(Vec<V> a, Vec<V> b) {  // a - b
+  return fma_v(b, splat<V>(-1.f), a);
+}
+
+template <int V>
+__device__ __forceinline__ Vec<V> negated(Vec<V> s) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) s.v[i] = -s.v[i];
+  return s;
+}
+
 // f = sigmoid(z) and 1 - f: the smaller of the two from exp(-|z|), which
 // neither overflows nor cancels, to a few ulp of itself; the larger is one
 // minus it, correctly rounded.
@@ -149,62 +202,103 @@ __device__ __forceinline__ void sigmoid_pair(float z, float& f, float& omf) {
 // Activations of the linear operator (values of the `act` argument).
 enum Act : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3, kActSigmoid = 4 };
 
-// FAST (results rounded to 16 bits): the normal distribution function
-// through Abramowitz & Stegun 7.1.26, erfc(x) = (a1 t + .. + a5 t^5) e^(-x^2)
-// with t = 1 / (1 + p x), |error| <= 1.5e-7: one exponential and one
-// reciprocal in place of erff's two polynomial branches.  e is e^(-z^2/2).
-__device__ __forceinline__ float normal_cdf_fast(float z, float& e) {
-  const float t = rcp(__fmaf_rn(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
-  e = ex2(mul_rn(mul_rn(-0.72134752044448170f, z), z));
-  float q = __fmaf_rn(1.061405429f, t, -1.453152027f);
-  q = __fmaf_rn(q, t, 1.421413741f);
-  q = __fmaf_rn(q, t, -0.284496736f);
-  q = __fmaf_rn(q, t, 0.254829592f);
-  q = mul_rn(mul_rn(mul_rn(q, t), 0.5f), e);
-  return z < 0.f ? q : add_rn(1.f, -q);
+// Upper tail of the normal distribution at |z| (results rounded to 16 bits),
+// through Abramowitz & Stegun 7.1.26: erfc(x) = (a1 t + .. + a5 t^5) e^(-x^2)
+// with t = 1 / (1 + p x), |error| <= 1.5e-7, x = |z| / sqrt 2; one exponential
+// and one reciprocal in place of erff's two polynomial branches.  The factor
+// 1/2 is in the coefficients.  az is |z| (cut at 30, where the tail is 0, so
+// that an infinity times it is not a NaN), e is e^(-z^2 / 2).
+template <int V>
+__device__ __forceinline__ Vec<V> normal_tail(Vec<V> z, Vec<V>& az, Vec<V>& e) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) az.v[i] = fminf(fabsf(z.v[i]), 30.f);
+  Vec<V> t = fma_v(az, splat<V>(0.3275911f * 0.70710678118654752f), splat<V>(1.f));
+  e = mul_v(mul_v(z, z), splat<V>(-0.72134752044448170f));
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    t.v[i] = rcp(t.v[i]);
+    e.v[i] = ex2(e.v[i]);
+  }
+  Vec<V> q = fma_v(splat<V>(0.5f * 1.061405429f), t, splat<V>(-0.5f * 1.453152027f));
+  q = fma_v(q, t, splat<V>(0.5f * 1.421413741f));
+  q = fma_v(q, t, splat<V>(-0.5f * 0.284496736f));
+  q = fma_v(q, t, splat<V>(0.5f * 0.254829592f));
+  return mul_v(mul_v(q, t), e);
 }
 
-// The roundings are explicit: a call that saves z gives the bits of one that
-// does not, whatever the compiler contracts around it.
-template <int ACT, bool FAST>
-__device__ __forceinline__ float act_value(float z) {
-  if (ACT == kActRelu) return z < 0.f ? 0.f : z;  // a NaN stays a NaN
-  if (ACT == kActGelu && FAST) {
-    float e;
-    return mul_rn(z, normal_cdf_fast(z, e));
+// act(z).  FAST: for results of 16 bits.  The roundings are explicit: a call
+// that saves z gives the bits of one that does not, whatever the compiler
+// contracts around it.
+template <int ACT, bool FAST, int V>
+__device__ __forceinline__ Vec<V> act_value(Vec<V> z) {
+  if constexpr (ACT == kActGelu && FAST) {  // z Phi(z) = max(z, 0) - |z| tail(|z|)
+    Vec<V> az, e, r;
+    const Vec<V> q = normal_tail(z, az, e);
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = fmaxf(z.v[i], 0.f);
+    return fma_v(negated(az), q, r);
+  } else if constexpr (ACT == kActSilu || ACT == kActSigmoid) {
+    Vec<V> f = mul_v(z, splat<V>(-1.4426950408889634f));
+#pragma unroll
+    for (int i = 0; i < V; ++i) f.v[i] = ex2(f.v[i]);
+    f = add_v(f, splat<V>(1.f));
+#pragma unroll
+    for (int i = 0; i < V; ++i) f.v[i] = rcp(f.v[i]);
+    return ACT == kActSilu ? mul_v(z, f) : f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float& v = z.v[i];
+      if (ACT == kActRelu) v = v < 0.f ? 0.f : v;  // a NaN stays a NaN
+      if (ACT == kActGelu) {
+        const float h = mul_rn(0.5f, v);
+        v = __fmaf_rn(h, erff(mul_rn(v, 0.70710678118654752f)), h);
+      }
+    }
+    return z;
   }
-  if (ACT == kActGelu) {
-    const float h = mul_rn(0.5f, z);
-    return __fmaf_rn(h, erff(mul_rn(z, 0.70710678118654752f)), h);
-  }
-  if (ACT == kActSilu || ACT == kActSigmoid) {
-    float f, omf;
-    sigmoid_pair(z, f, omf);
-    return ACT == kActSilu ? mul_rn(z, f) : f;
-  }
-  return z;
 }
 
 // d act / dz at z.
-template <int ACT, bool FAST>
-__device__ __forceinline__ float act_slope(float z) {
-  if (ACT == kActRelu) return z > 0.f ? 1.f : (z != z ? z : 0.f);
-  if (ACT == kActGelu) {
-    float cdf, e;
-    if (FAST) {
-      cdf = normal_cdf_fast(z, e);
-    } else {
-      cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-      e = ex2(-0.72134752044448170f * z * z);
+template <int ACT, bool FAST, int V>
+__device__ __forceinline__ Vec<V> act_slope(Vec<V> z) {
+  if constexpr (ACT == kActGelu && FAST) {  // Phi(z) + z phi(z)
+    Vec<V> az, e;
+    Vec<V> c = fma_v(normal_tail(z, az, e), splat<V>(-1.f), splat<V>(0.5f));
+#pragma unroll
+    for (int i = 0; i < V; ++i) c.v[i] = copysignf(c.v[i], z.v[i]);
+    return fma_v(mul_v(z, splat<V>(0.39894228040143268f)), e, add_v(c, splat<V>(0.5f)));
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float& v = z.v[i];
+      if (ACT == kActRelu) v = v > 0.f ? 1.f : (v != v ? v : 0.f);
+      if (ACT == kActGelu) {
+        const float cdf = 0.5f * (1.f + erff(v * 0.70710678118654752f));
+        v = fmaf(v, 0.39894228040143268f * ex2(-0.72134752044448170f * v * v), cdf);
+      }
+      if (ACT == kActSilu || ACT == kActSigmoid) {
+        float f, omf;
+        sigmoid_pair(v, f, omf);
+        v = ACT == kActSilu ? f * fmaf(v, omf, 1.f) : f * omf;
+      }
+      if (ACT == kActNone) v = 1.f;
     }
-    return fmaf(z, 0.39894228040143268f * e, cdf);
+    return z;
   }
-  if (ACT == kActSilu || ACT == kActSigmoid) {
-    float f, omf;
-    sigmoid_pair(z, f, omf);
-    return ACT == kActSilu ? f * fmaf(z, omf, 1.f) : f * omf;
+}
+
+// One value, the activation chosen at run time.
+template <bool FAST>
+__device__ __forceinline__ float activate1(float v, int act) {
+  const Vec<1> z = {{v}};
+  switch (act) {
+    case kActRelu: return act_value<kActRelu, FAST>(z).v[0];
+    case kActGelu: return act_value<kActGelu, FAST>(z).v[0];
+    case kActSilu: return act_value<kActSilu, FAST>(z).v[0];
+    case kActSigmoid: return act_value<kActSigmoid, FAST>(z).v[0];
+    default: return v;
   }
-  return 1.f;
 }
 
 }  // namespace tw

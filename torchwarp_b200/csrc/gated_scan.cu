@@ -10,27 +10,29 @@
 // there are 0, its gradients 0, and x and g are not read.
 //
 // One pass over the data.  The channels of all sequences, c = b D + d, are
-// numbered through; a block of 128 threads owns 32 (or 16) lanes of them,
-// pairs in 16 bits, and walks time in tiles of 4 (or 8) runs x 16 frames.  A
-// thread reads its 16 frames into registers, composes them to (A, B) with
-// h_out = A h_in + B, learns its h_in from the runs before it, and goes over
-// its frames again in registers to write the outputs.  Few channels: up to 8
-// blocks of a cluster take neighbouring tiles and compose their (A, B) through
-// each other's shared memory, so that a long sequence still fills the GPU.
+// numbered through; a block of 128 threads owns 32 lanes of channel pairs (or
+// 16, or 8) and walks time in tiles of 4 (8, 16) runs of 8 frames.  A thread
+// reads its 8 frames into registers, composes them to (A, B) with h_out = A
+// h_in + B, learns its h_in from the runs before it, and goes over its frames
+// again in registers to write the outputs.  Few channels: up to 8 blocks of a
+// cluster take neighbouring tiles and compose their (A, B) through each
+// other's shared memory, so that a long sequence still fills the GPU.
 // Everything is summed in a fixed order.
 //
-// The forward saves h before every 16th frame in float32 (0.25 bytes a value);
+// The forward saves h before every 8th frame in float32 (0.5 bytes a value);
 // the backward recomputes the states of a thread's frames from it, so no
-// rounded output enters a gradient and the outputs are not read again.
+// rounded output enters a gradient and the outputs are not read again.  8
+// frames of two channels, the next tile's loads under way among them, fit 128
+// registers; 16 did not (32 x 1024 x 1024 bfloat16: 200 us with the spills).
 #include "../../include/torchwarp_b200.h"
 #include "element.cuh"
 
 namespace tw {
 namespace {
 
-constexpr int SCAN_FRAMES = 16;  // of a thread
+constexpr int SCAN_FRAMES = 8;  // of a thread
 constexpr int SCAN_THREADS = 128;
-// LPR lanes a frame: 128 / LPR runs of 16 frames a tile.
+// LPR lanes a frame: 128 / LPR runs a tile.
 constexpr int tile_of(int lpr) { return SCAN_THREADS / lpr * SCAN_FRAMES; }
 
 __device__ __forceinline__ int live_len(const int64_t* lengths, int b, int T) {
@@ -39,55 +41,8 @@ __device__ __forceinline__ int live_len(const int64_t* lengths, int b, int T) {
   return n < 0 ? 0 : n > T ? T : (int)n;
 }
 
-// V floats that go through the arithmetic together: pairs use the packed
-// instructions (two results each), which halve the issue slots of what a
-// frame costs beside its loads and two special functions.
-template <int V> struct Vec { float v[V]; };
-
-template <int V>
-__device__ __forceinline__ Vec<V> splat(float x) {
-  Vec<V> r;
-#pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = x;
-  return r;
-}
-__device__ __forceinline__ uint64_t two(const Vec<2>& a) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.v[0]), "f"(a.v[1]));
-  return r;
-}
-__device__ __forceinline__ Vec<2> of_two(uint64_t a) {
-  Vec<2> r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.v[0]), "=f"(r.v[1]) : "l"(a));
-  return r;
-}
-__device__ __forceinline__ Vec<1> fma_v(Vec<1> a, Vec<1> b, Vec<1> c) {
-  return {{fmaf(a.v[0], b.v[0], c.v[0])}};
-}
-__device__ __forceinline__ Vec<2> fma_v(Vec<2> a, Vec<2> b, Vec<2> c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(two(a)), "l"(two(b)), "l"(two(c)));
-  return of_two(r);
-}
-__device__ __forceinline__ Vec<1> add_v(Vec<1> a, Vec<1> b) { return {{a.v[0] + b.v[0]}}; }
-__device__ __forceinline__ Vec<2> add_v(Vec<2> a, Vec<2> b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(two(a)), "l"(two(b)));
-  return of_two(r);
-}
-__device__ __forceinline__ Vec<1> mul_v(Vec<1> a, Vec<1> b) { return {{a.v[0] * b.v[0]}}; }
-__device__ __forceinline__ Vec<2> mul_v(Vec<2> a, Vec<2> b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(two(a)), "l"(two(b)));
-  return of_two(r);
-}
-template <int V>
-__device__ __forceinline__ Vec<V> sub_v(Vec<V> a, Vec<V> b) {  // a - b
-  return fma_v(b, splat<V>(-1.f), a);
-}
-
-// A gate as one number: the smaller of 1 - f and f, which keeps its relative
-// precision, negative when it is f.  +0 keeps the state.
+// A gate as one number n: the smaller of 1 - f and f, which keeps its relative
+// precision, negative when it is 1 - f.  -0 keeps the state.
 template <int V>
 __device__ __forceinline__ Vec<V> gate_of(Vec<V> z) {
   const Vec<V> t = mul_v(z, splat<V>(1.4426950408889634f));
@@ -99,44 +54,35 @@ __device__ __forceinline__ Vec<V> gate_of(Vec<V> z) {
   for (int i = 0; i < V; ++i) r.v[i] = rcp(r.v[i]);
   r = mul_v(e, r);
 #pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = copysignf(r.v[i], z.v[i]);
+  for (int i = 0; i < V; ++i)
+    r.v[i] = __uint_as_float((__float_as_uint(r.v[i]) & 0x7FFFFFFFu) |
+                             (~__float_as_uint(z.v[i]) & 0x80000000u));
   return r;
 }
-// b where the gate is f (opens), else a.
+// a where n is 1 - f, b where it is f.
 template <int V>
-__device__ __forceinline__ Vec<V> pick(Vec<V> s, Vec<V> a, Vec<V> b) {
+__device__ __forceinline__ Vec<V> pick(Vec<V> n, Vec<V> a, Vec<V> b) {
   Vec<V> r;
 #pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = __float_as_int(s.v[i]) < 0 ? b.v[i] : a.v[i];
+  for (int i = 0; i < V; ++i) r.v[i] = __float_as_int(n.v[i]) < 0 ? a.v[i] : b.v[i];
   return r;
 }
 // f h + (1 - f) x as a step from the nearer of the two, so that the rounding
-// of a gate near 1 does not decay a state that should last.
+// of a gate near 1 does not decay a state that should last: h - (1 - f)(h - x)
+// or x + f (h - x).  diff is h - x.
 template <int V>
-__device__ __forceinline__ Vec<V> advance(Vec<V> s, Vec<V> h, Vec<V> x) {
-  return fma_v(s, sub_v(x, h), pick(s, h, x));
+__device__ __forceinline__ Vec<V> advance(Vec<V> n, Vec<V> h, Vec<V> x, Vec<V> diff) {
+  return fma_v(n, diff, pick(n, h, x));
 }
-// f l and (1 - f) l, likewise: together they are l.
+// f l, likewise.
 template <int V>
-__device__ __forceinline__ Vec<V> decay(Vec<V> ns, Vec<V> s, Vec<V> l) {
-  return fma_v(ns, l, pick(s, l, splat<V>(0.f)));
+__device__ __forceinline__ Vec<V> decay(Vec<V> n, Vec<V> l) {
+  return fma_v(n, l, pick(n, l, splat<V>(0.f)));
 }
+// (1 - f) l, from -l.
 template <int V>
-__device__ __forceinline__ Vec<V> passed(Vec<V> s, Vec<V> l) {
-  return fma_v(s, l, pick(s, splat<V>(0.f), l));
-}
-template <int V>
-__device__ __forceinline__ Vec<V> negated(Vec<V> s) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) s.v[i] = -s.v[i];
-  return s;
-}
-// f (1 - f) = |s| (1 - |s|)
-template <int V>
-__device__ __forceinline__ Vec<V> slope_of(Vec<V> s) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) s.v[i] = fabsf(s.v[i]);
-  return fma_v(negated(s), s, s);
+__device__ __forceinline__ Vec<V> passed(Vec<V> n, Vec<V> l, Vec<V> neg_l) {
+  return fma_v(n, neg_l, pick(n, splat<V>(0.f), l));
 }
 
 // VC neighbouring channels of a frame, as they lie in memory.
@@ -145,6 +91,12 @@ template <typename T, int VC> struct Frame {
   __device__ __forceinline__ Vec<1> get() const { return {{to_f(t)}}; }
   static __device__ __forceinline__ Frame zero() { return {from_f<T>(0.f)}; }
   static __device__ __forceinline__ Frame of(Vec<1> v) { return {from_f<T>(v.v[0])}; }
+};
+template <> struct Frame<float, 2> {
+  float2 t;
+  __device__ __forceinline__ Vec<2> get() const { return {{t.x, t.y}}; }
+  static __device__ __forceinline__ Frame zero() { return {make_float2(0.f, 0.f)}; }
+  static __device__ __forceinline__ Frame of(Vec<2> v) { return {make_float2(v.v[0], v.v[1])}; }
 };
 template <typename T> struct Frame<T, 2> {
   uint32_t u;
@@ -157,19 +109,31 @@ template <typename T> struct Frame<T, 2> {
   static __device__ __forceinline__ Frame of(Vec<2> v) { return {Pair<T>::pack(v.v[0], v.v[1])}; }
 };
 
-// A thread's frames t0.. of an array whose frames are `step` bytes apart;
-// frames from `n` on are zero and not read.
+// p + step, hidden from the compiler: it would otherwise keep the addresses of
+// all frames of all arrays in registers at once, 70 of them.
+template <typename P, typename S>
+__device__ __forceinline__ void walk(P*& p, S step) {
+  p += step;
+  asm("" : "+l"(p));
+}
+
+// A thread's frames from p on, `step` bytes apart; frames from `n` on are zero
+// and not read.
 template <typename T, int VC>
 __device__ __forceinline__ void load_frames(Frame<T, VC> (&f)[SCAN_FRAMES], const char* p,
                                             size_t step, int n) {
   if (n >= SCAN_FRAMES) {
 #pragma unroll
-    for (int k = 0; k < SCAN_FRAMES; ++k, p += step)
+    for (int k = 0; k < SCAN_FRAMES; ++k) {
       f[k] = *reinterpret_cast<const Frame<T, VC>*>(p);
+      walk(p, step);
+    }
   } else {
 #pragma unroll
-    for (int k = 0; k < SCAN_FRAMES; ++k, p += step)
+    for (int k = 0; k < SCAN_FRAMES; ++k) {
       f[k] = k < n ? *reinterpret_cast<const Frame<T, VC>*>(p) : Frame<T, VC>::zero();
+      walk(p, step);
+    }
   }
 }
 
@@ -306,16 +270,17 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
   load_frames<T, VC>(xr, xp + (size_t)t0 * xs, xs, ch.L - t0);
   for (int it = 0; it < steps; ++it, t0 += TILE * S) {
     const int n = ch.L - t0;
-    Vec<VC> s[SCAN_FRAMES], xv[SCAN_FRAMES];
+    Vec<VC> s[SCAN_FRAMES];
+    Frame<T, VC> xk[SCAN_FRAMES];  // as it lies: pairs in one register
 #pragma unroll
     for (int k = 0; k < SCAN_FRAMES; ++k) {
       s[k] = gate_of(gr[k].get());
-      xv[k] = xr[k].get();
+      xk[k] = xr[k];
     }
     if (n < SCAN_FRAMES)
 #pragma unroll
       for (int k = 0; k < SCAN_FRAMES; ++k)
-        if (k >= n) s[k] = splat<VC>(0.f);
+        if (k >= n) s[k] = splat<VC>(-0.f);
     // the next tile's loads are under way while the blocks wait for each other
     const int t1 = t0 + TILE * S;
     load_frames<T, VC>(gr, gp + (size_t)t1 * gs, gs, ch.L - t1);
@@ -323,8 +288,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
     Vec<VC> A = splat<VC>(1.f), B = splat<VC>(0.f), h;
 #pragma unroll
     for (int k = 0; k < SCAN_FRAMES; ++k) {
-      B = advance(s[k], B, xv[k]);
-      A = decay(negated(s[k]), s[k], A);
+      const Vec<VC> x = xk[k].get();
+      B = advance(s[k], B, x, sub_v(B, x));
+      A = decay(s[k], A);
     }
     compose<VC, LPR, false>(sh, it, S, rank, part, lane, A, B, run, h);
     if (carry && ch.live && t0 < TT)
@@ -334,16 +300,20 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
     char* o = yp + (size_t)t0 * ys;
     if (n >= SCAN_FRAMES) {
 #pragma unroll
-      for (int k = 0; k < SCAN_FRAMES; ++k, o += ys) {
-        h = advance(s[k], h, xv[k]);
+      for (int k = 0; k < SCAN_FRAMES; ++k) {
+        const Vec<VC> x = xk[k].get();
+        h = advance(s[k], h, x, sub_v(h, x));
         *reinterpret_cast<Frame<T, VC>*>(o) = Frame<T, VC>::of(h);
+        walk(o, ys);
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < SCAN_FRAMES; ++k, o += ys) {
-        h = advance(s[k], h, xv[k]);
+      for (int k = 0; k < SCAN_FRAMES; ++k) {
+        const Vec<VC> x = xk[k].get();
+        h = advance(s[k], h, x, sub_v(h, x));
         if (ch.live && t0 + k < TT)
           *reinterpret_cast<Frame<T, VC>*>(o) = k < n ? Frame<T, VC>::of(h) : Frame<T, VC>::zero();
+        walk(o, ys);
       }
     }
     if (S == 1 && part == SCAN_THREADS / LPR - 1)
@@ -358,9 +328,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
   if (S > 1) cluster_sync_all();  // the others may still read this block's tile
 }
 
-// The same walk from the end.  Pairs of 16 bits load a tile when its turn
-// comes (its registers leave no room for the next one's); single channels
-// load a tile ahead.
+// The same walk from the end.
 template <typename T, int VC, int LPR>
 __global__ void __launch_bounds__(SCAN_THREADS, 4)
     scan_bwd_kernel(const T* __restrict__ dy, size_t yb, size_t yt,
@@ -369,7 +337,6 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
                     const int64_t* __restrict__ lengths, const float* __restrict__ carry,
                     size_t BD, int TT, int D, int S, T* __restrict__ dx, T* __restrict__ dg,
                     float* __restrict__ dh0) {
-  constexpr bool AHEAD = VC == 1;
   constexpr int TILE = tile_of(LPR);
   __shared__ ScanShared<VC, LPR> sh;
   const int part = threadIdx.x / LPR, lane = threadIdx.x & (LPR - 1);
@@ -401,44 +368,46 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
     for (int v = 0; v < VC; ++v)
       hr.v[v] = n > 0 ? carry[(tt / SCAN_FRAMES) * BD + ch.c + v] : 0.f;
   };
-  if (AHEAD) load(t0);
+  load(t0);
   for (int it = 0; it < steps; ++it, t0 -= TILE * S) {
     const int n = ch.L - t0;
-    if (!AHEAD) load(t0);
     Vec<VC> s[SCAN_FRAMES], diff[SCAN_FRAMES];  // the gates; h_{t-1} - x_t
-    Vec<VC> yv[AHEAD ? SCAN_FRAMES : 1], h = hr, lam;
+    Vec<VC> h = hr, lam;
+    Frame<T, VC> yk[SCAN_FRAMES];
 #pragma unroll
     for (int k = 0; k < SCAN_FRAMES; ++k) {
       s[k] = gate_of(gr[k].get());
-      if (AHEAD) yv[k] = yr[k].get();
+      yk[k] = yr[k];
     }
     if (n < SCAN_FRAMES)
 #pragma unroll
       for (int k = 0; k < SCAN_FRAMES; ++k)
-        if (k >= n) s[k] = splat<VC>(0.f);
+        if (k >= n) s[k] = splat<VC>(-0.f);
 #pragma unroll
     for (int k = 0; k < SCAN_FRAMES; ++k) {
-      diff[k] = sub_v(h, xr[k].get());
-      h = fma_v(negated(s[k]), diff[k], pick(s[k], h, xr[k].get()));
+      const Vec<VC> x = xr[k].get();
+      diff[k] = sub_v(h, x);
+      h = advance(s[k], h, x, diff[k]);
     }
-    if (AHEAD) load(t0 - TILE * S);
+    load(t0 - TILE * S);  // under way while the blocks wait for each other
     Vec<VC> A = splat<VC>(1.f), B = splat<VC>(0.f);
 #pragma unroll
     for (int k = SCAN_FRAMES - 1; k >= 0; --k) {
-      const Vec<VC> ns = negated(s[k]);
-      B = decay(ns, s[k], add_v(AHEAD ? yv[k] : yr[k].get(), B));
-      A = decay(ns, s[k], A);
+      B = decay(s[k], add_v(yk[k].get(), B));
+      A = decay(s[k], A);
     }
     compose<VC, LPR, true>(sh, it, S, rank, part, lane, A, B, run, lam);
     const size_t last = (at + (size_t)(t0 + SCAN_FRAMES - 1) * D) * sizeof(T);
     char* ox = reinterpret_cast<char*>(dx) + last;
     char* og = reinterpret_cast<char*>(dg) + last;
 #pragma unroll
-    for (int k = SCAN_FRAMES - 1; k >= 0; --k, ox -= os, og -= os) {
-      const Vec<VC> l = add_v(AHEAD ? yv[k] : yr[k].get(), lam);
-      lam = decay(negated(s[k]), s[k], l);
-      const Frame<T, VC> vx = Frame<T, VC>::of(passed(s[k], l));
-      const Frame<T, VC> vg = Frame<T, VC>::of(mul_v(mul_v(l, diff[k]), slope_of(s[k])));
+    for (int k = SCAN_FRAMES - 1; k >= 0; --k) {
+      const Vec<VC> l = add_v(yk[k].get(), lam);
+      lam = decay(s[k], l);
+      const Vec<VC> pass = passed(s[k], l, negated(l));
+      const Frame<T, VC> vx = Frame<T, VC>::of(pass);
+      // f (1 - f) l (h - x)
+      const Frame<T, VC> vg = Frame<T, VC>::of(mul_v(decay(s[k], pass), diff[k]));
       if (n >= SCAN_FRAMES) {
         *reinterpret_cast<Frame<T, VC>*>(ox) = vx;
         *reinterpret_cast<Frame<T, VC>*>(og) = vg;
@@ -446,6 +415,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
         *reinterpret_cast<Frame<T, VC>*>(ox) = k < n ? vx : Frame<T, VC>::zero();
         *reinterpret_cast<Frame<T, VC>*>(og) = k < n ? vg : Frame<T, VC>::zero();
       }
+      walk(ox, -os);
+      walk(og, -os);
     }
     if (S == 1 && part == 0)
 #pragma unroll
@@ -466,8 +437,9 @@ __global__ void __launch_bounds__(SCAN_THREADS)
   const size_t id = (size_t)blockIdx.x * SCAN_THREADS + threadIdx.x;
   if (id >= (size_t)B * D) return;
   const size_t b = id / D, d = id - b * D;
-  const Vec<1> s = gate_of(Vec<1>{{to_f(g[b * gs + d])}});
-  const float h = advance(s, Vec<1>{{state[id]}}, Vec<1>{{to_f(x[b * xs + d])}}).v[0];
+  const Vec<1> n = gate_of(Vec<1>{{to_f(g[b * gs + d])}});
+  const Vec<1> was = {{state[id]}}, in = {{to_f(x[b * xs + d])}};
+  const float h = advance(n, was, in, sub_v(was, in)).v[0];
   state[id] = h;
   y[id] = from_f<T>(h);
 }
@@ -476,7 +448,7 @@ int check(const char* who, int B, int TT, int D) {
   if (B < 0 || TT < 0 || D <= 0)
     return set_error(kInvalid, "%s: invalid sizes B=%d T=%d D=%d (need B, T >= 0, D > 0)", who, B,
                      TT, D);
-  if ((size_t)B * D / 16 >= 0x7fffffffu / 8 || TT > 0x7fffffff - 8 * 256)
+  if ((size_t)B * D / 8 >= 0x7fffffffu / 8 || TT > 0x7fffffff - 8 * 128)
     return set_error(kUnsupported, "%s: sizes too large", who);
   return kOk;
 }
@@ -491,22 +463,20 @@ unsigned grid_of(int B, int D) {
   return (unsigned)(((size_t)B * D + SCAN_THREADS - 1) / SCAN_THREADS);
 }
 
-// How the channels and the time of a call are spread over blocks.  Whole
-// 128-byte (pairs, float) or 64-byte lines a frame while that gives the SMs
-// three blocks each; else more blocks take part of the time, as many as there
-// are tiles; else half lines.
+// How the channels and the time of a call are spread over blocks: 32 lanes of
+// channels a frame while that gives the SMs three blocks each; else more
+// blocks take part of the time, as many as there are tiles; else fewer lanes.
 struct ScanPlan {
   int lpr, S;
   size_t groups;
 };
 ScanPlan scan_plan(size_t BD, int vc, int TT) {
   ScanPlan p = {32, 1, 0};
-  for (;;) {
+  for (;; p.lpr /= 2) {
     p.groups = (BD + p.lpr * vc - 1) / (p.lpr * vc);
     p.S = 1;
     while (p.S < 8 && p.groups * p.S < 148 * 3 && (long long)p.S * tile_of(p.lpr) < TT) p.S *= 2;
-    if (p.lpr == 16 || p.groups * p.S >= 148 * 3) return p;
-    p.lpr = 16;
+    if (p.lpr == 8 || p.groups * p.S >= 148 * 3) return p;
   }
 }
 
@@ -528,9 +498,17 @@ int launch(const char* who, void (*kernel)(Params...), size_t groups, int S, voi
   return kOk;
 }
 
+template <typename T>
 bool pairs_ok(const void* p, size_t s1, size_t s2) {
-  return (uintptr_t)p % 4 == 0 && s1 % 2 == 0 && s2 % 2 == 0;
+  return (uintptr_t)p % (2 * sizeof(T)) == 0 && s1 % 2 == 0 && s2 % 2 == 0;
 }
+
+// The instance of a kernel for plan p and `pairs`.
+#define TW_SCAN_KERNEL(KERNEL)                                                   \
+  (pairs ? (p.lpr == 32 ? KERNEL<T, 2, 32> : p.lpr == 16 ? KERNEL<T, 2, 16>      \
+                                                         : KERNEL<T, 2, 8>)      \
+         : (p.lpr == 32 ? KERNEL<T, 1, 32> : p.lpr == 16 ? KERNEL<T, 1, 16>      \
+                                                         : KERNEL<T, 1, 8>))
 
 template <typename T>
 int fwd(const void* x, size_t xb, size_t xt, const void* g, size_t gb, size_t gt, const float* h0,
@@ -546,17 +524,11 @@ int fwd(const void* x, size_t xb, size_t xt, const void* g, size_t gb, size_t gt
                      tw_gated_scan_carry_bytes(B, TT, D));
   const char* who = "tw_gated_scan_forward";
   const size_t BD = (size_t)B * D;
-  if constexpr (sizeof(T) == 2) if (D % 2 == 0 && pairs_ok(x, xb, xt) && pairs_ok(g, gb, gt) &&
-                                    pairs_ok(y, 0, 0)) {
-    const ScanPlan p = scan_plan(BD, 2, TT);
-    return launch(who, p.lpr == 32 ? scan_fwd_kernel<T, 2, 32> : scan_fwd_kernel<T, 2, 16>,
-                  p.groups, p.S, stream, (const T*)x, xb, xt, (const T*)g,
-                  gb, gt, h0, lengths, BD, TT, D, p.S, (T*)y, state, (float*)carry);
-  }
-  const ScanPlan p = scan_plan(BD, 1, TT);
-  return launch(who, p.lpr == 32 ? scan_fwd_kernel<T, 1, 32> : scan_fwd_kernel<T, 1, 16>, p.groups,
-                p.S, stream, (const T*)x, xb, xt, (const T*)g,
-                gb, gt, h0, lengths, BD, TT, D, p.S, (T*)y, state, (float*)carry);
+  const bool pairs = D % 2 == 0 && pairs_ok<T>(x, xb, xt) && pairs_ok<T>(g, gb, gt) &&
+                     pairs_ok<T>(y, 0, 0);
+  const ScanPlan p = scan_plan(BD, pairs ? 2 : 1, TT);
+  return launch(who, TW_SCAN_KERNEL(scan_fwd_kernel), p.groups, p.S, stream, (const T*)x, xb, xt,
+                (const T*)g, gb, gt, h0, lengths, BD, TT, D, p.S, (T*)y, state, (float*)carry);
 }
 
 template <typename T>
@@ -573,20 +545,12 @@ int bwd(const void* dy, size_t yb, size_t yt, const float* dstate, const void* x
                      tw_gated_scan_carry_bytes(B, TT, D));
   const char* who = "tw_gated_scan_backward";
   const size_t BD = (size_t)B * D;
-  if constexpr (sizeof(T) == 2) if (D % 2 == 0 && pairs_ok(x, xb, xt) && pairs_ok(g, gb, gt) &&
-                                    pairs_ok(dy, yb, yt) && pairs_ok(dx, 0, 0) &&
-                                    pairs_ok(dg, 0, 0)) {
-    const ScanPlan p = scan_plan(BD, 2, TT);
-    return launch(who, p.lpr == 32 ? scan_bwd_kernel<T, 2, 32> : scan_bwd_kernel<T, 2, 16>,
-                  p.groups, p.S, stream, (const T*)dy, yb, yt, dstate,
-                  (const T*)x, xb, xt, (const T*)g, gb, gt, lengths, (const float*)carry, BD, TT,
-                  D, p.S, (T*)dx, (T*)dg, dh0);
-  }
-  const ScanPlan p = scan_plan(BD, 1, TT);
-  return launch(who, p.lpr == 32 ? scan_bwd_kernel<T, 1, 32> : scan_bwd_kernel<T, 1, 16>, p.groups,
-                p.S, stream, (const T*)dy, yb, yt, dstate,
-                (const T*)x, xb, xt, (const T*)g, gb, gt, lengths, (const float*)carry, BD, TT, D,
-                p.S, (T*)dx, (T*)dg, dh0);
+  const bool pairs = D % 2 == 0 && pairs_ok<T>(x, xb, xt) && pairs_ok<T>(g, gb, gt) &&
+                     pairs_ok<T>(dy, yb, yt) && pairs_ok<T>(dx, 0, 0) && pairs_ok<T>(dg, 0, 0);
+  const ScanPlan p = scan_plan(BD, pairs ? 2 : 1, TT);
+  return launch(who, TW_SCAN_KERNEL(scan_bwd_kernel), p.groups, p.S, stream, (const T*)dy, yb, yt,
+                dstate, (const T*)x, xb, xt, (const T*)g, gb, gt, lengths, (const float*)carry, BD,
+                TT, D, p.S, (T*)dx, (T*)dg, dh0);
 }
 
 template <typename T>

@@ -41,6 +41,63 @@ __device__ __forceinline__ float row_sum(float v, int tpr, float* red) {
   }
 }
 
+// N values of a thread, two an instruction where N is even.
+template <int N> struct Width { static constexpr int W = N % 2 == 0 ? 2 : 1; };
+template <int N>
+__device__ __forceinline__ Vec<Width<N>::W> at(const float* v, int i) {
+  Vec<Width<N>::W> r;
+#pragma unroll
+  for (int k = 0; k < Width<N>::W; ++k) r.v[k] = v[i + k];
+  return r;
+}
+template <int N>
+__device__ __forceinline__ void put(float* v, int i, Vec<Width<N>::W> r) {
+#pragma unroll
+  for (int k = 0; k < Width<N>::W; ++k) v[i + k] = r.v[k];
+}
+#define TW_EACH for (int i = 0, W = Width<N>::W; i < N; i += W)
+template <int N> __device__ __forceinline__ void shift_n(float* v, float c) {
+#pragma unroll
+  TW_EACH put<N>(v, i, add_v(at<N>(v, i), splat<Width<N>::W>(c)));
+}
+template <int N> __device__ __forceinline__ void scale_n(float* v, float c) {
+#pragma unroll
+  TW_EACH put<N>(v, i, mul_v(at<N>(v, i), splat<Width<N>::W>(c)));
+}
+template <int N> __device__ __forceinline__ void times_n(float* v, const float* p) {
+#pragma unroll
+  TW_EACH put<N>(v, i, mul_v(at<N>(v, i), at<N>(p, i)));
+}
+template <int N> __device__ __forceinline__ void plus_n(float* v, const float* p) {
+#pragma unroll
+  TW_EACH put<N>(v, i, add_v(at<N>(v, i), at<N>(p, i)));
+}
+template <int N>  // v += p q
+__device__ __forceinline__ void fma_n(float* v, const float* p, const float* q) {
+#pragma unroll
+  TW_EACH put<N>(v, i, fma_v(at<N>(p, i), at<N>(q, i), at<N>(v, i)));
+}
+template <int N> __device__ __forceinline__ float total(Vec<Width<N>::W> s) {
+  float t = s.v[0];
+  if (Width<N>::W == 2) t += s.v[Width<N>::W - 1];
+  return t;
+}
+template <int N> __device__ __forceinline__ float sum_of(const float* v) {
+  Vec<Width<N>::W> s = splat<Width<N>::W>(0.f);
+#pragma unroll
+  TW_EACH s = add_v(s, at<N>(v, i));
+  return total<N>(s);
+}
+template <int N> __device__ __forceinline__ float dot_of(const float* p, const float* q) {
+  Vec<Width<N>::W> s = splat<Width<N>::W>(0.f);
+#pragma unroll
+  TW_EACH s = fma_v(at<N>(p, i), at<N>(q, i), s);
+  return total<N>(s);
+}
+template <int N> __device__ __forceinline__ float square_sum_of(const float* v) {
+  return dot_of<N>(v, v);
+}
+
 // Rows that fit the registers of `tpr` threads, E values each (VEC: in
 // 16-byte pieces, so that a row is read with whole-sector loads; else value
 // by value, neighbours in neighbouring lanes).  BLOCK: one row a block, else
@@ -49,17 +106,17 @@ __device__ __forceinline__ float row_sum(float v, int tpr, float* red) {
 template <typename T, typename P, bool VEC, int E, bool BLOCK>
 __global__ void __launch_bounds__(LN_THREADS)
     ln_fwd_kernel(const T* __restrict__ x, size_t xs, const P* __restrict__ w,
-                  const P* __restrict__ b, size_t rows, int D, int tpr, float eps,
+                  const P* __restrict__ b, size_t rows, int D, int tpr_log, float inv_d, float eps,
                   T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
   constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, NV = E / V;
   __shared__ float red[LN_THREADS / 32];
+  const int tpr = BLOCK ? blockDim.x : 1 << tpr_log;
   const int t = BLOCK ? threadIdx.x : threadIdx.x & (tpr - 1);
   const size_t r = BLOCK ? blockIdx.x
-                         : (size_t)blockIdx.x * (LN_THREADS / tpr) + threadIdx.x / tpr;
+                         : ((size_t)blockIdx.x * LN_THREADS + threadIdx.x) >> tpr_log;
   const bool in = r < rows;
   const T* xr = x + (in ? r : rows - 1) * xs;
   float v[E];
-  float s = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int d = (j * tpr + t) * V;
@@ -70,36 +127,26 @@ __global__ void __launch_bounds__(LN_THREADS)
       for (int q = 0; q < V; ++q) v[j * V + q] = 0.f;
     }
   }
-#pragma unroll
-  for (int i = 0; i < E; ++i) s += v[i];
-  const float mu = row_sum<BLOCK>(s, tpr, red) / D;
-  s = 0.f;
+  const float mu = row_sum<BLOCK>(sum_of<E>(v), tpr, red) * inv_d;
 #pragma unroll
   for (int j = 0; j < NV; ++j)
-    if ((j * tpr + t) * V < D)
-#pragma unroll
-      for (int q = 0; q < V; ++q) {
-        v[j * V + q] -= mu;
-        s = fmaf(v[j * V + q], v[j * V + q], s);
-      }
-  const float rs = 1.f / sqrtf(row_sum<BLOCK>(s, tpr, red) / D + eps);
+    if ((j * tpr + t) * V < D) shift_n<V>(v + j * V, -mu);
+  const float rs = rsqrtf(row_sum<BLOCK>(square_sum_of<E>(v), tpr, red) * inv_d + eps);
   if (!in) return;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int d = (j * tpr + t) * V;
     if (d < D) {
-      float o[V], p[V];
-#pragma unroll
-      for (int q = 0; q < V; ++q) o[q] = mul_rn(v[j * V + q], rs);
+      float* o = v + j * V;
+      float p[V];
+      scale_n<V>(o, rs);
       if (w) {
         load_n<VEC, V>(w + d, p);
-#pragma unroll
-        for (int q = 0; q < V; ++q) o[q] = mul_rn(o[q], p[q]);
+        times_n<V>(o, p);
       }
       if (b) {
         load_n<VEC, V>(b + d, p);
-#pragma unroll
-        for (int q = 0; q < V; ++q) o[q] = add_rn(o[q], p[q]);
+        plus_n<V>(o, p);
       }
       store_n<VEC, V>(y + r * D + d, o);
     }
@@ -155,23 +202,17 @@ __global__ void __launch_bounds__(BLOCK ? LN_THREADS : BWD_THREADS, BLOCK ? 1 : 
       float g[V], h[V];
       gr[j].get(g);
       hr[j].get(h);
-#pragma unroll
-      for (int q = 0; q < V; ++q) {
-        h[q] = (h[q] - mu) * rs;
-        ab[j * V + q] += g[q];
-        aw[j * V + q] = fmaf(g[q], h[q], aw[j * V + q]);
-      }
+      shift_n<V>(h, -mu);
+      scale_n<V>(h, rs);
+      plus_n<V>(ab + j * V, g);
+      fma_n<V>(aw + j * V, g, h);
       if (w && d < D) {
         float wv[V];
         load_n<VEC, V>(w + d, wv);
-#pragma unroll
-        for (int q = 0; q < V; ++q) g[q] *= wv[q];
+        times_n<V>(g, wv);
       }
-#pragma unroll
-      for (int q = 0; q < V; ++q) {
-        s1 += g[q];
-        s2 = fmaf(g[q], h[q], s2);
-      }
+      s1 += sum_of<V>(g);
+      s2 += dot_of<V>(g, h);
     }
     if (dx) {
       const float c1 = row_sum<BLOCK>(s1, tpr, red) * inv_d;
@@ -186,11 +227,14 @@ __global__ void __launch_bounds__(BLOCK ? LN_THREADS : BWD_THREADS, BLOCK ? 1 : 
           if (w) {
             float wv[V];
             load_n<VEC, V>(w + d, wv);
-#pragma unroll
-            for (int q = 0; q < V; ++q) g[q] *= wv[q];
+            times_n<V>(g, wv);
           }
-#pragma unroll
-          for (int q = 0; q < V; ++q) g[q] = rs * (g[q] - c1 - (h[q] - mu) * rs * c2);
+          shift_n<V>(h, -mu);
+          scale_n<V>(h, rs);
+          scale_n<V>(h, -c2);
+          shift_n<V>(g, -c1);
+          plus_n<V>(g, h);
+          scale_n<V>(g, rs);
           store_n<VEC, V>(dx + r * D + d, g);
         }
       }
@@ -285,7 +329,7 @@ __global__ void __launch_bounds__(LN_THREADS)
       const float c = to_f(xr[d]) - mu;
       s = fmaf(c, c, s);
     }
-    const float rs = 1.f / sqrtf(block_sum(s, red) / D + eps);
+    const float rs = rsqrtf(block_sum(s, red) / D + eps);
     for (int d = threadIdx.x; d < D; d += LN_THREADS) {
       const float xh = mul_rn(to_f(xr[d]) - mu, rs);
       y[r * D + d] = from_f<T>(add_rn(mul_rn(xh, w ? to_f(w[d]) : 1.f), b ? to_f(b[d]) : 0.f));
@@ -399,6 +443,12 @@ bool aligned16(const void* p, size_t stride_bytes) {
   return (uintptr_t)p % 16 == 0 && stride_bytes % 16 == 0;
 }
 
+int log2_of(int n) {
+  int l = 0;
+  while ((1 << l) < n) ++l;
+  return l;
+}
+
 // The instance of a row kernel for a plan.
 #define TW_ROW_KERNEL(KERNEL)                                                          \
   (!vec ? (plan.tpr > 32 ? KERNEL<T, P, false, 16, true>                               \
@@ -422,7 +472,8 @@ int fwd_p(const void* x, size_t xs, const void* w, const void* b, size_t rows, i
   if (blocks > 0x7fffffff) return set_error(kUnsupported, "tw_layer_norm_forward: too many rows");
   auto kernel = TW_ROW_KERNEL(ln_fwd_kernel);
   kernel<<<(unsigned)blocks, plan.tpr > 32 ? plan.tpr : LN_THREADS, 0, st>>>(
-      (const T*)x, xs, (const P*)w, (const P*)b, rows, D, plan.tpr, eps, (T*)y, mean, rstd);
+      (const T*)x, xs, (const P*)w, (const P*)b, rows, D, log2_of(plan.tpr), 1.f / D, eps,
+      (T*)y, mean, rstd);
   return launched("tw_layer_norm_forward");
 }
 

@@ -71,17 +71,6 @@ __device__ __forceinline__ float scatter_sum(float (&v)[C], int lane) {
   return s;
 }
 
-template <bool FAST>
-__device__ __forceinline__ float activate1(float v, int act) {
-  switch (act) {
-    case kActRelu: return act_value<kActRelu, FAST>(v);
-    case kActGelu: return act_value<kActGelu, FAST>(v);
-    case kActSilu: return act_value<kActSilu, FAST>(v);
-    case kActSigmoid: return act_value<kActSigmoid, FAST>(v);
-    default: return v;
-  }
-}
-
 // M <= MT rows: a warp owns 4 output columns, its lanes the contraction.
 // Bound by the one read of the weight; x stays in the caches.
 template <typename T, int MT, bool VEC>
@@ -235,11 +224,15 @@ __device__ __forceinline__ void pack_block(const PackJob<T>& j, int bx, int by, 
         if (ACT != kActNone) zv[i] = c0 + i < C ? to_f(zp[i]) : 0.f;
       }
     }
+    if (ACT != kActNone)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (ACT != kActNone) v[i] *= act_slope<ACT, sizeof(T) == 2>(zv[i]);
-      s[i] += v[i];
-    }
+      for (int i = 0; i < 8; i += 2) {
+        const Vec<2> d = act_slope<ACT, sizeof(T) == 2>(Vec<2>{{zv[i], zv[i + 1]}});
+        v[i] *= d.v[0];
+        v[i + 1] *= d.v[1];
+      }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] += v[i];
     if (dst) {
       E* o = dst + (size_t)r * Cp + c0;
       if constexpr (PL == 3) {

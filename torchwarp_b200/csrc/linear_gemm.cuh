@@ -229,27 +229,23 @@ __device__ __forceinline__ void free_tmem(uint32_t addr, unsigned cols) {
     tmem_dealloc(addr, cols);
 }
 
+template <int ACT, bool FAST>
+__device__ __forceinline__ void activate_all(float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    const Vec<2> r = act_value<ACT, FAST>(Vec<2>{{v[i], v[i + 1]}});
+    v[i] = r.v[0];
+    v[i + 1] = r.v[1];
+  }
+}
 template <bool FAST>
 __device__ __forceinline__ void activate(float (&v)[32], int act) {
   switch (act) {
-    case kActRelu:
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = act_value<kActRelu, FAST>(v[i]);
-      break;
-    case kActGelu:
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = act_value<kActGelu, FAST>(v[i]);
-      break;
-    case kActSilu:
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = act_value<kActSilu, FAST>(v[i]);
-      break;
-    case kActSigmoid:
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = act_value<kActSigmoid, FAST>(v[i]);
-      break;
-    default:
-      break;
+    case kActRelu: activate_all<kActRelu, FAST>(v); break;
+    case kActGelu: activate_all<kActGelu, FAST>(v); break;
+    case kActSilu: activate_all<kActSilu, FAST>(v); break;
+    case kActSigmoid: activate_all<kActSigmoid, FAST>(v); break;
+    default: break;
   }
 }
 
@@ -634,13 +630,7 @@ __global__ void __launch_bounds__(256)
     const size_t m = i / g.N, c = i - m * g.N;
     if (g.bias) v = add_rn(v, to_f(g.bias[c]));
     if (g.z) g.z[i] = from_f<T>(v);
-    switch (g.act) {
-      case kActRelu: v = act_value<kActRelu, FAST>(v); break;
-      case kActGelu: v = act_value<kActGelu, FAST>(v); break;
-      case kActSilu: v = act_value<kActSilu, FAST>(v); break;
-      case kActSigmoid: v = act_value<kActSigmoid, FAST>(v); break;
-      default: break;
-    }
+    v = activate1<FAST>(v, g.act);
     if (g.res) v = add_rn(v, to_f(g.res[m * g.ldr + c]));
     g.out[i] = from_f<T>(v);
   }
