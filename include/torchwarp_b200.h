@@ -455,11 +455,14 @@ int tw_linear_backward_f16(const void* dy, size_t lddy, const void* x, size_t ld
  * (zeros); lengths [B] or NULL: from frame lengths[b] on a sequence keeps its
  * state, its outputs and gradients are 0 and its inputs are not read.
  * y [B, T, D], state [B, D] float32: the last state.  carry: states saved for
- * the backward (tw_gated_scan_carry_bytes), or NULL.
+ * the backward, tw_gated_scan_carry_bytes; without a backward a scratch of
+ * tw_gated_scan_workspace_bytes, or NULL (a long sequence of few channels is
+ * then not cut into parts that run at once).  16-byte aligned.
  * Backward for dL/dy and dL/dstate (NULL: none): dx, dgate [B, T, D], dh0
- * [B, D] float32 or NULL.
+ * [B, D] float32 or NULL; workspace: tw_gated_scan_workspace_bytes.
  * Step: one frame, x, gate, y [B, D]; state is updated in place. */
-size_t tw_gated_scan_carry_bytes(int B, int T, int D);
+size_t tw_gated_scan_carry_bytes(int B, int T, int D, int dtype_bytes);
+size_t tw_gated_scan_workspace_bytes(int B, int T, int D, int dtype_bytes);
 int tw_gated_scan_forward_f32(const void* x, size_t x_batch, size_t x_time, const void* gate,
                               size_t g_batch, size_t g_time, const float* h0,
                               const int64_t* lengths, int B, int T, int D, void* y, float* state,
@@ -469,7 +472,7 @@ int tw_gated_scan_backward_f32(const void* dy, size_t dy_batch, size_t dy_time,
                                const void* gate, size_t g_batch, size_t g_time,
                                const int64_t* lengths, const void* carry, size_t carry_bytes,
                                int B, int T, int D, void* dx, void* dgate, float* dh0,
-                               void* stream);
+                               void* workspace, size_t ws_bytes, void* stream);
 int tw_gated_scan_step_f32(const void* x, size_t x_batch, const void* gate, size_t g_batch,
                            float* state, int B, int D, void* y, void* stream);
 int tw_gated_scan_forward_bf16(const void* x, size_t x_batch, size_t x_time, const void* gate,
@@ -481,7 +484,7 @@ int tw_gated_scan_backward_bf16(const void* dy, size_t dy_batch, size_t dy_time,
                                const void* gate, size_t g_batch, size_t g_time,
                                const int64_t* lengths, const void* carry, size_t carry_bytes,
                                int B, int T, int D, void* dx, void* dgate, float* dh0,
-                               void* stream);
+                               void* workspace, size_t ws_bytes, void* stream);
 int tw_gated_scan_step_bf16(const void* x, size_t x_batch, const void* gate, size_t g_batch,
                            float* state, int B, int D, void* y, void* stream);
 int tw_gated_scan_forward_f16(const void* x, size_t x_batch, size_t x_time, const void* gate,
@@ -493,7 +496,7 @@ int tw_gated_scan_backward_f16(const void* dy, size_t dy_batch, size_t dy_time,
                                const void* gate, size_t g_batch, size_t g_time,
                                const int64_t* lengths, const void* carry, size_t carry_bytes,
                                int B, int T, int D, void* dx, void* dgate, float* dh0,
-                               void* stream);
+                               void* workspace, size_t ws_bytes, void* stream);
 int tw_gated_scan_step_f16(const void* x, size_t x_batch, const void* gate, size_t g_batch,
                            float* state, int B, int D, void* y, void* stream);
 

@@ -96,7 +96,8 @@ SIGNATURES = {
     "tw_optimal_path_f64": (_c_i, [_c_p] + [_c_i] * 6 + [_c_p] * 5),
     "tw_layer_norm_workspace_bytes": (_c_sz, [_c_sz, _c_i]),
     "tw_linear_workspace_bytes": (_c_sz, [_c_i] * 7),
-    "tw_gated_scan_carry_bytes": (_c_sz, [_c_i] * 3),
+    "tw_gated_scan_carry_bytes": (_c_sz, [_c_i] * 4),
+    "tw_gated_scan_workspace_bytes": (_c_sz, [_c_i] * 4),
 }
 
 # the encoder operators, one entry per element type
@@ -113,7 +114,7 @@ for _t in ("f32", "bf16", "f16"):
         "tw_gated_scan_forward_" + _t: (_c_i, [_c_p, _c_sz, _c_sz] * 2 + [_c_p] * 2 + [_c_i] * 3
                                         + [_c_p] * 3 + [_c_sz, _c_p]),
         "tw_gated_scan_backward_" + _t: (_c_i, [_c_p, _c_sz, _c_sz, _c_p] + [_c_p, _c_sz, _c_sz] * 2
-                                         + [_c_p] * 2 + [_c_sz] + [_c_i] * 3 + [_c_p] * 4),
+                                         + [_c_p] * 2 + [_c_sz] + [_c_i] * 3 + [_c_p] * 4 + [_c_sz, _c_p]),
         "tw_gated_scan_step_" + _t: (_c_i, [_c_p, _c_sz] * 2 + [_c_p] + [_c_i] * 2 + [_c_p] * 2),
         "tw_adamw_step_" + _t: (_c_i, [_c_p, _c_i, _c_i] + [_c_p] * 5 + [_c_d, _c_p] + [_c_d] * 4
                                 + [_c_sz, _c_p]),

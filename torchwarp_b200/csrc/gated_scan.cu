@@ -10,30 +10,44 @@
 // there are 0, its gradients 0, and x and g are not read.
 //
 // One pass over the data.  The channels of all sequences, c = b D + d, are
-// numbered through; a block of 128 threads owns 32 lanes of channel pairs (or
-// 16, or 8) and walks time in tiles of 4 (8, 16) runs of 8 frames.  A thread
-// reads its 8 frames into registers, composes them to (A, B) with h_out = A
-// h_in + B, learns its h_in from the runs before it, and goes over its frames
-// again in registers to write the outputs.  Few channels: up to 8 blocks of a
-// cluster take neighbouring tiles and compose their (A, B) through each
-// other's shared memory, so that a long sequence still fills the GPU.
+// numbered through; a block of 128 threads owns a line of them (128 or 64
+// bytes a frame, two channels a lane) and walks time in tiles of 4 to 16 runs
+// of 16 frames (8 of float32).  cp.async brings a tile to shared memory while
+// the one before it is worked on.  A thread composes the frames of its run to
+// (A, B) with h_out = A h_in + B, learns its h_in from the runs before it, and
+// goes over its frames again to write the outputs in the place of the inputs,
+// from where whole 16-byte pieces go out.  Few channels: time is cut into
+// segments, a first kernel composes each to one (A, B), and a segment's blocks
+// start from what the segments before them give.  That reads two arrays twice,
+// and still took 38 us forward and 54 us backward for 1 x 32768 x 256 float32
+// where 8 blocks of a cluster, exchanging (A, B) at every tile, took 105 and
+// 127: a step of those waits for the slowest of the 8.
 // Everything is summed in a fixed order.
 //
-// The forward saves h before every 8th frame in float32 (0.5 bytes a value);
-// the backward recomputes the states of a thread's frames from it, so no
-// rounded output enters a gradient and the outputs are not read again.  8
-// frames of two channels, the next tile's loads under way among them, fit 128
-// registers; 16 did not (32 x 1024 x 1024 bfloat16: 200 us with the spills).
+// The forward saves h before every run in float32 (0.25 bytes a 16-bit value,
+// 0.5 a float32 one); the backward recomputes the states of a run from it, so
+// no rounded output enters a gradient and the outputs are not read again.
+//
+// Rows that are not 16-byte aligned take a second form, one channel a lane,
+// whose frames go through registers: there each frame's address costs the
+// instructions that a 16-byte copy shares among 4 to 8 values.  Its long
+// sequences of few channels are shared by up to 8 blocks of a cluster, which
+// take neighbouring tiles and compose their (A, B) through each other's shared
+// memory.
 #include "../../include/torchwarp_b200.h"
 #include "element.cuh"
 
 namespace tw {
 namespace {
 
-constexpr int SCAN_FRAMES = 8;  // of a thread
 constexpr int SCAN_THREADS = 128;
+// Frames of a run: what a thread holds of the gates (and in the backward of
+// the differences) of two channels without spilling.
+constexpr int frames_of(size_t type_bytes) { return type_bytes == 4 ? 8 : 16; }
 // LPR lanes a frame: 128 / LPR runs a tile.
-constexpr int tile_of(int lpr) { return SCAN_THREADS / lpr * SCAN_FRAMES; }
+constexpr int tile_of(int lpr, size_t type_bytes) {
+  return SCAN_THREADS / lpr * frames_of(type_bytes);
+}
 
 __device__ __forceinline__ int live_len(const int64_t* lengths, int b, int T) {
   if (!lengths) return T;
@@ -119,18 +133,18 @@ __device__ __forceinline__ void walk(P*& p, S step) {
 
 // A thread's frames from p on, `step` bytes apart; frames from `n` on are zero
 // and not read.
-template <typename T, int VC>
-__device__ __forceinline__ void load_frames(Frame<T, VC> (&f)[SCAN_FRAMES], const char* p,
+template <typename T, int VC, int FR>
+__device__ __forceinline__ void load_frames(Frame<T, VC> (&f)[FR], const char* p,
                                             size_t step, int n) {
-  if (n >= SCAN_FRAMES) {
+  if (n >= FR) {
 #pragma unroll
-    for (int k = 0; k < SCAN_FRAMES; ++k) {
+    for (int k = 0; k < FR; ++k) {
       f[k] = *reinterpret_cast<const Frame<T, VC>*>(p);
       walk(p, step);
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < SCAN_FRAMES; ++k) {
+    for (int k = 0; k < FR; ++k) {
       f[k] = k < n ? *reinterpret_cast<const Frame<T, VC>*>(p) : Frame<T, VC>::zero();
       walk(p, step);
     }
@@ -248,7 +262,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
                     size_t gb, size_t gt, const float* __restrict__ h0,
                     const int64_t* __restrict__ lengths, size_t BD, int TT, int D, int S,
                     T* __restrict__ y, float* __restrict__ state, float* __restrict__ carry) {
-  constexpr int TILE = tile_of(LPR);
+  constexpr int FR = frames_of(sizeof(T)), TILE = tile_of(LPR, sizeof(T));
   __shared__ ScanShared<VC, LPR> sh;
   const int part = threadIdx.x / LPR, lane = threadIdx.x & (LPR - 1);
   const int rank = blockIdx.x % S;
@@ -264,30 +278,30 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
     if (part == 0) sh.start[0][lane * VC + v] = run.v[v];
   }
   const int steps = (TT + TILE * S - 1) / (TILE * S);
-  int t0 = rank * TILE + part * SCAN_FRAMES;
-  Frame<T, VC> xr[SCAN_FRAMES], gr[SCAN_FRAMES];
-  load_frames<T, VC>(gr, gp + (size_t)t0 * gs, gs, ch.L - t0);
-  load_frames<T, VC>(xr, xp + (size_t)t0 * xs, xs, ch.L - t0);
+  int t0 = rank * TILE + part * FR;
+  Frame<T, VC> xr[FR], gr[FR];
+  load_frames(gr, gp + (size_t)t0 * gs, gs, ch.L - t0);
+  load_frames(xr, xp + (size_t)t0 * xs, xs, ch.L - t0);
   for (int it = 0; it < steps; ++it, t0 += TILE * S) {
     const int n = ch.L - t0;
-    Vec<VC> s[SCAN_FRAMES];
-    Frame<T, VC> xk[SCAN_FRAMES];  // as it lies: pairs in one register
+    Vec<VC> s[FR];
+    Frame<T, VC> xk[FR];  // as it lies: pairs in one register
 #pragma unroll
-    for (int k = 0; k < SCAN_FRAMES; ++k) {
+    for (int k = 0; k < FR; ++k) {
       s[k] = gate_of(gr[k].get());
       xk[k] = xr[k];
     }
-    if (n < SCAN_FRAMES)
+    if (n < FR)
 #pragma unroll
-      for (int k = 0; k < SCAN_FRAMES; ++k)
+      for (int k = 0; k < FR; ++k)
         if (k >= n) s[k] = splat<VC>(-0.f);
     // the next tile's loads are under way while the blocks wait for each other
     const int t1 = t0 + TILE * S;
-    load_frames<T, VC>(gr, gp + (size_t)t1 * gs, gs, ch.L - t1);
-    load_frames<T, VC>(xr, xp + (size_t)t1 * xs, xs, ch.L - t1);
+    load_frames(gr, gp + (size_t)t1 * gs, gs, ch.L - t1);
+    load_frames(xr, xp + (size_t)t1 * xs, xs, ch.L - t1);
     Vec<VC> A = splat<VC>(1.f), B = splat<VC>(0.f), h;
 #pragma unroll
-    for (int k = 0; k < SCAN_FRAMES; ++k) {
+    for (int k = 0; k < FR; ++k) {
       const Vec<VC> x = xk[k].get();
       B = advance(s[k], B, x, sub_v(B, x));
       A = decay(s[k], A);
@@ -296,11 +310,11 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
     if (carry && ch.live && t0 < TT)
 #pragma unroll
       for (int v = 0; v < VC; ++v)
-        carry[(size_t)(t0 / SCAN_FRAMES) * BD + ch.c + v] = h.v[v];
+        carry[(size_t)(t0 / FR) * BD + ch.c + v] = h.v[v];
     char* o = yp + (size_t)t0 * ys;
-    if (n >= SCAN_FRAMES) {
+    if (n >= FR) {
 #pragma unroll
-      for (int k = 0; k < SCAN_FRAMES; ++k) {
+      for (int k = 0; k < FR; ++k) {
         const Vec<VC> x = xk[k].get();
         h = advance(s[k], h, x, sub_v(h, x));
         *reinterpret_cast<Frame<T, VC>*>(o) = Frame<T, VC>::of(h);
@@ -308,7 +322,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < SCAN_FRAMES; ++k) {
+      for (int k = 0; k < FR; ++k) {
         const Vec<VC> x = xk[k].get();
         h = advance(s[k], h, x, sub_v(h, x));
         if (ch.live && t0 + k < TT)
@@ -337,7 +351,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
                     const int64_t* __restrict__ lengths, const float* __restrict__ carry,
                     size_t BD, int TT, int D, int S, T* __restrict__ dx, T* __restrict__ dg,
                     float* __restrict__ dh0) {
-  constexpr int TILE = tile_of(LPR);
+  constexpr int FR = frames_of(sizeof(T)), TILE = tile_of(LPR, sizeof(T));
   __shared__ ScanShared<VC, LPR> sh;
   const int part = threadIdx.x / LPR, lane = threadIdx.x & (LPR - 1);
   const int rank = blockIdx.x % S;
@@ -355,36 +369,36 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
     if (part == 0) sh.start[0][lane * VC + v] = run.v[v];
   }
   const int steps = (TT + TILE * S - 1) / (TILE * S);
-  int t0 = ((steps - 1) * S + rank) * TILE + part * SCAN_FRAMES;
-  Frame<T, VC> xr[SCAN_FRAMES], gr[SCAN_FRAMES], yr[SCAN_FRAMES];
+  int t0 = ((steps - 1) * S + rank) * TILE + part * FR;
+  Frame<T, VC> xr[FR], gr[FR], yr[FR];
   Vec<VC> hr;
   auto load = [&](int t) {
     const int n = t >= 0 ? ch.L - t : 0;
     const size_t tt = t >= 0 ? t : 0;
-    load_frames<T, VC>(gr, gp + tt * gs, gs, n);
-    load_frames<T, VC>(yr, yp + tt * ys, ys, n);
-    load_frames<T, VC>(xr, xp + tt * xs, xs, n);
+    load_frames(gr, gp + tt * gs, gs, n);
+    load_frames(yr, yp + tt * ys, ys, n);
+    load_frames(xr, xp + tt * xs, xs, n);
 #pragma unroll
     for (int v = 0; v < VC; ++v)
-      hr.v[v] = n > 0 ? carry[(tt / SCAN_FRAMES) * BD + ch.c + v] : 0.f;
+      hr.v[v] = n > 0 ? carry[(tt / FR) * BD + ch.c + v] : 0.f;
   };
   load(t0);
   for (int it = 0; it < steps; ++it, t0 -= TILE * S) {
     const int n = ch.L - t0;
-    Vec<VC> s[SCAN_FRAMES], diff[SCAN_FRAMES];  // the gates; h_{t-1} - x_t
+    Vec<VC> s[FR], diff[FR];  // the gates; h_{t-1} - x_t
     Vec<VC> h = hr, lam;
-    Frame<T, VC> yk[SCAN_FRAMES];
+    Frame<T, VC> yk[FR];
 #pragma unroll
-    for (int k = 0; k < SCAN_FRAMES; ++k) {
+    for (int k = 0; k < FR; ++k) {
       s[k] = gate_of(gr[k].get());
       yk[k] = yr[k];
     }
-    if (n < SCAN_FRAMES)
+    if (n < FR)
 #pragma unroll
-      for (int k = 0; k < SCAN_FRAMES; ++k)
+      for (int k = 0; k < FR; ++k)
         if (k >= n) s[k] = splat<VC>(-0.f);
 #pragma unroll
-    for (int k = 0; k < SCAN_FRAMES; ++k) {
+    for (int k = 0; k < FR; ++k) {
       const Vec<VC> x = xr[k].get();
       diff[k] = sub_v(h, x);
       h = advance(s[k], h, x, diff[k]);
@@ -392,23 +406,23 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
     load(t0 - TILE * S);  // under way while the blocks wait for each other
     Vec<VC> A = splat<VC>(1.f), B = splat<VC>(0.f);
 #pragma unroll
-    for (int k = SCAN_FRAMES - 1; k >= 0; --k) {
+    for (int k = FR - 1; k >= 0; --k) {
       B = decay(s[k], add_v(yk[k].get(), B));
       A = decay(s[k], A);
     }
     compose<VC, LPR, true>(sh, it, S, rank, part, lane, A, B, run, lam);
-    const size_t last = (at + (size_t)(t0 + SCAN_FRAMES - 1) * D) * sizeof(T);
+    const size_t last = (at + (size_t)(t0 + FR - 1) * D) * sizeof(T);
     char* ox = reinterpret_cast<char*>(dx) + last;
     char* og = reinterpret_cast<char*>(dg) + last;
 #pragma unroll
-    for (int k = SCAN_FRAMES - 1; k >= 0; --k) {
+    for (int k = FR - 1; k >= 0; --k) {
       const Vec<VC> l = add_v(yk[k].get(), lam);
       lam = decay(s[k], l);
       const Vec<VC> pass = passed(s[k], l, negated(l));
       const Frame<T, VC> vx = Frame<T, VC>::of(pass);
       // f (1 - f) l (h - x)
       const Frame<T, VC> vg = Frame<T, VC>::of(mul_v(decay(s[k], pass), diff[k]));
-      if (n >= SCAN_FRAMES) {
+      if (n >= FR) {
         *reinterpret_cast<Frame<T, VC>*>(ox) = vx;
         *reinterpret_cast<Frame<T, VC>*>(og) = vg;
       } else if (ch.live && t0 + k < TT) {
@@ -428,6 +442,366 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
     for (int v = 0; v < VC; ++v)
       dh0[ch.c + v] = S > 1 ? run.v[v] : sh.start[steps & 1][lane * VC + v];
   if (S > 1) cluster_sync_all();
+}
+
+// ------------------------------------------- tiles in shared memory
+
+// Like common.cuh's, and a barrier to the compiler: a slot is refilled after
+// it was read.
+__device__ __forceinline__ void fetch16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src),
+               "r"(in ? 16 : 0)
+               : "memory");
+}
+
+template <typename T, int LPR> struct Staged {
+  static constexpr int FR = frames_of(sizeof(T)), RUNS = SCAN_THREADS / LPR;
+  static constexpr int TILE = tile_of(LPR, sizeof(T));
+  static constexpr int LINE = LPR * 2 * (int)sizeof(T);              // bytes a frame
+  static constexpr int PITCH = FR * LINE;                            // of a run
+  static constexpr int SLOT = RUNS * PITCH;                          // of an array's tile
+  // Half lines: odd runs swap neighbouring frames, so that the two runs that a
+  // half-warp reads at once lie in different banks.
+  static constexpr bool SWAP = LINE < 128;
+  static constexpr int CPL = LINE / 16, ROWS = SCAN_THREADS / CPL;   // 16-byte pieces of a frame
+  static constexpr int PASSES = TILE / ROWS, STEP = ROWS / FR * PITCH;
+  static constexpr int STAGES = 2;
+};
+
+// A run's frames of a lane in a slot.
+template <typename T, int LPR> struct RunFrames {
+  using G = Staged<T, LPR>;
+  using F = Frame<T, 2>;
+  F* even;
+  F* odd;
+  __device__ __forceinline__ RunFrames(uint8_t* slot, int part, int lane) {
+    F* p = reinterpret_cast<F*>(slot + part * G::PITCH) + lane;
+    const int by = G::SWAP && (part & 1) ? LPR : 0;
+    even = p + by;
+    odd = p - by;
+  }
+  __device__ __forceinline__ F& operator[](int k) const { return (k & 1 ? odd : even)[k * LPR]; }
+};
+
+// A thread's share of moving tiles: piece `threadIdx % CPL` of every ROWS-th
+// frame.
+template <typename T, int LPR> struct Mover {
+  using G = Staged<T, LPR>;
+  size_t b, d;
+  bool live;
+  int L, row;
+  uint32_t at;  // in a slot
+  __device__ __forceinline__ Mover(size_t first, size_t BD, int D, int TT,
+                                   const int64_t* lengths) {
+    const int piece = threadIdx.x % G::CPL;
+    row = threadIdx.x / G::CPL;
+    const size_t c = first + piece * (16 / sizeof(T));
+    live = c < BD;
+    b = live ? c / D : 0;
+    d = live ? c - b * D : 0;
+    L = live ? live_len(lengths, (int)b, TT) : 0;
+    const int r = row / G::FR, k = row % G::FR;
+    at = r * G::PITCH + (G::SWAP ? k ^ (r & 1) : k) * G::LINE + piece * 16;
+  }
+  // frames t.. of an array (its frames `step` bytes apart, p at this thread's
+  // piece of frame 0) into the slot at shared address `slot`; past L: zeros
+  __device__ __forceinline__ void fetch(uint32_t slot, const char* p, size_t step, int t) const {
+    const char* q = p + (size_t)(t + row) * step;
+#pragma unroll
+    for (int i = 0; i < G::PASSES; ++i) {
+      const bool in = t + row + i * G::ROWS < L;
+      fetch16(slot + at + i * G::STEP, in ? q : p, in);
+      q += G::ROWS * step;
+    }
+  }
+  __device__ __forceinline__ void put(const uint8_t* slot, char* p, size_t step, int t,
+                                      int TT) const {
+    char* q = p + (size_t)(t + row) * step;
+#pragma unroll
+    for (int i = 0; i < G::PASSES; ++i) {
+      if (live && t + row + i * G::ROWS < TT)
+        *reinterpret_cast<uint4*>(q) = *reinterpret_cast<const uint4*>(slot + at + i * G::STEP);
+      q += G::ROWS * step;
+    }
+  }
+};
+
+// What segments of time do to the state: (A, B) of every segment and channel.
+struct Segments {
+  int tiles;         // of a segment
+  int count;
+  float2* sums;      // [count][BD], or NULL when there is one segment
+};
+
+// The state that enters segment z: from `h`, through the segments before it
+// (REV: after it).
+template <bool REV>
+__device__ __forceinline__ float entering(const Segments& seg, int z, size_t BD, size_t c,
+                                          float h) {
+  const int n = REV ? seg.count - 1 - z : z;
+#pragma unroll 8
+  for (int i = 0; i < n; ++i) {
+    const float2 ab = seg.sums[(size_t)(REV ? seg.count - 1 - i : i) * BD + c];
+    h = fmaf(ab.x, h, ab.y);
+  }
+  return h;
+}
+
+// (A, B) of each segment: of f h + (1 - f) v forward in time, or REV of
+// f (l + v) backward.
+template <typename T, int LPR, bool REV>
+__global__ void __launch_bounds__(SCAN_THREADS, 4)
+    scan_sum_tiles_kernel(const T* __restrict__ v, size_t vb, size_t vt, const T* __restrict__ g,
+                          size_t gb, size_t gt, const int64_t* __restrict__ lengths, size_t BD,
+                          int TT, int D, Segments seg) {
+  using G = Staged<T, LPR>;
+  constexpr int FR = G::FR;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ ScanShared<2, LPR> sh;
+  const int part = threadIdx.x / LPR, lane = threadIdx.x & (LPR - 1);
+  // the last segment in time's order is not needed
+  const int z = blockIdx.x % (seg.count - 1) + (REV ? 1 : 0);
+  const size_t first = (size_t)(blockIdx.x / (seg.count - 1)) * (2 * LPR);
+  const Channel ch(first, lane, 2, BD, D, TT, lengths);
+  const Mover<T, LPR> mv(first, BD, D, TT, lengths);
+  const char* vp = reinterpret_cast<const char*>(v + mv.b * vb + mv.d);
+  const char* gp = reinterpret_cast<const char*>(g + mv.b * gb + mv.d);
+  const size_t vs = vt * sizeof(T), gs = gt * sizeof(T);
+  const int steps = min(seg.tiles, (TT + G::TILE - 1) / G::TILE - z * seg.tiles);
+  auto tile_of_step = [&](int it) {
+    return (z * seg.tiles + (REV ? steps - 1 - it : it)) * G::TILE;
+  };
+  auto fetch = [&](int it) {
+    if (it < steps) {
+      const uint32_t slot = smem_u32(ring) + (it % G::STAGES) * 2 * G::SLOT;
+      mv.fetch(slot, gp, gs, tile_of_step(it));
+      mv.fetch(slot + G::SLOT, vp, vs, tile_of_step(it));
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < G::STAGES; ++i) fetch(i);
+  float2 total[2] = {make_float2(1.f, 0.f), make_float2(1.f, 0.f)};  // of run 0's threads
+  for (int it = 0; it < steps; ++it) {
+    uint8_t* gsl = ring + (it % G::STAGES) * 2 * G::SLOT;
+    const int n = ch.L - (tile_of_step(it) + part * FR), p = it & 1;
+    const RunFrames<T, LPR> gf(gsl, part, lane), vf(gsl + G::SLOT, part, lane);
+    cp_async_wait<G::STAGES - 1>();
+    __syncthreads();
+    Vec<2> A = splat<2>(1.f), B = splat<2>(0.f);
+#pragma unroll
+    for (int i = 0; i < FR; ++i) {
+      const int k = REV ? FR - 1 - i : i;
+      const Vec<2> s = k < n ? gate_of(gf[k].get()) : splat<2>(-0.f), x = vf[k].get();
+      B = REV ? decay(s, add_v(x, B)) : advance(s, B, x, sub_v(B, x));
+      A = decay(s, A);
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      sh.a[p][part][lane * 2 + q] = A.v[q];
+      sh.b[p][part][lane * 2 + q] = B.v[q];
+    }
+    __syncthreads();
+    if (part == 0)
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int i = 0; i < G::RUNS; ++i) {
+          const int w = REV ? G::RUNS - 1 - i : i;
+          const float wa = sh.a[p][w][lane * 2 + q];
+          total[q].y = fmaf(wa, total[q].y, sh.b[p][w][lane * 2 + q]);
+          total[q].x *= wa;
+        }
+    fetch(it + G::STAGES);  // all have read this tile
+  }
+  if (ch.live && part == 0)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) seg.sums[(size_t)z * BD + ch.c + q] = total[q];
+}
+
+template <typename T, int LPR>
+__global__ void __launch_bounds__(SCAN_THREADS, 4)
+    scan_fwd_tiles_kernel(const T* __restrict__ x, size_t xb, size_t xt, const T* __restrict__ g,
+                          size_t gb, size_t gt, const float* __restrict__ h0,
+                          const int64_t* __restrict__ lengths, size_t BD, int TT, int D, Segments seg,
+                          T* __restrict__ y, float* __restrict__ state,
+                          float* __restrict__ carry) {
+  using G = Staged<T, LPR>;
+  constexpr int FR = G::FR;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ ScanShared<2, LPR> sh;
+  const int part = threadIdx.x / LPR, lane = threadIdx.x & (LPR - 1);
+  const int z = blockIdx.x % seg.count;
+  const size_t first = (size_t)(blockIdx.x / seg.count) * (2 * LPR);
+  const Channel ch(first, lane, 2, BD, D, TT, lengths);
+  const Mover<T, LPR> mv(first, BD, D, TT, lengths);
+  const char* xp = reinterpret_cast<const char*>(x + mv.b * xb + mv.d);
+  const char* gp = reinterpret_cast<const char*>(g + mv.b * gb + mv.d);
+  char* yp = reinterpret_cast<char*>(y + mv.b * (size_t)TT * D + mv.d);
+  const size_t xs = xt * sizeof(T), gs = gt * sizeof(T), ys = D * sizeof(T);
+  Vec<2> run = splat<2>(0.f);
+  if (part == 0)
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+      sh.start[0][lane * 2 + v] =
+          ch.live ? entering<false>(seg, z, BD, ch.c + v, h0 ? h0[ch.c + v] : 0.f) : 0.f;
+  const int tiles = (TT + G::TILE - 1) / G::TILE, tile0 = z * seg.tiles;
+  const int steps = min(seg.tiles, tiles - tile0);
+  auto fetch = [&](int it) {
+    if (it < steps) {
+      const uint32_t slot = smem_u32(ring) + (it % G::STAGES) * 2 * G::SLOT;
+      const int t = (tile0 + it) * G::TILE;
+      mv.fetch(slot, gp, gs, t);
+      mv.fetch(slot + G::SLOT, xp, xs, t);
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < G::STAGES; ++i) fetch(i);
+  for (int it = 0; it < steps; ++it) {
+    uint8_t* gsl = ring + (it % G::STAGES) * 2 * G::SLOT;
+    uint8_t* xsl = gsl + G::SLOT;
+    const int tile = (tile0 + it) * G::TILE, t0 = tile + part * FR, n = ch.L - t0;
+    using F = Frame<T, 2>;
+    const RunFrames<T, LPR> gf(gsl, part, lane), xf(xsl, part, lane);
+    cp_async_wait<G::STAGES - 1>();
+    __syncthreads();
+    Vec<2> s[FR], A = splat<2>(1.f), B = splat<2>(0.f), h;
+#pragma unroll
+    for (int k = 0; k < FR; ++k) s[k] = gate_of(gf[k].get());
+    if (n < FR)
+#pragma unroll
+      for (int k = 0; k < FR; ++k)
+        if (k >= n) s[k] = splat<2>(-0.f);
+#pragma unroll
+    for (int k = 0; k < FR; ++k) {
+      const Vec<2> xv = xf[k].get();
+      B = advance(s[k], B, xv, sub_v(B, xv));
+      A = decay(s[k], A);
+    }
+    compose<2, LPR, false>(sh, it, 1, 0, part, lane, A, B, run, h);
+    if (carry && ch.live && t0 < TT)
+      *reinterpret_cast<float2*>(carry + (size_t)(t0 / FR) * BD + ch.c) =
+          make_float2(h.v[0], h.v[1]);
+#pragma unroll
+    for (int k = 0; k < FR; ++k) {
+      const Vec<2> xv = xf[k].get();
+      h = advance(s[k], h, xv, sub_v(h, xv));
+      xf[k] = k < n ? F::of(h) : F::zero();
+    }
+    if (part == G::RUNS - 1)
+#pragma unroll
+      for (int v = 0; v < 2; ++v) sh.start[(it + 1) & 1][lane * 2 + v] = h.v[v];
+    __syncthreads();
+    mv.put(xsl, yp, ys, tile, TT);
+    fetch(it + G::STAGES);  // into the places this thread has just read
+  }
+  __syncthreads();
+  if (ch.live && part == 0 && z == seg.count - 1)
+#pragma unroll
+    for (int v = 0; v < 2; ++v) state[ch.c + v] = sh.start[steps & 1][lane * 2 + v];
+}
+
+// The same walk from the end.
+template <typename T, int LPR>
+__global__ void __launch_bounds__(SCAN_THREADS, 4)
+    scan_bwd_tiles_kernel(const T* __restrict__ dy, size_t yb, size_t yt,
+                          const float* __restrict__ dstate, const T* __restrict__ x, size_t xb,
+                          size_t xt, const T* __restrict__ g, size_t gb, size_t gt,
+                          const int64_t* __restrict__ lengths, const float* __restrict__ carry,
+                          size_t BD, int TT, int D, Segments seg, T* __restrict__ dx, T* __restrict__ dg,
+                          float* __restrict__ dh0) {
+  using G = Staged<T, LPR>;
+  constexpr int FR = G::FR;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ ScanShared<2, LPR> sh;
+  const int part = threadIdx.x / LPR, lane = threadIdx.x & (LPR - 1);
+  const int z = blockIdx.x % seg.count;
+  const size_t first = (size_t)(blockIdx.x / seg.count) * (2 * LPR);
+  const Channel ch(first, lane, 2, BD, D, TT, lengths);
+  const Mover<T, LPR> mv(first, BD, D, TT, lengths);
+  const char* xp = reinterpret_cast<const char*>(x + mv.b * xb + mv.d);
+  const char* gp = reinterpret_cast<const char*>(g + mv.b * gb + mv.d);
+  const char* yp = reinterpret_cast<const char*>(dy + mv.b * yb + mv.d);
+  const size_t out = mv.b * (size_t)TT * D + mv.d;
+  char* ox = reinterpret_cast<char*>(dx + out);
+  char* og = reinterpret_cast<char*>(dg + out);
+  const size_t xs = xt * sizeof(T), gs = gt * sizeof(T), ys = yt * sizeof(T), os = D * sizeof(T);
+  // f_{t+1} lam_{t+1} beyond the frames done
+  Vec<2> run = splat<2>(0.f);
+  if (part == 0)
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+      sh.start[0][lane * 2 + v] =
+          ch.live ? entering<true>(seg, z, BD, ch.c + v, dstate ? dstate[ch.c + v] : 0.f) : 0.f;
+  const int tiles = (TT + G::TILE - 1) / G::TILE, tile0 = z * seg.tiles;
+  const int steps = min(seg.tiles, tiles - tile0);
+  auto fetch = [&](int it) {
+    if (it < steps) {
+      const uint32_t slot = smem_u32(ring) + (it % G::STAGES) * 3 * G::SLOT;
+      const int t = (tile0 + steps - 1 - it) * G::TILE;
+      mv.fetch(slot, gp, gs, t);
+      mv.fetch(slot + G::SLOT, xp, xs, t);
+      mv.fetch(slot + 2 * G::SLOT, yp, ys, t);
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < G::STAGES; ++i) fetch(i);
+  for (int it = 0; it < steps; ++it) {
+    uint8_t* gsl = ring + (it % G::STAGES) * 3 * G::SLOT;
+    uint8_t* xsl = gsl + G::SLOT;
+    uint8_t* ysl = xsl + G::SLOT;
+    const int tile = (tile0 + steps - 1 - it) * G::TILE, t0 = tile + part * FR,
+              n = ch.L - t0;
+    using F = Frame<T, 2>;
+    const RunFrames<T, LPR> gf(gsl, part, lane), xf(xsl, part, lane), yf(ysl, part, lane);
+    float2 h2 = make_float2(0.f, 0.f);
+    if (n > 0)
+      h2 = *reinterpret_cast<const float2*>(carry + (size_t)(t0 / FR) * BD + ch.c);
+    cp_async_wait<G::STAGES - 1>();
+    __syncthreads();
+    Vec<2> s[FR], diff[FR];  // the gates; h_{t-1} - x_t
+    Vec<2> A = splat<2>(1.f), B = splat<2>(0.f), h = {{h2.x, h2.y}}, lam;
+#pragma unroll
+    for (int k = 0; k < FR; ++k) s[k] = gate_of(gf[k].get());
+    if (n < FR)
+#pragma unroll
+      for (int k = 0; k < FR; ++k)
+        if (k >= n) s[k] = splat<2>(-0.f);
+#pragma unroll
+    for (int k = FR - 1; k >= 0; --k) {
+      B = decay(s[k], add_v(yf[k].get(), B));
+      A = decay(s[k], A);
+    }
+#pragma unroll
+    for (int k = 0; k < FR; ++k) {
+      const Vec<2> xv = xf[k].get();
+      diff[k] = sub_v(h, xv);
+      h = advance(s[k], h, xv, diff[k]);
+    }
+    compose<2, LPR, true>(sh, it, 1, 0, part, lane, A, B, run, lam);
+#pragma unroll
+    for (int k = FR - 1; k >= 0; --k) {
+      const Vec<2> l = add_v(yf[k].get(), lam);
+      lam = decay(s[k], l);
+      const Vec<2> pass = passed(s[k], l, negated(l));
+      xf[k] = k < n ? F::of(pass) : F::zero();
+      // f (1 - f) l (h - x)
+      gf[k] = k < n ? F::of(mul_v(decay(s[k], pass), diff[k])) : F::zero();
+    }
+    if (part == 0)
+#pragma unroll
+      for (int v = 0; v < 2; ++v) sh.start[(it + 1) & 1][lane * 2 + v] = lam.v[v];
+    __syncthreads();
+    mv.put(xsl, ox, os, tile, TT);
+    mv.put(gsl, og, os, tile, TT);
+    fetch(it + G::STAGES);  // into places that this thread, or all before the barrier, have read
+  }
+  __syncthreads();
+  if (ch.live && dh0 && part == 0 && z == 0)
+#pragma unroll
+    for (int v = 0; v < 2; ++v) dh0[ch.c + v] = sh.start[steps & 1][lane * 2 + v];
 }
 
 template <typename T>
@@ -463,29 +837,72 @@ unsigned grid_of(int B, int D) {
   return (unsigned)(((size_t)B * D + SCAN_THREADS - 1) / SCAN_THREADS);
 }
 
-// How the channels and the time of a call are spread over blocks: 32 lanes of
-// channels a frame while that gives the SMs three blocks each; else more
-// blocks take part of the time, as many as there are tiles; else fewer lanes.
+// How the channels of a call are spread over blocks of the second form, 32 or
+// 16 lanes a frame, and its time over S blocks of a cluster: whole lanes while
+// the SMs get three blocks each, then as many time blocks as there are tiles.
 struct ScanPlan {
   int lpr, S;
   size_t groups;
 };
-ScanPlan scan_plan(size_t BD, int vc, int TT) {
+ScanPlan scan_plan(size_t BD, int TT, size_t type_bytes) {
   ScanPlan p = {32, 1, 0};
-  for (;; p.lpr /= 2) {
-    p.groups = (BD + p.lpr * vc - 1) / (p.lpr * vc);
+  for (;; p.lpr = 16) {
+    p.groups = (BD + p.lpr - 1) / p.lpr;
     p.S = 1;
-    while (p.S < 8 && p.groups * p.S < 148 * 3 && (long long)p.S * tile_of(p.lpr) < TT) p.S *= 2;
-    if (p.lpr == 8 || p.groups * p.S >= 148 * 3) return p;
+    while (p.S < 8 && p.groups * p.S < 148 * 3 &&
+           (long long)p.S * tile_of(p.lpr, type_bytes) < TT)
+      p.S *= 2;
+    if (p.lpr == 16 || p.groups * p.S >= 148 * 3) return p;
   }
 }
 
+// Of the first form.  Whole 128-byte lines while they give the SMs two blocks
+// each; half lines while those give them three for two; below that segments of
+// time, of at least 2 tiles, as many as the SMs hold blocks of (4 each; more
+// would start when the first end: 640 blocks took 240 us where 576 take 175, 4 x
+// 32768 x 256 float32 backward).
+struct TilePlan {
+  bool whole;
+  int segments, tiles;  // tiles of a segment
+  size_t groups;
+};
+template <typename T>
+TilePlan tile_plan(size_t BD, int TT) {
+  constexpr int MOST = 64 / sizeof(T);  // lanes of a whole line, two channels each
+  const size_t lines = (BD + 2 * MOST - 1) / (2 * MOST), halves = (BD + MOST - 1) / MOST;
+  TilePlan p = {lines >= 148 * 2 || halves < 222, 1, 0, 0};
+  p.groups = p.whole ? lines : halves;
+  const int tile = tile_of(p.whole ? MOST : MOST / 2, sizeof(T));
+  const int tiles = (TT + tile - 1) / tile;
+  if (halves < 222 && lines) {
+    const size_t want = 148 * 4 / lines;
+    p.segments = want < (size_t)(tiles / 2) ? (int)want : tiles / 2;
+    if (p.segments < 1) p.segments = 1;
+  }
+  p.tiles = (tiles + p.segments - 1) / p.segments;
+  p.segments = p.tiles ? (tiles + p.tiles - 1) / p.tiles : 1;
+  return p;
+}
+
+template <typename T>
+size_t sums_bytes(int B, int TT, int D) {
+  if (D * sizeof(T) % 16) return 0;
+  const TilePlan p = tile_plan<T>((size_t)B * D, TT);
+  return p.segments > 1 ? (size_t)p.segments * B * D * sizeof(float2) : 0;
+}
+
 template <typename... Params, typename... Args>
-int launch(const char* who, void (*kernel)(Params...), size_t groups, int S, void* stream,
-           Args... args) {
+int launch(const char* who, void (*kernel)(Params...), size_t groups, int S, size_t smem,
+           void* stream, Args... args) {
+  if (smem) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        (const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return set_error(kLaunch, "%s: %s", who, cudaGetErrorString(e));
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(groups * S));
   cfg.blockDim = dim3(SCAN_THREADS);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -498,59 +915,134 @@ int launch(const char* who, void (*kernel)(Params...), size_t groups, int S, voi
   return kOk;
 }
 
-template <typename T>
-bool pairs_ok(const void* p, size_t s1, size_t s2) {
-  return (uintptr_t)p % (2 * sizeof(T)) == 0 && s1 % 2 == 0 && s2 % 2 == 0;
-}
-
-// The instance of a kernel for plan p and `pairs`.
-#define TW_SCAN_KERNEL(KERNEL)                                                   \
-  (pairs ? (p.lpr == 32 ? KERNEL<T, 2, 32> : p.lpr == 16 ? KERNEL<T, 2, 16>      \
-                                                         : KERNEL<T, 2, 8>)      \
-         : (p.lpr == 32 ? KERNEL<T, 1, 32> : p.lpr == 16 ? KERNEL<T, 1, 16>      \
-                                                         : KERNEL<T, 1, 8>))
-
-template <typename T>
-int fwd(const void* x, size_t xb, size_t xt, const void* g, size_t gb, size_t gt, const float* h0,
-        const int64_t* lengths, int B, int TT, int D, void* y, float* state, void* carry,
-        size_t carry_bytes, void* stream) {
-  set_error(kOk, "%s", "");
-  if (int e = check("tw_gated_scan_forward", B, TT, D)) return e;
-  if (B == 0) return kOk;
-  if (!state || (TT && (!x || !g || !y)))
-    return set_error(kInvalid, "tw_gated_scan_forward: null pointer argument");
-  if (carry && carry_bytes < tw_gated_scan_carry_bytes(B, TT, D))
-    return set_error(kWorkspace, "tw_gated_scan_forward: carry needs %zu bytes",
-                     tw_gated_scan_carry_bytes(B, TT, D));
+// The first form's launches: the segments' sums when there are several, then
+// the scan.
+template <typename T, int LPR>
+int fwd_tiles(const TilePlan& p, const T* x, size_t xb, size_t xt, const T* g, size_t gb,
+              size_t gt, const float* h0, const int64_t* lengths, size_t BD, int TT, int D, T* y,
+              float* state, float* carry, float2* sums, void* stream) {
+  using G = Staged<T, LPR>;
   const char* who = "tw_gated_scan_forward";
-  const size_t BD = (size_t)B * D;
-  const bool pairs = D % 2 == 0 && pairs_ok<T>(x, xb, xt) && pairs_ok<T>(g, gb, gt) &&
-                     pairs_ok<T>(y, 0, 0);
-  const ScanPlan p = scan_plan(BD, pairs ? 2 : 1, TT);
-  return launch(who, TW_SCAN_KERNEL(scan_fwd_kernel), p.groups, p.S, stream, (const T*)x, xb, xt,
-                (const T*)g, gb, gt, h0, lengths, BD, TT, D, p.S, (T*)y, state, (float*)carry);
+  const size_t smem = G::STAGES * 2 * G::SLOT;
+  const Segments seg = {p.tiles, p.segments, sums};
+  if (p.segments > 1)
+    if (int e = launch(who, scan_sum_tiles_kernel<T, LPR, false>, p.groups * (p.segments - 1), 1,
+                       smem, stream, x, xb, xt, g, gb, gt, lengths, BD, TT, D, seg))
+      return e;
+  return launch(who, scan_fwd_tiles_kernel<T, LPR>, p.groups * p.segments, 1, smem, stream, x, xb,
+                xt, g, gb, gt, h0, lengths, BD, TT, D, seg, y, state, carry);
+}
+
+template <typename T, int LPR>
+int bwd_tiles(const TilePlan& p, const T* dy, size_t yb, size_t yt, const float* dstate,
+              const T* x, size_t xb, size_t xt, const T* g, size_t gb, size_t gt,
+              const int64_t* lengths, const float* carry, size_t BD, int TT, int D, T* dx, T* dg,
+              float* dh0, float2* sums, void* stream) {
+  using G = Staged<T, LPR>;
+  const char* who = "tw_gated_scan_backward";
+  const Segments seg = {p.tiles, p.segments, sums};
+  if (p.segments > 1)
+    if (int e = launch(who, scan_sum_tiles_kernel<T, LPR, true>, p.groups * (p.segments - 1), 1,
+                       (size_t)G::STAGES * 2 * G::SLOT, stream, dy, yb, yt, g, gb, gt, lengths, BD,
+                       TT, D, seg))
+      return e;
+  return launch(who, scan_bwd_tiles_kernel<T, LPR>, p.groups * p.segments, 1,
+                (size_t)G::STAGES * 3 * G::SLOT, stream, dy, yb, yt, dstate, x, xb, xt, g, gb, gt,
+                lengths, carry, BD, TT, D, seg, dx, dg, dh0);
+}
+
+// Whether frames can move in 16-byte pieces.
+template <typename T>
+bool pieces(const void* p, size_t s1, size_t s2) {
+  return (uintptr_t)p % 16 == 0 && s1 * sizeof(T) % 16 == 0 && s2 * sizeof(T) % 16 == 0;
+}
+
+// The saved states of a call; its segments' sums lie behind them.
+template <typename T>
+size_t states_bytes(int B, int TT, int D) {
+  const int fr = frames_of(sizeof(T));
+  const size_t n = (size_t)B * D * ((TT + fr - 1) / fr) * sizeof(float);
+  return (n + 15) / 16 * 16;
 }
 
 template <typename T>
-int bwd(const void* dy, size_t yb, size_t yt, const float* dstate, const void* x, size_t xb,
-        size_t xt, const void* g, size_t gb, size_t gt, const int64_t* lengths, const void* carry,
-        size_t carry_bytes, int B, int TT, int D, void* dx, void* dg, float* dh0, void* stream) {
+int fwd(const void* xv, size_t xb, size_t xt, const void* gv, size_t gb, size_t gt,
+        const float* h0, const int64_t* lengths, int B, int TT, int D, void* y, float* state,
+        void* carry, size_t carry_bytes, void* stream) {
   set_error(kOk, "%s", "");
-  if (int e = check("tw_gated_scan_backward", B, TT, D)) return e;
+  const char* who = "tw_gated_scan_forward";
+  if (int e = check(who, B, TT, D)) return e;
   if (B == 0) return kOk;
-  if (TT && (!dy || !x || !g || !carry || !dx || !dg))
-    return set_error(kInvalid, "tw_gated_scan_backward: null pointer argument");
-  if (carry_bytes < tw_gated_scan_carry_bytes(B, TT, D))
-    return set_error(kWorkspace, "tw_gated_scan_backward: carry needs %zu bytes",
-                     tw_gated_scan_carry_bytes(B, TT, D));
-  const char* who = "tw_gated_scan_backward";
+  if (!state || (TT && (!xv || !gv || !y)))
+    return set_error(kInvalid, "tw_gated_scan_forward: null pointer argument");
+  const size_t states = states_bytes<T>(B, TT, D), sums = sums_bytes<T>(B, TT, D);
+  const bool saves = carry && carry_bytes >= states + sums;
+  if (carry && !saves && (sums == 0 || carry_bytes < sums))
+    return set_error(kWorkspace, "tw_gated_scan_forward: carry needs %zu bytes (%zu without a "
+                     "backward)", states + sums, sums);
+  const T* x = (const T*)xv;
+  const T* g = (const T*)gv;
   const size_t BD = (size_t)B * D;
-  const bool pairs = D % 2 == 0 && pairs_ok<T>(x, xb, xt) && pairs_ok<T>(g, gb, gt) &&
-                     pairs_ok<T>(dy, yb, yt) && pairs_ok<T>(dx, 0, 0) && pairs_ok<T>(dg, 0, 0);
-  const ScanPlan p = scan_plan(BD, pairs ? 2 : 1, TT);
-  return launch(who, TW_SCAN_KERNEL(scan_bwd_kernel), p.groups, p.S, stream, (const T*)dy, yb, yt,
-                dstate, (const T*)x, xb, xt, (const T*)g, gb, gt, lengths, (const float*)carry, BD,
-                TT, D, p.S, (T*)dx, (T*)dg, dh0);
+  float* saved = saves ? (float*)carry : nullptr;
+  if (D * sizeof(T) % 16 == 0 && pieces<T>(x, xb, xt) && pieces<T>(g, gb, gt) &&
+      pieces<T>(y, 0, 0) && (uintptr_t)carry % 16 == 0) {
+    TilePlan p = tile_plan<T>(BD, TT);
+    if (p.segments > 1 && !carry) {  // no room for their sums
+      p.tiles *= p.segments;
+      p.segments = 1;
+    }
+    float2* room = (float2*)((char*)carry + (saves ? states : 0));
+    constexpr int MOST = 64 / sizeof(T);
+    return p.whole ? fwd_tiles<T, MOST>(p, x, xb, xt, g, gb, gt, h0, lengths, BD, TT, D, (T*)y,
+                                        state, saved, room, stream)
+                   : fwd_tiles<T, MOST / 2>(p, x, xb, xt, g, gb, gt, h0, lengths, BD, TT, D,
+                                            (T*)y, state, saved, room, stream);
+  }
+  const ScanPlan p = scan_plan(BD, TT, sizeof(T));
+  return launch(who, p.lpr == 32 ? scan_fwd_kernel<T, 1, 32> : scan_fwd_kernel<T, 1, 16>,
+                p.groups, p.S, 0, stream, x, xb, xt, g, gb, gt, h0, lengths, BD, TT, D, p.S,
+                (T*)y, state, saved);
+}
+
+template <typename T>
+int bwd(const void* dyv, size_t yb, size_t yt, const float* dstate, const void* xv, size_t xb,
+        size_t xt, const void* gv, size_t gb, size_t gt, const int64_t* lengths,
+        const void* carry, size_t carry_bytes, int B, int TT, int D, void* dx, void* dg,
+        float* dh0, void* ws, size_t ws_bytes, void* stream) {
+  set_error(kOk, "%s", "");
+  const char* who = "tw_gated_scan_backward";
+  if (int e = check(who, B, TT, D)) return e;
+  if (B == 0) return kOk;
+  if (TT && (!dyv || !xv || !gv || !carry || !dx || !dg))
+    return set_error(kInvalid, "tw_gated_scan_backward: null pointer argument");
+  if (carry_bytes < states_bytes<T>(B, TT, D))
+    return set_error(kWorkspace, "tw_gated_scan_backward: carry needs %zu bytes",
+                     states_bytes<T>(B, TT, D));
+  const size_t sums = sums_bytes<T>(B, TT, D);
+  if (sums && (!ws || (uintptr_t)ws % 16 || ws_bytes < sums))
+    return set_error(kWorkspace, "tw_gated_scan_backward: workspace needs %zu bytes, 16-byte "
+                     "aligned", sums);
+  const T* dy = (const T*)dyv;
+  const T* x = (const T*)xv;
+  const T* g = (const T*)gv;
+  const size_t BD = (size_t)B * D;
+  if (D * sizeof(T) % 16 == 0 && pieces<T>(x, xb, xt) && pieces<T>(g, gb, gt) &&
+      pieces<T>(dy, yb, yt) && pieces<T>(dx, 0, 0) && pieces<T>(dg, 0, 0) &&
+      (uintptr_t)carry % 8 == 0) {
+    const TilePlan p = tile_plan<T>(BD, TT);
+    constexpr int MOST = 64 / sizeof(T);
+    return p.whole
+               ? bwd_tiles<T, MOST>(p, dy, yb, yt, dstate, x, xb, xt, g, gb, gt, lengths,
+                                    (const float*)carry, BD, TT, D, (T*)dx, (T*)dg, dh0,
+                                    (float2*)ws, stream)
+               : bwd_tiles<T, MOST / 2>(p, dy, yb, yt, dstate, x, xb, xt, g, gb, gt, lengths,
+                                        (const float*)carry, BD, TT, D, (T*)dx, (T*)dg, dh0,
+                                        (float2*)ws, stream);
+  }
+  const ScanPlan p = scan_plan(BD, TT, sizeof(T));
+  return launch(who, p.lpr == 32 ? scan_bwd_kernel<T, 1, 32> : scan_bwd_kernel<T, 1, 16>,
+                p.groups, p.S, 0, stream, dy, yb, yt, dstate, x, xb, xt, g, gb, gt, lengths,
+                (const float*)carry, BD, TT, D, p.S, (T*)dx, (T*)dg, dh0);
 }
 
 template <typename T>
@@ -571,9 +1063,16 @@ int step(const void* x, size_t xs, const void* g, size_t gs, float* state, int B
 
 extern "C" {
 
-size_t tw_gated_scan_carry_bytes(int B, int T, int D) {
+size_t tw_gated_scan_carry_bytes(int B, int T, int D, int dtype_bytes) {
   if (B <= 0 || T <= 0 || D <= 0) return 0;
-  return (size_t)B * D * ((T + tw::SCAN_FRAMES - 1) / tw::SCAN_FRAMES) * sizeof(float);
+  return tw_gated_scan_workspace_bytes(B, T, D, dtype_bytes) +
+         (dtype_bytes == 4 ? tw::states_bytes<float>(B, T, D)
+                           : tw::states_bytes<__nv_bfloat16>(B, T, D));
+}
+size_t tw_gated_scan_workspace_bytes(int B, int T, int D, int dtype_bytes) {
+  if (B <= 0 || T <= 0 || D <= 0) return 0;
+  return dtype_bytes == 4 ? tw::sums_bytes<float>(B, T, D)
+                          : tw::sums_bytes<__nv_bfloat16>(B, T, D);
 }
 
 #define TW_GATED_SCAN(SUFFIX, E)                                                                 \
@@ -588,9 +1087,9 @@ size_t tw_gated_scan_carry_bytes(int B, int T, int D) {
       const void* dy, size_t dy_batch, size_t dy_time, const float* dstate, const void* x,       \
       size_t x_batch, size_t x_time, const void* gate, size_t g_batch, size_t g_time,            \
       const int64_t* lengths, const void* carry, size_t carry_bytes, int B, int T, int D,        \
-      void* dx, void* dgate, float* dh0, void* stream) {                                         \
+      void* dx, void* dgate, float* dh0, void* workspace, size_t ws_bytes, void* stream) {                                         \
     return tw::bwd<E>(dy, dy_batch, dy_time, dstate, x, x_batch, x_time, gate, g_batch, g_time,  \
-                      lengths, carry, carry_bytes, B, T, D, dx, dgate, dh0, stream);             \
+                      lengths, carry, carry_bytes, B, T, D, dx, dgate, dh0, workspace, ws_bytes, stream);             \
   }                                                                                              \
   int tw_gated_scan_step_##SUFFIX(const void* x, size_t x_batch, const void* gate,               \
                                   size_t g_batch, float* state, int B, int D, void* y,           \

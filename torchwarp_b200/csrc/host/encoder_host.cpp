@@ -365,12 +365,9 @@ std::tuple<Tensor, Tensor, Tensor> gated_scan_forward(const Tensor& x_in, const 
   const int64_t b = x_in.size(0), t = x_in.size(1), d = x_in.size(2);
   Tensor y = dense_like(x_in);
   Tensor state = at::empty({b, d}, x_in.options().dtype(at::kFloat));
-  Tensor carry;
-  size_t n = 0;
-  if (save) {
-    n = tw_gated_scan_carry_bytes(dim32(b), dim32(t), dim32(d));
-    carry = at::empty({(int64_t)n}, x_in.options().dtype(at::kByte));
-  }
+  const auto size = save ? tw_gated_scan_carry_bytes : tw_gated_scan_workspace_bytes;
+  const size_t n = size(dim32(b), dim32(t), dim32(d), (int)x_in.element_size());
+  Tensor carry = bytes(n, x_in);
   if (b) {
     c10::cuda::CUDAGuard guard(x_in.device());
     const Tensor x = frames_of(x_in), gate = frames_of(gate_in);
@@ -381,6 +378,7 @@ std::tuple<Tensor, Tensor, Tensor> gated_scan_forward(const Tensor& x_in, const 
                      dim32(d), ptr(y), state.data_ptr<float>(), ptr(carry), n, stream_of(x)),
                  "tw_gated_scan_forward");
   }
+  if (save && !carry.defined()) carry = at::empty({0}, x_in.options().dtype(at::kByte));
   return {y, state, carry};
 }
 
@@ -398,11 +396,15 @@ std::tuple<Tensor, Tensor, Tensor> gated_scan_backward(const Tensor& dy_in, cons
         dy_in.defined() ? frames_of(dy_in.to(x.scalar_type())) : at::zeros_like(dx);
     const Tensor ds =
         dstate_in.defined() ? dstate_in.to(at::kFloat).contiguous() : dstate_in;
+    const size_t n = tw_gated_scan_workspace_bytes(dim32(b), dim32(t), dim32(d),
+                                                   (int)x.element_size());
+    Tensor ws = bytes(n, x);
     check_status(TW_PICK(tw_gated_scan_backward, x.scalar_type())(
                      ptr(dy), dy.stride(0), dy.stride(1), (const float*)ptr(ds), ptr(x),
                      x.stride(0), x.stride(1), ptr(gate), gate.stride(0), gate.stride(1),
                      (const int64_t*)ptr(lengths), ptr(carry), (size_t)carry.numel(), dim32(b),
-                     dim32(t), dim32(d), ptr(dx), ptr(dgate), dh0.data_ptr<float>(), stream_of(x)),
+                     dim32(t), dim32(d), ptr(dx), ptr(dgate), dh0.data_ptr<float>(), ptr(ws), n,
+                     stream_of(x)),
                  "tw_gated_scan_backward");
   }
   return {dx, dgate, dh0};

@@ -159,18 +159,26 @@ __global__ void __launch_bounds__(LN_THREADS)
 
 // dx, and this block's sums for dw and db: a thread keeps the same columns
 // for all its rows, so both sums stay in registers until the block's last
-// row.  x and dy are read once and kept as they lie (half the registers).
-// With 32 values a thread that is about 150 registers: blocks of 4 warps, three
-// a SM, hold 12 warps where blocks of 8 held one of 178 registers each (146 us
-// for 32768 x 1024 bfloat16).  part: [gridDim.x][2][D] (NULL: only dx).
+// row.  x and dy are read once.  AHEAD: each thread brings its own pieces of
+// the next row to shared memory with cp.async while it works on this one, and
+// reads them from there for both passes; no barrier, as nobody else reads
+// them.  Blocks of 4 warps, as many as the registers of 32 values a thread
+// allow.  32768 x 1024 bfloat16: 146 us with blocks of 8 warps and the row in
+// registers, 62 with 4, 50 with the next row ahead.  part:
+// [gridDim.x][2][D] (NULL: only dx).
 template <typename T, typename P, bool VEC, int E, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? LN_THREADS : BWD_THREADS, BLOCK ? 1 : 3)
+__global__ void __launch_bounds__(BLOCK ? LN_THREADS : BWD_THREADS,
+                                  BLOCK ? 1 : VEC && sizeof(T) == 2 ? 4 : 3)
     ln_bwd_kernel(const T* __restrict__ dy, size_t dys, const T* __restrict__ x, size_t xs,
                   const P* __restrict__ w, const float* __restrict__ mean,
                   const float* __restrict__ rstd, size_t rows, int D, int tpr,
                   T* __restrict__ dx, float* __restrict__ part) {
   constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, NV = E / V;
-  extern __shared__ float acc_s[];  // [2][D] of the block's warps, one after the other
+  constexpr bool AHEAD = VEC && !BLOCK;
+  // first the rows ahead: [2][x, dy][NV] pieces of every thread; at the end
+  // [2][D] sums of the block's warps, one after the other
+  extern __shared__ __align__(16) uint8_t room[];
+  float* acc_s = reinterpret_cast<float*>(room);
   __shared__ float red[LN_THREADS / 32];
   const int t = BLOCK ? threadIdx.x : threadIdx.x & (tpr - 1);
   const int per = BLOCK ? 1 : BWD_THREADS / tpr;  // rows of a block's step
@@ -178,30 +186,69 @@ __global__ void __launch_bounds__(BLOCK ? LN_THREADS : BWD_THREADS, BLOCK ? 1 : 
   float aw[E], ab[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) aw[i] = ab[i] = 0.f;
-  for (size_t r0 = (size_t)blockIdx.x * per; r0 < rows; r0 += (size_t)gridDim.x * per) {
-    const size_t r = r0 + (BLOCK ? 0 : threadIdx.x / tpr);
-    const bool in = r < rows;
-    const size_t rc = in ? r : rows - 1;
-    const float mu = mean[rc], rs = rstd[rc];
-    Raw<VEC, V, T> gr[NV], hr[NV];
-    float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int d = (j * tpr + t) * V;
-      if (in && d < D) {
-        gr[j].load(dy + rc * dys + d);
-        hr[j].load(x + rc * xs + d);
-      } else {
-        gr[j].zero();
-        hr[j].zero();
-      }
+  const size_t stride = (size_t)gridDim.x * per;
+  const size_t mine = BLOCK ? 0 : threadIdx.x / tpr;
+  auto piece = [&](int stage, int array, int j) {
+    return room + ((((stage * 2 + array) * NV + j) * BWD_THREADS + threadIdx.x) << 4);
+  };
+  float mu_next = 0.f, rs_next = 0.f;
+  auto fetch = [&](size_t r, int stage) {
+    if (r < rows) {
+      mu_next = mean[r];
+      rs_next = rstd[r];
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int d = (j * tpr + t) * V;
+      const bool in = r < rows && d < D;
+      cp_async16(piece(stage, 0, j), in ? x + r * xs + d : x, in ? 16 : 0);
+      cp_async16(piece(stage, 1, j), in ? dy + r * dys + d : dy, in ? 16 : 0);
+    }
+    cp_async_commit();
+  };
+  int stage = 0;
+  if (AHEAD) fetch((size_t)blockIdx.x * per + mine, 0);
+  for (size_t r0 = (size_t)blockIdx.x * per; r0 < rows; r0 += stride) {
+    const size_t r = r0 + mine;
+    const bool in = r < rows;
+    const size_t rc = in ? r : rows - 1;
+    float mu, rs;
+    Raw<VEC, V, T> gr[NV], hr[NV];  // in shared memory when AHEAD
+    float s1 = 0.f, s2 = 0.f;
+    if constexpr (AHEAD) {
+      mu = mu_next;
+      rs = rs_next;
+      fetch(r + stride, stage ^ 1);
+      asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+    } else {
+      mu = mean[rc];
+      rs = rstd[rc];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int d = (j * tpr + t) * V;
+        if (in && d < D) {
+          gr[j].load(dy + rc * dys + d);
+          hr[j].load(x + rc * xs + d);
+        } else {
+          gr[j].zero();
+          hr[j].zero();
+        }
+      }
+    }
+    auto row = [&](int j, float* g, float* h) {
+      if constexpr (AHEAD) {
+        unpack16<T>(*reinterpret_cast<const uint4*>(piece(stage, 1, j)), g);
+        unpack16<T>(*reinterpret_cast<const uint4*>(piece(stage, 0, j)), h);
+      } else {
+        gr[j].get(g);
+        hr[j].get(h);
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int d = (j * tpr + t) * V;
       float g[V], h[V];
-      gr[j].get(g);
-      hr[j].get(h);
+      row(j, g, h);
       shift_n<V>(h, -mu);
       scale_n<V>(h, rs);
       plus_n<V>(ab + j * V, g);
@@ -222,8 +269,7 @@ __global__ void __launch_bounds__(BLOCK ? LN_THREADS : BWD_THREADS, BLOCK ? 1 : 
         const int d = (j * tpr + t) * V;
         if (in && d < D) {
           float g[V], h[V];
-          gr[j].get(g);
-          hr[j].get(h);
+          row(j, g, h);
           if (w) {
             float wv[V];
             load_n<VEC, V>(w + d, wv);
@@ -239,6 +285,13 @@ __global__ void __launch_bounds__(BLOCK ? LN_THREADS : BWD_THREADS, BLOCK ? 1 : 
         }
       }
     }
+    stage ^= 1;
+    // this row's pieces were read before the copies that replace them start
+    asm volatile("" ::: "memory");
+  }
+  if (AHEAD) {
+    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+    __syncthreads();  // the rows' room becomes the sums'
   }
   if (!part) return;
   if (!BLOCK) {  // the rows of a warp's other lanes, then the warps in their order
@@ -398,11 +451,12 @@ __global__ void __launch_bounds__(LN_THREADS)
 // checks are one a value and 32 of them spill.  tpr 0: too long for a block.
 struct RowPlan {
   int e, tpr, per;  // per: rows of a block
+  int per_sm;       // backward blocks a SM holds at 32 values a thread
 };
 
-RowPlan row_plan(int D, bool vec) {
+RowPlan row_plan(int D, bool vec, int per_sm = 3) {
   const int most = vec ? 32 : 16;
-  RowPlan p = {most, 0, 1};
+  RowPlan p = {most, 0, 1, per_sm};
   if (D > most * LN_THREADS) return p;
   if (D <= 32 * most) {
     p.e = D <= 256 ? 8 : D <= 512 ? 16 : 32;
@@ -418,7 +472,7 @@ RowPlan row_plan(int D, bool vec) {
 // Blocks of the backward: what a SM holds, fewer when there are fewer rows.
 int bwd_per(const RowPlan& p) { return p.tpr > 32 ? 1 : BWD_THREADS / p.tpr; }
 int bwd_blocks(size_t rows, const RowPlan& p) {
-  const int per_sm = p.tpr > 32 ? 1024 / p.tpr / 2 : p.e == 8 ? 8 : p.e == 16 ? 5 : 3;
+  const int per_sm = p.tpr > 32 ? 1024 / p.tpr / 2 : p.e == 8 ? 8 : p.e == 16 ? 5 : p.per_sm;
   const size_t steps = (rows + bwd_per(p) - 1) / bwd_per(p), most = 148 * (per_sm < 1 ? 1 : per_sm);
   return (int)(steps < most ? steps : most);
 }
@@ -497,7 +551,7 @@ int bwd_p(const void* dy, size_t dys, const void* x, size_t xs, const void* w, c
           cudaStream_t st) {
   const bool vec = D * sizeof(T) % 16 == 0 && aligned16(x, xs * sizeof(T)) &&
                    aligned16(dy, dys * sizeof(T)) && aligned16(w, 0) && aligned16(dx, 0);
-  const RowPlan plan = row_plan(D, vec);
+  const RowPlan plan = row_plan(D, vec, sizeof(T) == 2 ? 4 : 3);
   if (plan.tpr == 0) {
     if (dx && rows)
       ln_dx_long_kernel<T, P><<<grid_of(rows), LN_THREADS, 0, st>>>(
@@ -511,7 +565,15 @@ int bwd_p(const void* dy, size_t dys, const void* x, size_t xs, const void* w, c
   float* part = dw || db ? (float*)ws : nullptr;
   if (blocks) {
     auto kernel = TW_ROW_KERNEL(ln_bwd_kernel);
-    const size_t smem = part && plan.tpr <= 32 ? 2 * (size_t)D * sizeof(float) : 0;
+    size_t smem = part && plan.tpr <= 32 ? 2 * (size_t)D * sizeof(float) : 0;
+    const size_t ahead = (size_t)plan.e * sizeof(T) * 2 * 2 * BWD_THREADS;
+    if (vec && plan.tpr <= 32 && smem < ahead) smem = ahead;
+    if (smem > 48 * 1024) {
+      const cudaError_t e = cudaFuncSetAttribute(
+          (const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      if (e != cudaSuccess)
+        return set_error(kLaunch, "tw_layer_norm_backward: %s", cudaGetErrorString(e));
+    }
     kernel<<<blocks, plan.tpr > 32 ? plan.tpr : BWD_THREADS, smem, st>>>(
         (const T*)dy, dys, (const T*)x, xs, (const P*)w, mean, rstd, rows, D, plan.tpr, (T*)dx,
         part);
@@ -547,7 +609,7 @@ size_t tw_layer_norm_workspace_bytes(size_t rows, int D) {
   if (D <= 0) return 0;
   int blocks = 0;  // of either way to read a row
   for (int vec = 0; vec < 2; ++vec) {
-    const tw::RowPlan p = tw::row_plan(D, vec != 0);
+    const tw::RowPlan p = tw::row_plan(D, vec != 0, 4);
     const int b = p.tpr ? tw::bwd_blocks(rows, p) : 0;
     if (b > blocks) blocks = b;
   }

@@ -112,7 +112,8 @@ def gated_scan(x: Tensor, gate: Tensor, h0: Optional[Tensor],
 def _(x, gate, h0, lengths):
     b, t, d = x.shape
     return (x.new_empty((b, t, d)), x.new_empty((b, d), dtype=torch.float32),
-            x.new_empty(nat.lib().tw_gated_scan_carry_bytes(b, t, d), dtype=torch.uint8))
+            x.new_empty(nat.lib().tw_gated_scan_carry_bytes(b, t, d, x.element_size()),
+                        dtype=torch.uint8))
 
 
 @torch.library.custom_op("torchwarp_b200::gated_scan_backward", mutates_args=())
