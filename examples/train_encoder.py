@@ -11,11 +11,15 @@ its states carried along, and gives the features that it gives for whole sequenc
 """
 
 import argparse
+import sys
+from pathlib import Path
 
 import torch
 
-import torchwarp_b200 as torchwarp
-import torchwarp_b200.functional as TF
+sys.path.insert(0, str(Path(__file__).resolve().parents[1]))  # the package beside this folder
+
+import torchwarp_b200 as torchwarp  # noqa: E402
+import torchwarp_b200.functional as TF  # noqa: E402
 
 
 def curves(batch, frames, classes, generator, device):
@@ -25,7 +29,7 @@ def curves(batch, frames, classes, generator, device):
     time = pace.cumsum(1) / pace.sum(1, keepdim=True)
     angle = 6.28 * time * (1 + label).unsqueeze(1)
     clean = torch.stack([angle.sin(), angle.cos(), (2 * angle).sin()], -1)
-    noise = 0.3 * torch.randn(clean.shape, generator=generator, device=device)
+    noise = 1.0 * torch.randn(clean.shape, generator=generator, device=device)
     return clean + noise, label
 
 
@@ -46,10 +50,10 @@ def main():
     references = torch.stack([angle.sin(), angle.cos(), (2 * angle).sin()], -1)
 
     def scores(x):
-        """[batch, classes]: minus the alignment cost with each reference, in mean per frame."""
+        """[batch, classes]: minus the alignment cost with each reference, a frame and feature."""
         a, b = encoder(x), encoder(references)
         pairs = TF.soft_dtw(a.repeat_interleave(classes, 0), b.repeat(len(a), 1, 1), gamma=1.0)
-        return -pairs.view(len(a), classes) / frames
+        return -pairs.view(len(a), classes) / (frames * dim)
 
     for step in range(args.steps):
         x, label = curves(32, frames, classes, generator, device)

@@ -253,6 +253,7 @@ template <typename T, int ACT>
 __global__ void __launch_bounds__(256, 4)
     linear_pack_kernel(const __grid_constant__ PackJobs<T> jobs) {
   __shared__ float red[PACK_ROWS][PACK_COLS + 8];
+  let_next_start();  // the first of a call: behind an ordinary launch
   int k = jobs.count - 1;
   while (k > 0 && (int)blockIdx.x < jobs.j[k].first) --k;
   const PackJob<T>& j = jobs.j[k];
@@ -282,6 +283,8 @@ __global__ void __launch_bounds__(1024)
   __shared__ float red[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 32 + tx;
   float s = 0.f;
+  after_previous();
+  let_next_start();
   if (c < C)
 #pragma unroll 8
     for (int b = ty; b < blocks; b += 32) s += sums[(size_t)b * C + c];
@@ -450,6 +453,7 @@ int fwd(const void* xv, size_t ldx, const void* wv, size_t ldw, const void* bias
   p.z = act == kActNone ? nullptr : z;
   p.partial = (float*)(base + l.partial);
   if (int e = packing.run("tw_linear_forward", st)) return e;
+  p.after = packing.blocks != 0;
   return gemm_run<T>(p, st);
 }
 
@@ -488,8 +492,14 @@ int bwd(const void* dyv, size_t ldy, const void* xv, size_t ldx, const void* wv,
   if (dx) bw = packing.operand(w, ldw, N, K, false, pw, base + l.w);
   if (dw) bx = packing.operand(x, ldx, M, K, false, px, base + l.x);
   if (int e = packing.run("tw_linear_backward", st)) return e;
-  if (db) linear_db_kernel<T><<<(N + 31) / 32, 1024, 0, st>>>(sums, row_blocks(M), N, (T*)db);
+  if (db) {
+    const cudaError_t e = launch_after(true, linear_db_kernel<T>, dim3((N + 31) / 32), dim3(1024),
+                                       0, 1, st, (const float*)sums, row_blocks(M), N, (T*)db);
+    if (e != cudaSuccess)
+      return set_error(kLaunch, "tw_linear_backward: %s", cudaGetErrorString(e));
+  }
   GemmProblem p = {};
+  p.after = packing.blocks != 0;
   p.partial = (float*)(base + l.partial);
   if (dx) {
     p.a = dz;
@@ -499,6 +509,7 @@ int bwd(const void* dyv, size_t ldy, const void* xv, size_t ldx, const void* wv,
     p.K = N;
     p.out = dx;
     if (int e = gemm_run<T>(p, st)) return e;
+    p.after = true;
   }
   if (dw) {
     p.a = dz;

@@ -387,6 +387,8 @@ __global__ void __launch_bounds__(Geom<T, CG, TN>::THREADS, 1)
   if (CG == 2) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = sh.tmem_base;
+  after_previous();  // all above overlaps its end
+  let_next_start();
   // the alignment of shared memory is the same in every CTA, so a pair
   // leaves together
   const bool dead = *abort != 0;
@@ -624,6 +626,8 @@ __global__ void __launch_bounds__(256)
     gemm_join_kernel(const float* __restrict__ partial, int splits, const GemmArgs<T> g) {
   const size_t n = (size_t)g.M * g.N;
   constexpr bool FAST = sizeof(T) == 2;
+  after_previous();
+  let_next_start();
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
     float v = 0.f;
     for (int s = 0; s < splits; ++s) v += __ldcs(partial + s * n + i);
@@ -704,26 +708,16 @@ int gemm_launch(const GemmProblem& p, const GemmPlan& plan, cudaStream_t st) {
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
   if (err != cudaSuccess) return set_error(kLaunch, "tw_linear: %s", cudaGetErrorString(err));
   const int most = 148 / CG;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(CG * (g.items < most ? g.items : most)));
-  cfg.blockDim = dim3(G::THREADS);
-  cfg.dynamicSmemBytes = G::SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = CG == 2 ? 1 : 0;
-  err = cudaLaunchKernelEx(&cfg, kernel, mapA, mapB, mapY, mapZ, g);
-  if (err != cudaSuccess) return set_error(kLaunch, "tw_linear: %s", cudaGetErrorString(err));
-  if (g.partial) {
+  const unsigned grid = (unsigned)(CG * (g.items < most ? g.items : most));
+  err = launch_after(p.after, kernel, dim3(grid), dim3(G::THREADS), G::SMEM, CG, st, mapA, mapB,
+                     mapY, mapZ, g);
+  if (err == cudaSuccess && g.partial) {
     const size_t n = (size_t)p.M * p.N, blocks = (n + 255) / 256;
-    gemm_join_kernel<T><<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, st>>>(
-        p.partial, g.splits, g);
-    err = cudaGetLastError();
-    if (err != cudaSuccess) return set_error(kLaunch, "tw_linear: %s", cudaGetErrorString(err));
+    err = launch_after(true, gemm_join_kernel<T>,
+                       dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), dim3(256), 0, 1, st,
+                       (const float*)p.partial, g.splits, g);
   }
+  if (err != cudaSuccess) return set_error(kLaunch, "tw_linear: %s", cudaGetErrorString(err));
   return kOk;
 }
 

@@ -31,6 +31,7 @@ struct GemmProblem {
   void* out;
   void* z;
   float* partial;
+  bool after;  // the kernel before this one on the stream is the operator's own
 };
 
 // How a product is cut: CTAs per tile (1, or a pair), tile width, and parts
