@@ -63,14 +63,29 @@ __device__ __forceinline__ uint32_t lowbias32(uint32_t h) {  // C. Wellons, hash
   return h ^ (h >> 16);
 }
 
-// The e4m3 code of y >= 0 (in units of the scale), rounded up when the
-// fraction of a spacing that is cut off plus u in [0, 1) reaches 1.
-__device__ __forceinline__ float round_e4m3(float y, float u) {
-  int e = (int)(__float_as_uint(y) >> 23) - 127;
-  e = e < -6 ? -6 : e;
-  const float ulp = __uint_as_float((unsigned)(e - 3 + 127) << 23);
-  const float inv = __uint_as_float((unsigned)(3 - e + 127) << 23);
-  return fminf(floorf(__fadd_rn(y * inv, u)) * ulp, 448.f);
+// The e4m3 value next to y >= 0 (in units of the scale): below, or above with
+// the probability of the part of a spacing that is cut off, r in [0, 2^20)
+// being the random number.  A float has 20 bits below e4m3's three, so adding
+// r and clearing them does it; below 2^-6, where e4m3's spacing stays 2^-9,
+// after adding 2^-6, which has that spacing.
+__device__ __forceinline__ float round_e4m3(float y, uint32_t r) {
+  const float low = y < 0.015625f ? 0.015625f : 0.f;
+  const uint32_t bits = (__float_as_uint(y + low) + r) & 0xFFF00000u;
+  return fminf(__uint_as_float(bits) - low, 448.f);
+}
+
+// b^t by squaring, to a few ulp.
+__device__ __forceinline__ double power(double b, int t) {
+  double r = 1.0;
+  for (; t > 0; t >>= 1, b *= b)
+    if (t & 1) r *= b;
+  return r;
+}
+
+__device__ __forceinline__ float sqrt_fast(float x) {
+  float y;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -120,17 +135,24 @@ __global__ void __launch_bounds__(AD_THREADS)
     adamw_kernel(const __grid_constant__ AdamTable tab, AdamState s, AdamScalars a) {
   __shared__ float sc[4];
   __shared__ uint32_t skey;
-  if (threadIdx.x == 0) {
+  if (threadIdx.x < 2) {  // one thread for each beta
     const int t = *(volatile int*)a.step + 1;
     const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
-    sc[0] = (float)(1.0 - lr * a.wd);
-    sc[1] = (float)(lr / (1.0 - pow(a.b1, (double)t)));
-    sc[2] = (float)(1.0 / sqrt(1.0 - pow(a.b2, (double)t)));
-    skey = a.seed * 0x9E3779B1u + (uint32_t)t * 0x85EBCA77u;
-    __threadfence();
-    if (a.last && atomicAdd(&a.step[1], 1) == (int)gridDim.x - 1) {
-      a.step[1] = 0;
-      a.step[0] = t;
+    const double rest = 1.0 - power(threadIdx.x ? a.b2 : a.b1, t);
+    if (threadIdx.x == 0) {
+      sc[0] = (float)(1.0 - lr * a.wd);
+      sc[1] = (float)(lr / rest);
+      skey = a.seed * 0x9E3779B1u + (uint32_t)t * 0x85EBCA77u;
+    } else {
+      sc[2] = (float)(1.0 / sqrt(rest));
+    }
+    __syncwarp(3);
+    if (threadIdx.x == 0) {
+      __threadfence();
+      if (a.last && atomicAdd(&a.step[1], 1) == (int)gridDim.x - 1) {
+        a.step[1] = 0;
+        a.step[0] = t;
+      }
     }
   }
   __syncthreads();
@@ -182,7 +204,7 @@ __global__ void __launch_bounds__(AD_THREADS)
     for (int i = 0; i < 8; ++i) {
       const float v = fmaf(b2, BITS8 ? r[i] * r[i] : r[i], c2 * (gv[i] * gv[i]));
       m[i] = fmaf(b1, m[i], c1 * gv[i]);
-      r[i] = sqrtf(v);
+      r[i] = sqrt_fast(v);
       pv[i] = pv[i] * keep - alpha * __fdividef(m[i], fmaf(r[i], root2, eps));
       if (!BITS8) r[i] = v;
       mmax = fmaxf(mmax, fabsf(m[i]));
@@ -208,9 +230,9 @@ __global__ void __launch_bounds__(AD_THREADS)
       for (int i = 0; i < 8; ++i) {
         const uint32_t h = lowbias32((uint32_t)(sl + i) ^ key);
         const float yr = r[i] * irs;
-        m[i] = copysignf(round_e4m3(fabsf(m[i]) * ims, (float)(h & 0xFFFFu) * (1.f / 65536.f)),
+        m[i] = copysignf(round_e4m3(fabsf(m[i]) * ims, (h & 0xFFFFu) << 4),
                          m[i]);
-        r[i] = round_e4m3(yr, (float)(h >> 16) * (1.f / 65536.f));
+        r[i] = round_e4m3(yr, (h >> 16) << 4);
         // a second moment that is not zero stays above zero: it divides m
         if (yr > 0.f) r[i] = fmaxf(r[i], 0.001953125f);
       }

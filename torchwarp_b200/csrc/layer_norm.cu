@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(LN_THREADS)
 // checks are one a value and 32 of them spill.  tpr 0: too long for a block.
 struct RowPlan {
   int e, tpr, per;  // per: rows of a block
-  int per_sm;       // backward blocks a SM holds at 32 values a thread
+  int per_sm;       // backward blocks a SM holds at 32 values a thread (16: one more)
 };
 
 RowPlan row_plan(int D, bool vec, int per_sm = 3) {
@@ -472,7 +472,7 @@ RowPlan row_plan(int D, bool vec, int per_sm = 3) {
 // Blocks of the backward: what a SM holds, fewer when there are fewer rows.
 int bwd_per(const RowPlan& p) { return p.tpr > 32 ? 1 : BWD_THREADS / p.tpr; }
 int bwd_blocks(size_t rows, const RowPlan& p) {
-  const int per_sm = p.tpr > 32 ? 1024 / p.tpr / 2 : p.e == 8 ? 8 : p.e == 16 ? 5 : p.per_sm;
+  const int per_sm = p.tpr > 32 ? 1024 / p.tpr / 2 : p.e == 8 ? 8 : p.e == 16 ? p.per_sm + 1 : p.per_sm;
   const size_t steps = (rows + bwd_per(p) - 1) / bwd_per(p), most = 148 * (per_sm < 1 ? 1 : per_sm);
   return (int)(steps < most ? steps : most);
 }
@@ -551,7 +551,7 @@ int bwd_p(const void* dy, size_t dys, const void* x, size_t xs, const void* w, c
           cudaStream_t st) {
   const bool vec = D * sizeof(T) % 16 == 0 && aligned16(x, xs * sizeof(T)) &&
                    aligned16(dy, dys * sizeof(T)) && aligned16(w, 0) && aligned16(dx, 0);
-  const RowPlan plan = row_plan(D, vec, sizeof(T) == 2 ? 4 : 3);
+  const RowPlan plan = row_plan(D, vec, !vec ? 2 : sizeof(T) == 2 ? 4 : 3);
   if (plan.tpr == 0) {
     if (dx && rows)
       ln_dx_long_kernel<T, P><<<grid_of(rows), LN_THREADS, 0, st>>>(
