@@ -513,7 +513,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<int64_t>& o
   for (size_t i = 0; i < params.size(); ++i) {
     const Tensor& p = params[i];
     Tensor g = p.grad();
-    if (!g.defined()) continue;
+    if (!g.defined() || p.numel() == 0) continue;
     if (p.scalar_type() != type || g.scalar_type() != type || g.layout() != at::kStrided)
       bad_type("a gradient must be dense and of its parameter's type " + type_of(type) + ", got " +
                type_of(g.scalar_type()));
