@@ -284,12 +284,14 @@ __device__ __forceinline__ void stage_piece(uint8_t* box, const float (&v)[32], 
 template <> __device__ __forceinline__ void stage_piece<float>(uint8_t*, const float (&)[32], int) {}
 
 // Bias, activation, residual and the stores of a warp's 32 x 32 piece at
-// (m0, n0); `bias` is that of column n0 + lane, bias_s the warp's room for 32.
+// (m0, n0); `bias` is that of column n0 + lane, bias_s the warp's room for 32,
+// `ahead` the row's residual when it was fetched before (16-bit, aligned, a
+// whole piece).
 template <typename T>
 __device__ __forceinline__ void finish_piece(float (&v)[32], int m0, int n0, const GemmArgs<T>& g,
-                                             T bias, T* bias_s, uint8_t* stg,
-                                             const CUtensorMap* mapY, const CUtensorMap* mapZ,
-                                             int lane, int split) {
+                                             T bias, T* bias_s, const Raw<true, 32, T>& ahead,
+                                             uint8_t* stg, const CUtensorMap* mapY,
+                                             const CUtensorMap* mapZ, int lane, int split) {
   if (m0 >= g.M || n0 >= g.N) return;
   if (g.partial) {
     store_piece<float>(reinterpret_cast<float*>(stg), v, g.partial + (size_t)split * g.M * g.N, m0,
@@ -321,12 +323,13 @@ __device__ __forceinline__ void finish_piece(float (&v)[32], int m0, int n0, con
   if (g.res) {
     if (g.res_vec && n0 + 32 <= g.N) {
       if (m0 + lane < g.M) {
-        const uint4* r = reinterpret_cast<const uint4*>(g.res + (size_t)(m0 + lane) * g.ldr + n0);
         constexpr int PER = 16 / sizeof(T);
+        Raw<true, 32, T> here;
+        if (sizeof(T) == 4) here.load(g.res + (size_t)(m0 + lane) * g.ldr + n0);
 #pragma unroll
         for (int c = 0; c < 32 / PER; ++c) {
           float q[PER];
-          unpack16<T>(__ldg(r + c), q);
+          unpack16<T>(sizeof(T) == 4 ? here.w[c] : ahead.w[c], q);
 #pragma unroll
           for (int i = 0; i < PER; ++i) v[c * PER + i] = add_rn(v[c * PER + i], q[i]);
         }
@@ -554,6 +557,12 @@ __global__ void __launch_bounds__(Geom<T, CG, TN>::THREADS, 1)
           asm volatile("prefetch.global.L2 [%0];" ::"l"(g.res + (size_t)(m0 + lane) * g.ldr + n0 +
                                                         32 * c));
       }
+      Raw<true, 32, T> ahead;
+      auto fetch_residual = [&](int c) {
+        if (sizeof(T) == 2 && g.res_vec && m0 + lane < g.M && n0 + 32 * c + 32 <= g.N)
+          ahead.load(g.res + (size_t)(m0 + lane) * g.ldr + n0 + 32 * c);
+      };
+      fetch_residual(0);
       if (PL == 1) {
         const int a = si & 1;
         if (!wait_for(&sh.accf[a], (unsigned)(si >> 1) & 1u, abort)) {
@@ -573,8 +582,9 @@ __global__ void __launch_bounds__(Geom<T, CG, TN>::THREADS, 1)
               else mbar_arrive(&sh.acce[a]);
             }
           }
-          finish_piece<T>(v, m0, n0 + 32 * c, g, bias[c], bias_s, stg, &mapY, &mapZ, lane,
+          finish_piece<T>(v, m0, n0 + 32 * c, g, bias[c], bias_s, ahead, stg, &mapY, &mapZ, lane,
                           split);
+          if (c + 1 < NP) fetch_residual(c + 1);
         }
       } else {
         const int k0 = split * g.per_split, k1 = min(g.nK, k0 + g.per_split);
@@ -609,8 +619,8 @@ __global__ void __launch_bounds__(Geom<T, CG, TN>::THREADS, 1)
         if (!ok) break;
 #pragma unroll
         for (int c = 0; c < NP; ++c)
-          finish_piece<T>(acc[c], m0, n0 + 32 * c, g, bias[c], bias_s, stg, &mapY, &mapZ, lane,
-                          split);
+          finish_piece<T>(acc[c], m0, n0 + 32 * c, g, bias[c], bias_s, ahead, stg, &mapY, &mapZ,
+                          lane, split);
       }
     }
     if (lane == 0) bulk_wait_all();
