@@ -460,23 +460,33 @@ __device__ __forceinline__ void fetch16(uint32_t dst, const void* src, bool in) 
                : "memory");
 }
 
-template <typename T, int LPR> struct Staged {
-  static constexpr int FR = frames_of(sizeof(T)), RUNS = SCAN_THREADS / LPR;
-  static constexpr int TILE = tile_of(LPR, sizeof(T));
+// NT threads a block, LPR lanes a frame.  NT 32 and LPR 32: one warp walks its
+// channels through all of time, a run at a time; nothing is composed and
+// nobody waits for anybody, so a frame costs half the instructions.
+template <typename T, int LPR, int NT> struct Staged {
+  static constexpr int FR = frames_of(sizeof(T)), RUNS = NT / LPR;
+  static constexpr int TILE = RUNS * FR;
   static constexpr int LINE = LPR * 2 * (int)sizeof(T);              // bytes a frame
   static constexpr int PITCH = FR * LINE;                            // of a run
   static constexpr int SLOT = RUNS * PITCH;                          // of an array's tile
   // Half lines: odd runs swap neighbouring frames, so that the two runs that a
   // half-warp reads at once lie in different banks.
   static constexpr bool SWAP = LINE < 128;
-  static constexpr int CPL = LINE / 16, ROWS = SCAN_THREADS / CPL;   // 16-byte pieces of a frame
-  static constexpr int PASSES = TILE / ROWS, STEP = ROWS / FR * PITCH;
-  static constexpr int STAGES = 2;
+  static constexpr int CPL = LINE / 16, ROWS = NT / CPL;             // 16-byte pieces of a frame
+  static constexpr int PASSES = TILE / ROWS;
+  static constexpr int STEP = ROWS >= FR ? ROWS / FR * PITCH : ROWS * LINE;
+  static constexpr int STAGES = NT == 32 ? 6 : 2;
 };
 
+template <int NT>
+__device__ __forceinline__ void block_sync() {
+  if (NT == 32) __syncwarp();
+  else __syncthreads();
+}
+
 // A run's frames of a lane in a slot.
-template <typename T, int LPR> struct RunFrames {
-  using G = Staged<T, LPR>;
+template <typename T, int LPR, int NT> struct RunFrames {
+  using G = Staged<T, LPR, NT>;
   using F = Frame<T, 2>;
   F* even;
   F* odd;
@@ -491,8 +501,8 @@ template <typename T, int LPR> struct RunFrames {
 
 // A thread's share of moving tiles: piece `threadIdx % CPL` of every ROWS-th
 // frame.
-template <typename T, int LPR> struct Mover {
-  using G = Staged<T, LPR>;
+template <typename T, int LPR, int NT> struct Mover {
+  using G = Staged<T, LPR, NT>;
   size_t b, d;
   bool live;
   int L, row;
@@ -560,7 +570,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
     scan_sum_tiles_kernel(const T* __restrict__ v, size_t vb, size_t vt, const T* __restrict__ g,
                           size_t gb, size_t gt, const int64_t* __restrict__ lengths, size_t BD,
                           int TT, int D, Segments seg) {
-  using G = Staged<T, LPR>;
+  using G = Staged<T, LPR, SCAN_THREADS>;
   constexpr int FR = G::FR;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ ScanShared<2, LPR> sh;
@@ -569,7 +579,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
   const int z = blockIdx.x % (seg.count - 1) + (REV ? 1 : 0);
   const size_t first = (size_t)(blockIdx.x / (seg.count - 1)) * (2 * LPR);
   const Channel ch(first, lane, 2, BD, D, TT, lengths);
-  const Mover<T, LPR> mv(first, BD, D, TT, lengths);
+  const Mover<T, LPR, SCAN_THREADS> mv(first, BD, D, TT, lengths);
   const char* vp = reinterpret_cast<const char*>(v + mv.b * vb + mv.d);
   const char* gp = reinterpret_cast<const char*>(g + mv.b * gb + mv.d);
   const size_t vs = vt * sizeof(T), gs = gt * sizeof(T);
@@ -591,7 +601,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
   for (int it = 0; it < steps; ++it) {
     uint8_t* gsl = ring + (it % G::STAGES) * 2 * G::SLOT;
     const int n = ch.L - (tile_of_step(it) + part * FR), p = it & 1;
-    const RunFrames<T, LPR> gf(gsl, part, lane), vf(gsl + G::SLOT, part, lane);
+    const RunFrames<T, LPR, SCAN_THREADS> gf(gsl, part, lane), vf(gsl + G::SLOT, part, lane);
     cp_async_wait<G::STAGES - 1>();
     __syncthreads();
     Vec<2> A = splat<2>(1.f), B = splat<2>(0.f);
@@ -625,22 +635,23 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
     for (int q = 0; q < 2; ++q) seg.sums[(size_t)z * BD + ch.c + q] = total[q];
 }
 
-template <typename T, int LPR>
-__global__ void __launch_bounds__(SCAN_THREADS, 4)
+template <typename T, int LPR, int NT>
+__global__ void __launch_bounds__(NT, NT == 32 ? 8 : 4)
     scan_fwd_tiles_kernel(const T* __restrict__ x, size_t xb, size_t xt, const T* __restrict__ g,
                           size_t gb, size_t gt, const float* __restrict__ h0,
                           const int64_t* __restrict__ lengths, size_t BD, int TT, int D, Segments seg,
                           T* __restrict__ y, float* __restrict__ state,
                           float* __restrict__ carry) {
-  using G = Staged<T, LPR>;
+  using G = Staged<T, LPR, NT>;
   constexpr int FR = G::FR;
   extern __shared__ __align__(128) uint8_t ring[];
+  constexpr bool ALONE = G::RUNS == 1;
   __shared__ ScanShared<2, LPR> sh;
   const int part = threadIdx.x / LPR, lane = threadIdx.x & (LPR - 1);
   const int z = blockIdx.x % seg.count;
   const size_t first = (size_t)(blockIdx.x / seg.count) * (2 * LPR);
   const Channel ch(first, lane, 2, BD, D, TT, lengths);
-  const Mover<T, LPR> mv(first, BD, D, TT, lengths);
+  const Mover<T, LPR, NT> mv(first, BD, D, TT, lengths);
   const char* xp = reinterpret_cast<const char*>(x + mv.b * xb + mv.d);
   const char* gp = reinterpret_cast<const char*>(g + mv.b * gb + mv.d);
   char* yp = reinterpret_cast<char*>(y + mv.b * (size_t)TT * D + mv.d);
@@ -649,7 +660,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
   if (part == 0)
 #pragma unroll
     for (int v = 0; v < 2; ++v)
-      sh.start[0][lane * 2 + v] =
+      run.v[v] = sh.start[0][lane * 2 + v] =
           ch.live ? entering<false>(seg, z, BD, ch.c + v, h0 ? h0[ch.c + v] : 0.f) : 0.f;
   const int tiles = (TT + G::TILE - 1) / G::TILE, tile0 = z * seg.tiles;
   const int steps = min(seg.tiles, tiles - tile0);
@@ -669,9 +680,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
     uint8_t* xsl = gsl + G::SLOT;
     const int tile = (tile0 + it) * G::TILE, t0 = tile + part * FR, n = ch.L - t0;
     using F = Frame<T, 2>;
-    const RunFrames<T, LPR> gf(gsl, part, lane), xf(xsl, part, lane);
+    const RunFrames<T, LPR, NT> gf(gsl, part, lane), xf(xsl, part, lane);
     cp_async_wait<G::STAGES - 1>();
-    __syncthreads();
+    block_sync<NT>();
     Vec<2> s[FR], A = splat<2>(1.f), B = splat<2>(0.f), h;
 #pragma unroll
     for (int k = 0; k < FR; ++k) s[k] = gate_of(gf[k].get());
@@ -679,36 +690,46 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
 #pragma unroll
       for (int k = 0; k < FR; ++k)
         if (k >= n) s[k] = splat<2>(-0.f);
+    if constexpr (ALONE) {
+      h = run;
+    } else {
 #pragma unroll
-    for (int k = 0; k < FR; ++k) {
-      const Vec<2> xv = xf[k].get();
-      B = advance(s[k], B, xv, sub_v(B, xv));
-      A = decay(s[k], A);
+      for (int k = 0; k < FR; ++k) {
+        const Vec<2> xv = xf[k].get();
+        B = advance(s[k], B, xv, sub_v(B, xv));
+        A = decay(s[k], A);
+      }
+      compose<2, LPR, false>(sh, it, 1, 0, part, lane, A, B, run, h);
     }
-    compose<2, LPR, false>(sh, it, 1, 0, part, lane, A, B, run, h);
     if (carry && ch.live && t0 < TT)
       *reinterpret_cast<float2*>(carry + (size_t)(t0 / FR) * BD + ch.c) =
           make_float2(h.v[0], h.v[1]);
+    auto finish = [&](bool all) {
 #pragma unroll
-    for (int k = 0; k < FR; ++k) {
-      const Vec<2> xv = xf[k].get();
-      h = advance(s[k], h, xv, sub_v(h, xv));
-      xf[k] = k < n ? F::of(h) : F::zero();
-    }
+      for (int k = 0; k < FR; ++k) {
+        const Vec<2> xv = xf[k].get();
+        h = advance(s[k], h, xv, sub_v(h, xv));
+        xf[k] = all || k < n ? F::of(h) : F::zero();
+      }
+    };
+    if (n >= FR) finish(true);
+    else finish(false);
+    if (ALONE) run = h;
     if (part == G::RUNS - 1)
 #pragma unroll
       for (int v = 0; v < 2; ++v) sh.start[(it + 1) & 1][lane * 2 + v] = h.v[v];
-    __syncthreads();
+    block_sync<NT>();
     mv.put(xsl, yp, ys, tile, TT);
     fetch(it + G::STAGES);  // into the places this thread has just read
   }
-  __syncthreads();
+  block_sync<NT>();
   if (ch.live && part == 0 && z == seg.count - 1)
 #pragma unroll
     for (int v = 0; v < 2; ++v) state[ch.c + v] = sh.start[steps & 1][lane * 2 + v];
 }
 
-// The same walk from the end.
+// The same walk from the end, always in the 128-thread form: alone, a warp
+// took 101 us where the four runs take 85 (32 x 1024 x 1024 bfloat16).
 template <typename T, int LPR>
 __global__ void __launch_bounds__(SCAN_THREADS, 4)
     scan_bwd_tiles_kernel(const T* __restrict__ dy, size_t yb, size_t yt,
@@ -717,7 +738,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
                           const int64_t* __restrict__ lengths, const float* __restrict__ carry,
                           size_t BD, int TT, int D, Segments seg, T* __restrict__ dx, T* __restrict__ dg,
                           float* __restrict__ dh0) {
-  using G = Staged<T, LPR>;
+  using G = Staged<T, LPR, SCAN_THREADS>;
   constexpr int FR = G::FR;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ ScanShared<2, LPR> sh;
@@ -725,7 +746,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
   const int z = blockIdx.x % seg.count;
   const size_t first = (size_t)(blockIdx.x / seg.count) * (2 * LPR);
   const Channel ch(first, lane, 2, BD, D, TT, lengths);
-  const Mover<T, LPR> mv(first, BD, D, TT, lengths);
+  const Mover<T, LPR, SCAN_THREADS> mv(first, BD, D, TT, lengths);
   const char* xp = reinterpret_cast<const char*>(x + mv.b * xb + mv.d);
   const char* gp = reinterpret_cast<const char*>(g + mv.b * gb + mv.d);
   const char* yp = reinterpret_cast<const char*>(dy + mv.b * yb + mv.d);
@@ -761,7 +782,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
     const int tile = (tile0 + steps - 1 - it) * G::TILE, t0 = tile + part * FR,
               n = ch.L - t0;
     using F = Frame<T, 2>;
-    const RunFrames<T, LPR> gf(gsl, part, lane), xf(xsl, part, lane), yf(ysl, part, lane);
+    const RunFrames<T, LPR, SCAN_THREADS> gf(gsl, part, lane), xf(xsl, part, lane), yf(ysl, part, lane);
     float2 h2 = make_float2(0.f, 0.f);
     if (n > 0)
       h2 = *reinterpret_cast<const float2*>(carry + (size_t)(t0 / FR) * BD + ch.c);
@@ -787,15 +808,25 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
       h = advance(s[k], h, xv, diff[k]);
     }
     compose<2, LPR, true>(sh, it, 1, 0, part, lane, A, B, run, lam);
+    // With a = |n| and b = a l: the smaller of f l and (1 - f) l is b, the other
+    // l - b; f (1 - f) l = b - a b.
+    auto finish = [&](bool all) {
 #pragma unroll
-    for (int k = FR - 1; k >= 0; --k) {
-      const Vec<2> l = add_v(yf[k].get(), lam);
-      lam = decay(s[k], l);
-      const Vec<2> pass = passed(s[k], l, negated(l));
-      xf[k] = k < n ? F::of(pass) : F::zero();
-      // f (1 - f) l (h - x)
-      gf[k] = k < n ? F::of(mul_v(decay(s[k], pass), diff[k])) : F::zero();
-    }
+      for (int k = FR - 1; k >= 0; --k) {
+        const Vec<2> l = add_v(yf[k].get(), lam);
+        Vec<2> a;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) a.v[v] = fabsf(s[k].v[v]);
+        const Vec<2> b = mul_v(a, l), c = sub_v(l, b);
+        lam = pick(s[k], c, b);
+        const F vx = F::of(pick(s[k], b, c));
+        const F vg = F::of(mul_v(fma_v(negated(a), b, b), diff[k]));
+        xf[k] = all || k < n ? vx : F::zero();
+        gf[k] = all || k < n ? vg : F::zero();
+      }
+    };
+    if (n >= FR) finish(true);
+    else finish(false);
     if (part == 0)
 #pragma unroll
       for (int v = 0; v < 2; ++v) sh.start[(it + 1) & 1][lane * 2 + v] = lam.v[v];
@@ -870,17 +901,24 @@ ScanPlan scan_plan(size_t BD, int TT, size_t type_bytes) {
 // would start when the first end: 640 blocks took 240 us where 576 take 175, 4 x
 // 32768 x 256 float32 backward).
 struct TilePlan {
-  bool whole;
+  bool whole, alone;
   int segments, tiles;  // tiles of a segment
   size_t groups;
 };
+
+// Forward, 16 bits, and lines for three warps a SM at least: a warp alone walks
+// a line (32 x 1024 x 1024 bfloat16: 51 us against 56 of blocks whose four runs
+// are composed; 64 x 64 x 2048: 13.4 against 16.9).  float32 is within a fifth
+// of a copy's time without it.
+constexpr size_t ALONE_FROM = 148 * 3;
 template <typename T>
-TilePlan tile_plan(size_t BD, int TT) {
+TilePlan tile_plan(size_t BD, int TT, bool forward) {
   constexpr int MOST = 64 / sizeof(T);  // lanes of a whole line, two channels each
   const size_t lines = (BD + 2 * MOST - 1) / (2 * MOST), halves = (BD + MOST - 1) / MOST;
-  TilePlan p = {lines >= 148 * 2 || halves < 222, 1, 0, 0};
+  TilePlan p = {lines >= 148 * 2 || halves < 222, forward && sizeof(T) == 2 && lines >= ALONE_FROM, 1,
+                0, 0};
   p.groups = p.whole ? lines : halves;
-  const int tile = tile_of(p.whole ? MOST : MOST / 2, sizeof(T));
+  const int tile = p.alone ? frames_of(sizeof(T)) : tile_of(p.whole ? MOST : MOST / 2, sizeof(T));
   const int tiles = (TT + tile - 1) / tile;
   if (halves < 222 && lines) {
     const size_t want = 148 * 4 / lines;
@@ -895,13 +933,13 @@ TilePlan tile_plan(size_t BD, int TT) {
 template <typename T>
 size_t sums_bytes(int B, int TT, int D) {
   if (D * sizeof(T) % 16) return 0;
-  const TilePlan p = tile_plan<T>((size_t)B * D, TT);
+  const TilePlan p = tile_plan<T>((size_t)B * D, TT, false);  // same segments
   return p.segments > 1 ? (size_t)p.segments * B * D * sizeof(float2) : 0;
 }
 
 template <typename... Params, typename... Args>
-int launch(const char* who, void (*kernel)(Params...), size_t groups, int S, size_t smem,
-           void* stream, Args... args) {
+int launch(const char* who, void (*kernel)(Params...), size_t groups, int S, int threads,
+           size_t smem, void* stream, Args... args) {
   if (smem) {
     const cudaError_t e = cudaFuncSetAttribute(
         (const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -909,7 +947,7 @@ int launch(const char* who, void (*kernel)(Params...), size_t groups, int S, siz
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(groups * S));
-  cfg.blockDim = dim3(SCAN_THREADS);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[1];
@@ -925,20 +963,20 @@ int launch(const char* who, void (*kernel)(Params...), size_t groups, int S, siz
 
 // The first form's launches: the segments' sums when there are several, then
 // the scan.
-template <typename T, int LPR>
+template <typename T, int LPR, int NT>
 int fwd_tiles(const TilePlan& p, const T* x, size_t xb, size_t xt, const T* g, size_t gb,
               size_t gt, const float* h0, const int64_t* lengths, size_t BD, int TT, int D, T* y,
               float* state, float* carry, float2* sums, void* stream) {
-  using G = Staged<T, LPR>;
+  using G = Staged<T, LPR, NT>;
+  using GS = Staged<T, LPR, SCAN_THREADS>;
   const char* who = "tw_gated_scan_forward";
-  const size_t smem = G::STAGES * 2 * G::SLOT;
   const Segments seg = {p.tiles, p.segments, sums};
   if (p.segments > 1)
     if (int e = launch(who, scan_sum_tiles_kernel<T, LPR, false>, p.groups * (p.segments - 1), 1,
-                       smem, stream, x, xb, xt, g, gb, gt, lengths, BD, TT, D, seg))
+                       SCAN_THREADS, (size_t)GS::STAGES * 2 * GS::SLOT, stream, x, xb, xt, g, gb, gt, lengths, BD, TT, D, seg))
       return e;
-  return launch(who, scan_fwd_tiles_kernel<T, LPR>, p.groups * p.segments, 1, smem, stream, x, xb,
-                xt, g, gb, gt, h0, lengths, BD, TT, D, seg, y, state, carry);
+  return launch(who, scan_fwd_tiles_kernel<T, LPR, NT>, p.groups * p.segments, 1, NT,
+                (size_t)G::STAGES * 2 * G::SLOT, stream, x, xb, xt, g, gb, gt, h0, lengths, BD, TT, D, seg, y, state, carry);
 }
 
 template <typename T, int LPR>
@@ -946,15 +984,15 @@ int bwd_tiles(const TilePlan& p, const T* dy, size_t yb, size_t yt, const float*
               const T* x, size_t xb, size_t xt, const T* g, size_t gb, size_t gt,
               const int64_t* lengths, const float* carry, size_t BD, int TT, int D, T* dx, T* dg,
               float* dh0, float2* sums, void* stream) {
-  using G = Staged<T, LPR>;
+  using G = Staged<T, LPR, SCAN_THREADS>;
   const char* who = "tw_gated_scan_backward";
   const Segments seg = {p.tiles, p.segments, sums};
   if (p.segments > 1)
     if (int e = launch(who, scan_sum_tiles_kernel<T, LPR, true>, p.groups * (p.segments - 1), 1,
-                       (size_t)G::STAGES * 2 * G::SLOT, stream, dy, yb, yt, g, gb, gt, lengths, BD,
+                       SCAN_THREADS, (size_t)G::STAGES * 2 * G::SLOT, stream, dy, yb, yt, g, gb, gt, lengths, BD,
                        TT, D, seg))
       return e;
-  return launch(who, scan_bwd_tiles_kernel<T, LPR>, p.groups * p.segments, 1,
+  return launch(who, scan_bwd_tiles_kernel<T, LPR>, p.groups * p.segments, 1, SCAN_THREADS,
                 (size_t)G::STAGES * 3 * G::SLOT, stream, dy, yb, yt, dstate, x, xb, xt, g, gb, gt,
                 lengths, carry, BD, TT, D, seg, dx, dg, dh0);
 }
@@ -994,21 +1032,25 @@ int fwd(const void* xv, size_t xb, size_t xt, const void* gv, size_t gb, size_t 
   float* saved = saves ? (float*)carry : nullptr;
   if (D * sizeof(T) % 16 == 0 && pieces<T>(x, xb, xt) && pieces<T>(g, gb, gt) &&
       pieces<T>(y, 0, 0) && (uintptr_t)carry % 16 == 0) {
-    TilePlan p = tile_plan<T>(BD, TT);
+    TilePlan p = tile_plan<T>(BD, TT, true);
     if (p.segments > 1 && !carry) {  // no room for their sums
       p.tiles *= p.segments;
       p.segments = 1;
     }
     float2* room = (float2*)((char*)carry + (saves ? states : 0));
     constexpr int MOST = 64 / sizeof(T);
-    return p.whole ? fwd_tiles<T, MOST>(p, x, xb, xt, g, gb, gt, h0, lengths, BD, TT, D, (T*)y,
+    if constexpr (MOST == 32)
+      if (p.alone)
+        return fwd_tiles<T, 32, 32>(p, x, xb, xt, g, gb, gt, h0, lengths, BD, TT, D, (T*)y, state,
+                                    saved, room, stream);
+    return p.whole ? fwd_tiles<T, MOST, SCAN_THREADS>(p, x, xb, xt, g, gb, gt, h0, lengths, BD, TT, D, (T*)y,
                                         state, saved, room, stream)
-                   : fwd_tiles<T, MOST / 2>(p, x, xb, xt, g, gb, gt, h0, lengths, BD, TT, D,
+                   : fwd_tiles<T, MOST / 2, SCAN_THREADS>(p, x, xb, xt, g, gb, gt, h0, lengths, BD, TT, D,
                                             (T*)y, state, saved, room, stream);
   }
   const ScanPlan p = scan_plan(BD, TT, sizeof(T));
   return launch(who, p.lpr == 32 ? scan_fwd_kernel<T, 1, 32> : scan_fwd_kernel<T, 1, 16>,
-                p.groups, p.S, 0, stream, x, xb, xt, g, gb, gt, h0, lengths, BD, TT, D, p.S,
+                p.groups, p.S, SCAN_THREADS, 0, stream, x, xb, xt, g, gb, gt, h0, lengths, BD, TT, D, p.S,
                 (T*)y, state, saved);
 }
 
@@ -1037,7 +1079,7 @@ int bwd(const void* dyv, size_t yb, size_t yt, const float* dstate, const void* 
   if (D * sizeof(T) % 16 == 0 && pieces<T>(x, xb, xt) && pieces<T>(g, gb, gt) &&
       pieces<T>(dy, yb, yt) && pieces<T>(dx, 0, 0) && pieces<T>(dg, 0, 0) &&
       (uintptr_t)carry % 8 == 0) {
-    const TilePlan p = tile_plan<T>(BD, TT);
+    const TilePlan p = tile_plan<T>(BD, TT, false);
     constexpr int MOST = 64 / sizeof(T);
     return p.whole
                ? bwd_tiles<T, MOST>(p, dy, yb, yt, dstate, x, xb, xt, g, gb, gt, lengths,
@@ -1049,7 +1091,7 @@ int bwd(const void* dyv, size_t yb, size_t yt, const float* dstate, const void* 
   }
   const ScanPlan p = scan_plan(BD, TT, sizeof(T));
   return launch(who, p.lpr == 32 ? scan_bwd_kernel<T, 1, 32> : scan_bwd_kernel<T, 1, 16>,
-                p.groups, p.S, 0, stream, dy, yb, yt, dstate, x, xb, xt, g, gb, gt, lengths,
+                p.groups, p.S, SCAN_THREADS, 0, stream, dy, yb, yt, dstate, x, xb, xt, g, gb, gt, lengths,
                 (const float*)carry, BD, TT, D, p.S, (T*)dx, (T*)dg, dh0);
 }
 
