@@ -1,0 +1,102 @@
+"""The encoder operators' custom ops, which ``torch.compile`` calls, without a GPU: an eager call's
+checks hold in the ops and in their fakes, where a bad argument is refused before any launch."""
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from torchwarp_b200.encoder import _ops
+
+X, H, I, U = (2, 3, 8), torch.float16, torch.int64, torch.uint8
+D = torch.float64
+
+# t(shape, dtype): a tensor, real or a tracer's
+CALLS = [
+    (TypeError, lambda t: _ops.layer_norm(t(X, D), None, None, 1e-5)),
+    (ValueError, lambda t: _ops.layer_norm(t((3, 0)), None, None, 1e-5)),
+    (ValueError, lambda t: _ops.layer_norm(t(X), t((7,)), None, 1e-5)),
+    (ValueError, lambda t: _ops.layer_norm(t(X), None, t((9,)), 1e-5)),
+    (TypeError, lambda t: _ops.layer_norm(t(X), t((8,), H), None, 1e-5)),
+    (TypeError, lambda t: _ops.layer_norm(t(X, H), t((8,)), t((8,), H), 1e-5)),
+    (ValueError, lambda t: _ops.layer_norm(t(X), None, None, -1.0)),
+    (ValueError, lambda t: _ops.layer_norm_backward(t((1, 3, 8)), t(X), None, None, t((2, 6)))),
+    (ValueError, lambda t: _ops.layer_norm_backward(t(X), t(X), None, None, t((2, 5)))),
+    (ValueError, lambda t: _ops.layer_norm_backward(t(X), t(X), None, None, t((2, 6), D))),
+    (ValueError, lambda t: _ops.layer_norm_backward(t(X), t(X), t((7,)), None, t((2, 6)))),
+    (TypeError, lambda t: _ops.linear(t(X, D), t((4, 8), D), None, None, 0)),
+    (ValueError, lambda t: _ops.linear(t(X), t((4, 7)), None, None, 0)),
+    (ValueError, lambda t: _ops.linear(t(X), t((8,)), None, None, 0)),
+    (ValueError, lambda t: _ops.linear(t(X), t((4, 8)), t((3,)), None, 0)),
+    (ValueError, lambda t: _ops.linear(t(X), t((4, 8)), None, t((2, 3, 1)), 0)),
+    (TypeError, lambda t: _ops.linear(t(X), t((4, 8), H), None, None, 0)),
+    (ValueError, lambda t: _ops.linear_backward(t((2, 3, 3)), t(X), t((4, 8)), t((0,)), 0)),
+    (ValueError, lambda t: _ops.linear_backward(t((2, 3, 4)), t(X), t((4, 8)), t((5, 4)), 2)),
+    (ValueError, lambda t: _ops.linear_backward(t((2, 3, 4)), t(X), t((4, 8)), t((6, 4), H), 2)),
+    (TypeError, lambda t: _ops.gated_scan(t(X, D), t(X, D), None, None)),
+    (ValueError, lambda t: _ops.gated_scan(t(X), t((2, 2, 8)), None, None)),
+    (TypeError, lambda t: _ops.gated_scan(t(X), t(X, H), None, None)),
+    (ValueError, lambda t: _ops.gated_scan(t(X), t(X), t((2, 7)), None)),
+    (TypeError, lambda t: _ops.gated_scan(t(X), t(X), t((2, 8), H), None)),
+    (ValueError, lambda t: _ops.gated_scan(t(X), t(X), None, t((3,), I))),
+    (TypeError, lambda t: _ops.gated_scan(t(X), t(X), None, t((2,)))),
+    (ValueError, lambda t: _ops.gated_scan_backward(t((1, 3, 8)), None, t(X), t(X), None,
+                                                    t((64,), U))),
+    (ValueError, lambda t: _ops.gated_scan_backward(None, t((2, 7)), t(X), t(X), None,
+                                                    t((64,), U))),
+    (ValueError, lambda t: _ops.gated_scan_backward(t(X), None, t(X), t(X), None, t((64,)))),
+]
+
+
+def real(shape, dtype=torch.float32):
+    return torch.zeros(shape, dtype=dtype)
+
+
+def traced(shape, dtype=torch.float32):
+    return torch.empty(shape, dtype=dtype, device="cuda")
+
+
+@pytest.mark.parametrize("error,call", CALLS)
+def test_refusals_of_the_ops(error, call):
+    with pytest.raises(error):
+        call(real)
+
+
+@pytest.mark.parametrize("error,call", CALLS)
+def test_refusals_while_tracing(error, call):
+    with FakeTensorMode():
+        with pytest.raises(error):
+            call(traced)
+
+
+@pytest.mark.parametrize("call", [
+    lambda t: _ops.layer_norm(t(X), t((8,)), None, 1e-5),
+    lambda t: _ops.linear(t(X), t((4, 8)), None, None, 0),
+    lambda t: _ops.gated_scan(t(X), t(X), None, t((2,), I)),
+])
+def test_no_cpu_fallback_of_the_ops(call):
+    with pytest.raises(RuntimeError, match="CUDA"):
+        call(real)
+    with FakeTensorMode():
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call(real)
+
+
+def test_devices_do_not_mix_while_tracing():
+    with FakeTensorMode():
+        x = torch.empty(2, 3, 8, device="cuda")
+        for call in (lambda: _ops.layer_norm(x, torch.empty(8), None, 1e-5),
+                     lambda: _ops.linear(x, torch.empty(4, 8), None, None, 0),
+                     lambda: _ops.gated_scan(x, x, None, torch.empty(2, dtype=torch.int64))):
+            with pytest.raises(RuntimeError):
+                call()
+
+
+def test_shapes_while_tracing():
+    with FakeTensorMode():
+        x, w = torch.empty(2, 3, 8, device="cuda"), torch.empty(4, 8, device="cuda")
+        y, stats = _ops.layer_norm(x, None, None, 1e-5)
+        assert y.shape == x.shape and stats.shape == (2, 6)
+        y, z = _ops.linear(x, w, None, None, 2)
+        assert y.shape == (2, 3, 4) and z.shape == (6, 4)
+        y, state, _ = _ops.gated_scan(x, x, None, torch.empty(2, dtype=torch.int32, device="cuda"))
+        assert y.shape == x.shape and state.shape == (2, 8) and state.dtype == torch.float32

@@ -1,0 +1,66 @@
+"""The encoder operators where inputs, tensors or programs are unlike a plain eager call (B200)."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module")
+def tw():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    import torchwarp_b200
+    return torchwarp_b200
+
+
+@pytest.fixture(autouse=True, scope="module")
+def _no_device_error():
+    yield
+    if torch.cuda.is_available():
+        from torchwarp_b200 import _native
+        assert _native.lib().tw_device_error() == 0
+
+
+@pytest.fixture
+def randn():
+    g = torch.Generator(device=DEV).manual_seed(0)
+    return lambda *shape, dtype=torch.float32: torch.randn(*shape, device=DEV,
+                                                           generator=g).to(dtype)
+
+
+# ------------------------------------------------------------ compiled calls
+
+def test_compiled_calls_take_strided_parameters(tw, randn):
+    TF = tw.functional
+    x, gate = randn(4, 30, 16), randn(4, 30, 16)
+    w, nw, nb, b = randn(16, 16), randn(32)[::2], randn(32)[1::2], randn(48)[::3]
+    lengths = torch.tensor([30, 0, 7, 0, 29, 0, 1, 0], device=DEV)[::2]
+
+    def f(x, gate):
+        y = TF.linear(TF.layer_norm(x, nw, nb), w, b, activation="silu")
+        return TF.gated_scan(y, gate, lengths=lengths)
+
+    torch._dynamo.reset()
+    want, got = f(x, gate), torch.compile(f, fullgraph=True, backend="aot_eager")(x, gate)
+    assert torch.equal(got.output, want.output) and torch.equal(got.state, want.state)
+    for kind in (torch.int32, torch.int64):
+        torch._dynamo.reset()
+        n = lengths.to(kind)
+        out = torch.compile(lambda x, g: TF.gated_scan(x, g, lengths=n), backend="aot_eager")(x, gate)
+        assert torch.equal(out.output, TF.gated_scan(x, gate, lengths=lengths).output)
+
+
+def test_compiled_calls_refuse_bad_arguments(tw, randn):
+    """While the function is traced: nothing is launched."""
+    TF = tw.functional
+    x = randn(4, 30, 16)
+    for f in (lambda x: TF.layer_norm(x, x.new_ones(15)), lambda x: TF.linear(x, x.new_ones(8, 17)),
+              lambda x: TF.linear(x, x.new_ones(8, 16), residual=x.new_ones(4, 1, 8)),
+              lambda x: TF.gated_scan(x, x[:, :1]),
+              lambda x: TF.gated_scan(x, x, lengths=torch.zeros(4, dtype=torch.int64))):
+        torch._dynamo.reset()
+        with pytest.raises(Exception, match="must (have|be)|CUDA"):
+            torch.compile(f, fullgraph=True, backend="aot_eager")(x)

@@ -36,9 +36,15 @@ void check_status(int status, const char* what) {
                       "): " + tw_last_error());
 }
 
+// Checks compare sym_size, so that they also hold for a tracer's tensors, whose
+// sizes may be symbols.
+std::string text_of(const c10::SymInt& n) {
+  const auto v = n.maybe_as_int();
+  return v ? std::to_string(*v) : n.toSymNodeImplUnowned()->str();
+}
 std::string shape_of(const Tensor& t) {
   std::string s = "[";
-  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + text_of(t.sym_size(i));
   return s + "]";
 }
 
@@ -68,12 +74,16 @@ void require_cuda(const Tensor& t) {
     throw std::runtime_error("torchwarp_b200 runs only on CUDA tensors (B200, sm_100a); got a "
                              "tensor on " + t.device().str() + ". There is no CPU fallback.");
 }
-void check_device(const Tensor& first, const Tensor& t) {
-  if (!t.defined()) return;
-  require_cuda(t);
-  if (t.device() != first.device())
-    bad_value("all tensors must be on one device, got " + first.device().str() + " and " +
-              t.device().str());
+// `first` and those of `others` that are there lie on one GPU.
+void check_devices(const Tensor& first, std::initializer_list<const Tensor*> others) {
+  require_cuda(first);
+  for (const Tensor* t : others) {
+    if (!t->defined()) continue;
+    require_cuda(*t);
+    if (t->device() != first.device())
+      bad_value("all tensors must be on one device, got " + first.device().str() + " and " +
+                t->device().str());
+  }
 }
 
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
@@ -112,10 +122,14 @@ Tensor frames_of(const Tensor& x) {
 // autograd sees them: an autograd Function counts only the tensors it is given.
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 Tensor def(const OptTensor& t) { return t.value_or(Tensor()); }
+Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
 
 // The entry of the element type.
-#define TW_PICK(NAME, TYPE)                                                        \
-  ((TYPE) == at::kFloat ? NAME##_f32 : (TYPE) == at::kBFloat16 ? NAME##_bf16 : NAME##_f16)
+#define TW_PICK(NAME, TYPE)                                                              \
+  ((TYPE) == at::kFloat      ? NAME##_f32                                                \
+   : (TYPE) == at::kBFloat16 ? NAME##_bf16                                               \
+   : (TYPE) == at::kHalf     ? NAME##_f16                                                \
+                             : throw py::type_error("no " #NAME " of " + type_of(TYPE)))
 
 void* stream_of(const Tensor& t) {
   return (void*)c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
@@ -140,7 +154,45 @@ variable_list first_order(variable_list out) {
   return out;
 }
 
+void check_shape_of(const char* name, const Tensor& t, const Tensor& x) {
+  if (t.sym_sizes() != x.sym_sizes())
+    bad_value(std::string(name) + " must have x's shape " + shape_of(x) + ", got " + shape_of(t));
+}
+
 // -------------------------------------------------------------- layer norm
+
+void check_parameter(const char* name, const Tensor& p, const Tensor& x) {
+  if (p.dim() != 1 || p.sym_size(0) != x.sym_size(-1))
+    bad_value(std::string(name) + " must have shape [" + text_of(x.sym_size(-1)) + "], got " +
+              shape_of(p));
+  if (p.scalar_type() != x.scalar_type() && p.scalar_type() != at::kFloat)
+    bad_type(std::string(name) + " must be float32 or of x's type " + type_of(x.scalar_type()) +
+             ", got " + type_of(p.scalar_type()));
+}
+
+// The checks of a call, whichever way it comes: eager, or through the custom
+// ops and their fakes.
+void check_layer_norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps) {
+  check_type("x", x);
+  if (x.dim() < 1 || x.sym_size(-1) == 0) bad_value("x must have shape [..., D] with D > 0");
+  if (x.sym_size(-1) > INT_MAX) bad_value("x must have fewer than 2^31 columns");
+  if (w.defined()) check_parameter("weight", w, x);
+  if (b.defined()) check_parameter("bias", b, x);
+  if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type())
+    bad_type("weight and bias must have one type");
+  if (!(eps >= 0)) bad_value("eps must be >= 0");
+  check_devices(x, {&w, &b});
+}
+void check_layer_norm_backward(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& b,
+                               const Tensor& stats) {
+  check_shape_of("dy", dy, x);
+  if (x.dim() < 1 || stats.dim() != 2 || stats.sym_size(0) != 2 ||
+      stats.sym_size(1) * x.sym_size(-1) != x.sym_numel() || stats.scalar_type() != at::kFloat ||
+      !stats.is_contiguous())
+    bad_value("stats must be what the forward saved");
+  check_layer_norm(x, w, b, 0);
+  check_devices(x, {&dy, &stats});
+}
 
 std::tuple<Tensor, Tensor> layer_norm_forward(const Tensor& x, const Tensor& w, const Tensor& b,
                                               double eps, bool save) {
@@ -208,34 +260,52 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   }
 };
 
-void check_parameter(const char* name, const Tensor& p, const Tensor& x) {
-  if (p.dim() != 1 || p.size(0) != x.size(-1))
-    bad_value(std::string(name) + " must have shape [" + std::to_string(x.size(-1)) + "], got " +
-              shape_of(p));
-  if (p.scalar_type() != x.scalar_type() && p.scalar_type() != at::kFloat)
-    bad_type(std::string(name) + " must be float32 or of x's type " + type_of(x.scalar_type()) +
-             ", got " + type_of(p.scalar_type()));
-}
-
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
-  check_type("x", x);
-  if (x.dim() < 1 || x.size(-1) == 0) bad_value("x must have shape [..., D] with D > 0");
-  Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
-  if (w.defined()) check_parameter("weight", w, x);
-  if (b.defined()) check_parameter("bias", b, x);
-  if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type())
-    bad_type("weight and bias must have one type");
-  if (!(eps >= 0)) bad_value("eps must be >= 0");
-  require_cuda(x);
-  check_device(x, w);
-  check_device(x, b);
-  if (w.defined()) w = w.contiguous();
-  if (b.defined()) b = b.contiguous();
+  Tensor w = def(weight), b = def(bias);
+  check_layer_norm(x, w, b, eps);
+  w = dense(w);
+  b = dense(b);
   if (wants_grad({&x, &w, &b})) return LayerNormFn::apply(x, opt(w), opt(b), eps);
   return std::get<0>(layer_norm_forward(x, w, b, eps, false));
 }
 
 // ------------------------------------------------------------------ linear
+
+// A tensor's shape is x's but for its last dimension, `n`.
+bool rows_like(const Tensor& t, const Tensor& x, const c10::SymInt& n) {
+  bool same = t.dim() == x.dim() && t.sym_size(-1) == n;
+  for (int64_t i = 0; same && i + 1 < x.dim(); ++i) same = t.sym_size(i) == x.sym_size(i);
+  return same;
+}
+
+void check_linear(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r) {
+  check_type("x", x);
+  if (w.dim() != 2 || w.sym_size(0) == 0 || w.sym_size(1) == 0)
+    bad_value("weight must have shape [N, K] with N, K > 0");
+  const c10::SymInt n = w.sym_size(0), k = w.sym_size(1);
+  if (x.dim() < 1 || x.sym_size(-1) != k)
+    bad_value("x must have shape [..., " + text_of(k) + "], got " + shape_of(x));
+  if (b.defined() && (b.dim() != 1 || b.sym_size(0) != n))
+    bad_value("bias must have shape [" + text_of(n) + "], got " + shape_of(b));
+  if (r.defined() && !rows_like(r, x, n))
+    bad_value("residual must have the result's shape [..., " + text_of(n) + "], got " +
+              shape_of(r));
+  check_same_type("weight", w, x);
+  if (b.defined()) check_same_type("bias", b, x);
+  if (r.defined()) check_same_type("residual", r, x);
+  check_devices(x, {&w, &b, &r});
+}
+void check_linear_backward(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& z,
+                           int64_t act) {
+  if (x.dim() < 1 || w.dim() != 2 || !rows_like(dy, x, w.sym_size(0)))
+    bad_value("dy must have the result's shape, got " + shape_of(dy));
+  if (act && (!z.defined() || z.dim() != 2 || z.sym_size(0) * w.sym_size(1) != x.sym_numel() ||
+              z.sym_size(1) != w.sym_size(0) || z.scalar_type() != x.scalar_type() ||
+              !z.is_contiguous()))
+    bad_value("z must be what the forward saved");
+  check_linear(x, w, Tensor(), Tensor());
+  check_devices(x, {&dy, &z});
+}
 
 // 1 when a row of 16-bit elements may start off a 16-byte boundary.
 int unaligned(const Rows& r) {
@@ -325,34 +395,57 @@ Tensor linear(Tensor x, Tensor w, const OptTensor& bias, const OptTensor& residu
     if (b.defined()) b = b.to(t);
     if (r.defined()) r = r.to(t);
   }
-  check_type("x", x);
-  if (w.dim() != 2 || w.size(0) == 0 || w.size(1) == 0)
-    bad_value("weight must have shape [N, K] with N, K > 0");
-  const int64_t n = w.size(0), k = w.size(1);
-  if (x.dim() < 1 || x.size(-1) != k)
-    bad_value("x must have shape [..., " + std::to_string(k) + "], got " + shape_of(x));
-  if (b.defined() && (b.dim() != 1 || b.size(0) != n))
-    bad_value("bias must have shape [" + std::to_string(n) + "], got " + shape_of(b));
-  if (r.defined()) {
-    bool same = r.dim() == x.dim() && r.size(-1) == n;
-    for (int64_t i = 0; same && i + 1 < x.dim(); ++i) same = r.size(i) == x.size(i);
-    if (!same)
-      bad_value("residual must have the result's shape [..., " + std::to_string(n) + "], got " +
-                shape_of(r));
-  }
-  check_same_type("weight", w, x);
-  if (b.defined()) check_same_type("bias", b, x);
-  if (r.defined()) check_same_type("residual", r, x);
-  require_cuda(x);
-  check_device(x, w);
-  check_device(x, b);
-  check_device(x, r);
-  if (b.defined()) b = b.contiguous();
+  check_linear(x, w, b, r);
+  b = dense(b);
   if (wants_grad({&x, &w, &b, &r})) return LinearFn::apply(x, w, opt(b), opt(r), act);
   return std::get<0>(linear_forward(x, w, b, r, act, false));
 }
 
 // -------------------------------------------------------------- gated scan
+
+void check_gate(const Tensor& gate, const Tensor& x) {
+  check_shape_of("gate", gate, x);
+  check_same_type("gate", gate, x);
+}
+void check_state(const char* name, const Tensor& state, const Tensor& x) {
+  const c10::SymInt batch = x.sym_size(0), dim = x.sym_size(-1);
+  if (state.dim() != 2 || state.sym_size(0) != batch || state.sym_size(1) != dim)
+    bad_value(std::string(name) + " must have shape [" + text_of(batch) + ", " + text_of(dim) +
+              "], got " + shape_of(state));
+}
+void check_gated_scan(const Tensor& x, const Tensor& gate, const Tensor& h0,
+                      const Tensor& lengths) {
+  check_type("x", x);
+  if (x.dim() != 3 || x.sym_size(2) == 0)
+    bad_value("x must have shape [batch, time, feature] with features");
+  check_gate(gate, x);
+  if (h0.defined()) {
+    check_state("state", h0, x);
+    if (h0.scalar_type() != at::kFloat)
+      bad_type("state must be float32, got " + type_of(h0.scalar_type()));
+  }
+  if (lengths.defined()) {
+    if (lengths.dim() != 1 || lengths.sym_size(0) != x.sym_size(0))
+      bad_value("lengths must have shape [" + text_of(x.sym_size(0)) + "], got " +
+                shape_of(lengths));
+    if (lengths.scalar_type() != at::kLong && lengths.scalar_type() != at::kInt)
+      bad_type("lengths must be int64 or int32, got " + type_of(lengths.scalar_type()));
+  }
+  check_devices(x, {&gate, &h0, &lengths});
+}
+void check_gated_scan_backward(const Tensor& dy, const Tensor& dstate, const Tensor& x,
+                               const Tensor& gate, const Tensor& lengths, const Tensor& carry) {
+  if (dy.defined()) check_shape_of("dy", dy, x);
+  if (x.dim() == 3 && dstate.defined()) check_state("dstate", dstate, x);
+  if (carry.scalar_type() != at::kByte || !carry.is_contiguous())  // its size: the C ABI
+    bad_value("carry must be what the forward saved");
+  check_gated_scan(x, gate, Tensor(), lengths);
+  check_devices(x, {&dy, &dstate, &carry});
+}
+// lengths as the kernels read them.
+Tensor whole_lengths(const Tensor& lengths) {
+  return lengths.defined() ? lengths.to(at::kLong).contiguous() : lengths;
+}
 
 int dim32(int64_t v) {
   TORCH_CHECK(v <= INT_MAX, "gated_scan: a size is too large");
@@ -427,39 +520,11 @@ struct GatedScanFn : torch::autograd::Function<GatedScanFn> {
   }
 };
 
-void check_gate(const Tensor& gate, const Tensor& x) {
-  if (gate.sizes() != x.sizes())
-    bad_value("gate must have x's shape " + shape_of(x) + ", got " + shape_of(gate));
-  check_same_type("gate", gate, x);
-}
-void check_state(const Tensor& state, int64_t batch, int64_t dim) {
-  if (state.dim() != 2 || state.size(0) != batch || state.size(1) != dim)
-    bad_value("state must have shape [" + std::to_string(batch) + ", " + std::to_string(dim) +
-              "], got " + shape_of(state));
-  if (state.scalar_type() != at::kFloat)
-    bad_type("state must be float32, got " + type_of(state.scalar_type()));
-}
-
 std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gate, const OptTensor& state,
                                       const OptTensor& lengths_in) {
-  check_type("x", x);
-  if (x.dim() != 3 || x.size(2) == 0)
-    bad_value("x must have shape [batch, time, feature] with features");
-  check_gate(gate, x);
-  Tensor h0 = state.value_or(Tensor()), lengths = lengths_in.value_or(Tensor());
-  if (h0.defined()) check_state(h0, x.size(0), x.size(2));
-  if (lengths.defined()) {
-    if (lengths.dim() != 1 || lengths.size(0) != x.size(0))
-      bad_value("lengths must have shape [" + std::to_string(x.size(0)) + "], got " +
-                shape_of(lengths));
-    if (lengths.scalar_type() != at::kLong && lengths.scalar_type() != at::kInt)
-      bad_type("lengths must be int64 or int32, got " + type_of(lengths.scalar_type()));
-  }
-  require_cuda(x);
-  check_device(x, gate);
-  check_device(x, h0);
-  check_device(x, lengths);
-  if (lengths.defined()) lengths = lengths.to(at::kLong).contiguous();
+  const Tensor h0 = def(state);
+  check_gated_scan(x, gate, h0, def(lengths_in));
+  const Tensor lengths = whole_lengths(def(lengths_in));
   if (wants_grad({&x, &gate, &h0})) {
     variable_list out = GatedScanFn::apply(x, gate, opt(h0), opt(lengths));
     return {out[0], out[1]};
@@ -475,14 +540,14 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const OptTensor& sta
   check_gate(gate, x);
   if (!state_in.has_value()) bad_value("state must be a [B,D] tensor: it is updated in place");
   const Tensor& state = *state_in;
-  const int64_t b = x.size(0), d = x.size(1);
-  check_state(state, b, d);
+  check_state("state", state, x);
+  if (state.scalar_type() != at::kFloat)
+    bad_type("state must be float32, got " + type_of(state.scalar_type()));
   if (!state.is_contiguous()) bad_value("state must be contiguous: it is updated in place");
-  require_cuda(x);
-  check_device(x, gate);
-  check_device(x, state);
+  check_devices(x, {&gate, &state});
   if (wants_grad({&x, &gate, &state}))
     throw std::runtime_error("gated_scan_step is not differentiable; use gated_scan, or no_grad");
+  const int64_t b = x.size(0), d = x.size(1);
   Tensor y = dense_like(x);
   if (b) {
     c10::cuda::CUDAGuard guard(x.device());
@@ -566,29 +631,55 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   // without autograd, for the custom ops of torch.compile
   m.def("layer_norm_forward", [](const Tensor& x, const OptTensor& w, const OptTensor& b,
                                  double eps) {
-    return layer_norm_forward(x, def(w), def(b), eps, true);
+    check_layer_norm(x, def(w), def(b), eps);
+    return layer_norm_forward(x, dense(def(w)), dense(def(b)), eps, true);
   });
   m.def("layer_norm_backward", [](const Tensor& dy, const Tensor& x, const OptTensor& w,
-                                  const OptTensor& param, const Tensor& stats) {
-    const Tensor p = w.has_value() ? *w : def(param);
-    return layer_norm_backward(dy, x, def(w), p.defined() ? p.scalar_type() : x.scalar_type(),
-                               stats, true, true, true);
+                                  const OptTensor& b, const Tensor& stats) {
+    check_layer_norm_backward(dy, x, def(w), def(b), stats);
+    const Tensor p = w.has_value() ? *w : def(b);
+    return layer_norm_backward(dy, x, dense(def(w)),
+                               p.defined() ? p.scalar_type() : x.scalar_type(), stats, true, true,
+                               true);
   });
   m.def("linear_forward", [](const Tensor& x, const Tensor& w, const OptTensor& b,
                              const OptTensor& r, int64_t act) {
-    auto [y, z] = linear_forward(x, w, def(b), def(r), act, true);
+    check_linear(x, w, def(b), def(r));
+    auto [y, z] = linear_forward(x, w, dense(def(b)), def(r), act, true);
     return std::make_tuple(y, opt(z));
   });
   m.def("linear_backward", [](const Tensor& dy, const Tensor& x, const Tensor& w,
                               const OptTensor& z, int64_t act) {
+    check_linear_backward(dy, x, w, def(z), act);
     return linear_backward(dy, x, w, def(z), act, true, true, true);
   });
   m.def("gated_scan_forward", [](const Tensor& x, const Tensor& g, const OptTensor& h0,
                                  const OptTensor& n) {
-    return gated_scan_forward(x, g, def(h0), def(n), true);
+    check_gated_scan(x, g, def(h0), def(n));
+    return gated_scan_forward(x, g, def(h0), whole_lengths(def(n)), true);
   });
   m.def("gated_scan_backward", [](const OptTensor& dy, const OptTensor& ds, const Tensor& x,
                                   const Tensor& g, const OptTensor& n, const Tensor& carry) {
-    return gated_scan_backward(def(dy), def(ds), x, g, def(n), carry);
+    check_gated_scan_backward(def(dy), def(ds), x, g, def(n), carry);
+    return gated_scan_backward(def(dy), def(ds), x, g, whole_lengths(def(n)), carry);
   });
+  // and for their fakes
+  m.def("check_layer_norm", [](const Tensor& x, const OptTensor& w, const OptTensor& b,
+                               double eps) { check_layer_norm(x, def(w), def(b), eps); });
+  m.def("check_layer_norm_backward",
+        [](const Tensor& dy, const Tensor& x, const OptTensor& w, const OptTensor& b,
+           const Tensor& stats) { check_layer_norm_backward(dy, x, def(w), def(b), stats); });
+  m.def("check_linear", [](const Tensor& x, const Tensor& w, const OptTensor& b,
+                           const OptTensor& r) { check_linear(x, w, def(b), def(r)); });
+  m.def("check_linear_backward", [](const Tensor& dy, const Tensor& x, const Tensor& w,
+                                    const OptTensor& z, int64_t act) {
+    check_linear_backward(dy, x, w, def(z), act);
+  });
+  m.def("check_gated_scan", [](const Tensor& x, const Tensor& g, const OptTensor& h0,
+                               const OptTensor& n) { check_gated_scan(x, g, def(h0), def(n)); });
+  m.def("check_gated_scan_backward",
+        [](const OptTensor& dy, const OptTensor& ds, const Tensor& x, const Tensor& g,
+           const OptTensor& n, const Tensor& carry) {
+          check_gated_scan_backward(def(dy), def(ds), x, g, def(n), carry);
+        });
 }

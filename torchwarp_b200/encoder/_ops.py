@@ -3,7 +3,8 @@
 Eager calls go straight to the host extension (``csrc/host/encoder_host.cpp``), which checks the
 arguments, allocates, records autograd and calls the C ABI.  ``torch.compile`` needs ops it can
 trace: ``torchwarp_b200::layer_norm``, ``linear`` and ``gated_scan`` with fakes and registered
-backwards, over the same extension.  Backward passes are first order only.
+backwards, over the same extension.  Ops and fakes make the extension's checks of an eager call, so
+a bad argument is refused while a function is traced.  Backward passes are first order only.
 """
 
 from typing import Optional, Tuple
@@ -26,6 +27,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor],
 
 @layer_norm.register_fake
 def _(x, weight, bias, eps):
+    nat.host().check_layer_norm(x, weight, bias, eps)
     return (x.new_empty(x.shape),
             x.new_empty((2, x.numel() // x.shape[-1]), dtype=torch.float32))
 
@@ -38,6 +40,7 @@ def layer_norm_backward(dy: Tensor, x: Tensor, weight: Optional[Tensor], bias: O
 
 @layer_norm_backward.register_fake
 def _(dy, x, weight, bias, stats):
+    nat.host().check_layer_norm_backward(dy, x, weight, bias, stats)
     like = weight if weight is not None else bias if bias is not None else x
     return x.new_empty(x.shape), like.new_empty(x.shape[-1]), like.new_empty(x.shape[-1])
 
@@ -67,6 +70,7 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional
 
 @linear.register_fake
 def _(x, weight, bias, residual, act):
+    nat.host().check_linear(x, weight, bias, residual)
     n, k = weight.shape
     return (x.new_empty((*x.shape[:-1], n)),
             x.new_empty((x.numel() // k, n) if act else (0,)))
@@ -80,6 +84,7 @@ def linear_backward(dy: Tensor, x: Tensor, weight: Tensor, z: Tensor,
 
 @linear_backward.register_fake
 def _(dy, x, weight, z, act):
+    nat.host().check_linear_backward(dy, x, weight, z if act else None, act)
     return (x.new_empty(x.shape), weight.new_empty(weight.shape),
             weight.new_empty(weight.shape[0]))
 
@@ -110,6 +115,7 @@ def gated_scan(x: Tensor, gate: Tensor, h0: Optional[Tensor],
 
 @gated_scan.register_fake
 def _(x, gate, h0, lengths):
+    nat.host().check_gated_scan(x, gate, h0, lengths)
     b, t, d = x.shape
     return (x.new_empty((b, t, d)), x.new_empty((b, d), dtype=torch.float32),
             x.new_empty(nat.lib().tw_gated_scan_carry_bytes(b, t, d, x.element_size()),
@@ -125,6 +131,7 @@ def gated_scan_backward(dy: Optional[Tensor], dstate: Optional[Tensor], x: Tenso
 
 @gated_scan_backward.register_fake
 def _(dy, dstate, x, gate, lengths, carry):
+    nat.host().check_gated_scan_backward(dy, dstate, x, gate, lengths, carry)
     b, t, d = x.shape
     return (x.new_empty((b, t, d)), x.new_empty((b, t, d)),
             x.new_empty((b, d), dtype=torch.float32))

@@ -81,8 +81,6 @@ def gated_scan(x, gate, state=None, *, lengths=None):
         GatedScanOutput(output [B,T,D] of x's type, state [B,D] float32).
     """
     if torch.compiler.is_compiling():
-        if lengths is not None:
-            lengths = lengths.to(torch.int64)
         return GatedScanOutput(*_ops.gated_scan(x, gate, state, lengths)[:2])
     return GatedScanOutput(*nat.host().gated_scan(x, gate, state, lengths))
 
