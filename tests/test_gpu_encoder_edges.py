@@ -64,3 +64,72 @@ def test_compiled_calls_refuse_bad_arguments(tw, randn):
         torch._dynamo.reset()
         with pytest.raises(Exception, match="must (have|be)|CUDA"):
             torch.compile(f, fullgraph=True, backend="aot_eager")(x)
+
+
+# ------------------------------------------------------------------- AdamW
+
+def _stepped(tw, randn, sizes, **kw):
+    ps = [torch.nn.Parameter(randn(n)) for n in sizes]
+    for p in ps:
+        p.grad = randn(p.numel())
+    opt = tw.AdamW(ps, **kw)
+    opt.step()
+    return ps, opt
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_refuses_other_parameters_than_its_states(tw, randn, bits):
+    """A replaced, added, dropped, longer or shorter parameter: nothing is written."""
+    def refused(change, back):
+        ps, opt = _stepped(tw, randn, [300, 40, 7], state_bits=bits)
+        was = [v.clone() for v in opt.flat_state().values()]
+        group = opt.param_groups[0]["params"]
+        values = [p.detach().clone() for p in group]
+        change(group)
+        with pytest.raises(ValueError):
+            opt.step()
+        back(group, ps)
+        for v, w in zip(opt.flat_state().values(), was):
+            assert torch.equal(v.float(), w.float())
+        for p, v in zip(ps, values):
+            assert torch.equal(p.detach(), v)
+        opt.step()
+
+    def put(group, ps):
+        group[:] = ps
+
+    def resize(n):
+        def change(group):
+            group[0].grad = None
+            group[0].data = randn(n)
+            group[0].grad = randn(n)
+        return change
+
+    new = torch.nn.Parameter(randn(40))
+    new.grad = randn(40)
+    refused(lambda g: g.__setitem__(1, new), put)
+    refused(lambda g: g.append(new), put)
+    refused(lambda g: g.pop(), put)
+    refused(lambda g: g.reverse(), put)
+    for n in (4000, 301, 299, 0):
+        ps, opt = _stepped(tw, randn, [300, 40, 7], state_bits=bits)
+        was = [v.clone() for v in opt.flat_state().values()]
+        resize(n)(ps)
+        with pytest.raises(ValueError):
+            opt.step()
+        for v, w in zip(opt.flat_state().values(), was):
+            assert torch.equal(v.float(), w.float())
+
+
+def test_adamw_takes_new_groups_later(tw, randn):
+    ps, opt = _stepped(tw, randn, [300])
+    new = torch.nn.Parameter(randn(5))
+    new.grad = randn(5)
+    opt.add_param_group({"params": [new], "lr": 1e-2})
+    was = new.detach().clone()
+    kept = opt.flat_state(0)["exp_avg"].clone()
+    ps[0].grad = None
+    opt.step()
+    # a first step moves a weight by lr along its gradient's sign
+    torch.testing.assert_close(new.detach(), was * (1 - 1e-4) - 1e-2 * new.grad.sign())
+    assert torch.equal(opt.flat_state(0)["exp_avg"], kept)

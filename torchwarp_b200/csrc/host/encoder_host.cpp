@@ -564,20 +564,26 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const OptTensor& sta
 
 // ------------------------------------------------------------------ AdamW
 
-// One AdamW step over `params`, whose states start at `offsets` in the flat
-// buffers; a parameter without a gradient is left out.
-void adamw_step(const std::vector<Tensor>& params, const std::vector<int64_t>& offsets,
+// One AdamW step over `params`, which had `sizes` values each when the flat
+// buffers of their states were made, one after the other on boundaries of 256
+// values; a parameter without a gradient is left out.
+void adamw_step(const std::vector<Tensor>& params, const std::vector<int64_t>& sizes,
                 int64_t bits, const Tensor& m, const OptTensor& ms, const Tensor& v,
                 const OptTensor& vs, const Tensor& step, double lr, const OptTensor& lr_tensor,
                 double beta1, double beta2, double eps, double weight_decay, int64_t seed) {
-  TORCH_CHECK(params.size() == offsets.size(), "adamw_step: one offset a parameter");
+  TORCH_CHECK(params.size() == sizes.size(), "adamw_step: one size a parameter");
   std::vector<uint64_t> table;
   std::vector<Tensor> keep;
   table.reserve(4 * params.size());
   const at::ScalarType type = params.empty() ? at::kFloat : params[0].scalar_type();
-  for (size_t i = 0; i < params.size(); ++i) {
+  int64_t offset = 0;
+  for (size_t i = 0; i < params.size(); offset += (sizes[i] + 255) / 256 * 256, ++i) {
     const Tensor& p = params[i];
     Tensor g = p.grad();
+    if (g.defined() && (p.numel() != sizes[i] || g.numel() != sizes[i]))
+      bad_value("a parameter has " + std::to_string(p.numel()) + " values and its gradient " +
+                std::to_string(g.numel()) + ", where its states were made for " +
+                std::to_string(sizes[i]));
     if (!g.defined() || p.numel() == 0) continue;
     if (p.scalar_type() != type || g.scalar_type() != type || g.layout() != at::kStrided)
       bad_type("a gradient must be dense and of its parameter's type " + type_of(type) + ", got " +
@@ -591,8 +597,9 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<int64_t>& o
       keep.push_back(g);
     }
     table.insert(table.end(), {(uint64_t)p.data_ptr(), (uint64_t)g.data_ptr(), (uint64_t)p.numel(),
-                               (uint64_t)offsets[i]});
+                               (uint64_t)offset});
   }
+  TORCH_CHECK(m.numel() >= offset && v.numel() >= offset, "adamw_step: the states are too short");
   const float* lr_device = nullptr;
   if (lr_tensor.has_value()) {
     const Tensor& t = *lr_tensor;

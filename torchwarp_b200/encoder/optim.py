@@ -1,5 +1,7 @@
 """AdamW over all parameters of a group in one launch, with 32-bit or 8-bit states."""
 
+import operator
+
 import torch
 
 from .. import _native as nat
@@ -17,10 +19,8 @@ class _Bucket:
         if self.dtype not in (torch.float32, torch.bfloat16, torch.float16):
             raise TypeError("parameters must be float32, bfloat16 or float16, got {}".format(
                 self.dtype))
-        self.offsets, at = [], 0
-        for p in params:
-            self.offsets.append(at)
-            at += -(-p.numel() // _BLOCK) * _BLOCK
+        self.sizes = [p.numel() for p in params]
+        at = sum(-(-n // _BLOCK) * _BLOCK for n in self.sizes)
         dev = self.device
         self.step = torch.zeros(2, dtype=torch.int32, device=dev)
         if bits == 32:
@@ -55,8 +55,9 @@ class AdamW(torch.optim.Optimizer):
             float32 scale per 256 values, rounded stochastically.
         seed: Of that rounding; one seed gives one result.
 
-    The states of a group's parameters lie in flat buffers (``flat_state``).  The step count is
-    the group's and lives on the device; a parameter without a gradient is left out of a step.
+    The states of a group's parameters lie in flat buffers (``flat_state``), made at the first step:
+    from then on the group keeps its parameters, and they their sizes.  The step count is the
+    group's and lives on the device; a parameter without a gradient is left out of a step.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *,
@@ -77,12 +78,15 @@ class AdamW(torch.optim.Optimizer):
     def _group_buckets(self, index):
         """Made at the first step, when the parameters are where they will stay."""
         group = self.param_groups[index]["params"]
-        have = self._buckets.get(index)
-        if have is None or sum(len(b.params) for b in have) != len(group):
+        if index not in self._buckets:
             kinds = {}
             for p in group:
                 kinds.setdefault((p.device, p.dtype), []).append(p)
-            have = self._buckets[index] = [_Bucket(ps, self._bits) for ps in kinds.values()]
+            self._buckets[index] = tuple(group), [_Bucket(ps, self._bits) for ps in kinds.values()]
+        members, have = self._buckets[index]
+        if len(members) != len(group) or not all(map(operator.is_, members, group)):
+            raise ValueError("the parameters of group {} are not those that its states were made "
+                             "for; new ones come with add_param_group".format(index))
         return have
 
     @torch.no_grad()
@@ -96,7 +100,7 @@ class AdamW(torch.optim.Optimizer):
             on_device = isinstance(lr, torch.Tensor)
             for b in self._group_buckets(index):
                 m, ms, v, vs = b.buffers()
-                nat.host().adamw_step(b.params, b.offsets, self._bits, m, ms, v, vs, b.step,
+                nat.host().adamw_step(b.params, b.sizes, self._bits, m, ms, v, vs, b.step,
                                       0.0 if on_device else lr, lr if on_device else None,
                                       *group["betas"], group["eps"], group["weight_decay"],
                                       self._seed & 0xFFFFFFFF)
