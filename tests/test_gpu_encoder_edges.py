@@ -133,3 +133,39 @@ def test_adamw_takes_new_groups_later(tw, randn):
     # a first step moves a weight by lr along its gradient's sign
     torch.testing.assert_close(new.detach(), was * (1 - 1e-4) - 1e-2 * new.grad.sign())
     assert torch.equal(opt.flat_state(0)["exp_avg"], kept)
+
+
+# ------------------------------------------------------------------ linear
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu", "sigmoid"])
+@pytest.mark.parametrize("m", [4, 200])
+def test_linear_slopes_where_the_saved_z_is_infinite(tw, randn, m, act, dtype):
+    """z past the type's largest value is saved as an infinity; the slope there is 0 or 1.
+    Tolerances: those of tests/test_gpu_encoder.py for gradients, 4 roundings to the type and 64
+    of float32 in the 2-norm."""
+    big = {torch.float16: 7e4, torch.bfloat16: 3.395e38, torch.float32: 1e30}[dtype]
+    unit = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 0.0}[dtype]
+    k = 16
+    x, w = randn(m, k) * 0.5, randn(24, k) * 0.25
+    x[:, 0], x[1, 0], w[:, 0], w[0, 0], w[1, 0] = 0, 64, 0, -big / 64, big / 64
+    x, w = (v.to(dtype).requires_grad_(True) for v in (x, w))
+    dy = randn(m, 24, dtype=dtype)
+    grads = torch.autograd.grad(tw.functional.linear(x, w, activation=act), (x, w), dy)
+    xd, wd = x.detach().double(), w.detach().double()
+    z = xd @ wd.t()
+    assert float(z[1, 1]) > 0.9 * big and float(z[1, 0]) < -0.9 * big
+    if act == "relu":
+        slope = (z > 0).double()
+    elif act == "gelu":
+        slope = torch.special.ndtr(z) + z * torch.exp(-z * z / 2) * 0.3989422804014327
+    else:
+        f = torch.sigmoid(z)
+        slope = f * (1 + z * (1 - f)) if act == "silu" else f * (1 - f)
+    dz = dy.double() * slope
+    # the columns of w that hold `big` meet dx alone: compare the others, and that those are finite
+    for got, want in zip(grads, (dz @ wd, dz.t() @ xd)):
+        assert torch.isfinite(got).all() or dtype != torch.float16
+        got, want = got.double()[:, 1:], want[:, 1:]
+        err, bound = float((got - want).norm()), (4 * unit + 64 * 2.0 ** -24) * float(want.norm())
+        assert err <= bound + 2.0 ** -24 * want.numel() ** 0.5, (err, bound)

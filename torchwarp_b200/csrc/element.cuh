@@ -296,15 +296,20 @@ __device__ __forceinline__ Vec<V> act_value(Vec<V> z) {
   }
 }
 
-// d act / dz at z.
+// d act / dz at z.  z may be infinite where the forward was not: a saved z is
+// rounded to 16 bits.  Where a factor vanishes or is 1, the z it meets is cut
+// to a finite value; a NaN stays in the other factor.
 template <int ACT, bool FAST, int V>
 __device__ __forceinline__ Vec<V> act_slope(Vec<V> z) {
   if constexpr (ACT == kActGelu && FAST) {  // Phi(z) + z phi(z)
     Vec<V> az, e;
     Vec<V> c = fma_v(normal_tail(z, az, e), splat<V>(-1.f), splat<V>(0.5f));
 #pragma unroll
-    for (int i = 0; i < V; ++i) c.v[i] = copysignf(c.v[i], z.v[i]);
-    return fma_v(mul_v(z, splat<V>(0.39894228040143268f)), e, add_v(c, splat<V>(0.5f)));
+    for (int i = 0; i < V; ++i) {
+      c.v[i] = copysignf(c.v[i], z.v[i]);
+      az.v[i] = copysignf(az.v[i], z.v[i]);  // at the cut e is 0
+    }
+    return fma_v(mul_v(az, splat<V>(0.39894228040143268f)), e, add_v(c, splat<V>(0.5f)));
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -312,12 +317,13 @@ __device__ __forceinline__ Vec<V> act_slope(Vec<V> z) {
       if (ACT == kActRelu) v = v > 0.f ? 1.f : (v != v ? v : 0.f);
       if (ACT == kActGelu) {
         const float cdf = 0.5f * (1.f + erff(v * 0.70710678118654752f));
-        v = fmaf(v, 0.39894228040143268f * ex2(-0.72134752044448170f * v * v), cdf);
+        const float e = 0.39894228040143268f * ex2(-0.72134752044448170f * v * v);
+        v = fmaf(fmaxf(fminf(v, 30.f), -30.f), e, cdf);
       }
       if (ACT == kActSilu || ACT == kActSigmoid) {
         float f, omf;
         sigmoid_pair(v, f, omf);
-        v = ACT == kActSilu ? f * fmaf(v, omf, 1.f) : f * omf;
+        v = ACT == kActSilu ? f * fmaf(fmaxf(fminf(v, 128.f), -128.f), omf, 1.f) : f * omf;
       }
       if (ACT == kActNone) v = 1.f;
     }
