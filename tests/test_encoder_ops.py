@@ -100,3 +100,27 @@ def test_shapes_while_tracing():
         assert y.shape == (2, 3, 4) and z.shape == (6, 4)
         y, state, _ = _ops.gated_scan(x, x, None, torch.empty(2, dtype=torch.int32, device="cuda"))
         assert y.shape == x.shape and state.shape == (2, 8) and state.dtype == torch.float32
+
+
+def test_forward_mode_is_refused():
+    """An eager call and the ops alike, whichever input has the tangent, also without gradients."""
+    from torch.autograd import forward_ad
+    import torchwarp_b200.functional as TF
+
+    calls = [
+        (lambda x, w, b: TF.layer_norm(x, w, b), [X, (8,), (8,)]),
+        (lambda x, w, b, r: TF.linear(x, w, b, residual=r), [X, (4, 8), (4,), (2, 3, 4)]),
+        (lambda x, g, h: TF.gated_scan(x, g, h), [X, X, (2, 8)]),
+        (lambda x, g, h: TF.gated_scan_step(x, g, h), [(2, 8)] * 3),
+        (lambda x, w, b: _ops.layer_norm(x, w, b, 1e-5), [X, (8,), (8,)]),
+        (lambda x, w, b, r: _ops.linear(x, w, b, r, 0), [X, (4, 8), (4,), (2, 3, 4)]),
+        (lambda x, g, h: _ops.gated_scan(x, g, h, None), [X, X, (2, 8)]),
+    ]
+    for call, shapes in calls:
+        for which in range(len(shapes)):
+            for grad in (False, True):
+                with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+                    args = [real(s) for s in shapes]
+                    args[which] = forward_ad.make_dual(args[which], torch.ones(shapes[which]))
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        call(*args)

@@ -93,6 +93,14 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 
+// The operators have no forward-mode derivative: a tangent is refused, not lost.
+void no_tangents(const char* name, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined())
+      throw std::runtime_error(std::string(name) + " has no forward-mode derivative; its "
+                               "backward is first order");
+}
+
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 Tensor dense_like(const Tensor& x) { return at::empty(x.sizes(), x.options()); }
@@ -181,6 +189,7 @@ void check_layer_norm(const Tensor& x, const Tensor& w, const Tensor& b, double 
   if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type())
     bad_type("weight and bias must have one type");
   if (!(eps >= 0)) bad_value("eps must be >= 0");
+  no_tangents("layer_norm", {&x, &w, &b});
   check_devices(x, {&w, &b});
 }
 void check_layer_norm_backward(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& b,
@@ -293,6 +302,7 @@ void check_linear(const Tensor& x, const Tensor& w, const Tensor& b, const Tenso
   check_same_type("weight", w, x);
   if (b.defined()) check_same_type("bias", b, x);
   if (r.defined()) check_same_type("residual", r, x);
+  no_tangents("linear", {&x, &w, &b, &r});
   check_devices(x, {&w, &b, &r});
 }
 void check_linear_backward(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& z,
@@ -431,6 +441,7 @@ void check_gated_scan(const Tensor& x, const Tensor& gate, const Tensor& h0,
     if (lengths.scalar_type() != at::kLong && lengths.scalar_type() != at::kInt)
       bad_type("lengths must be int64 or int32, got " + type_of(lengths.scalar_type()));
   }
+  no_tangents("gated_scan", {&x, &gate, &h0});
   check_devices(x, {&gate, &h0, &lengths});
 }
 void check_gated_scan_backward(const Tensor& dy, const Tensor& dstate, const Tensor& x,
@@ -544,6 +555,7 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const OptTensor& sta
   if (state.scalar_type() != at::kFloat)
     bad_type("state must be float32, got " + type_of(state.scalar_type()));
   if (!state.is_contiguous()) bad_value("state must be contiguous: it is updated in place");
+  no_tangents("gated_scan_step", {&x, &gate, &state});
   check_devices(x, {&gate, &state});
   if (wants_grad({&x, &gate, &state}))
     throw std::runtime_error("gated_scan_step is not differentiable; use gated_scan, or no_grad");

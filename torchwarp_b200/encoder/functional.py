@@ -2,7 +2,7 @@
 gated linear recurrence over time.
 
 All take float32, bfloat16 or float16 CUDA tensors, compute in float32 and round a result once.
-They are differentiable once.  Under autocast ``linear`` runs in the autocast type; the others run
+They are differentiable once, in reverse mode (a forward-mode tangent is refused).  Under autocast ``linear`` runs in the autocast type; the others run
 in the type of their input (with float32 parameters, states and statistics).
 """
 
