@@ -124,3 +124,25 @@ def test_forward_mode_is_refused():
                     args[which] = forward_ad.make_dual(args[which], torch.ones(shapes[which]))
                     with pytest.raises(RuntimeError, match="forward-mode"):
                         call(*args)
+
+
+def test_tracers_see_the_operators():
+    """Fake tensors and make_fx: shapes and graph nodes come from the ops, nothing is launched."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    import torchwarp_b200.functional as TF
+
+    def f(x, w, b, r, g, h):
+        y = TF.linear(TF.layer_norm(x, b), w, b, activation="gelu", residual=r)
+        out, last = TF.gated_scan(y, g, h)
+        return out, last, TF.gated_scan_step(y[:, 0], g[:, 0], h)
+
+    shapes = [X, (8, 8), (8,), X, X, (2, 8)]
+    with FakeTensorMode():
+        out, last, y = f(*[traced(s) for s in shapes])
+        assert out.shape == X and last.shape == (2, 8) and y.shape == (2, 8)
+        args = [traced(s) for s in shapes]
+    with torch.no_grad():
+        graph = make_fx(f)(*args).graph
+    names = [str(n.target) for n in graph.nodes if "torchwarp" in str(n.target)]
+    assert names == ["torchwarp_b200.{}.default".format(n) for n in
+                     ("layer_norm", "linear", "gated_scan", "gated_scan_step")]

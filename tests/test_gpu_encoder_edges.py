@@ -169,3 +169,79 @@ def test_linear_slopes_where_the_saved_z_is_infinite(tw, randn, m, act, dtype):
         got, want = got.double()[:, 1:], want[:, 1:]
         err, bound = float((got - want).norm()), (4 * unit + 64 * 2.0 ** -24) * float(want.norm())
         assert err <= bound + 2.0 ** -24 * want.numel() ** 0.5, (err, bound)
+
+
+# ------------------------------------------------------ tracers, transforms
+
+def _program(tw, randn):
+    TF = tw.functional
+    w, b = randn(32, 32) / 6, randn(32)
+
+    def f(x, gate, lengths, w, b):
+        y = TF.linear(TF.layer_norm(x, b), w, b, activation="gelu", residual=x)
+        out, last = TF.gated_scan(y, gate, lengths=lengths)
+        return out, last
+
+    def args(*t):
+        return randn(3, 20, 32), randn(3, 20, 32), torch.tensor(t, device=DEV), w, b
+    return f, args
+
+
+def test_traced_programs_compute(tw, randn):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, args = _program(tw, randn)
+    a, b = args(20, 3, 7), args(5, 20, 0)
+    want = f(*b)
+    for program in (torch.jit.trace(f, a), make_fx(f)(*a), make_fx(f, tracing_mode="fake")(*a),
+                    make_fx(f, tracing_mode="symbolic")(*a)):
+        for got, w in zip(program(*b), want):
+            assert torch.equal(got, w)
+
+    def stream(x, gate, state):
+        return tw.functional.gated_scan_step(x, gate, state)
+
+    s = [randn(4, 32) for _ in range(3)]
+    for trace in (lambda: torch.jit.trace(stream, [v.clone() for v in s], check_trace=False),
+                  lambda: make_fx(stream)(*[v.clone() for v in s])):
+        program = trace()
+        x, gate, state = (randn(4, 32) for _ in range(3))
+        other = state.clone()
+        assert torch.equal(program(x, gate, state), stream(x, gate, other))
+        assert torch.equal(state, other)
+
+
+def test_dispatch_modes_and_subclasses(tw, randn):
+    """An operator under a mode gives the bits and the gradients of a plain call."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Log(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    f, args = _program(tw, randn)
+    x, *rest = args(20, 3, 7)
+    x.requires_grad_(True)
+    want = f(x, *rest)[0]
+    wg, = torch.autograd.grad(want.sum(), x)
+    names = []
+    with Log():
+        got = f(x, *rest)[0]
+        gg, = torch.autograd.grad(got.sum(), x)
+    for name in ("layer_norm", "linear", "gated_scan"):
+        assert "torchwarp_b200.{}.default".format(name) in names
+        assert "torchwarp_b200.{}_backward.default".format(name) in names
+    assert torch.equal(got, want) and torch.equal(gg, wg)
+
+
+def test_function_transforms(tw, randn):
+    """vmap goes slice by slice; derivatives by torch.func, which the operators lack, raise."""
+    f, args = _program(tw, randn)
+    x, *rest = args(20, 3, 7)
+    with pytest.raises(Exception):
+        torch.func.grad(lambda x: f(x, *rest)[0].square().sum())(x)
+    with pytest.raises(Exception):
+        torch.func.jvp(lambda x: f(x, *rest)[0], (x,), (x,))
+    for got, want in zip(torch.func.vmap(f, (0, 0, 0, None, None))(
+            *(torch.stack([v, v.flip(0)]) for v in (x, *rest[:2])), *rest[2:]), f(x, *rest)):
+        assert torch.equal(got[0], want) and torch.equal(got[1], want.flip(0))

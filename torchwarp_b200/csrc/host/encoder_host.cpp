@@ -6,7 +6,9 @@
 // the host side is C++: one conversion of the arguments, no interpreter in
 // the backward.  Backward passes are first order: their results carry a node
 // that raises when it is differentiated.
+#include <ATen/TracerMode.h>
 #include <ATen/autocast_mode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -91,6 +93,25 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+
+// Whether a call has to go through the dispatcher: torch.jit.trace, a dispatch
+// mode (make_fx, fake tensors), a transform or a tensor subclass would see only
+// the allocation of an eager call's results.
+bool dispatched(std::initializer_list<const Tensor*> ts) {
+  if (at::tracer::impl::is_dispatch_enabled() ||
+      c10::impl::TorchDispatchModeTLS::any_modes_set())
+    return true;
+  constexpr c10::DispatchKeySet wrapped({c10::DispatchKey::Python, c10::DispatchKey::Functionalize,
+                                         c10::DispatchKey::FuncTorchBatched,
+                                         c10::DispatchKey::FuncTorchGradWrapper});
+  for (const Tensor* t : ts)
+    if (t->defined() && t->key_set().has_any(wrapped)) return true;
+  return false;
+}
+// The custom op of that name.
+py::object op(const char* name) {
+  return py::module_::import("torchwarp_b200.encoder._ops").attr(name);
 }
 
 // The operators have no forward-mode derivative: a tangent is refused, not lost.
@@ -189,7 +210,6 @@ void check_layer_norm(const Tensor& x, const Tensor& w, const Tensor& b, double 
   if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type())
     bad_type("weight and bias must have one type");
   if (!(eps >= 0)) bad_value("eps must be >= 0");
-  no_tangents("layer_norm", {&x, &w, &b});
   check_devices(x, {&w, &b});
 }
 void check_layer_norm_backward(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& b,
@@ -271,6 +291,9 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
 
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
   Tensor w = def(weight), b = def(bias);
+  no_tangents("layer_norm", {&x, &w, &b});
+  if (dispatched({&x, &w, &b}))
+    return op("layer_norm")(x, weight, bias, eps).cast<std::pair<Tensor, Tensor>>().first;
   check_layer_norm(x, w, b, eps);
   w = dense(w);
   b = dense(b);
@@ -302,7 +325,6 @@ void check_linear(const Tensor& x, const Tensor& w, const Tensor& b, const Tenso
   check_same_type("weight", w, x);
   if (b.defined()) check_same_type("bias", b, x);
   if (r.defined()) check_same_type("residual", r, x);
-  no_tangents("linear", {&x, &w, &b, &r});
   check_devices(x, {&w, &b, &r});
 }
 void check_linear_backward(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& z,
@@ -405,6 +427,9 @@ Tensor linear(Tensor x, Tensor w, const OptTensor& bias, const OptTensor& residu
     if (b.defined()) b = b.to(t);
     if (r.defined()) r = r.to(t);
   }
+  no_tangents("linear", {&x, &w, &b, &r});
+  if (dispatched({&x, &w, &b, &r}))
+    return op("linear")(x, w, opt(b), opt(r), act).cast<std::pair<Tensor, Tensor>>().first;
   check_linear(x, w, b, r);
   b = dense(b);
   if (wants_grad({&x, &w, &b, &r})) return LinearFn::apply(x, w, opt(b), opt(r), act);
@@ -441,7 +466,6 @@ void check_gated_scan(const Tensor& x, const Tensor& gate, const Tensor& h0,
     if (lengths.scalar_type() != at::kLong && lengths.scalar_type() != at::kInt)
       bad_type("lengths must be int64 or int32, got " + type_of(lengths.scalar_type()));
   }
-  no_tangents("gated_scan", {&x, &gate, &h0});
   check_devices(x, {&gate, &h0, &lengths});
 }
 void check_gated_scan_backward(const Tensor& dy, const Tensor& dstate, const Tensor& x,
@@ -533,9 +557,15 @@ struct GatedScanFn : torch::autograd::Function<GatedScanFn> {
 
 std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gate, const OptTensor& state,
                                       const OptTensor& lengths_in) {
-  const Tensor h0 = def(state);
-  check_gated_scan(x, gate, h0, def(lengths_in));
-  const Tensor lengths = whole_lengths(def(lengths_in));
+  const Tensor h0 = def(state), n = def(lengths_in);
+  no_tangents("gated_scan", {&x, &gate, &h0});
+  if (dispatched({&x, &gate, &h0, &n})) {
+    auto out = op("gated_scan")(x, gate, state, lengths_in)
+                   .cast<std::tuple<Tensor, Tensor, Tensor>>();
+    return {std::get<0>(out), std::get<1>(out)};
+  }
+  check_gated_scan(x, gate, h0, n);
+  const Tensor lengths = whole_lengths(n);
   if (wants_grad({&x, &gate, &h0})) {
     variable_list out = GatedScanFn::apply(x, gate, opt(h0), opt(lengths));
     return {out[0], out[1]};
@@ -544,21 +574,22 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gate, const
   return {y, last};
 }
 
-Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const OptTensor& state_in) {
+void check_gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& state) {
   check_type("x", x);
   if (x.dim() != 2 || x.size(1) == 0)
     bad_value("x must have shape [batch, feature] with features");
   check_gate(gate, x);
-  if (!state_in.has_value()) bad_value("state must be a [B,D] tensor: it is updated in place");
-  const Tensor& state = *state_in;
+  if (!state.defined()) bad_value("state must be a [B,D] tensor: it is updated in place");
   check_state("state", state, x);
   if (state.scalar_type() != at::kFloat)
     bad_type("state must be float32, got " + type_of(state.scalar_type()));
   if (!state.is_contiguous()) bad_value("state must be contiguous: it is updated in place");
-  no_tangents("gated_scan_step", {&x, &gate, &state});
   check_devices(x, {&gate, &state});
   if (wants_grad({&x, &gate, &state}))
     throw std::runtime_error("gated_scan_step is not differentiable; use gated_scan, or no_grad");
+}
+
+Tensor gated_scan_step_forward(const Tensor& x, const Tensor& gate, const Tensor& state) {
   const int64_t b = x.size(0), d = x.size(1);
   Tensor y = dense_like(x);
   if (b) {
@@ -569,6 +600,15 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const OptTensor& sta
                      dim32(d), ptr(y), stream_of(x)),
                  "tw_gated_scan_step");
   }
+  return y;
+}
+
+Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const OptTensor& state_in) {
+  const Tensor state = def(state_in);
+  no_tangents("gated_scan_step", {&x, &gate, &state});
+  check_gated_scan_step(x, gate, state);
+  if (dispatched({&x, &gate, &state})) return op("gated_scan_step")(x, gate, state).cast<Tensor>();
+  const Tensor y = gated_scan_step_forward(x, gate, state);
   // written through a raw pointer: autograd has to see the change
   if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
   return y;
@@ -647,11 +687,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gated_scan", &gated_scan);
   m.def("gated_scan_step", &gated_scan_step);
   m.def("adamw_step", &adamw_step);
-  // without autograd, for the custom ops of torch.compile
+  // without autograd, for the custom ops
   m.def("layer_norm_forward", [](const Tensor& x, const OptTensor& w, const OptTensor& b,
                                  double eps) {
-    check_layer_norm(x, def(w), def(b), eps);
-    return layer_norm_forward(x, dense(def(w)), dense(def(b)), eps, true);
+    const Tensor weight = def(w), bias = def(b);
+    no_tangents("layer_norm", {&x, &weight, &bias});
+    check_layer_norm(x, weight, bias, eps);
+    return layer_norm_forward(x, dense(weight), dense(bias), eps, true);
   });
   m.def("layer_norm_backward", [](const Tensor& dy, const Tensor& x, const OptTensor& w,
                                   const OptTensor& b, const Tensor& stats) {
@@ -663,8 +705,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   });
   m.def("linear_forward", [](const Tensor& x, const Tensor& w, const OptTensor& b,
                              const OptTensor& r, int64_t act) {
-    check_linear(x, w, def(b), def(r));
-    auto [y, z] = linear_forward(x, w, dense(def(b)), def(r), act, true);
+    const Tensor bias = def(b), residual = def(r);
+    no_tangents("linear", {&x, &w, &bias, &residual});
+    check_linear(x, w, bias, residual);
+    auto [y, z] = linear_forward(x, w, dense(bias), residual, act, true);
     return std::make_tuple(y, opt(z));
   });
   m.def("linear_backward", [](const Tensor& dy, const Tensor& x, const Tensor& w,
@@ -674,13 +718,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   });
   m.def("gated_scan_forward", [](const Tensor& x, const Tensor& g, const OptTensor& h0,
                                  const OptTensor& n) {
-    check_gated_scan(x, g, def(h0), def(n));
-    return gated_scan_forward(x, g, def(h0), whole_lengths(def(n)), true);
+    const Tensor state = def(h0);
+    no_tangents("gated_scan", {&x, &g, &state});
+    check_gated_scan(x, g, state, def(n));
+    return gated_scan_forward(x, g, state, whole_lengths(def(n)), true);
   });
   m.def("gated_scan_backward", [](const OptTensor& dy, const OptTensor& ds, const Tensor& x,
                                   const Tensor& g, const OptTensor& n, const Tensor& carry) {
     check_gated_scan_backward(def(dy), def(ds), x, g, def(n), carry);
     return gated_scan_backward(def(dy), def(ds), x, g, whole_lengths(def(n)), carry);
+  });
+  m.def("gated_scan_step_forward", [](const Tensor& x, const Tensor& g, const Tensor& state) {
+    no_tangents("gated_scan_step", {&x, &g, &state});
+    check_gated_scan_step(x, g, state);
+    return gated_scan_step_forward(x, g, state);
   });
   // and for their fakes
   m.def("check_layer_norm", [](const Tensor& x, const OptTensor& w, const OptTensor& b,
@@ -696,6 +747,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   });
   m.def("check_gated_scan", [](const Tensor& x, const Tensor& g, const OptTensor& h0,
                                const OptTensor& n) { check_gated_scan(x, g, def(h0), def(n)); });
+  m.def("check_gated_scan_step", [](const Tensor& x, const Tensor& g, const Tensor& state) {
+    check_gated_scan_step(x, g, state);
+  });
   m.def("check_gated_scan_backward",
         [](const OptTensor& dy, const OptTensor& ds, const Tensor& x, const Tensor& g,
            const OptTensor& n, const Tensor& carry) {

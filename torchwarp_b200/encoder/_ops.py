@@ -1,9 +1,10 @@
-"""The encoder operators as torch custom ops, for ``torch.compile``.
+"""The encoder operators as torch custom ops, for ``torch.compile``, tracers and transforms.
 
 Eager calls go straight to the host extension (``csrc/host/encoder_host.cpp``), which checks the
 arguments, allocates, records autograd and calls the C ABI.  ``torch.compile`` needs ops it can
-trace: ``torchwarp_b200::layer_norm``, ``linear`` and ``gated_scan`` with fakes and registered
-backwards, over the same extension.  Ops and fakes make the extension's checks of an eager call, so
+trace: ``torchwarp_b200::layer_norm``, ``linear``, ``gated_scan`` with fakes and registered
+backwards, and ``gated_scan_step``, over the same extension.  The extension itself calls them where
+a tracer, a dispatch mode, a transform or a tensor subclass has to see the operator.  Ops and fakes make the extension's checks of an eager call, so
 a bad argument is refused while a function is traced.  Backward passes are first order only.
 """
 
@@ -150,3 +151,14 @@ def _gated_scan_bwd(ctx, dy, dstate, _carry):
 
 
 gated_scan.register_autograd(_gated_scan_bwd, setup_context=_gated_scan_setup)
+
+
+@torch.library.custom_op("torchwarp_b200::gated_scan_step", mutates_args=("state",))
+def gated_scan_step(x: Tensor, gate: Tensor, state: Tensor) -> Tensor:
+    return nat.host().gated_scan_step_forward(x, gate, state)
+
+
+@gated_scan_step.register_fake
+def _(x, gate, state):
+    nat.host().check_gated_scan_step(x, gate, state)
+    return x.new_empty(x.shape)
