@@ -245,3 +245,19 @@ def test_function_transforms(tw, randn):
     for got, want in zip(torch.func.vmap(f, (0, 0, 0, None, None))(
             *(torch.stack([v, v.flip(0)]) for v in (x, *rest[:2])), *rest[2:]), f(x, *rest)):
         assert torch.equal(got[0], want) and torch.equal(got[1], want.flip(0))
+
+
+def test_compiled_forward_mode_is_refused(tw, randn):
+    from torch.autograd import forward_ad
+    x = randn(2, 20, 32)
+    for f in (lambda x: tw.functional.layer_norm(x), lambda x: tw.functional.linear(x, x[0, :4]),
+              lambda x: tw.functional.gated_scan(x, x).output):
+        def level(x):
+            with forward_ad.dual_level():
+                return forward_ad.unpack_dual(f(forward_ad.make_dual(x, x))).tangent
+        for g in (lambda x: torch.func.jvp(f, (x,), (x,))[1], level):
+            torch._dynamo.reset()
+            with pytest.raises(Exception, match="forward-mode"):
+                torch.compile(g, backend="aot_eager")(x)
+        torch._dynamo.reset()  # and a call after it compiles
+        assert torch.equal(torch.compile(f, backend="aot_eager", fullgraph=True)(x), f(x))

@@ -9,9 +9,26 @@ in the type of their input (with float32 parameters, states and statistics).
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native as nat
 from . import _ops
+
+
+@torch.compiler.assume_constant_result
+def _forward_mode():
+    return forward_ad._current_level >= 0
+
+
+def _compiling():
+    """Whether a call is being traced by torch.compile, where it becomes a custom op.  An op does
+    not see the tangents of what it is traced with: forward mode is refused there as a whole."""
+    if not torch.compiler.is_compiling():
+        return False
+    if _forward_mode():
+        raise RuntimeError("the encoder operators have no forward-mode derivative; their backward "
+                           "is first order")
+    return True
 
 
 class GatedScanOutput(NamedTuple):
@@ -32,7 +49,7 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5):
     Returns:
         [..., D] of x's type.
     """
-    if torch.compiler.is_compiling():
+    if _compiling():
         return _ops.layer_norm(x, weight, bias, float(eps))[0]
     return nat.host().layer_norm(x, weight, bias, eps)
 
@@ -56,7 +73,7 @@ def linear(x, weight, bias=None, *, activation=None, residual=None):
         raise ValueError("activation must be one of {}, got {!r}".format(
             [a for a in _ops.ACTIVATIONS if a not in (None, "none")] + [None], activation))
     act = _ops.ACTIVATIONS[activation]
-    if torch.compiler.is_compiling():
+    if _compiling():
         if torch.is_autocast_enabled("cuda"):
             dtype = torch.get_autocast_dtype("cuda")
             x, weight, bias, residual = (None if t is None else t.to(dtype)
@@ -80,7 +97,7 @@ def gated_scan(x, gate, state=None, *, lengths=None):
     Returns:
         GatedScanOutput(output [B,T,D] of x's type, state [B,D] float32).
     """
-    if torch.compiler.is_compiling():
+    if _compiling():
         return GatedScanOutput(*_ops.gated_scan(x, gate, state, lengths)[:2])
     return GatedScanOutput(*nat.host().gated_scan(x, gate, state, lengths))
 
