@@ -261,3 +261,20 @@ def test_compiled_forward_mode_is_refused(tw, randn):
                 torch.compile(g, backend="aot_eager")(x)
         torch._dynamo.reset()  # and a call after it compiles
         assert torch.equal(torch.compile(f, backend="aot_eager", fullgraph=True)(x), f(x))
+
+
+def test_compiled_stream(tw, randn):
+    """A frame of a live stream in one compiled graph: eager's bits, the states updated in place."""
+    torch._dynamo.reset()
+    enc = tw.SequenceEncoder(5, 32, layers=2, device=DEV)
+    step = torch.compile(enc.step, fullgraph=True, backend="aot_eager")
+    a, b = enc.init_state(3), enc.init_state(3)
+    for _ in range(4):
+        x = randn(3, 5)
+        got, want = step(x, a), enc.step(x, b)
+        assert torch.equal(got, want)
+        for u, v in zip(a, b):
+            assert torch.equal(u, v)
+    x = randn(3, 16).requires_grad_(True)
+    with pytest.raises(Exception, match="not differentiable"):
+        torch.compile(tw.functional.gated_scan_step, backend="aot_eager")(x, x, randn(3, 16))

@@ -112,4 +112,9 @@ def gated_scan_step(x, gate, state):
     Returns:
         [B,D] of x's type.  Not differentiable.
     """
+    if _compiling():
+        if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad
+                                        or state.requires_grad):
+            raise RuntimeError("gated_scan_step is not differentiable; use gated_scan, or no_grad")
+        return _ops.gated_scan_step(x, gate, state)
     return nat.host().gated_scan_step(x, gate, state)
