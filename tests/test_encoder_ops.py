@@ -146,3 +146,32 @@ def test_tracers_see_the_operators():
     names = [str(n.target) for n in graph.nodes if "torchwarp" in str(n.target)]
     assert names == ["torchwarp_b200.{}.default".format(n) for n in
                      ("layer_norm", "linear", "gated_scan", "gated_scan_step")]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_symbolic_lengths_stay_symbolic(dtype):
+    """A dynamic time dimension is not fixed by the fakes, which give the sizes of the real ops."""
+    from torch.fx.experimental.symbolic_shapes import (DimDynamic, ShapeEnv,
+                                                       StatelessSymbolicContext)
+    from torchwarp_b200 import _native
+
+    env, plain = ShapeEnv(), torch.empty(3, 33, 20, dtype=dtype, device="meta")
+    with FakeTensorMode(shape_env=env) as mode:
+        dyn = StatelessSymbolicContext([DimDynamic.STATIC, DimDynamic.DYNAMIC, DimDynamic.STATIC])
+        x = mode.from_tensor(plain, symbolic_context=dyn)
+        x = torch.empty_like(x, device="cuda")
+        w, n = traced((8, 20), dtype), traced((3,), I)
+        assert isinstance(x.shape[1], torch.SymInt)
+        _, stats = _ops.layer_norm(x, None, None, 1e-5)
+        y, z = _ops.linear(x, w, None, None, 1)
+        out, state, carry = _ops.gated_scan(x, x, None, n)
+        dx, dg, dh = _ops.gated_scan_backward(out, state, x, x, n, carry)
+        assert all(isinstance(v, torch.SymInt) for v in (stats.shape[1], y.shape[1], z.shape[0],
+                                                         out.shape[1], carry.shape[0], dx.shape[1]))
+    assert not env.replacements  # nothing fixed the symbol
+    lib, size = _native.lib(), 4 if dtype == torch.float32 else 2
+    for b, t, d in ((3, 33, 20), (1, 5000, 16), (1, 1, 1), (4, 0, 8), (2, 17, 8)):
+        with FakeTensorMode():
+            carry = _ops.gated_scan(traced((b, t, d), dtype), traced((b, t, d), dtype), None, None)[2]
+        assert carry.numel() == (lib.tw_gated_scan_carry_bytes(b, t, d, size)
+                                 - lib.tw_gated_scan_workspace_bytes(b, t, d, size))

@@ -278,3 +278,27 @@ def test_compiled_stream(tw, randn):
     x = randn(3, 16).requires_grad_(True)
     with pytest.raises(Exception, match="not differentiable"):
         torch.compile(tw.functional.gated_scan_step, backend="aot_eager")(x, x, randn(3, 16))
+
+
+def test_compiled_once_for_all_lengths(tw, randn):
+    """Time marked dynamic: one graph, right at every length, forward and backward."""
+    from torch._dynamo.testing import CompileCounterWithBackend
+    TF = tw.functional
+    w, b = randn(48, 24), randn(48)
+
+    def f(x):
+        v, a = TF.linear(TF.layer_norm(x), w, b, activation="silu").split(24, -1)
+        return TF.gated_scan(v, a).output
+
+    torch._dynamo.reset()
+    counter = CompileCounterWithBackend("aot_eager")
+    g = torch.compile(f, backend=counter, fullgraph=True)
+    for t in (33, 700, 5, 129, 2000):
+        x = randn(3, t, 24).requires_grad_(True)
+        torch._dynamo.mark_dynamic(x, 1)
+        got = g(x)
+        dx, = torch.autograd.grad(got.square().sum(), x)
+        want = f(x)
+        wx, = torch.autograd.grad(want.square().sum(), x)
+        assert torch.equal(got, want) and torch.equal(dx, wx)
+    assert counter.frame_count == 1

@@ -493,8 +493,10 @@ std::tuple<Tensor, Tensor, Tensor> gated_scan_forward(const Tensor& x_in, const 
   const int64_t b = x_in.size(0), t = x_in.size(1), d = x_in.size(2);
   Tensor y = dense_like(x_in);
   Tensor state = at::empty({b, d}, x_in.options().dtype(at::kFloat));
-  const auto size = save ? tw_gated_scan_carry_bytes : tw_gated_scan_workspace_bytes;
-  const size_t n = size(dim32(b), dim32(t), dim32(d), (int)x_in.element_size());
+  // the saved states, and behind them the call's own scratch
+  const int es = (int)x_in.element_size();
+  const size_t scratch = tw_gated_scan_workspace_bytes(dim32(b), dim32(t), dim32(d), es);
+  const size_t n = save ? tw_gated_scan_carry_bytes((int)b, (int)t, (int)d, es) : scratch;
   Tensor carry = bytes(n, x_in);
   if (b) {
     c10::cuda::CUDAGuard guard(x_in.device());
@@ -507,6 +509,7 @@ std::tuple<Tensor, Tensor, Tensor> gated_scan_forward(const Tensor& x_in, const 
                  "tw_gated_scan_forward");
   }
   if (save && !carry.defined()) carry = at::empty({0}, x_in.options().dtype(at::kByte));
+  if (save && scratch) carry = carry.narrow(0, 0, (int64_t)(n - scratch));
   return {y, state, carry};
 }
 

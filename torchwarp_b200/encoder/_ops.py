@@ -118,9 +118,10 @@ def gated_scan(x: Tensor, gate: Tensor, h0: Optional[Tensor],
 def _(x, gate, h0, lengths):
     nat.host().check_gated_scan(x, gate, h0, lengths)
     b, t, d = x.shape
+    frames = 8 if x.element_size() == 4 else 16  # of a run, whose state is saved; sizes may be symbols
+    states = 4 * b * d * ((t + frames - 1) // frames)
     return (x.new_empty((b, t, d)), x.new_empty((b, d), dtype=torch.float32),
-            x.new_empty(nat.lib().tw_gated_scan_carry_bytes(b, t, d, x.element_size()),
-                        dtype=torch.uint8))
+            x.new_empty((states + 15) // 16 * 16, dtype=torch.uint8))
 
 
 @torch.library.custom_op("torchwarp_b200::gated_scan_backward", mutates_args=())
