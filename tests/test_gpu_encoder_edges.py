@@ -302,3 +302,40 @@ def test_compiled_once_for_all_lengths(tw, randn):
         wx, = torch.autograd.grad(want.square().sum(), x)
         assert torch.equal(got, want) and torch.equal(dx, wx)
     assert counter.frame_count == 1
+
+
+def test_compiled_inference_saves_nothing(tw, randn):
+    """What only a backward needs is written when one can follow, not in a call without gradients."""
+    TF = tw.functional
+    x, w = randn(3, 40, 32), randn(64, 32)
+
+    def f(x, w):
+        v, a = TF.linear(TF.layer_norm(x), w, activation="gelu").split(32, -1)
+        return TF.gated_scan(v, a)
+
+    def saves(x, w, grad):
+        graphs = []
+
+        def backend(gm, inputs):
+            graphs.append(gm)
+            return gm.forward
+
+        torch._dynamo.reset()
+        with torch.set_grad_enabled(grad):
+            got, want = torch.compile(f, backend=backend, fullgraph=True)(x, w), f(x, w)
+        assert torch.equal(got.output, want.output) and torch.equal(got.state, want.state)
+        return [n.args[-1] for n in graphs[0].graph.nodes if "torchwarp" in str(n.target)]
+
+    assert saves(x, w, True) == [False] * 3 and saves(x, w.requires_grad_(True), False) == [False] * 3
+    assert saves(x, w, True) == [False, True, True]
+    ops = torch.ops.torchwarp_b200
+    assert ops.layer_norm(x, None, None, 1e-5, False)[1].numel() == 0
+    assert ops.linear(x, w.detach(), None, None, 2, False)[1].numel() == 0
+    assert ops.gated_scan(x, x, None, None, False)[2].numel() == 0
+    # a backward without what it needs is refused
+    with pytest.raises(ValueError):
+        ops.layer_norm_backward(x, x, None, None, ops.layer_norm(x, None, None, 1e-5, False)[1])
+    with pytest.raises(ValueError):
+        ops.linear_backward(randn(3, 40, 64), x, w.detach(), randn(0), 2)
+    with pytest.raises(RuntimeError):
+        ops.gated_scan_backward(x, None, x, x, None, torch.empty(0, dtype=torch.uint8, device=DEV))

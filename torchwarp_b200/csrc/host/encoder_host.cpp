@@ -293,7 +293,8 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
   Tensor w = def(weight), b = def(bias);
   no_tangents("layer_norm", {&x, &w, &b});
   if (dispatched({&x, &w, &b}))
-    return op("layer_norm")(x, weight, bias, eps).cast<std::pair<Tensor, Tensor>>().first;
+    return op("layer_norm")(x, weight, bias, eps)
+        .cast<std::pair<Tensor, Tensor>>().first;
   check_layer_norm(x, w, b, eps);
   w = dense(w);
   b = dense(b);
@@ -429,7 +430,8 @@ Tensor linear(Tensor x, Tensor w, const OptTensor& bias, const OptTensor& residu
   }
   no_tangents("linear", {&x, &w, &b, &r});
   if (dispatched({&x, &w, &b, &r}))
-    return op("linear")(x, w, opt(b), opt(r), act).cast<std::pair<Tensor, Tensor>>().first;
+    return op("linear")(x, w, opt(b), opt(r), act)
+        .cast<std::pair<Tensor, Tensor>>().first;
   check_linear(x, w, b, r);
   b = dense(b);
   if (wants_grad({&x, &w, &b, &r})) return LinearFn::apply(x, w, opt(b), opt(r), act);
@@ -692,11 +694,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("adamw_step", &adamw_step);
   // without autograd, for the custom ops
   m.def("layer_norm_forward", [](const Tensor& x, const OptTensor& w, const OptTensor& b,
-                                 double eps) {
+                                 double eps, bool save) {
     const Tensor weight = def(w), bias = def(b);
     no_tangents("layer_norm", {&x, &weight, &bias});
     check_layer_norm(x, weight, bias, eps);
-    return layer_norm_forward(x, dense(weight), dense(bias), eps, true);
+    auto [y, stats] = layer_norm_forward(x, dense(weight), dense(bias), eps, save);
+    return std::make_tuple(y, opt(stats));
   });
   m.def("layer_norm_backward", [](const Tensor& dy, const Tensor& x, const OptTensor& w,
                                   const OptTensor& b, const Tensor& stats) {
@@ -707,11 +710,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                                true);
   });
   m.def("linear_forward", [](const Tensor& x, const Tensor& w, const OptTensor& b,
-                             const OptTensor& r, int64_t act) {
+                             const OptTensor& r, int64_t act, bool save) {
     const Tensor bias = def(b), residual = def(r);
     no_tangents("linear", {&x, &w, &bias, &residual});
     check_linear(x, w, bias, residual);
-    auto [y, z] = linear_forward(x, w, dense(bias), residual, act, true);
+    auto [y, z] = linear_forward(x, w, dense(bias), residual, act, save);
     return std::make_tuple(y, opt(z));
   });
   m.def("linear_backward", [](const Tensor& dy, const Tensor& x, const Tensor& w,
@@ -720,11 +723,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return linear_backward(dy, x, w, def(z), act, true, true, true);
   });
   m.def("gated_scan_forward", [](const Tensor& x, const Tensor& g, const OptTensor& h0,
-                                 const OptTensor& n) {
+                                 const OptTensor& n, bool save) {
     const Tensor state = def(h0);
     no_tangents("gated_scan", {&x, &g, &state});
     check_gated_scan(x, g, state, def(n));
-    return gated_scan_forward(x, g, state, whole_lengths(def(n)), true);
+    auto [y, last, carry] = gated_scan_forward(x, g, state, whole_lengths(def(n)), save);
+    return std::make_tuple(y, last, save ? opt(carry) : std::nullopt);
   });
   m.def("gated_scan_backward", [](const OptTensor& dy, const OptTensor& ds, const Tensor& x,
                                   const Tensor& g, const OptTensor& n, const Tensor& carry) {

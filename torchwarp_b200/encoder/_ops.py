@@ -5,7 +5,8 @@ arguments, allocates, records autograd and calls the C ABI.  ``torch.compile`` n
 trace: ``torchwarp_b200::layer_norm``, ``linear``, ``gated_scan`` with fakes and registered
 backwards, and ``gated_scan_step``, over the same extension.  The extension itself calls them where
 a tracer, a dispatch mode, a transform or a tensor subclass has to see the operator.  Ops and fakes make the extension's checks of an eager call, so
-a bad argument is refused while a function is traced.  Backward passes are first order only.
+a bad argument is refused while a function is traced.  ``save``: a backward will follow, and the
+results that it needs are not left empty.  Backward passes are first order only.
 """
 
 from typing import Optional, Tuple
@@ -22,15 +23,16 @@ ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4
 
 @torch.library.custom_op("torchwarp_b200::layer_norm", mutates_args=())
 def layer_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor],
-               eps: float) -> Tuple[Tensor, Tensor]:
-    return nat.host().layer_norm_forward(x, weight, bias, eps)
+               eps: float, save: bool = True) -> Tuple[Tensor, Tensor]:
+    y, stats = nat.host().layer_norm_forward(x, weight, bias, eps, save)
+    return y, stats if save else x.new_empty((2, 0), dtype=torch.float32)
 
 
 @layer_norm.register_fake
-def _(x, weight, bias, eps):
+def _(x, weight, bias, eps, save=True):
     nat.host().check_layer_norm(x, weight, bias, eps)
     return (x.new_empty(x.shape),
-            x.new_empty((2, x.numel() // x.shape[-1]), dtype=torch.float32))
+            x.new_empty((2, x.numel() // x.shape[-1] if save else 0), dtype=torch.float32))
 
 
 @torch.library.custom_op("torchwarp_b200::layer_norm_backward", mutates_args=())
@@ -47,14 +49,14 @@ def _(dy, x, weight, bias, stats):
 
 
 def _layer_norm_setup(ctx, inputs, output):
-    x, weight, bias, _ = inputs
+    x, weight, bias, _, _ = inputs
     ctx.save_for_backward(x, weight, bias, output[1])
 
 
 def _layer_norm_bwd(ctx, dy, _stats):
     x, weight, bias, stats = ctx.saved_tensors
     dx, dw, db = layer_norm_backward(dy, x, weight, bias, stats)
-    return dx, None if weight is None else dw, None if bias is None else db, None
+    return dx, None if weight is None else dw, None if bias is None else db, None, None
 
 
 layer_norm.register_autograd(_layer_norm_bwd, setup_context=_layer_norm_setup)
@@ -64,17 +66,17 @@ layer_norm.register_autograd(_layer_norm_bwd, setup_context=_layer_norm_setup)
 
 @torch.library.custom_op("torchwarp_b200::linear", mutates_args=())
 def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor],
-           act: int) -> Tuple[Tensor, Tensor]:
-    y, z = nat.host().linear_forward(x, weight, bias, residual, act)
+           act: int, save: bool = True) -> Tuple[Tensor, Tensor]:
+    y, z = nat.host().linear_forward(x, weight, bias, residual, act, save)
     return y, z if z is not None else x.new_empty(0)
 
 
 @linear.register_fake
-def _(x, weight, bias, residual, act):
+def _(x, weight, bias, residual, act, save=True):
     nat.host().check_linear(x, weight, bias, residual)
     n, k = weight.shape
     return (x.new_empty((*x.shape[:-1], n)),
-            x.new_empty((x.numel() // k, n) if act else (0,)))
+            x.new_empty((x.numel() // k, n) if act and save else (0,)))
 
 
 @torch.library.custom_op("torchwarp_b200::linear_backward", mutates_args=())
@@ -91,7 +93,7 @@ def _(dy, x, weight, z, act):
 
 
 def _linear_setup(ctx, inputs, output):
-    x, weight, bias, residual, act = inputs
+    x, weight, bias, residual, act, _ = inputs
     ctx.save_for_backward(x, weight, output[1])
     ctx.has = (bias is not None, residual is not None)
     ctx.act = act
@@ -100,7 +102,7 @@ def _linear_setup(ctx, inputs, output):
 def _linear_bwd(ctx, dy, _z):
     x, weight, z = ctx.saved_tensors
     dx, dw, db = linear_backward(dy, x, weight, z, ctx.act)
-    return dx, dw, db if ctx.has[0] else None, dy if ctx.has[1] else None, None
+    return dx, dw, db if ctx.has[0] else None, dy if ctx.has[1] else None, None, None
 
 
 linear.register_autograd(_linear_bwd, setup_context=_linear_setup)
@@ -110,16 +112,17 @@ linear.register_autograd(_linear_bwd, setup_context=_linear_setup)
 
 @torch.library.custom_op("torchwarp_b200::gated_scan", mutates_args=())
 def gated_scan(x: Tensor, gate: Tensor, h0: Optional[Tensor],
-               lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
-    return nat.host().gated_scan_forward(x, gate, h0, lengths)
+               lengths: Optional[Tensor], save: bool = True) -> Tuple[Tensor, Tensor, Tensor]:
+    y, state, carry = nat.host().gated_scan_forward(x, gate, h0, lengths, save)
+    return y, state, carry if save else x.new_empty(0, dtype=torch.uint8)
 
 
 @gated_scan.register_fake
-def _(x, gate, h0, lengths):
+def _(x, gate, h0, lengths, save=True):
     nat.host().check_gated_scan(x, gate, h0, lengths)
     b, t, d = x.shape
     frames = 8 if x.element_size() == 4 else 16  # of a run, whose state is saved; sizes may be symbols
-    states = 4 * b * d * ((t + frames - 1) // frames)
+    states = 4 * b * d * ((t + frames - 1) // frames) if save else 0
     return (x.new_empty((b, t, d)), x.new_empty((b, d), dtype=torch.float32),
             x.new_empty((states + 15) // 16 * 16, dtype=torch.uint8))
 
@@ -140,7 +143,7 @@ def _(dy, dstate, x, gate, lengths, carry):
 
 
 def _gated_scan_setup(ctx, inputs, output):
-    x, gate, h0, lengths = inputs
+    x, gate, h0, lengths, _ = inputs
     ctx.save_for_backward(x, gate, lengths, output[2])
     ctx.has_h0 = h0 is not None
 
@@ -148,7 +151,7 @@ def _gated_scan_setup(ctx, inputs, output):
 def _gated_scan_bwd(ctx, dy, dstate, _carry):
     x, gate, lengths, carry = ctx.saved_tensors
     dx, dgate, dh0 = gated_scan_backward(dy, dstate, x, gate, lengths, carry)
-    return dx, dgate, dh0 if ctx.has_h0 else None, None
+    return dx, dgate, dh0 if ctx.has_h0 else None, None, None
 
 
 gated_scan.register_autograd(_gated_scan_bwd, setup_context=_gated_scan_setup)

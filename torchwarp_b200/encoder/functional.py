@@ -31,6 +31,10 @@ def _compiling():
     return True
 
 
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class GatedScanOutput(NamedTuple):
     """Result of ``gated_scan``: ``output`` [B,T,D] and the last ``state`` [B,D] (float32)."""
 
@@ -50,7 +54,7 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5):
         [..., D] of x's type.
     """
     if _compiling():
-        return _ops.layer_norm(x, weight, bias, float(eps))[0]
+        return _ops.layer_norm(x, weight, bias, float(eps), _wants_grad(x, weight, bias))[0]
     return nat.host().layer_norm(x, weight, bias, eps)
 
 
@@ -78,7 +82,8 @@ def linear(x, weight, bias=None, *, activation=None, residual=None):
             dtype = torch.get_autocast_dtype("cuda")
             x, weight, bias, residual = (None if t is None else t.to(dtype)
                                          for t in (x, weight, bias, residual))
-        return _ops.linear(x, weight, bias, residual, act)[0]
+        return _ops.linear(x, weight, bias, residual, act,
+                           _wants_grad(x, weight, bias, residual))[0]
     return nat.host().linear(x, weight, bias, residual, act)
 
 
@@ -98,7 +103,8 @@ def gated_scan(x, gate, state=None, *, lengths=None):
         GatedScanOutput(output [B,T,D] of x's type, state [B,D] float32).
     """
     if _compiling():
-        return GatedScanOutput(*_ops.gated_scan(x, gate, state, lengths)[:2])
+        return GatedScanOutput(*_ops.gated_scan(x, gate, state, lengths,
+                                                 _wants_grad(x, gate, state))[:2])
     return GatedScanOutput(*nat.host().gated_scan(x, gate, state, lengths))
 
 
@@ -113,8 +119,7 @@ def gated_scan_step(x, gate, state):
         [B,D] of x's type.  Not differentiable.
     """
     if _compiling():
-        if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad
-                                        or state.requires_grad):
+        if _wants_grad(x, gate, state):
             raise RuntimeError("gated_scan_step is not differentiable; use gated_scan, or no_grad")
         return _ops.gated_scan_step(x, gate, state)
     return nat.host().gated_scan_step(x, gate, state)
