@@ -28,6 +28,7 @@ OBJ_DIR = PKG.parent / "_build" / "obj"
 ROOT = PKG.parent
 HOST_SRC = CSRC / "host" / "encoder_host.cpp"
 HOST_LIB = OUT_DIR / "_encoder_host.so"
+HOST_STAMP = OBJ_DIR / "_encoder_host.stamp"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -42,7 +43,7 @@ def nvcc():
 
 
 def _headers():
-    return sorted(CSRC.glob("*.cuh")) + sorted((ROOT / "include").glob("*.h"))
+    return sorted(p for d in (CSRC, ROOT / "include") for e in ("*.cuh", "*.h") for p in d.glob(e))
 
 
 def _compile(src, force):
@@ -59,10 +60,6 @@ def _compile(src, force):
 
 def _build_host(force):
     """The host extension; returns an error text or None."""
-    deps = [HOST_SRC, ROOT / "include" / "torchwarp_b200.h"]
-    if not force and HOST_LIB.exists() and \
-            HOST_LIB.stat().st_mtime >= max(d.stat().st_mtime for d in deps):
-        return None
     import sysconfig
 
     import torch
@@ -78,8 +75,19 @@ def _build_host(force):
            *(a for i in includes for a in ("-isystem", i)), str(HOST_SRC), "-o", str(HOST_LIB),
            "-L", str(OUT_DIR), "-l:" + LIB.name, "-L", torch_lib, "-lc10", "-lc10_cuda",
            "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    deps = [HOST_SRC, ROOT / "include" / "torchwarp_b200.h"]
+    # another torch or interpreter needs another build of the same source
+    stamp = "{}\ntorch {}".format(" ".join(cmd), torch.__version__)
+    if not force and HOST_LIB.exists() and HOST_STAMP.exists() and \
+            HOST_STAMP.read_text() == stamp and \
+            HOST_LIB.stat().st_mtime >= max(d.stat().st_mtime for d in deps):
+        return None
+    HOST_STAMP.unlink(missing_ok=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
-    return None if r.returncode == 0 else "{}\n{}{}".format(" ".join(cmd), r.stdout, r.stderr)
+    if r.returncode != 0:
+        return "{}\n{}{}".format(" ".join(cmd), r.stdout, r.stderr)
+    HOST_STAMP.write_text(stamp)
+    return None
 
 
 def build(force=False, verbose=False):
