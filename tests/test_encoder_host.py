@@ -1,6 +1,9 @@
 """Host-side checks of the encoder operators that need no GPU: argument checks, the public names,
 the C ABI's refusals and the missing CPU fallback."""
 
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -120,3 +123,11 @@ def test_c_abi_refusals_without_a_gpu():
     assert lib.tw_adamw_step_f32(p, 1, 32, p, None, p, None, p, 1e-3, None, 1.0, 0.99, 1e-8, 0.0,
                                  0, None) == 1
     assert b"beta" in lib.tw_last_error()
+
+
+@pytest.mark.parametrize("again", [copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))])
+def test_adamw_is_copied_whole(again):
+    opt = again(tw.AdamW(_params(), lr=0.5, state_bits=8, seed=7))
+    assert (opt._bits, opt._seed, opt.param_groups[0]["lr"]) == (8, 7, 0.5)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        opt.step()

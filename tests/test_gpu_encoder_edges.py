@@ -1,5 +1,8 @@
 """The encoder operators where inputs, tensors or programs are unlike a plain eager call (B200)."""
 
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -339,3 +342,30 @@ def test_compiled_inference_saves_nothing(tw, randn):
         ops.linear_backward(randn(3, 40, 64), x, w.detach(), randn(0), 2)
     with pytest.raises(RuntimeError):
         ops.gated_scan_backward(x, None, x, x, None, torch.empty(0, dtype=torch.uint8, device=DEV))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("again", [copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))])
+def test_adamw_copies_go_on_by_themselves(tw, randn, bits, again):
+    """A copy has its own weights and states, and takes the steps that the optimizer takes."""
+    ps, opt = _stepped(tw, randn, [300, 5], state_bits=bits, seed=4)
+    ps.append(torch.nn.Parameter(randn(40).half()))
+    ps[-1].grad = randn(40).half()
+    opt.add_param_group({"params": ps[-1:]})
+    opt.step()
+    other = again(opt)
+    qs = [p for g in other.param_groups for p in g["params"]]
+    for p, q in zip(ps, qs):
+        assert p is not q and torch.equal(p, q)
+        q.grad = p.grad.clone()
+    for _ in range(2):
+        opt.step()
+    for p, q in zip(ps, qs):
+        assert not torch.equal(p, q)
+    for _ in range(2):
+        other.step()
+    for p, q in zip(ps, qs):
+        assert torch.equal(p, q)
+    for k in range(2):
+        for a, b in zip(opt.flat_state(k).values(), other.flat_state(k).values()):
+            assert a.data_ptr() != b.data_ptr() and torch.equal(a.float(), b.float())

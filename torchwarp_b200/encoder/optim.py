@@ -6,6 +6,7 @@ import torch
 
 from .. import _native as nat
 
+_CODE = torch.float8_e4m3fn
 _BLOCK = 256  # values that share a scale; every tensor's states start on such a boundary
 
 
@@ -27,12 +28,22 @@ class _Bucket:
             self.state = {"exp_avg": torch.zeros(at, device=dev),
                           "exp_avg_sq": torch.zeros(at, device=dev)}
         else:
-            code = dict(dtype=torch.float8_e4m3fn, device=dev)
+            code = dict(dtype=_CODE, device=dev)
             self.state = {"exp_avg": torch.zeros(at, **code),
                           "exp_avg_scale": torch.zeros(at // _BLOCK, device=dev),
                           "exp_avg_sqrt": torch.zeros(at, **code),
                           "exp_avg_sqrt_scale": torch.zeros(at // _BLOCK, device=dev)}
         self.bits = bits
+
+    # pickle takes no float8 tensors: codes travel as bytes
+    def __getstate__(self):
+        return {**self.__dict__, "state": {k: v.view(torch.uint8) if v.dtype == _CODE else v
+                                           for k, v in self.state.items()}}
+
+    def __setstate__(self, saved):
+        self.__dict__.update(saved)
+        self.state = {k: v.view(_CODE) if v.dtype == torch.uint8 else v
+                      for k, v in self.state.items()}
 
     def buffers(self):
         """First moments and their scales, second moments and theirs."""
@@ -74,6 +85,11 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("state_bits must be 8 or 32")
         self._bits, self._seed, self._buckets = state_bits, int(seed), {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def __getstate__(self):
+        """Copies and pickles keep the states and whose they are, not only the groups."""
+        return {**super().__getstate__(), "_bits": self._bits, "_seed": self._seed,
+                "_buckets": self._buckets}
 
     def _group_buckets(self, index):
         """Made at the first step, when the parameters are where they will stay."""
