@@ -369,3 +369,18 @@ def test_adamw_copies_go_on_by_themselves(tw, randn, bits, again):
     for k in range(2):
         for a, b in zip(opt.flat_state(k).values(), other.flat_state(k).values()):
             assert a.data_ptr() != b.data_ptr() and torch.equal(a.float(), b.float())
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_steps_without_gradients_do_not_count(tw, randn, bits):
+    """The first step that has a gradient is the first: it moves a weight by lr."""
+    p = torch.nn.Parameter(randn(300))
+    opt = tw.AdamW([p], lr=1e-2, weight_decay=0.0, state_bits=bits)
+    for _ in range(3):
+        opt.step()
+    was, p.grad = p.detach().clone(), randn(300)
+    opt.step()
+    torch.testing.assert_close(p.detach(), was - 1e-2 * p.grad.sign(), rtol=1e-5, atol=1e-6)
+    p.grad, was = None, p.detach().clone()
+    opt.step()
+    assert torch.equal(p, was) and opt.state_dict()["buckets"][0]["step"].tolist() == [1]

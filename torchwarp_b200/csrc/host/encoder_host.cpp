@@ -623,7 +623,8 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const OptTensor& sta
 
 // One AdamW step over `params`, which had `sizes` values each when the flat
 // buffers of their states were made, one after the other on boundaries of 256
-// values; a parameter without a gradient is left out.
+// values; a parameter without a gradient is left out, and with none at all
+// nothing is done.
 void adamw_step(const std::vector<Tensor>& params, const std::vector<int64_t>& sizes,
                 int64_t bits, const Tensor& m, const OptTensor& ms, const Tensor& v,
                 const OptTensor& vs, const Tensor& step, double lr, const OptTensor& lr_tensor,
@@ -634,6 +635,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<int64_t>& s
   table.reserve(4 * params.size());
   const at::ScalarType type = params.empty() ? at::kFloat : params[0].scalar_type();
   int64_t offset = 0;
+  bool any = false;
   for (size_t i = 0; i < params.size(); offset += (sizes[i] + 255) / 256 * 256, ++i) {
     const Tensor& p = params[i];
     Tensor g = p.grad();
@@ -641,6 +643,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<int64_t>& s
       bad_value("a parameter has " + std::to_string(p.numel()) + " values and its gradient " +
                 std::to_string(g.numel()) + ", where its states were made for " +
                 std::to_string(sizes[i]));
+    any = any || g.defined();
     if (!g.defined() || p.numel() == 0) continue;
     if (p.scalar_type() != type || g.scalar_type() != type || g.layout() != at::kStrided)
       bad_type("a gradient must be dense and of its parameter's type " + type_of(type) + ", got " +
@@ -656,6 +659,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<int64_t>& s
     table.insert(table.end(), {(uint64_t)p.data_ptr(), (uint64_t)g.data_ptr(), (uint64_t)p.numel(),
                                (uint64_t)offset});
   }
+  if (!any) return;  // no step
   TORCH_CHECK(m.numel() >= offset && v.numel() >= offset, "adamw_step: the states are too short");
   const float* lr_device = nullptr;
   if (lr_tensor.has_value()) {

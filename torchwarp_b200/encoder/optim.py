@@ -68,7 +68,8 @@ class AdamW(torch.optim.Optimizer):
 
     The states of a group's parameters lie in flat buffers (``flat_state``), made at the first step:
     from then on the group keeps its parameters, and they their sizes.  The step count is the
-    group's and lives on the device; a parameter without a gradient is left out of a step.
+    group's (of the parameters of one type in it) and lives on the device; a parameter without a
+    gradient is left out of a step, and a step in which none has one is not counted.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *,
