@@ -384,3 +384,37 @@ def test_adamw_steps_without_gradients_do_not_count(tw, randn, bits):
     p.grad, was = None, p.detach().clone()
     opt.step()
     assert torch.equal(p, was) and opt.state_dict()["buckets"][0]["step"].tolist() == [1]
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_refused_checkpoints_change_nothing(tw, randn, bits):
+    _, opt = _stepped(tw, randn, [300, 7], state_bits=bits, lr=1e-2, seed=1)
+    _, longer = _stepped(tw, randn, [600, 7], state_bits=bits, lr=1.0, seed=2)
+    _, fewer = _stepped(tw, randn, [300], state_bits=bits, lr=1.0, seed=2)
+    _, other = _stepped(tw, randn, [300, 7], state_bits=40 - bits, lr=1.0, seed=2)
+    short = _stepped(tw, randn, [300, 7], state_bits=bits, lr=1.0, seed=2)[1].state_dict()
+    del short["buckets"][0]["step"]
+    was = copy.deepcopy(opt.state_dict())
+    for bad in (longer.state_dict(), fewer.state_dict(), other.state_dict(), short):
+        with pytest.raises(ValueError):
+            opt.load_state_dict(bad)
+        now = opt.state_dict()
+        assert now["param_groups"] == was["param_groups"] and now["seed"] == 1
+        for a, b in zip(now["buckets"], was["buckets"]):
+            assert all(torch.equal(a[k].float(), b[k].float()) for k in b)
+
+
+def test_adamw_state_dict_is_one_moment(tw, randn):
+    """The step count follows the states of the same dictionary; a copy keeps both."""
+    ps, opt = _stepped(tw, randn, [300])
+    live, kept = opt.state_dict(), copy.deepcopy(opt.state_dict())
+    weights = [p.detach().clone() for p in ps]
+    opt.step()
+    after = [p.detach().clone() for p in ps]
+    assert live["buckets"][0]["step"].item() == 2 and kept["buckets"][0]["step"].item() == 1
+    assert torch.equal(live["buckets"][0]["exp_avg"], opt.flat_state()["exp_avg"])
+    for p, w in zip(ps, weights):
+        p.detach().copy_(w)
+    opt.load_state_dict(kept)
+    opt.step()
+    assert all(torch.equal(p, a) for p, a in zip(ps, after))

@@ -132,11 +132,12 @@ class AdamW(torch.optim.Optimizer):
         return dict(buckets[index].state)
 
     def state_dict(self):
-        """Hyperparameters by group, and the flat states of every bucket."""
+        """Hyperparameters by group, and the flat states of every bucket: the live tensors, their
+        step count among them, as ``torch.optim`` gives them."""
         out = super().state_dict()
         out["state_bits"] = self._bits
         out["seed"] = self._seed
-        out["buckets"] = [{"step": b.step[:1].clone(), **b.state}
+        out["buckets"] = [{"step": b.step[:1], **b.state}
                           for i in range(len(self.param_groups)) for b in self._group_buckets(i)]
         return out
 
@@ -144,12 +145,14 @@ class AdamW(torch.optim.Optimizer):
         if state_dict.get("state_bits") != self._bits:
             raise ValueError("the saved states have {} bits, this optimizer's {}".format(
                 state_dict.get("state_bits"), self._bits))
-        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        # all is checked before anything changes (the groups by the base class, first thing)
         mine = [b for i in range(len(self.param_groups)) for b in self._group_buckets(i)]
         saved = state_dict["buckets"]
-        if len(mine) != len(saved) or any(v.shape != s[k].shape for b, s in zip(mine, saved)
-                                          for k, v in b.state.items()):
+        if len(mine) != len(saved) or any(k not in s or v.shape != s[k].shape
+                                          for b, s in zip(mine, saved)
+                                          for k, v in {**b.state, "step": b.step[:1]}.items()):
             raise ValueError("the saved states belong to other parameters")
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         self._seed = int(state_dict["seed"])
         for b, s in zip(mine, saved):
             b.step[:1].copy_(s["step"])
