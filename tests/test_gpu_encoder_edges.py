@@ -418,3 +418,36 @@ def test_adamw_state_dict_is_one_moment(tw, randn):
     opt.load_state_dict(kept)
     opt.step()
     assert all(torch.equal(p, a) for p, a in zip(ps, after))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_adamw_8_bit_bad_gradients_stay_in_their_place(tw, randn, dtype):
+    """An infinite or NaN gradient spoils its own weight, not the 255 whose scale it shares: they
+    take the bits that they take when it is zero."""
+    bad = {3: float("inf"), 40: float("-inf"), 41: float("nan"), 700: float("inf"), 899: float("nan")}
+    start = randn(900, dtype=dtype)
+    grads = [randn(900, dtype=dtype) * 1e-2 for _ in range(3)]
+    for g in grads:
+        g[list(bad)] = 0
+
+    def run(first):
+        p = torch.nn.Parameter(start.clone())
+        opt = tw.AdamW([p], lr=1e-2, state_bits=8, seed=9)
+        for g in [first] + grads[1:]:
+            p.grad = g
+            opt.step()
+        return p.detach(), opt.flat_state()
+
+    wrong = grads[0].clone()
+    for k, v in bad.items():
+        wrong[k] = v
+    (p, s), (q, t) = run(wrong), run(grads[0])
+    fine = torch.ones(900, dtype=torch.bool, device=DEV)
+    fine[list(bad)] = False
+    assert torch.isnan(p[~fine]).all() and torch.equal(p[fine], q[fine])
+    for k in s:
+        if k.endswith("scale"):
+            assert torch.equal(s[k], t[k])
+        else:
+            a, b = s[k].float()[:900], t[k].float()[:900]
+            assert torch.isnan(a[~fine]).all() and torch.equal(a[fine], b[fine])

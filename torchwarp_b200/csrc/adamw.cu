@@ -11,7 +11,8 @@
 // far less than half an e4m3 spacing, so rounding to nearest would never
 // move it.  The random bits are a hash of the value's place, the step and
 // the seed, so a step is reproducible.  The weight's update uses m and v in
-// float32, before they are rounded.
+// float32, before they are rounded.  An infinity or NaN becomes the code of
+// NaN and has no part in its block's scale.
 //
 // The step count lives on the device, so a step can be captured in a CUDA
 // graph: every block reads it, the last block to have read it stores the new
@@ -63,6 +64,13 @@ __device__ __forceinline__ uint32_t lowbias32(uint32_t h) {  // C. Wellons, hash
   return h ^ (h >> 16);
 }
 
+// The maximum that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // The e4m3 value next to y >= 0 (in units of the scale): below, or above with
 // the probability of the part of a spacing that is cut off, r in [0, 2^20)
 // being the random number.  A float has 20 bits below e4m3's three, so adding
@@ -90,7 +98,7 @@ __device__ __forceinline__ float sqrt_fast(float x) {
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 
@@ -113,7 +121,7 @@ __device__ __forceinline__ void decode8(uint2 c, float scale, float* v) {
     v[2 * i + 1] = f.y * scale;
   }
 }
-__device__ __forceinline__ uint2 encode8(const float* v) {
+__device__ __forceinline__ unsigned long long encode8(const float* v) {
   uint32_t w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -122,7 +130,7 @@ __device__ __forceinline__ uint2 encode8(const float* v) {
            (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2], v[4 * i + 3]),
                                               __NV_SATFINITE, __NV_E4M3)
                << 16;
-  return make_uint2(w[0], w[1]);
+  return (unsigned long long)w[1] << 32 | w[0];
 }
 
 // A warp takes a unit of 256 values a turn, 8 neighbours a lane.  Bound by HBM
@@ -210,8 +218,8 @@ __global__ void __launch_bounds__(AD_THREADS)
       r[i] = sqrt_fast(v);
       pv[i] = pv[i] * keep - alpha * __fdividef(m[i], fmaf(r[i], root2, eps));
       if (!BITS8) r[i] = v;
-      mmax = fmaxf(mmax, fabsf(m[i]));
-      rmax = fmaxf(rmax, r[i]);
+      mmax = max_nan(mmax, fabsf(m[i]));
+      rmax = max_nan(rmax, r[i]);
     }
     if (vec) {
       store_n<true, 8>(p, pv);
@@ -224,8 +232,31 @@ __global__ void __launch_bounds__(AD_THREADS)
       store_n<true, 8>(s.m32 + sl, m);
       store_n<true, 8>(s.v32 + sl, r);
     } else {
+      unsigned long long spoiled_m = 0, spoiled_r = 0;  // codes of NaN
+      mmax = warp_max(mmax);
+      rmax = warp_max(rmax);
+      if (!(mmax < INFINITY && rmax < INFINITY)) {
+        // an infinity or NaN stays in its place, as the code of NaN: the scale
+        // is that of the finite values
+        mmax = rmax = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (!(fabsf(m[i]) < INFINITY)) {
+            m[i] = 0.f;
+            spoiled_m |= 0x7Full << (8 * i);
+          }
+          if (!(r[i] < INFINITY)) {
+            r[i] = 0.f;
+            spoiled_r |= 0x7Full << (8 * i);
+          }
+          mmax = fmaxf(mmax, fabsf(m[i]));
+          rmax = fmaxf(rmax, r[i]);
+        }
+        mmax = warp_max(mmax);
+        rmax = warp_max(rmax);
+      }
       // a block below 1e-37, whose scale has no reciprocal, is zero
-      float nms = warp_max(mmax) / 448.f, nrs = warp_max(rmax) / 448.f;
+      float nms = mmax / 448.f, nrs = rmax / 448.f;
       if (nms < 1e-37f) nms = 0.f;
       if (nrs < 1e-37f) nrs = 0.f;
       const float ims = nms > 0.f ? 1.f / nms : 0.f, irs = nrs > 0.f ? 1.f / nrs : 0.f;
@@ -239,8 +270,9 @@ __global__ void __launch_bounds__(AD_THREADS)
         // a second moment that is not zero stays above zero: it divides m
         if (yr > 0.f) r[i] = fmaxf(r[i], 0.001953125f);
       }
-      *reinterpret_cast<uint2*>(s.m8 + sl) = encode8(m);
-      *reinterpret_cast<uint2*>(s.r8 + sl) = encode8(r);
+      // a spoiled value was made zero: 0x7F over its code, whatever its sign
+      *reinterpret_cast<unsigned long long*>(s.m8 + sl) = encode8(m) | spoiled_m;
+      *reinterpret_cast<unsigned long long*>(s.r8 + sl) = encode8(r) | spoiled_r;
       if (lane == 0) {
         s.ms[so / AD_UNIT] = nms;
         s.rs[so / AD_UNIT] = nrs;
