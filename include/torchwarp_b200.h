@@ -388,7 +388,7 @@ int tw_optimal_path_f64(const double* cost, int B, int K, int T, int U, int max_
  * encoder in front of an alignment loss computes, for float (f32),
  * bfloat16 (bf16) and half (f16) elements; `void*` tensors hold elements of
  * the entry's type.  Rows may be strided: strides are in elements, the last
- * dimension is contiguous.  Outputs are dense.  Sums, statistics and states
+ * dimension is contiguous; rows that are read may overlap.  Outputs are dense.  Sums, statistics and states
  * are float32; a result is rounded once, when it is stored.
  * ------------------------------------------------------------------- */
 

@@ -451,3 +451,26 @@ def test_adamw_8_bit_bad_gradients_stay_in_their_place(tw, randn, dtype):
         else:
             a, b = s[k].float()[:900], t[k].float()[:900]
             assert torch.isnan(a[~fine]).all() and torch.equal(a[fine], b[fine])
+
+
+# ------------------------------------------------------ windows of a signal
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size,hop", [(64, 16), (64, 1), (33, 8), (400, 160), (9000, 512)])
+def test_overlapping_rows(tw, randn, size, hop, dtype):
+    """Windows as a view of their signal give what a copy of them gives."""
+    TF = tw.functional
+    rows = randn(2, 30 * hop + size, dtype=dtype).unfold(-1, size, hop)
+    w, b = randn(size, dtype=dtype), randn(size, dtype=dtype)
+    lw = (randn(24, size) / size ** 0.5).to(dtype)
+    for f in (lambda x: TF.layer_norm(x, w, b), lambda x: TF.linear(x, lw, activation="silu")):
+        view, dense = (v.detach().requires_grad_(True) for v in (rows, rows.contiguous()))
+        assert view.stride(1) == hop
+        y, want = f(view), f(dense)
+        dy = randn(*y.shape, dtype=dtype)
+        dx, = torch.autograd.grad(y, view, dy)
+        wx, = torch.autograd.grad(want, dense, dy)
+        # alignment may choose another form of a kernel: 16 roundings of float32, one to the type
+        unit = 2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -20
+        for got, ref in ((y.detach(), want.detach()), (dx, wx)):
+            assert float((got.float() - ref.float()).norm()) <= unit * float(ref.float().norm())

@@ -478,11 +478,9 @@ int bwd_blocks(size_t rows, const RowPlan& p) {
   return (int)(steps < most ? steps : most);
 }
 
-int check(const char* who, size_t rows, int D, size_t xs) {
+int check(const char* who, size_t rows, int D) {
   if (D <= 0) return set_error(kInvalid, "%s: invalid D=%d (need D > 0)", who, D);
   if (rows > (size_t)1 << 40) return set_error(kInvalid, "%s: too many rows", who);
-  if (rows > 1 && xs < (size_t)D && xs != 0)
-    return set_error(kInvalid, "%s: row stride %zu is below D=%d", who, xs, D);
   return kOk;
 }
 
@@ -536,7 +534,7 @@ template <typename T>
 int fwd(const void* x, size_t xs, const void* w, const void* b, int pf32, size_t rows, int D,
         double eps, void* y, float* mean, float* rstd, void* stream) {
   set_error(kOk, "%s", "");
-  if (int e = check("tw_layer_norm_forward", rows, D, xs)) return e;
+  if (int e = check("tw_layer_norm_forward", rows, D)) return e;
   if (!(eps >= 0)) return set_error(kInvalid, "tw_layer_norm_forward: eps must be >= 0");
   if (rows == 0) return kOk;
   if (!x || !y || (mean == nullptr) != (rstd == nullptr))
@@ -589,8 +587,7 @@ int bwd(const void* dy, size_t dys, const void* x, size_t xs, const void* w, int
         const float* mean, const float* rstd, size_t rows, int D, void* dx, void* dw, void* db,
         void* ws, size_t ws_bytes, void* stream) {
   set_error(kOk, "%s", "");
-  if (int e = check("tw_layer_norm_backward", rows, D, xs)) return e;
-  if (int e = check("tw_layer_norm_backward", rows, D, dys)) return e;
+  if (int e = check("tw_layer_norm_backward", rows, D)) return e;
   if (rows && (!dy || !x || !mean || !rstd))
     return set_error(kInvalid, "tw_layer_norm_backward: null pointer argument");
   if (ws_bytes < tw_layer_norm_workspace_bytes(rows, D) || (ws_bytes && !ws))

@@ -46,7 +46,7 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5):
     """Layer norm over the last dimension: ``(x - mean) / sqrt(var + eps) * weight + bias``.
 
     Args:
-        x: [..., D] float32, bfloat16 or float16; rows may be strided.
+        x: [..., D] float32, bfloat16 or float16; rows may be strided and may overlap.
         weight, bias: [D] of x's type or float32 (both of one type), or None.
         eps: Added to the variance (>= 0).
 
