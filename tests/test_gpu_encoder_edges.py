@@ -474,3 +474,29 @@ def test_overlapping_rows(tw, randn, size, hop, dtype):
         unit = 2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -20
         for got, ref in ((y.detach(), want.detach()), (dx, wx)):
             assert float((got.float() - ref.float()).norm()) <= unit * float(ref.float().norm())
+
+
+# ---------------------------------------------------------------- autocast
+
+@pytest.mark.parametrize("compiled", [False, True])
+def test_autocast_casts_what_torch_casts(tw, randn, compiled):
+    torch._dynamo.reset()
+    f = tw.functional.linear
+    if compiled:
+        f = torch.compile(f, backend="aot_eager")
+    x, w, b = randn(20, 32), randn(8, 32), randn(8)
+    with torch.autocast("cuda", torch.bfloat16):
+        y = f(x, w.half(), b)
+        assert torch.equal(y, tw.functional.linear(x.bfloat16(), w.half().bfloat16(), b.bfloat16()))
+        for bad in ((x.double(), w), (x, w.double()), (x.long(), w), (x, w, b.double())):
+            torch._dynamo.reset()
+            with pytest.raises(Exception, match="must be"):
+                f(*bad)
+    leaf = w.clone().requires_grad_(True)
+    with torch.autocast("cuda", torch.bfloat16):  # a weight used twice
+        loss = (f(x, leaf, b).float() + f(2 * x, leaf, b).float()).sum()
+    dw, = torch.autograd.grad(loss, leaf)
+    want = 3 * x.bfloat16().float().sum(0).expand(8, 32)
+    assert dw.dtype == torch.float32
+    # each of the two gradients, and their sum, is rounded to bfloat16
+    torch.testing.assert_close(dw, want, rtol=2.0 ** -6, atol=2.0 ** -6)

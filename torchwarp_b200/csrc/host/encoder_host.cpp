@@ -422,11 +422,11 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
 Tensor linear(Tensor x, Tensor w, const OptTensor& bias, const OptTensor& residual, int64_t act) {
   Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
   if (at::autocast::is_autocast_enabled(at::kCUDA)) {
+    // torch's own rule and cache: float64 and integers keep their type (and are
+    // refused), a weight is cast once a region
     const at::ScalarType t = at::autocast::get_autocast_dtype(at::kCUDA);
-    x = x.to(t);
-    w = w.to(t);
-    if (b.defined()) b = b.to(t);
-    if (r.defined()) r = r.to(t);
+    for (Tensor* v : {&x, &w, &b, &r})
+      if (v->defined()) *v = at::autocast::cached_cast(t, *v, at::kCUDA);
   }
   no_tangents("linear", {&x, &w, &b, &r});
   if (dispatched({&x, &w, &b, &r}))

@@ -68,7 +68,7 @@ def linear(x, weight, bias=None, *, activation=None, residual=None):
         activation: None, "relu", "gelu" (with erf), "silu" or "sigmoid".
         residual: [..., N] (the result's shape) or None, added after the activation.
 
-    All tensors have one type (under autocast they are cast to the autocast type).
+    All tensors have one type (under autocast float32 and 16-bit ones are cast to its type).
 
     Returns:
         [..., N] of that type.  float32 products keep float32 precision.
@@ -80,8 +80,9 @@ def linear(x, weight, bias=None, *, activation=None, residual=None):
     if _compiling():
         if torch.is_autocast_enabled("cuda"):
             dtype = torch.get_autocast_dtype("cuda")
-            x, weight, bias, residual = (None if t is None else t.to(dtype)
-                                         for t in (x, weight, bias, residual))
+            x, weight, bias, residual = (
+                t.to(dtype) if t is not None and t.is_floating_point() and t.dtype != torch.float64
+                else t for t in (x, weight, bias, residual))
         return _ops.linear(x, weight, bias, residual, act,
                            _wants_grad(x, weight, bias, residual))[0]
     return nat.host().linear(x, weight, bias, residual, act)
