@@ -500,3 +500,55 @@ def test_autocast_casts_what_torch_casts(tw, randn, compiled):
     assert dw.dtype == torch.float32
     # each of the two gradients, and their sum, is rounded to bfloat16
     torch.testing.assert_close(dw, want, rtol=2.0 ** -6, atol=2.0 ** -6)
+
+
+# --------------------------------------------------------------- infinities
+
+def _same_but_rounding(got, want, unit):
+    """NaN and infinities in the same places, the rest within `unit` of the largest of its row."""
+    got, want = got.detach().double(), want.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    for sign in (1, -1):
+        assert torch.equal(got == sign * float("inf"), want == sign * float("inf"))
+    fine = torch.isfinite(want)
+    zero = torch.zeros_like(want)
+    err = torch.where(fine, got - want, zero).abs()
+    assert (err <= unit * torch.where(fine, want, zero).abs().amax(-1, keepdim=True)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", [(2, 64, 96), (8, 20, 33), (300, 64, 96), (20, 40, 4096),
+                                   (17, 129, 65), (700, 512, 256)])
+def test_linear_infinities_follow_the_definition(tw, randn, m, n, k, dtype):
+    """inf w is an infinity of w's sign, inf 0 and inf - inf are NaN, whatever the number of rows.
+    Rounding: one to the type (2^-8, 2^-11) and a few of float32 in sums of like terms."""
+    inf = float("inf")
+    x, w = randn(m, k, dtype=dtype), (randn(n, k) / k ** 0.5).to(dtype)
+    dy = randn(m, n, dtype=dtype)
+    x[1, 3], w[5, 3] = inf, 0
+    if m > 8:
+        x[7, 0], x[7, k - 1] = inf, -inf
+        x[9, 20] = float("nan")
+        w[11, 21], dy[13, 2] = -inf, inf
+    w[:, 1], x[0, 0] = w[:, 1].sign() * 0.5, 1  # one bfloat16 plane each
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    unit = {torch.float32: 2.0 ** -18, torch.bfloat16: 2.0 ** -7, torch.float16: 2.0 ** -10}[dtype]
+    y = tw.functional.linear(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    xd, wd, dyd = (v.detach().double().cpu() for v in (x, w, dy))
+
+    def product(a, b):
+        """a b^T by the definition: sums that hold infinities are the sum of those."""
+        out = torch.where(torch.isfinite(a), a, 0.0) @ torch.where(torch.isfinite(b), b, 0.0).t()
+        for i in range(len(a)):
+            if not torch.isfinite(a[i]).all():
+                out[i] = (a[i] * b).sum(1)
+        for j in range(len(b)):
+            if not torch.isfinite(b[j]).all():
+                out[:, j] = (a * b[j]).sum(1)
+        return out.to(DEV)
+
+    _same_but_rounding(y, product(xd, wd), unit)
+    _same_but_rounding(dx, product(dyd, wd.t()), unit)
+    _same_but_rounding(dw, product(dyd.t(), xd.t()), unit)

@@ -161,7 +161,7 @@ template <> struct Packed<float> {
   static constexpr int PL = 3;
 };
 
-// x = p0 + p1 + p2 exactly (8 + 8 + 8 bits), each the bfloat16 nearest to what
+// x = p0 + p1 + p2 exactly (8 + 8 + 8 bits; from 2^-110 on), each the bfloat16 nearest to what
 // is left: x becomes p0.  An infinity or NaN stays in p0.
 __device__ __forceinline__ void split3(float& x, float& p1, float& p2) {
   float h = __bfloat162float(__float2bfloat16_rn(x));

@@ -10,10 +10,13 @@
 // products where one CTA alone would load 48 KB.
 //
 // float32 operands come as three bfloat16 planes whose sum is exact (8 + 8 +
-// 8 mantissa bits).  The six products of weight 2^-16 and above are taken:
+// 8 mantissa bits) down to 2^-110, below which the last bits fall under
+// bfloat16's smallest value, 2^-133.  The six products of weight 2^-16 and above are taken:
 // p0 q0 in one accumulator, the five small ones in another, so that the
-// rounding of the large sum does not reach them.  The tensor core truncates
-// its accumulator; every SEG_CHUNKS chunks the two are added to float32
+// rounding of the large sum does not reach them.  An infinity or NaN is in p0
+// or q0 alone; in the small products it meets planes that are 0 or of the other
+// sign, so where the large sum is not finite it counts alone.  The tensor core
+// truncates its accumulator; every SEG_CHUNKS chunks the two are added to float32
 // registers, rounding to nearest, which keeps that bias to a few steps.
 //
 // Warps 0 .. EW - 1: epilogue (TMEM lane quadrant warp % 4, a share of the
@@ -606,8 +609,28 @@ __global__ void __launch_bounds__(Geom<T, CG, TN>::THREADS, 1)
             const uint32_t col = lanes + (uint32_t)(a * G::ACC + share * G::COLS + 32 * c);
             tmem_ld32(col, big);
             tmem_ld32(col + TN, small);
+            // in pairs; the values' sum tells, for one addition a pair, whether
+            // any of them is not finite
+            Vec<2> all[2] = {splat<2>(0.f), splat<2>(0.f)};
 #pragma unroll
-            for (int i = 0; i < 32; ++i) acc[c][i] += big[i] + small[i];
+            for (int i = 0; i < 32; i += 2) {
+              const Vec<2> t = add_v(Vec<2>{{big[i], big[i + 1]}}, Vec<2>{{small[i], small[i + 1]}});
+              small[i] = t.v[0];
+              small[i + 1] = t.v[1];
+              all[i / 2 & 1] = add_v(all[i / 2 & 1], t);
+            }
+            all[0] = add_v(all[0], all[1]);
+            if (!(fabsf(all[0].v[0] + all[0].v[1]) < INFINITY))
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!(fabsf(big[i]) < INFINITY)) small[i] = big[i];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const Vec<2> s = add_v(Vec<2>{{acc[c][i], acc[c][i + 1]}},
+                                     Vec<2>{{small[i], small[i + 1]}});
+              acc[c][i] = s.v[0];
+              acc[c][i + 1] = s.v[1];
+            }
           }
           tc_fence_before();
           __syncwarp();
