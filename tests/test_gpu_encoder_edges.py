@@ -552,3 +552,82 @@ def test_linear_infinities_follow_the_definition(tw, randn, m, n, k, dtype):
     _same_but_rounding(y, product(xd, wd), unit)
     _same_but_rounding(dx, product(dyd, wd.t()), unit)
     _same_but_rounding(dw, product(dyd.t(), xd.t()), unit)
+
+
+def _scan_by_definition(x, gate, h0, lengths, dy, dstate):
+    """f h + (1 - f) x and its adjoints in 64 bits; past its length a sequence keeps its state, has
+    outputs and gradients 0, and what it holds there is not read."""
+    t = x.shape[1]
+    live = (torch.arange(t, device=DEV) < lengths.unsqueeze(1)).unsqueeze(2)
+    x, f, dy = (torch.where(live, v.double(), 0.0) for v in (x, gate, dy))
+    f = torch.sigmoid(f)
+    omf = torch.sigmoid(-torch.where(live, gate.double(), 0.0))
+    h, hs = h0.double(), []
+    for k in range(t):
+        hs.append(h)
+        h = torch.where(live[:, k], f[:, k] * h + omf[:, k] * x[:, k], h)
+    y = torch.where(live, torch.stack(hs[1:] + [h], 1), 0.0)
+    last, lam = h, dstate.double()
+    dx, dg = torch.zeros_like(x), torch.zeros_like(x)
+    for k in range(t - 1, -1, -1):
+        on = live[:, k]
+        l = lam + dy[:, k]
+        dx[:, k] = torch.where(on, omf[:, k] * l, 0.0)
+        dg[:, k] = torch.where(on, l * (hs[k] - x[:, k]) * f[:, k] * omf[:, k], 0.0)
+        lam = torch.where(on, f[:, k] * l, lam)
+    return y, last, dx, dg, lam
+
+
+# sizes that reach each form of the scan: segments of time, blocks of a cluster (rows off 16 bytes),
+# one block, half lines, whole lines, a warp alone
+SCAN_FORMS = [(2, 700, 16), (1, 5000, 64), (1, 5000, 3), (3, 300, 33), (40, 130, 97), (5, 700, 2048),
+              (40, 700, 96), (5, 300, 2048), (29, 203, 1000), (32, 97, 1024)]
+
+
+def _scan_inputs(randn, b, t, d, dtype, mean=2.0):
+    lengths = torch.tensor([(t, 0, 1, t - 1, t // 3)[k % 5] for k in range(b)], device=DEV)
+    u = randn(b, t, 2 * d)
+    u[..., d:] = u[..., d:] * 1.5 + mean
+    x, gate = u.to(dtype).split(d, -1)
+    return x, gate, randn(b, d), lengths, randn(b, t, d, dtype=dtype), randn(b, d)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("b,t,d", SCAN_FORMS)
+def test_scan_infinities_follow_the_definition(tw, randn, b, t, d, dtype):
+    """An infinite state stays one, at live frames and past a sequence's length."""
+    inf = float("inf")
+    x, gate, h0, lengths, dy, ds = _scan_inputs(randn, b, t, d, dtype)
+    h0[:, 0], h0[0, 1], ds[:, 2 % d] = inf, -inf, inf
+    x[0, t // 2, 1 % d], x[0, 40, 2 % d], x[0, 60, 2 % d] = inf, -inf, inf
+    x[0, 33, d - 1], dy[0, 90, d // 2] = float("nan"), -inf
+    x, gate = x.detach().requires_grad_(True), gate.detach().requires_grad_(True)
+    h0.requires_grad_(True)
+    y, last = tw.functional.gated_scan(x, gate, h0, lengths=lengths)
+    grads = torch.autograd.grad((y, last), (x, gate, h0), (dy, ds))
+    want = _scan_by_definition(*(v.detach() for v in (x, gate, h0)), lengths, dy, ds)
+    assert torch.isinf(want[1]).any() and torch.isinf(want[2]).any()
+    unit = {torch.float32: 2.0 ** -16, torch.bfloat16: 2.0 ** -7, torch.float16: 2.0 ** -10}[dtype]
+    for got, w in zip((y, last) + grads, want):
+        _same_but_rounding(got, w, unit)
+
+
+def test_scan_infinite_state_through_closed_gates(tw, randn):
+    """Products of small gates that underflow keep an infinity; a gate of -inf does not."""
+    for d in (8, 5):
+        x, h0 = randn(3, 200, d), torch.full((3, d), float("inf"), device=DEV)
+        gate = torch.full((3, 200, d), -20.0, device=DEV)
+        gate[1, 50], gate[2, 199] = float("-inf"), float("-inf")
+        y, last = tw.functional.gated_scan(x, gate, h0)
+        assert torch.isinf(y[0]).all() and torch.isinf(last[0]).all()
+        assert torch.isinf(y[1, :50]).all() and torch.isnan(y[1, 50:]).all()
+        assert torch.isinf(y[2, :199]).all() and torch.isnan(last[2]).all()
+
+
+def test_scan_step_infinities(tw, randn):
+    state, x, gate = randn(4, 8), randn(4, 8), randn(4, 8)
+    state[0], state[1], x[2], x[1, 0] = float("inf"), float("-inf"), float("inf"), float("inf")
+    want = torch.sigmoid(gate) * state + torch.sigmoid(-gate) * x
+    y = tw.functional.gated_scan_step(x, gate, state)
+    _same_but_rounding(y, want, 2.0 ** -20)
+    _same_but_rounding(state, want, 2.0 ** -20)

@@ -105,6 +105,40 @@ __device__ __forceinline__ Vec<V> passed(Vec<V> n, Vec<V> l, Vec<V> neg_l) {
   return fma_v(n, neg_l, pick(n, splat<V>(0.f), l));
 }
 
+// The steps above hold for finite values; an infinity meets itself in h - x or
+// in l - (1 - f) l.  Once there, what is not finite stays so to the end of a run,
+// so a run looks once and then goes again by the definition (`define`,
+// `define_back`), reading global memory, frame by frame.
+template <int V>
+__device__ __forceinline__ bool finite(Vec<V> v) {
+  bool r = true;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r = r && fabsf(v.v[i]) < INFINITY;
+  return r;
+}
+template <int V>
+__device__ __forceinline__ void both_gates(Vec<V> n, Vec<V>& f, Vec<V>& omf) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float a = fabsf(n.v[i]);
+    f.v[i] = __float_as_int(n.v[i]) < 0 ? 1.f - a : a;
+    omf.v[i] = __float_as_int(n.v[i]) < 0 ? a : 1.f - a;
+  }
+}
+// f h + (1 - f) x
+template <int V>
+__device__ __forceinline__ Vec<V> advance_any(Vec<V> n, Vec<V> h, Vec<V> x) {
+  Vec<V> f, omf;
+  both_gates(n, f, omf);
+  return fma_v(f, h, mul_v(omf, x));
+}
+// A product of gates that are not zero is not zero: it carries an infinite
+// state.  1.4e-45 times a finite one is below its rounding.
+__device__ __forceinline__ float times_gate(float a, float by) {
+  const float r = a * by;
+  return r == 0.f && a != 0.f && by != 0.f ? 1.4e-45f : r;
+}
+
 // VC neighbouring channels of a frame, as they lie in memory.
 template <typename T, int VC> struct Frame {
   T t;
@@ -157,6 +191,81 @@ __device__ __forceinline__ void load_frames(Frame<T, VC> (&f)[FR], const char* p
   }
 }
 
+// A channel's run in global memory, for what is not finite: frames `step` bytes
+// apart from p on.
+template <typename T, int VC> struct Far {
+  const char* p;
+  size_t step;
+  __device__ __forceinline__ Vec<VC> operator[](int k) const {
+    return reinterpret_cast<const Frame<T, VC>*>(p + (size_t)k * step)->get();
+  }
+};
+// The states of n frames by the definition; put(k, h) takes each.
+template <typename T, int VC, typename Put>
+__device__ __forceinline__ Vec<VC> define(Far<T, VC> x, Far<T, VC> g, int n, Vec<VC> h, Put put) {
+#pragma unroll 1
+  for (int k = 0; k < n; ++k) {
+    h = advance_any(gate_of(g[k]), h, x[k]);
+    put(k, h);
+  }
+  return h;
+}
+// The adjoints of n frames, from the last: l beyond them to l before them;
+// put(k, dx, dg).  The state before each frame is walked to anew from h.
+template <typename T, int VC, typename Put>
+__device__ __forceinline__ Vec<VC> define_back(Far<T, VC> y, Far<T, VC> x, Far<T, VC> g, int n,
+                                               Vec<VC> h, Vec<VC> l, Put put) {
+#pragma unroll 1
+  for (int k = n - 1; k >= 0; --k) {
+    const Vec<VC> before = define(x, g, k, h, [](int, Vec<VC>) {});
+    Vec<VC> f, omf;
+    both_gates(gate_of(g[k]), f, omf);
+    l = add_v(y[k], l);
+    put(k, mul_v(omf, l), mul_v(mul_v(mul_v(l, sub_v(before, x[k])), f), omf));
+    l = mul_v(f, l);
+  }
+  return l;
+}
+// B of a run, anew, for one that is not finite: from state 0 forward, REV: of
+// f (l + v) from 0 backward.
+template <bool REV, typename T, int VC>
+__device__ __forceinline__ Vec<VC> define_sum(Far<T, VC> v, Far<T, VC> g, int n) {
+  Vec<VC> B = splat<VC>(0.f);
+#pragma unroll 1
+  for (int i = 0; i < n; ++i) {
+    const int k = REV ? n - 1 - i : i;
+    const Vec<VC> s = gate_of(g[k]);
+    Vec<VC> f, omf;
+    both_gates(s, f, omf);
+    B = REV ? mul_v(f, add_v(v[k], B)) : advance_any(s, B, v[k]);
+  }
+  return B;
+}
+// A run's A as times_gate would have it; gate(k): a frame's gate as it lies.
+template <int FR, int V, typename Gate>
+__device__ __forceinline__ void keep_product(Vec<V>& A, Gate gate) {
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (A.v[i] == 0.f) {
+      float least = 0.f;
+#pragma unroll
+      for (int k = 0; k < FR; ++k) least = fminf(least, gate(k).v[i]);
+      if (least > -87.f) A.v[i] = 1.4e-45f;  // below, sigmoid itself is 0
+    }
+}
+// The same from gate_of's numbers, where 0 that is not -0 is a closed gate.
+template <int FR, int V>
+__device__ __forceinline__ void keep_product(Vec<V>& A, const Vec<V> (&s)[FR]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (A.v[i] == 0.f) {
+      bool closed = false;
+#pragma unroll
+      for (int k = 0; k < FR; ++k) closed = closed || __float_as_uint(s[k].v[i]) == 0u;
+      if (!closed) A.v[i] = 1.4e-45f;
+    }
+}
+
 __device__ __forceinline__ float peer_read(const float* p, uint32_t rank) {
   uint32_t a;
   float v;
@@ -203,7 +312,7 @@ __device__ __forceinline__ void compose(ScanShared<VC, LPR>& sh, int it, int S, 
           const int w = REV ? RUNS - 1 - i : i;
           const float wa = sh.a[p][w][lane * VC + v];
           tb = fmaf(wa, tb, sh.b[p][w][lane * VC + v]);
-          ta *= wa;
+          ta = times_gate(ta, wa);
         }
         sh.tile_a[p][lane * VC + v] = ta;
         sh.tile_b[p][lane * VC + v] = tb;
@@ -312,13 +421,26 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
       B = advance(s[k], B, x, sub_v(B, x));
       A = decay(s[k], A);
     }
+    const Far<T, VC> fx = {xp + (size_t)t0 * xs, xs}, fg = {gp + (size_t)t0 * gs, gs};
+    const int in = min(n, FR);
+    bool plain = finite(B);
+    if (!plain) B = define_sum<false>(fx, fg, in);
+    keep_product<FR>(A, s);
     compose<VC, LPR, false>(sh, it, S, rank, part, lane, A, B, run, h);
+    plain = plain && finite(h);
     if (carry && ch.live && t0 < TT)
 #pragma unroll
       for (int v = 0; v < VC; ++v)
         carry[(size_t)(t0 / FR) * BD + ch.c + v] = h.v[v];
     char* o = yp + (size_t)t0 * ys;
-    if (n >= FR) {
+    if (!plain) {
+      h = define(fx, fg, in, h, [&](int k, Vec<VC> v) {
+        *reinterpret_cast<Frame<T, VC>*>(o + (size_t)k * ys) = Frame<T, VC>::of(v);
+      });
+#pragma unroll 1
+      for (int k = max(in, 0); ch.live && k < FR && t0 + k < TT; ++k)
+        *reinterpret_cast<Frame<T, VC>*>(o + (size_t)k * ys) = Frame<T, VC>::zero();
+    } else if (n >= FR) {
 #pragma unroll
       for (int k = 0; k < FR; ++k) {
         const Vec<VC> x = xk[k].get();
@@ -409,6 +531,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
       diff[k] = sub_v(h, x);
       h = advance(s[k], h, x, diff[k]);
     }
+    const Vec<VC> first = hr;
     load(t0 - TILE * S);  // under way while the blocks wait for each other
     Vec<VC> A = splat<VC>(1.f), B = splat<VC>(0.f);
 #pragma unroll
@@ -416,10 +539,29 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
       B = decay(s[k], add_v(yk[k].get(), B));
       A = decay(s[k], A);
     }
+    const Far<T, VC> fy = {yp + (size_t)t0 * ys, ys}, fx = {xp + (size_t)t0 * xs, xs},
+                     fg = {gp + (size_t)t0 * gs, gs};
+    const int in = min(n, FR);
+    bool plain = finite(B) && finite(h);
+    if (!finite(B)) B = define_sum<true>(fy, fg, in);
+    keep_product<FR>(A, s);
     compose<VC, LPR, true>(sh, it, S, rank, part, lane, A, B, run, lam);
+    plain = plain && finite(lam);
     const size_t last = (at + (size_t)(t0 + FR - 1) * D) * sizeof(T);
     char* ox = reinterpret_cast<char*>(dx) + last;
     char* og = reinterpret_cast<char*>(dg) + last;
+    if (!plain) {
+      auto at_frame = [&](char* p, int k) {
+        return reinterpret_cast<Frame<T, VC>*>(p - (FR - 1 - k) * os);
+      };
+      lam = define_back(fy, fx, fg, in, first, lam, [&](int k, Vec<VC> vx, Vec<VC> vg) {
+        *at_frame(ox, k) = Frame<T, VC>::of(vx);
+        *at_frame(og, k) = Frame<T, VC>::of(vg);
+      });
+#pragma unroll 1
+      for (int k = max(in, 0); ch.live && k < FR && t0 + k < TT; ++k)
+        *at_frame(ox, k) = *at_frame(og, k) = Frame<T, VC>::zero();
+    } else
 #pragma unroll
     for (int k = FR - 1; k >= 0; --k) {
       const Vec<VC> l = add_v(yk[k].get(), lam);
@@ -542,6 +684,12 @@ template <typename T, int LPR, int NT> struct Mover {
   }
 };
 
+template <typename T>
+__device__ __forceinline__ Far<T, 2> far_run(const T* p, size_t b, size_t t, const Channel& ch,
+                                             int t0) {
+  return {reinterpret_cast<const char*>(p + ch.b * b + (size_t)t0 * t + ch.d), t * sizeof(T)};
+}
+
 // What segments of time do to the state: (A, B) of every segment and channel.
 struct Segments {
   int tiles;         // of a segment
@@ -598,6 +746,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
 #pragma unroll
   for (int i = 0; i < G::STAGES; ++i) fetch(i);
   float2 total[2] = {make_float2(1.f, 0.f), make_float2(1.f, 0.f)};  // of run 0's threads
+  bool closed[2] = {false, false};
   for (int it = 0; it < steps; ++it) {
     uint8_t* gsl = ring + (it % G::STAGES) * 2 * G::SLOT;
     const int n = ch.L - (tile_of_step(it) + part * FR), p = it & 1;
@@ -612,6 +761,11 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
       B = REV ? decay(s, add_v(x, B)) : advance(s, B, x, sub_v(B, x));
       A = decay(s, A);
     }
+    if (!finite(B)) {
+      const int t0 = tile_of_step(it) + part * FR;
+      B = define_sum<REV>(far_run<T>(v, vb, vt, ch, t0), far_run<T>(g, gb, gt, ch, t0), min(n, FR));
+    }
+    keep_product<FR>(A, [&](int k) { return k < n ? gf[k].get() : splat<2>(0.f); });
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       sh.a[p][part][lane * 2 + q] = A.v[q];
@@ -627,12 +781,16 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
           const float wa = sh.a[p][w][lane * 2 + q];
           total[q].y = fmaf(wa, total[q].y, sh.b[p][w][lane * 2 + q]);
           total[q].x *= wa;
+          closed[q] = closed[q] || wa == 0.f;
         }
     fetch(it + G::STAGES);  // all have read this tile
   }
   if (ch.live && part == 0)
 #pragma unroll
-    for (int q = 0; q < 2; ++q) seg.sums[(size_t)z * BD + ch.c + q] = total[q];
+    for (int q = 0; q < 2; ++q) {
+      if (total[q].x == 0.f && !closed[q]) total[q].x = 1.4e-45f;  // as times_gate
+      seg.sums[(size_t)z * BD + ch.c + q] = total[q];
+    }
 }
 
 template <typename T, int LPR, int NT>
@@ -690,6 +848,10 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 8 : 4)
 #pragma unroll
       for (int k = 0; k < FR; ++k)
         if (k >= n) s[k] = splat<2>(-0.f);
+    const int in = min(n, FR);
+    bool plain = true;
+    auto far_x = [&] { return far_run<T>(x, xb, xt, ch, t0); };
+    auto far_g = [&] { return far_run<T>(g, gb, gt, ch, t0); };
     if constexpr (ALONE) {
       h = run;
     } else {
@@ -699,7 +861,11 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 8 : 4)
         B = advance(s[k], B, xv, sub_v(B, xv));
         A = decay(s[k], A);
       }
+      plain = finite(B);
+      if (!plain) B = define_sum<false>(far_x(), far_g(), in);
+      keep_product<FR>(A, s);
       compose<2, LPR, false>(sh, it, 1, 0, part, lane, A, B, run, h);
+      plain = plain && finite(h);
     }
     if (carry && ch.live && t0 < TT)
       *reinterpret_cast<float2*>(carry + (size_t)(t0 / FR) * BD + ch.c) =
@@ -712,9 +878,18 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 8 : 4)
         xf[k] = all || k < n ? F::of(h) : F::zero();
       }
     };
-    if (n >= FR) finish(true);
+    auto finish_any = [&](Vec<2> from) {
+      h = define(far_x(), far_g(), in, from, [&](int k, Vec<2> v) { xf[k] = F::of(v); });
+#pragma unroll 1
+      for (int k = max(in, 0); k < FR; ++k) xf[k] = F::zero();
+    };
+    if (!plain) finish_any(h);
+    else if (n >= FR) finish(true);
     else finish(false);
-    if (ALONE) run = h;
+    if (ALONE) {
+      if (!finite(h)) finish_any(run);
+      run = h;
+    }
     if (part == G::RUNS - 1)
 #pragma unroll
       for (int v = 0; v < 2; ++v) sh.start[(it + 1) & 1][lane * 2 + v] = h.v[v];
@@ -807,7 +982,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
       diff[k] = sub_v(h, xv);
       h = advance(s[k], h, xv, diff[k]);
     }
+    bool plain = finite(B) && finite(h);
+    const int in = min(n, FR);
+    auto far_y = [&] { return far_run<T>(dy, yb, yt, ch, t0); };
+    auto far_g = [&] { return far_run<T>(g, gb, gt, ch, t0); };
+    if (!finite(B)) B = define_sum<true>(far_y(), far_g(), in);
+    keep_product<FR>(A, s);
     compose<2, LPR, true>(sh, it, 1, 0, part, lane, A, B, run, lam);
+    plain = plain && finite(lam);
     // With a = |n| and b = a l: the smaller of f l and (1 - f) l is b, the other
     // l - b; f (1 - f) l = b - a b.
     auto finish = [&](bool all) {
@@ -825,8 +1007,19 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
         gf[k] = all || k < n ? vg : F::zero();
       }
     };
-    if (n >= FR) finish(true);
-    else finish(false);
+    if (!plain) {
+      lam = define_back(far_y(), far_run<T>(x, xb, xt, ch, t0), far_g(), in, Vec<2>{{h2.x, h2.y}}, lam,
+                        [&](int k, Vec<2> vx, Vec<2> vg) {
+                          xf[k] = F::of(vx);
+                          gf[k] = F::of(vg);
+                        });
+#pragma unroll 1
+      for (int k = max(in, 0); k < FR; ++k) xf[k] = gf[k] = F::zero();
+    } else if (n >= FR) {
+      finish(true);
+    } else {
+      finish(false);
+    }
     if (part == 0)
 #pragma unroll
       for (int v = 0; v < 2; ++v) sh.start[(it + 1) & 1][lane * 2 + v] = lam.v[v];
@@ -852,7 +1045,8 @@ __global__ void __launch_bounds__(SCAN_THREADS)
   const size_t b = id / D, d = id - b * D;
   const Vec<1> n = gate_of(Vec<1>{{to_f(g[b * gs + d])}});
   const Vec<1> was = {{state[id]}}, in = {{to_f(x[b * xs + d])}};
-  const float h = advance(n, was, in, sub_v(was, in)).v[0];
+  float h = advance(n, was, in, sub_v(was, in)).v[0];
+  if (!(fabsf(h) < INFINITY)) h = advance_any(n, was, in).v[0];
   state[id] = h;
   y[id] = from_f<T>(h);
 }
