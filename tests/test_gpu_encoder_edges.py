@@ -631,3 +631,28 @@ def test_scan_step_infinities(tw, randn):
     y = tw.functional.gated_scan_step(x, gate, state)
     _same_but_rounding(y, want, 2.0 ** -20)
     _same_but_rounding(state, want, 2.0 ** -20)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("b,t,d", SCAN_FORMS)
+def test_scan_forms(tw, randn, b, t, d, ragged, dtype):
+    """Each form over several tiles and a partial last one, whole and with lengths of 0, 1, T - 1
+    and inside a tile.  Tolerances: one rounding to the type and 64 of float32, in the 2-norm, and
+    float16's smallest step."""
+    x, gate, h0, lengths, dy, ds = _scan_inputs(randn, b, t, d, dtype)
+    if not ragged:
+        lengths.fill_(t)
+    x, gate = x.detach().requires_grad_(True), gate.detach().requires_grad_(True)
+    h0.requires_grad_(True)
+    y, last = tw.functional.gated_scan(x, gate, h0, lengths=lengths if ragged else None)
+    grads = torch.autograd.grad((y, last), (x, gate, h0), (dy, ds))
+    want = _scan_by_definition(*(v.detach() for v in (x, gate, h0)), lengths, dy, ds)
+    for got, w in zip((y, last) + grads, want):
+        unit = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[got.dtype]
+        err = float((got.detach().double() - w).norm())
+        floor = 2.0 ** -24 * w.numel() ** 0.5 if got.dtype == torch.float16 else 0.0
+        assert err <= (unit + 64 * 2.0 ** -24) * float(w.norm()) + floor
+    with torch.no_grad():
+        y2, last2 = tw.functional.gated_scan(x, gate, h0, lengths=lengths if ragged else None)
+    assert torch.equal(y, y2) and torch.equal(last, last2)
