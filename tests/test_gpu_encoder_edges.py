@@ -656,3 +656,32 @@ def test_scan_forms(tw, randn, b, t, d, ragged, dtype):
     with torch.no_grad():
         y2, last2 = tw.functional.gated_scan(x, gate, h0, lengths=lengths if ragged else None)
     assert torch.equal(y, y2) and torch.equal(last, last2)
+
+
+@pytest.mark.parametrize("m", [1, 20])
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+def test_float32_activation_tails(tw, m, act):
+    """Far from 0 the small side of silu and sigmoid keeps float32's relative precision, into its
+    subnormals: an exponential of 2 ulp, a sum, a division and a product of half an ulp each, 8
+    spacings of 2^-23 allowed; below 2^-126 the spacing is 2^-149.  z is the bias, and its gradient,
+    a sum before any product, is dz."""
+    z = torch.linspace(-104, 20, 300, device=DEV)
+    leaf = z.clone().requires_grad_(True)
+    zero = torch.zeros(m, 4, device=DEV)
+    y = tw.functional.linear(zero, torch.zeros(300, 4, device=DEV), leaf, activation=act)
+    dy = torch.zeros_like(y)
+    dy[0] = 1
+    dz, = torch.autograd.grad(y, leaf, dy)
+    assert (y == y[0]).all()
+    y = y[0]
+    f, omf = torch.sigmoid(z.double()), torch.sigmoid(-z.double())
+    if act == "silu":
+        want, slope = z.double() * f, f * (1 + z.double() * omf)
+        near = (1 + z.double() * omf).abs() > 0.1  # where the slope's factor does not cancel
+    else:
+        want, slope, near = f, f * omf, torch.ones_like(f, dtype=torch.bool)
+    for got, w, where in ((y.detach(), want, torch.ones_like(near)), (dz, slope, near)):
+        bound = 8 * 2.0 ** -23 * w.abs() + 104 * 2.0 ** -149
+        # the slope's factor and the large side of f add their own roundings
+        bound = bound if w is want else 8 * bound
+        assert ((got.double() - w).abs() <= bound)[where].all()

@@ -226,14 +226,50 @@ __device__ __forceinline__ Vec<V> negated(Vec<V> s) {
   return s;
 }
 
+// e^-|z| for float32 results: 2^(-|z| log2(e) / 2) squared, so that it reaches
+// the subnormals (ex2 flushes them), times 1 + what the product's rounding left
+// over; within 2^-21.  It is 0 from 110 on.
+template <int V>
+__device__ __forceinline__ Vec<V> exp_minus_abs(Vec<V> z) {
+  constexpr double C = 0.72134752044448170368;  // log2(e) / 2
+  constexpr float HI = (float)C, LO = (float)(C - (double)HI);
+  Vec<V> a, e;
+#pragma unroll
+  for (int i = 0; i < V; ++i)  // -|z|, not below -110; a NaN stays one
+    asm("max.NaN.f32 %0, %1, 0fC2DC0000;" : "=f"(a.v[i]) : "f"(fminf(z.v[i], -z.v[i])));
+  const Vec<V> t = mul_v(a, splat<V>(HI));
+  // minus (a log2(e) / 2 - t)
+  const Vec<V> rest = fma_v(a, splat<V>(-LO), fma_v(a, splat<V>(-HI), t));
+#pragma unroll
+  for (int i = 0; i < V; ++i) e.v[i] = ex2(t.v[i]);
+  e = mul_v(e, e);
+  return fma_v(e, mul_v(rest, splat<V>(-1.3862943611198906f)), e);
+}
+
 // f = sigmoid(z) and 1 - f: the smaller of the two from exp(-|z|), which
-// neither overflows nor cancels, to a few ulp of itself; the larger is one
-// minus it, correctly rounded.
-__device__ __forceinline__ void sigmoid_pair(float z, float& f, float& omf) {
-  const float e = ex2(-1.4426950408889634f * fabsf(z));
-  const float lo = e * rcp(1.f + e), hi = 1.f - lo;
-  f = z >= 0.f ? hi : lo;
-  omf = z >= 0.f ? lo : hi;
+// neither overflows nor cancels, to a few ulp of itself, down to the smallest
+// float; the larger is one minus it, correctly rounded.  FAST: for results of
+// 16 bits; the product z log2(e) is rounded, so the smaller one's relative
+// error grows as |z| 2^-24, and below 2^-126 it is 0.
+template <bool FAST, int V>
+__device__ __forceinline__ void sigmoid_pair(Vec<V> z, Vec<V>& f, Vec<V>& omf) {
+  Vec<V> e, r;
+  if constexpr (FAST) {
+    e = mul_v(z, splat<V>(1.4426950408889634f));
+#pragma unroll
+    for (int i = 0; i < V; ++i) e.v[i] = ex2(-fabsf(e.v[i]));
+  } else {
+    e = exp_minus_abs(z);
+  }
+  r = add_v(e, splat<V>(1.f));
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = rcp(r.v[i]);
+  const Vec<V> lo = mul_v(e, r), hi = sub_v(splat<V>(1.f), lo);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    f.v[i] = z.v[i] >= 0.f ? hi.v[i] : lo.v[i];
+    omf.v[i] = z.v[i] >= 0.f ? lo.v[i] : hi.v[i];
+  }
 }
 
 // Activations of the linear operator (values of the `act` argument).
@@ -274,13 +310,17 @@ __device__ __forceinline__ Vec<V> act_value(Vec<V> z) {
 #pragma unroll
     for (int i = 0; i < V; ++i) r.v[i] = fmaxf(z.v[i], 0.f);
     return fma_v(negated(az), q, r);
-  } else if constexpr (ACT == kActSilu || ACT == kActSigmoid) {
+  } else if constexpr ((ACT == kActSilu || ACT == kActSigmoid) && FAST) {
     Vec<V> f = mul_v(z, splat<V>(-1.4426950408889634f));
 #pragma unroll
     for (int i = 0; i < V; ++i) f.v[i] = ex2(f.v[i]);
     f = add_v(f, splat<V>(1.f));
 #pragma unroll
     for (int i = 0; i < V; ++i) f.v[i] = rcp(f.v[i]);
+    return ACT == kActSilu ? mul_v(z, f) : f;
+  } else if constexpr (ACT == kActSilu || ACT == kActSigmoid) {
+    Vec<V> f, omf;
+    sigmoid_pair<false>(z, f, omf);
     return ACT == kActSilu ? mul_v(z, f) : f;
   } else {
 #pragma unroll
@@ -310,6 +350,13 @@ __device__ __forceinline__ Vec<V> act_slope(Vec<V> z) {
       az.v[i] = copysignf(az.v[i], z.v[i]);  // at the cut e is 0
     }
     return fma_v(mul_v(az, splat<V>(0.39894228040143268f)), e, add_v(c, splat<V>(0.5f)));
+  } else if constexpr (ACT == kActSilu || ACT == kActSigmoid) {
+    Vec<V> f, omf;
+    sigmoid_pair<FAST>(z, f, omf);
+    if (ACT == kActSigmoid) return mul_v(f, omf);
+#pragma unroll
+    for (int i = 0; i < V; ++i) z.v[i] = fmaxf(fminf(z.v[i], 128.f), -128.f);
+    return mul_v(f, fma_v(z, omf, splat<V>(1.f)));
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -319,11 +366,6 @@ __device__ __forceinline__ Vec<V> act_slope(Vec<V> z) {
         const float cdf = 0.5f * (1.f + erff(v * 0.70710678118654752f));
         const float e = 0.39894228040143268f * ex2(-0.72134752044448170f * v * v);
         v = fmaf(fmaxf(fminf(v, 30.f), -30.f), e, cdf);
-      }
-      if (ACT == kActSilu || ACT == kActSigmoid) {
-        float f, omf;
-        sigmoid_pair(v, f, omf);
-        v = ACT == kActSilu ? f * fmaf(fmaxf(fminf(v, 128.f), -128.f), omf, 1.f) : f * omf;
       }
       if (ACT == kActNone) v = 1.f;
     }
