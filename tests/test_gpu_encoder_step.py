@@ -142,3 +142,20 @@ def test_gated_scan_past_32_bits(tw):
     torch.testing.assert_close(last, lasts, rtol=1e-5, atol=1e-6)
     for a, b in ((y[:, -100:], ys[:, -100:]), (dx[:, -100:], dxs[:, -100:])):
         torch.testing.assert_close(a.float(), b.float(), rtol=2.0 ** -7, atol=1e-6)
+
+
+def test_linear_bias_gradient_of_nearly_2_to_31_rows(tw):
+    """The last of the blocks of rows ends past 2^31: its rows count."""
+    import torchwarp_b200._native as nat
+    rows, n = 2 ** 31 - 1000, 8
+    dy = torch.zeros(rows, n, device=DEV, dtype=torch.bfloat16)
+    dy[-5:] = 3
+    lib = nat.lib()
+    size = lib.tw_linear_workspace_bytes(rows, n, 8, 2, 0, 1, 0)
+    ws = torch.empty(size, device=DEV, dtype=torch.uint8)
+    db = torch.empty(n, device=DEV, dtype=torch.bfloat16)
+    x = torch.empty(8, device=DEV, dtype=torch.bfloat16)  # not read: only db is asked for
+    status = lib.tw_linear_backward_bf16(dy.data_ptr(), n, x.data_ptr(), 8, x.data_ptr(), 8, None,
+                                         rows, n, 8, 0, None, None, db.data_ptr(), ws.data_ptr(),
+                                         size, torch.cuda.current_stream().cuda_stream)
+    assert status == 0 and (db == 15).all()

@@ -204,7 +204,8 @@ __device__ __forceinline__ void pack_block(const PackJob<T>& j, int bx, int by, 
   constexpr int PL = Packed<T>::PL;
   using E = typename Packed<T>::E;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int c0 = bx * PACK_COLS + tx * 8, r1 = min(j.R, (by + 1) * j.rb), C = j.C;
+  const int c0 = bx * PACK_COLS + tx * 8, C = j.C;
+  const int r0 = by * j.rb, r1 = r0 + min(j.R - r0, j.rb);  // (by + 1) rb may pass 2^31
   if (c0 >= j.Cp) return;
   const size_t ld = j.ld, pitch = j.pitch, plane = j.plane;
   const T* __restrict__ src = j.src + c0;
@@ -212,7 +213,7 @@ __device__ __forceinline__ void pack_block(const PackJob<T>& j, int bx, int by, 
   E* __restrict__ dst = j.dst;
   const bool vec = j.vec;
 #pragma unroll 2
-  for (int r = by * j.rb + ty; r < r1; r += PACK_ROWS) {
+  for (int r = r0 + ty; r < r1; r += PACK_ROWS) {
     const T* p = src + (size_t)r * ld;
     const T* zp = ACT == kActNone ? nullptr : z + (size_t)r * C;
     float v[8], zv[8];
@@ -312,7 +313,10 @@ int rows_per_block(int R) {
   const int rb = (R + 255) / 256;
   return rb < 16 ? 16 : (rb + 7) / 8 * 8;
 }
-int row_blocks(int R) { return (R + rows_per_block(R) - 1) / rows_per_block(R); }
+int row_blocks(int R) {
+  const int rb = rows_per_block(R);
+  return (int)(((long long)R + rb - 1) / rb);
+}
 
 template <typename T>
 bool tma_reads(const void* p, size_t ld, int rows, int cols) {
