@@ -660,12 +660,13 @@ def test_scan_forms(tw, randn, b, t, d, ragged, dtype):
 
 @pytest.mark.parametrize("m", [1, 20])
 @pytest.mark.parametrize("act", ["silu", "sigmoid"])
-def test_float32_activation_tails(tw, m, act):
+@pytest.mark.parametrize("least,most", [(-104, 20), (-6, 6), (-8, 5.9)])
+def test_float32_activation_tails(tw, least, most, m, act):
     """Far from 0 the small side of silu and sigmoid keeps float32's relative precision, into its
     subnormals: an exponential of 2 ulp, a sum, a division and a product of half an ulp each, 8
     spacings of 2^-23 allowed; below 2^-126 the spacing is 2^-149.  z is the bias, and its gradient,
     a sum before any product, is dz."""
-    z = torch.linspace(-104, 20, 300, device=DEV)
+    z = torch.linspace(least, most, 300, device=DEV)
     leaf = z.clone().requires_grad_(True)
     zero = torch.zeros(m, 4, device=DEV)
     y = tw.functional.linear(zero, torch.zeros(300, 4, device=DEV), leaf, activation=act)
