@@ -139,8 +139,9 @@ __device__ __forceinline__ unsigned long long encode8(const float* v) {
 // unit whose parameter or gradient is not 16-byte aligned, and a tensor's
 // last, partial unit, go value by value.  67 million float32 weights with
 // 32-bit states: 285 us, 6.6 TB/s, a copy's rate (622 us value by value).
-// 3.2 million bfloat16 weights with 8-bit states: 16 us, of which the bytes are
-// 3; the rounding's arithmetic bounds it.
+// 2.1 million bfloat16 weights with 8-bit states: 15 us, of which the bytes are
+// 3; half of the issue slots are empty, as each short-lived block reads the step,
+// raises the betas to it and meets at a barrier before its first load.
 template <typename T, bool BITS8>
 __global__ void __launch_bounds__(AD_THREADS)
     adamw_kernel(const __grid_constant__ AdamTable tab, AdamState s, AdamScalars a) {

@@ -10,25 +10,28 @@
 // there are 0, its gradients 0, and x and g are not read.
 //
 // One pass over the data.  The channels of all sequences, c = b D + d, are
-// numbered through; a block of 128 threads owns a line of them (128 or 64
-// bytes a frame, two channels a lane) and walks time in tiles of 4 to 16 runs
-// of 16 frames (8 of float32).  cp.async brings a tile to shared memory while
-// the one before it is worked on.  A thread composes the frames of its run to
-// (A, B) with h_out = A h_in + B, learns its h_in from the runs before it, and
-// goes over its frames again to write the outputs in the place of the inputs,
-// from where whole 16-byte pieces go out.  Few channels: time is cut into
-// segments, a first kernel composes each to one (A, B), and a segment's blocks
-// start from what the segments before them give.  That reads two arrays twice,
-// and still took 38 us forward and 54 us backward for 1 x 32768 x 256 float32
-// where 8 blocks of a cluster, exchanging (A, B) at every tile, took 105 and
-// 127: a step of those waits for the slowest of the 8.
+// numbered through; a block owns a line of them (128 or 64 bytes a frame, two
+// channels a lane) and walks time in tiles, which cp.async brings to shared
+// memory while the ones before are worked on.  A thread takes runs of 16 frames
+// (8 of float32) and writes the outputs in the place of the inputs, from where
+// whole 16-byte pieces go out.  Two ways to walk:
+//   alone (16 bits, forward, many lines): a block is one warp, a tile one run;
+//   the state passes from run to run in registers.
+//   composed: a block is 128 threads, a tile 4 to 16 runs.  A thread composes the
+//   frames of its run to (A, B) with h_out = A h_in + B, learns its h_in from the
+//   runs before it, and goes over its frames again.
+// Few channels: time is cut into segments, a first kernel composes each to one
+// (A, B), and a segment's blocks start from what the segments before them give.
+// That reads two arrays twice, and still takes 34 us forward and 50 us backward
+// for 1 x 32768 x 256 float32, where 8 blocks of a cluster, exchanging (A, B) at
+// every tile, took 105 and 127: a step of those waits for the slowest of the 8.
 // Everything is summed in a fixed order.
 //
-// 32 x 1024 x 1024: float32 78 us forward and 123 backward, 79% and 84% of what
-// a copy of the same bytes takes; bfloat16 56 and 85, where the bytes are half
-// and the instructions, some 30 a value forward (gate, composition, second
-// walk), are not: the schedulers issue in 55 to 60% of their cycles with the 12
-// to 14 warps that 512 blocks give an SM.
+// 32 x 1024 x 1024: float32 75 us forward and 121 backward, 82% and 85% of what
+// a copy of the same bytes takes; bfloat16 53 (alone) and 73 (composed), where
+// the bytes are half and the instructions, some 30 a value composed (gate,
+// composition, second walk), are not: with the few warps that 512 lines give an
+// SM the schedulers issue in 55 to 60% of their cycles.
 //
 // The forward saves h before every run in float32 (0.25 bytes a 16-bit value,
 // 0.5 a float32 one); the backward recomputes the states of a run from it, so
@@ -39,7 +42,7 @@
 // instructions that a 16-byte copy shares among 4 to 8 values.  Its long
 // sequences of few channels are shared by up to 8 blocks of a cluster, which
 // take neighbouring tiles and compose their (A, B) through each other's shared
-// memory.
+// memory (1 x 32768 x 257 float32: 121 us forward, 155 backward).
 #include "../../include/torchwarp_b200.h"
 #include "element.cuh"
 
@@ -277,6 +280,7 @@ __device__ __forceinline__ float peer_read(const float* p, uint32_t rank) {
   return v;
 }
 __device__ __forceinline__ void cluster_sync_all() {
+  __syncwarp();  // the barrier wants whole warps
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -1104,8 +1108,9 @@ struct TilePlan {
 };
 
 // Forward, 16 bits, and lines for three warps a SM at least: a warp alone walks
-// a line (32 x 1024 x 1024 bfloat16: 51 us against 56 of blocks whose four runs
-// are composed; 64 x 64 x 2048: 13.4 against 16.9).  float32 is within a fifth
+// a line (measured when it was added: 32 x 1024 x 1024 bfloat16 51 us against 56
+// of blocks whose four runs are composed; 64 x 64 x 2048 13.4 against 16.9; other
+// shapes were not compared).  float32 is within a fifth
 // of a copy's time without it.
 constexpr size_t ALONE_FROM = 148 * 3;
 template <typename T>
