@@ -686,3 +686,51 @@ def test_float32_activation_tails(tw, least, most, m, act):
         # the slope's factor and the large side of f add their own roundings
         bound = bound if w is want else 8 * bound
         assert ((got.double() - w).abs() <= bound)[where].all()
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float64])
+def test_states_are_float32_whatever_the_default_type(tw, randn, default):
+    x = randn(3, 20, 5)
+    results = []
+    for kind in (torch.float32, default):
+        torch.manual_seed(1)
+        enc = tw.SequenceEncoder(5, 16, layers=1, device=DEV, dtype=torch.float32)
+        torch.set_default_dtype(kind)
+        try:
+            states = enc.init_state(3)
+            y = enc.step(x[:, 0], states)
+            out = [y, *states]
+            for bits in (8, 32):
+                opt = tw.AdamW(enc.parameters(), state_bits=bits)
+                enc(x).square().sum().backward()
+                opt.step()
+                out += [v for k, v in opt.flat_state().items()]
+                for k, v in opt.flat_state().items():
+                    assert v.dtype == (torch.float8_e4m3fn if bits == 8 and "scale" not in k
+                                       else torch.float32)
+        finally:
+            torch.set_default_dtype(torch.float32)
+        results.append([v.float() for v in out] + [p.detach() for p in enc.parameters()])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+def test_adamw_step_refuses_states_of_another_kind(tw, randn):
+    """The host entry itself: nothing is launched on buffers that the kernel would overrun."""
+    from torchwarp_b200 import _native
+    p = torch.nn.Parameter(randn(600))
+    p.grad = randn(600)
+    f = dict(device=DEV, dtype=torch.float32)
+    m, s, step = torch.zeros(768, **f), torch.zeros(3, **f), torch.zeros(2, device=DEV,
+                                                                       dtype=torch.int32)
+    c = torch.zeros(768, device=DEV).to(torch.float8_e4m3fn)
+    rest = (step, 1e-3, None, 0.9, 0.999, 1e-8, 0.0, 0)
+    host = _native.host()
+    host.adamw_step([p], [600], 32, m, None, m.clone(), None, *rest)
+    host.adamw_step([p], [600], 8, c, s, c.clone(), s.clone(), *rest)
+    for bits, a, x, b, y in ((32, m.bfloat16(), None, m, None), (32, m, None, m.double(), None),
+                             (32, m[:767], None, m, None), (32, m, s, m, s), (32, m.cpu(), None, m, None),
+                             (8, c, s, m, s), (8, c, s[:2], c, s), (8, c, None, c, s),
+                             (8, c, s, c, s.bfloat16())):
+        with pytest.raises((RuntimeError, ValueError)):
+            host.adamw_step([p], [600], bits, a, x, b, y, *rest)

@@ -660,7 +660,18 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<int64_t>& s
                                (uint64_t)offset});
   }
   if (!any) return;  // no step
-  TORCH_CHECK(m.numel() >= offset && v.numel() >= offset, "adamw_step: the states are too short");
+  const at::ScalarType kind = bits == 8 ? at::kFloat8_e4m3fn : at::kFloat;
+  for (const Tensor* t : {&m, &v})
+    TORCH_CHECK(t->is_cuda() && t->is_contiguous() && t->scalar_type() == kind &&
+                    t->numel() >= offset,
+                "adamw_step: the states are too short or of another type");
+  for (const OptTensor* t : {&ms, &vs})
+    TORCH_CHECK(t->has_value() == (bits == 8) &&
+                    (bits != 8 || ((*t)->is_cuda() && (*t)->is_contiguous() &&
+                                   (*t)->scalar_type() == at::kFloat &&
+                                   (*t)->numel() * 256 >= offset)),
+                "adamw_step: the scales are too short or of another type");
+  TORCH_CHECK(step.is_cuda() && step.numel() == 2, "adamw_step: the step is two int32 values");
   const float* lr_device = nullptr;
   if (lr_tensor.has_value()) {
     const Tensor& t = *lr_tensor;

@@ -106,9 +106,9 @@ class SequenceEncoder(nn.Module):
         return self.norm(x)
 
     def init_state(self, batch):
-        """The states before the first frame, one [batch, dim] tensor a block."""
-        dev = self.embed.weight.device
-        return [torch.zeros(batch, self.dim, device=dev) for _ in self.blocks]
+        """The states before the first frame, one float32 [batch, dim] tensor a block."""
+        kw = {"dtype": torch.float32, "device": self.embed.weight.device}
+        return [torch.zeros(batch, self.dim, **kw) for _ in self.blocks]
 
     @torch.no_grad()
     def step(self, x, states):

@@ -23,16 +23,16 @@ class _Bucket:
         self.sizes = [p.numel() for p in params]
         at = sum(-(-n // _BLOCK) * _BLOCK for n in self.sizes)
         dev = self.device
+        f32 = dict(dtype=torch.float32, device=dev)
         self.step = torch.zeros(2, dtype=torch.int32, device=dev)
         if bits == 32:
-            self.state = {"exp_avg": torch.zeros(at, device=dev),
-                          "exp_avg_sq": torch.zeros(at, device=dev)}
+            self.state = {"exp_avg": torch.zeros(at, **f32), "exp_avg_sq": torch.zeros(at, **f32)}
         else:
             code = dict(dtype=_CODE, device=dev)
             self.state = {"exp_avg": torch.zeros(at, **code),
-                          "exp_avg_scale": torch.zeros(at // _BLOCK, device=dev),
+                          "exp_avg_scale": torch.zeros(at // _BLOCK, **f32),
                           "exp_avg_sqrt": torch.zeros(at, **code),
-                          "exp_avg_sqrt_scale": torch.zeros(at // _BLOCK, device=dev)}
+                          "exp_avg_sqrt_scale": torch.zeros(at // _BLOCK, **f32)}
         self.bits = bits
 
     # pickle takes no float8 tensors: codes travel as bytes
