@@ -734,3 +734,23 @@ def test_adamw_step_refuses_states_of_another_kind(tw, randn):
                              (8, c, s, c, s.bfloat16())):
         with pytest.raises((RuntimeError, ValueError)):
             host.adamw_step([p], [600], bits, a, x, b, y, *rest)
+
+
+def test_adamw_first_step_is_not_captured(tw, randn):
+    """A graph that made the states would zero them at every replay."""
+    p = torch.nn.Parameter(randn(300))
+    p.grad = randn(300)
+    opt = tw.AdamW([p], lr=1e-2)
+    was = p.detach().clone()
+    with pytest.raises(RuntimeError, match="before a step is captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    torch.cuda.synchronize()
+    assert torch.equal(p, was)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(2):
+        graph.replay()
+    assert opt.state_dict()["buckets"][0]["step"].item() == 3

@@ -20,6 +20,9 @@ class _Bucket:
         if self.dtype not in (torch.float32, torch.bfloat16, torch.float16):
             raise TypeError("parameters must be float32, bfloat16 or float16, got {}".format(
                 self.dtype))
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("take one step before a step is captured: a replay would zero the "
+                               "states that the captured one makes")
         self.sizes = [p.numel() for p in params]
         at = sum(-(-n // _BLOCK) * _BLOCK for n in self.sizes)
         dev = self.device
@@ -60,7 +63,8 @@ class AdamW(torch.optim.Optimizer):
     Args:
         params: Parameters or groups of them: float32, bfloat16 or float16 CUDA tensors.
         lr: Learning rate, a number or a one-element float32 CUDA tensor.  A step captured in a
-            CUDA graph reads the tensor at each replay; a number is captured as it is.
+            CUDA graph (after one that was not) reads the tensor at each replay; a number is
+            captured as it is.
         betas, eps, weight_decay: As in ``torch.optim.AdamW``.
         state_bits: 32, or 8: the first moment and the root of the second as e4m3 codes with a
             float32 scale per 256 values, rounded stochastically.
