@@ -754,3 +754,29 @@ def test_adamw_first_step_is_not_captured(tw, randn):
     for _ in range(2):
         graph.replay()
     assert opt.state_dict()["buckets"][0]["step"].item() == 3
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,t,d", SCAN_FORMS)
+def test_scan_bad_values_stay_in_their_channel(tw, randn, b, t, d, dtype):
+    """Every other channel, and in time all that a bad value does not reach, keeps its bits."""
+    x, gate, h0, lengths, dy, ds = _scan_inputs(randn, b, t, d, dtype)
+    c, at = (0, d - 1), t // 2
+
+    def run(spoil):
+        xs, hs, ys, es = x.clone(), h0.clone(), dy.clone(), ds.clone()
+        if spoil:
+            xs[0, at, c[0]], xs[0, at, c[1]] = float("nan"), float("inf")
+            hs[2 % b, 0], ys[0, at, d // 2], es[0, 1] = float("-inf"), float("nan"), float("inf")
+        leaves = [v.requires_grad_(True) for v in (xs, gate.detach().clone(), hs)]
+        y, last = tw.functional.gated_scan(*leaves, lengths=lengths)
+        return y, last, *torch.autograd.grad((y, last), leaves, (ys, es))
+
+    spoilt = torch.zeros(b, d, dtype=torch.bool, device=DEV)
+    spoilt[0, [0, d - 1, d // 2, 1]] = True
+    spoilt[2 % b, 0] = True
+    got, want = run(True), run(False)
+    for u, w in zip(got, want):
+        u, w = (v.transpose(1, 2) if v.dim() == 3 else v for v in (u, w))
+        assert torch.equal(u[~spoilt], w[~spoilt])
+    assert torch.equal(got[0][0, :at, d - 1], want[0][0, :at, d - 1])  # outputs before a bad input

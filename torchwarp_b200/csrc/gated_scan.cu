@@ -114,7 +114,8 @@ __device__ __forceinline__ Vec<V> passed(Vec<V> n, Vec<V> l, Vec<V> neg_l) {
 // The steps above hold for finite values; an infinity meets itself in h - x or
 // in l - (1 - f) l.  Once there, what is not finite stays so to the end of a run,
 // so a run looks once and then goes again by the definition (`define`,
-// `define_back`), reading global memory, frame by frame.
+// `define_back`), reading global memory, frame by frame.  A neighbour that shares
+// its thread, and frames before the first infinity, keep their bits.
 template <int V>
 __device__ __forceinline__ bool finite(Vec<V> v) {
   bool r = true;
@@ -131,18 +132,40 @@ __device__ __forceinline__ void both_gates(Vec<V> n, Vec<V>& f, Vec<V>& omf) {
     omf.v[i] = __float_as_int(n.v[i]) < 0 ? a : 1.f - a;
   }
 }
+// a where it is finite, else b.
+template <int V>
+__device__ __forceinline__ Vec<V> unless_odd(Vec<V> a, Vec<V> b) {
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (!(fabsf(a.v[i]) < INFINITY)) a.v[i] = b.v[i];
+  return a;
+}
 // f h + (1 - f) x
 template <int V>
 __device__ __forceinline__ Vec<V> advance_any(Vec<V> n, Vec<V> h, Vec<V> x) {
   Vec<V> f, omf;
   both_gates(n, f, omf);
-  return fma_v(f, h, mul_v(omf, x));
+  return unless_odd(advance(n, h, x, sub_v(h, x)), fma_v(f, h, mul_v(omf, x)));
 }
 // A product of gates that are not zero is not zero: it carries an infinite
 // state.  1.4e-45 times a finite one is below its rounding.
 __device__ __forceinline__ float times_gate(float a, float by) {
   const float r = a * by;
   return r == 0.f && a != 0.f && by != 0.f ? 1.4e-45f : r;
+}
+
+// f l, (1 - f) l and f (1 - f) l diff.  With a = |n| and b = a l: the smaller of
+// the first two is b, the other l - b; f (1 - f) l = b - a b.
+template <int V>
+__device__ __forceinline__ void gradients(Vec<V> n, Vec<V> l, Vec<V> diff, Vec<V>& fl, Vec<V>& dx,
+                                          Vec<V>& dg) {
+  Vec<V> a;
+#pragma unroll
+  for (int v = 0; v < V; ++v) a.v[v] = fabsf(n.v[v]);
+  const Vec<V> b = mul_v(a, l), c = sub_v(l, b);
+  fl = pick(n, c, b);
+  dx = pick(n, b, c);
+  dg = mul_v(fma_v(negated(a), b, b), diff);
 }
 
 // VC neighbouring channels of a frame, as they lie in memory.
@@ -224,11 +247,14 @@ __device__ __forceinline__ Vec<VC> define_back(Far<T, VC> y, Far<T, VC> x, Far<T
 #pragma unroll 1
   for (int k = n - 1; k >= 0; --k) {
     const Vec<VC> before = define(x, g, k, h, [](int, Vec<VC>) {});
-    Vec<VC> f, omf;
-    both_gates(gate_of(g[k]), f, omf);
-    l = add_v(y[k], l);
-    put(k, mul_v(omf, l), mul_v(mul_v(mul_v(l, sub_v(before, x[k])), f), omf));
-    l = mul_v(f, l);
+    const Vec<VC> n = gate_of(g[k]), diff = sub_v(before, x[k]);
+    const Vec<VC> all = add_v(y[k], l);
+    Vec<VC> f, omf, dx, dg;
+    both_gates(n, f, omf);
+    gradients(n, all, diff, l, dx, dg);
+    l = unless_odd(l, mul_v(f, all));
+    put(k, unless_odd(dx, mul_v(omf, all)),
+        unless_odd(dg, mul_v(mul_v(mul_v(all, diff), f), omf)));
   }
   return l;
 }
@@ -243,7 +269,12 @@ __device__ __forceinline__ Vec<VC> define_sum(Far<T, VC> v, Far<T, VC> g, int n)
     const Vec<VC> s = gate_of(g[k]);
     Vec<VC> f, omf;
     both_gates(s, f, omf);
-    B = REV ? mul_v(f, add_v(v[k], B)) : advance_any(s, B, v[k]);
+    if (REV) {
+      const Vec<VC> l = add_v(v[k], B);
+      B = unless_odd(decay(s, l), mul_v(f, l));
+    } else {
+      B = advance_any(s, B, v[k]);
+    }
   }
   return B;
 }
@@ -997,19 +1028,13 @@ __global__ void __launch_bounds__(SCAN_THREADS, 4)
     keep_product<FR>(A, s);
     compose<2, LPR, true>(sh, it, 1, 0, part, lane, A, B, run, lam);
     plain = plain && finite(lam);
-    // With a = |n| and b = a l: the smaller of f l and (1 - f) l is b, the other
-    // l - b; f (1 - f) l = b - a b.
     auto finish = [&](bool all) {
 #pragma unroll
       for (int k = FR - 1; k >= 0; --k) {
         const Vec<2> l = add_v(yf[k].get(), lam);
-        Vec<2> a;
-#pragma unroll
-        for (int v = 0; v < 2; ++v) a.v[v] = fabsf(s[k].v[v]);
-        const Vec<2> b = mul_v(a, l), c = sub_v(l, b);
-        lam = pick(s[k], c, b);
-        const F vx = F::of(pick(s[k], b, c));
-        const F vg = F::of(mul_v(fma_v(negated(a), b, b), diff[k]));
+        Vec<2> dxv, dgv;
+        gradients(s[k], l, diff[k], lam, dxv, dgv);
+        const F vx = F::of(dxv), vg = F::of(dgv);
         xf[k] = all || k < n ? vx : F::zero();
         gf[k] = all || k < n ? vg : F::zero();
       }
