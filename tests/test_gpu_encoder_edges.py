@@ -780,3 +780,17 @@ def test_scan_bad_values_stay_in_their_channel(tw, randn, b, t, d, dtype):
         u, w = (v.transpose(1, 2) if v.dim() == 3 else v for v in (u, w))
         assert torch.equal(u[~spoilt], w[~spoilt])
     assert torch.equal(got[0][0, :at, d - 1], want[0][0, :at, d - 1])  # outputs before a bad input
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", [None, "gelu", "silu", "sigmoid"])
+@pytest.mark.parametrize("m,n,k", [(4, 64, 32), (200, 130, 96), (20, 40, 4096)])
+def test_linear_values_do_not_depend_on_their_neighbours(tw, randn, m, n, k, act, dtype):
+    """Large, infinite and NaN values in some columns leave the bits of the others."""
+    x, w, b = randn(m, k, dtype=dtype), (randn(n, k) / k ** 0.5).to(dtype), randn(n, dtype=dtype)
+    want = tw.functional.linear(x, w, b, activation=act)
+    odd = torch.zeros(n, dtype=torch.bool, device=DEV)
+    odd[[0, 5, 9, 33]] = True
+    b[0], b[5], b[9], b[33] = 50, -90, float("inf"), float("nan")
+    got = tw.functional.linear(x, w, b, activation=act)
+    assert torch.equal(got[:, ~odd], want[:, ~odd])

@@ -246,19 +246,22 @@ __device__ __forceinline__ void activate_all(float (&v)[32]) {
     v[i + 1] = r.v[1];
   }
 }
-// silu (or sigmoid) of n float32 values of any size, one after the other: not
-// inlined, as a kernel of one or two tiles pays for every line of code once.
+// silu (or sigmoid) of n float32 values of any size, one after the other, in the
+// long form where a value needs it: not inlined, as a kernel of one or two tiles
+// pays for every line of code once.
 __device__ __noinline__ void sigmoid_far(float* v, int n, bool silu) {
 #pragma unroll 1
   for (int i = 0; i < n; ++i) {
     const Vec<1> z = {{v[i]}};
-    v[i] = (silu ? act_value<kActSilu, false>(z) : act_value<kActSigmoid, false>(z)).v[0];
+    const float f = fabsf(v[i]) <= 6.f ? act_value<kActSigmoid, true>(z).v[0]
+                                       : act_value<kActSigmoid, false>(z).v[0];
+    v[i] = silu ? mul_rn(v[i], f) : f;
   }
 }
 // float32: up to |z| = 6 the relative error of the 16-bit results' form of silu
 // and sigmoid is below 2^-20, a few ulp.  Pieces that go further are rare (7000 x
 // 257 x 385 training: 101.9 us with that form everywhere, 107.2 with the long one
-// inline, which is as much if no value needs it, 103.9 so).
+// inline, which is as much if no value needs it, 103.5 so).
 template <int ACT>
 __device__ __forceinline__ void activate_sigmoid(float (&v)[32]) {
   float m = 0.f;
