@@ -794,3 +794,31 @@ def test_linear_values_do_not_depend_on_their_neighbours(tw, randn, m, n, k, act
     b[0], b[5], b[9], b[33] = 50, -90, float("inf"), float("nan")
     got = tw.functional.linear(x, w, b, activation=act)
     assert torch.equal(got[:, ~odd], want[:, ~odd])
+
+
+def test_adamw_refused_step_changes_nothing(tw, randn):
+    """With several types and groups, what the last of them refuses holds the first back too."""
+    a, b = (torch.nn.Parameter(randn(40, 30, dtype=t)) for t in (torch.bfloat16, torch.float32))
+    c = torch.nn.Parameter(randn(7))
+    opt = tw.AdamW([{"params": [a, b]}, {"params": [c]}])
+    for p in (a, b, c):
+        p.grad = randn(*p.shape, dtype=p.dtype)
+    opt.step()
+
+    def held_back():
+        was = [p.detach().clone() for p in (a, b, c)]
+        steps = [s["step"].item() for s in opt.state_dict()["buckets"]]
+        with pytest.raises(ValueError):
+            opt.step()
+        assert all(torch.equal(p, w) for p, w in zip((a, b, c), was))
+        assert [s["step"].item() for s in opt.state_dict()["buckets"]] == steps == [1, 1, 1]
+
+    b.data = randn(30, 40).t()  # no longer contiguous
+    held_back()
+    b.data = randn(40, 30)
+    opt.param_groups[1]["lr"] = torch.ones(2, device=DEV)
+    held_back()
+    opt.param_groups[1]["lr"] = 1e-3
+    c.grad, c.data = None, randn(9)
+    c.grad = randn(9)
+    held_back()

@@ -621,10 +621,11 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const OptTensor& sta
 
 // ------------------------------------------------------------------ AdamW
 
-// One AdamW step over `params`, which had `sizes` values each when the flat
+// One AdamW step (or, CHECK, its checks alone) over `params`, which had `sizes` values each when the flat
 // buffers of their states were made, one after the other on boundaries of 256
 // values; a parameter without a gradient is left out, and with none at all
 // nothing is done.
+template <bool CHECK>
 void adamw_step(const std::vector<Tensor>& params, const std::vector<int64_t>& sizes,
                 int64_t bits, const Tensor& m, const OptTensor& ms, const Tensor& v,
                 const OptTensor& vs, const Tensor& step, double lr, const OptTensor& lr_tensor,
@@ -679,6 +680,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<int64_t>& s
       bad_value("lr must be a number or one float32 value on " + m.device().str());
     lr_device = t.data_ptr<float>();
   }
+  if (CHECK) return;
   c10::cuda::CUDAGuard guard(m.device());
   check_status(TW_PICK(tw_adamw_step, type)(
                    table.data(), (int)(table.size() / 4), (int)bits, ptr(m),
@@ -706,7 +708,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear", &linear);
   m.def("gated_scan", &gated_scan);
   m.def("gated_scan_step", &gated_scan_step);
-  m.def("adamw_step", &adamw_step);
+  m.def("adamw_step", &adamw_step<false>);
+  m.def("adamw_check", &adamw_step<true>);
+  // whether two sequences hold the same objects, in one order
+  m.def("same_objects", [](const py::tuple& a, const py::list& b) {
+    bool same = a.size() == b.size();
+    for (size_t i = 0; same && i < a.size(); ++i)
+      same = PyTuple_GET_ITEM(a.ptr(), i) == PyList_GET_ITEM(b.ptr(), i);
+    return same;
+  });
   // without autograd, for the custom ops
   m.def("layer_norm_forward", [](const Tensor& x, const OptTensor& w, const OptTensor& b,
                                  double eps, bool save) {

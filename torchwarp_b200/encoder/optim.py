@@ -1,7 +1,5 @@
 """AdamW over all parameters of a group in one launch, with 32-bit or 8-bit states."""
 
-import operator
-
 import torch
 
 from .. import _native as nat
@@ -105,7 +103,7 @@ class AdamW(torch.optim.Optimizer):
                 kinds.setdefault((p.device, p.dtype), []).append(p)
             self._buckets[index] = tuple(group), [_Bucket(ps, self._bits) for ps in kinds.values()]
         members, have = self._buckets[index]
-        if len(members) != len(group) or not all(map(operator.is_, members, group)):
+        if not nat.host().same_objects(members, group):
             raise ValueError("the parameters of group {} are not those that its states were made "
                              "for; new ones come with add_param_group".format(index))
         return have
@@ -116,15 +114,22 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        launches = []
         for index, group in enumerate(self.param_groups):
             lr = group["lr"]
             on_device = isinstance(lr, torch.Tensor)
             for b in self._group_buckets(index):
                 m, ms, v, vs = b.buffers()
-                nat.host().adamw_step(b.params, b.sizes, self._bits, m, ms, v, vs, b.step,
-                                      0.0 if on_device else lr, lr if on_device else None,
-                                      *group["betas"], group["eps"], group["weight_decay"],
-                                      self._seed & 0xFFFFFFFF)
+                launches.append((b.params, b.sizes, self._bits, m, ms, v, vs, b.step,
+                                 0.0 if on_device else lr, lr if on_device else None,
+                                 *group["betas"], group["eps"], group["weight_decay"],
+                                 self._seed & 0xFFFFFFFF))
+        host = nat.host()
+        if len(launches) > 1:  # a refused step changes nothing
+            for args in launches:
+                host.adamw_check(*args)
+        for args in launches:
+            host.adamw_step(*args)
         return loss
 
     def flat_state(self, index=0):
