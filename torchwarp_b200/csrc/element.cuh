@@ -353,10 +353,13 @@ __device__ __forceinline__ Vec<V> act_slope(Vec<V> z) {
   } else if constexpr (ACT == kActSilu || ACT == kActSigmoid) {
     Vec<V> f, omf;
     sigmoid_pair<FAST>(z, f, omf);
-    if (ACT == kActSigmoid) return mul_v(f, omf);
+    if constexpr (ACT == kActSigmoid) {
+      return mul_v(f, omf);
+    } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) z.v[i] = fmaxf(fminf(z.v[i], 128.f), -128.f);
-    return mul_v(f, fma_v(z, omf, splat<V>(1.f)));
+      for (int i = 0; i < V; ++i) z.v[i] = fmaxf(fminf(z.v[i], 128.f), -128.f);
+      return mul_v(f, fma_v(z, omf, splat<V>(1.f)));
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
